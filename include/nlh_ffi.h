@@ -515,6 +515,48 @@ int32_t nlh_copy_rows(const float* src, int64_t src_stride, float* dst, int32_t 
 /* dst [cols, rows] <- src [rows, cols] transposed. */
 int32_t nlh_transpose(const float* src, float* dst, int32_t rows, int32_t cols);
 
+/* ── Gated delta rule (additive, no counterpart in the reference) ──────────────────────────────
+ *   M_t = e^{g_t} M_{t-1} + u_t k_t^T,  u_t = theta_t (v_t - e^{g_t} M_{t-1} k_t),  y_t = scale M_t q_t
+ * beside the Delta rule above (core/src/delta_rule.rs), which takes its error before the decay. M [dv, dk]
+ * fp32, g = log_retain. k, q [batch, seq, heads_k, dk], v [batch, seq, heads_v, dv] and d_y like v, all bf16 or all fp32
+ * (is_bf16), log_retain and theta [batch, seq, heads_v] fp32; strides in elements, the last axis contiguous. Value head
+ * h reads key head h / (heads_v / heads_k). dk, dv in 1..128. m_initial [sequences, heads_v, dv, dk] or NULL (zeros).
+ * y, d_k, d_v, d_q (in the inputs' type) and d_log_retain, d_theta (fp32) are contiguous in the inputs' shapes.
+ * Packed batches: batch = 1, n_seqs > 0, seq_starts [n_seqs + 1] on the device, sequence i = tokens
+ * seq_starts[i] .. seq_starts[i + 1] - 1. Starts are clamped to [0, seq] and to their running maximum; a sequence may be
+ * empty (m_final = m_initial); tokens outside the sequences are not read, and their rows of y and of the gradients of v, log_retain
+ * and theta are not written (those of k and q neither, unless heads are shared).
+ * A log_retain below -200 counts as -200 (e^-200 is 0 in fp32), a theta below 2^-60 in magnitude as 2^-60. A value that is not
+ * finite, or above 4e34, may make any output of its sequence from the start of its chunk of 64 tokens a NaN (backward: of its whole sequence). */
+typedef struct nlh_gated_delta_desc {
+    int32_t batch, seq, heads_k, heads_v, dk, dv;
+    int32_t n_seqs;      /* sequences of a packed batch; 0: dense */
+    int32_t is_bf16;
+    int64_t k_batch, k_token, k_head;
+    int64_t v_batch, v_token, v_head;
+    int64_t q_batch, q_token, q_head;
+    int64_t gate_batch, gate_token, gate_head;
+    int64_t dy_batch, dy_token, dy_head;
+    float scale;
+} nlh_gated_delta_desc;
+/* Bytes of the buffer that the forward writes and the backward reads, and of the backward's scratch. Both belong to the
+ * caller, are 16-byte aligned and are in use until the call's work on the stream has ended. -1: bad descriptor. */
+int64_t nlh_gated_delta_saved_bytes(const nlh_gated_delta_desc* desc);
+int64_t nlh_gated_delta_backward_bytes(const nlh_gated_delta_desc* desc);
+int32_t nlh_gated_delta_forward(const nlh_gated_delta_desc* desc, const void* k, const void* v, const void* q,
+    const float* log_retain, const float* theta, const float* m_initial, const int32_t* seq_starts, void* y,
+    float* m_final, void* saved, int64_t saved_bytes);
+/* d_m_final [sequences, heads_v, dv, dk] or NULL (zeros); d_m_initial may be NULL. */
+int32_t nlh_gated_delta_backward(const nlh_gated_delta_desc* desc, const void* k, const void* v, const void* q,
+    const float* log_retain, const float* theta, const int32_t* seq_starts, const void* saved, int64_t saved_bytes,
+    const void* d_y, const float* d_m_final, void* d_k, void* d_v, void* d_q, float* d_log_retain, float* d_theta,
+    float* d_m_initial, void* workspace, int64_t workspace_bytes);
+/* Recurrent form: seq tokens (one, or a few) for each of batch sequences on stored states m [n_slots, heads_v, dv, dk],
+ * updated in place. slots [batch] on the device gives each sequence's state; NULL: sequence i has state i. A slot outside
+ * [0, n_slots) is skipped and its rows of y are not written. A slot named more than once is stepped in the order of the batch. */
+int32_t nlh_gated_delta_step(const nlh_gated_delta_desc* desc, const void* k, const void* v, const void* q,
+    const float* log_retain, const float* theta, float* m, const int32_t* slots, int32_t n_slots, void* y);
+
 /* ── Host-slice dispatch layer (compiled counterpart of core/src/dispatch.rs `*_dispatch`) ────
  * Same argument order and meaning as the reference functions its kernel tests call
  * (swa_forward_dispatch dispatch.rs:378, swa_backward_dispatch :408, delta :746/:775, titans

@@ -1,0 +1,1081 @@
+// Gated delta rule: chunked forward and backward, recurrent step. Mathematics and products: gated_delta.cuh.
+//
+// Only the state in front of each chunk is a recurrence; the rest of a chunk is known once that state is.
+// So a pass has three parts: what needs no state, for all chunks at once (prep); the states, one after the
+// other, divided over the columns of V, which never meet (state); what needs them, for all chunks at once
+// (out). The backward has the same three parts. Every sum has one order: no atomics.
+#include "gated_delta.cuh"
+#include "nlh_common.cuh"
+#include "../../include/nlh_ffi.h"
+
+namespace nlh {
+namespace gd {
+
+// ── ragged batches: sequence, first token and length of every chunk slot ──
+// Starts are taken at their running maximum inside [0, seq], so that no value of them can lead out of the buffers:
+// the lengths are not negative and add up to seq at most, which bounds the chunks by seq / 64 + n_seqs.
+__device__ __forceinline__ int block_scan(int v, bool take_max, int* s_warp)
+{
+    const int lane = threadIdx.x & 31, w = threadIdx.x >> 5;
+    for (int o = 1; o < 32; o <<= 1) {
+        const int y = __shfl_up_sync(0xffffffffu, v, o);
+        if (lane >= o) v = take_max ? max(v, y) : v + y;
+    }
+    if (lane == 31) s_warp[w] = v;
+    __syncthreads();
+    for (int j = 0; j < w; j++) v = take_max ? max(v, s_warp[j]) : v + s_warp[j];
+    return v;
+}
+__global__ void __launch_bounds__(1024) gd_map_kernel(Args A)
+{
+    __shared__ int s_warp[32], s_last;
+    for (int pass = 0; pass < 2; pass++) {          // running maximum of the starts, then the sum of the chunks before each
+        int carry = 0;
+        for (int base = 0; base <= A.n_seqs; base += 1024) {
+            const int i = base + threadIdx.x;
+            int v = 0, n = 0;
+            if (pass == 0) v = i <= A.n_seqs ? min(max(A.starts[i], 0), A.seq) : 0;
+            else v = n = i < A.n_seqs ? (A.start[i + 1] - A.start[i] + C - 1) / C : 0;
+            v = block_scan(v, pass == 0, s_warp);
+            v = pass == 0 ? max(v, carry) : v + carry;
+            if (i <= A.n_seqs) (pass == 0 ? A.start : A.off)[i] = v - n;
+            if (threadIdx.x == 1023) s_last = v;
+            __syncthreads();
+            carry = s_last;
+            __syncthreads();
+        }
+    }
+    for (int slot = threadIdx.x; slot < A.slots; slot += 1024) {
+        int lo = 0, hi = A.n_seqs;                  // off[lo] <= slot; the last such lo
+        while (lo < hi) {
+            const int mid = (lo + hi + 1) >> 1;
+            if (A.off[mid] <= slot) lo = mid; else hi = mid - 1;
+        }
+        int4 m = make_int4(0, 0, 0, 0);
+        if (lo < A.n_seqs) {
+            const int t0 = A.start[lo] + (slot - A.off[lo]) * C;
+            m = make_int4(lo, t0, min(C, A.start[lo + 1] - t0), 0);
+        }
+        A.map[slot] = m;
+    }
+}
+
+__device__ __forceinline__ int first_slot(const Args& A, int seq) { return A.starts ? A.off[seq] : seq * A.nc; }
+__device__ __forceinline__ int chunk_count(const Args& A, int seq) { return A.starts ? A.off[seq + 1] - A.off[seq] : A.nc; }
+
+// ── prep: gates and T = (I + B diag(theta))^-1 of a chunk ──
+// One CTA of four warps per chunk and value head. T is built from the inverses of its 16 x 16 diagonal blocks
+// (forward substitution, a thread per column) by [[P, 0], [R, S]]^-1 = [[P', 0], [-S' R P', S']] twice, in fp32 FMA.
+// A theta of 0 is taken as 2^-60: then u is 2^-60 e, which no sum of fp32 sees, and the gradient e.x / theta of
+// theta needs no case of its own (x, the gradient of v, carries the factor theta).
+template <typename T>
+__global__ void __launch_bounds__(128) gd_prep_kernel(Args A)
+{
+    extern __shared__ float4 smem4[];
+    float* Ks = reinterpret_cast<float*>(smem4);
+    float *Am = Ks + C * LD, *Tm = Am + C * LD;
+    __shared__ float2 s_g[C];
+    __shared__ float s_theta[C];
+    const int slot = blockIdx.x / A.hv, h = blockIdx.x - slot * A.hv;
+    const Chunk ch = get_chunk(A, slot);
+    if (ch.len <= 0) return;
+    const long long tile = (long long)slot * A.hv + h;
+    const int tid = threadIdx.x, lane = tid & 31, w = tid >> 5, g = lane >> 2, t = lane & 3;
+
+    if (w == 0) {
+        const long long at = ch.b * A.gb + ch.t0 * A.gt + h * A.gh;
+        double x[2], th[2];
+#pragma unroll
+        for (int j = 0; j < 2; j++) {
+            const int i = 2 * lane + j;
+            float gv = 0.f, tv = 0.f;
+            if (i < ch.len) { gv = A.g[at + i * A.gt]; tv = A.theta[at + i * A.gt]; }
+            x[j] = gv < G_FLOOR ? G_FLOOR : gv;
+            th[j] = fabsf(tv) < THETA_TINY ? THETA_TINY : tv;
+        }
+        double s = x[0] + x[1];
+        for (int o = 1; o < 32; o <<= 1) { const double y = __shfl_up_sync(0xffffffffu, s, o); if (lane >= o) s += y; }
+        const double last = __shfl_sync(0xffffffffu, s, 31);
+#pragma unroll
+        for (int j = 0; j < 2; j++) {
+            const int i = 2 * lane + j;
+            const double G = j == 1 ? s : s - x[1];
+            const float hi = (float)G;
+            const float4 o = make_float4(hi, (float)(G - hi), expf(hi), expf((float)(last - G)));
+            A.gates[tile * C + i] = o;
+            A.theta_eff[tile * C + i] = (float)th[j];
+            s_g[i] = make_float2(o.x, o.y);
+            s_theta[i] = (float)th[j];
+        }
+    }
+    float lo[4][4], hi[4][4];
+    zero(lo);
+    zero(hi);
+    const T* kp = (const T*)A.k + ch.b * A.kb + ch.t0 * A.kt + (h / A.share) * A.kh;
+    for (int c0 = 0; c0 < A.dk; c0 += 64) {
+        __syncthreads();
+        load_tile<T, 64, 128>(Ks, LD, kp + c0, A.kt, ch.len, A.dk - c0);
+        __syncthreads();
+        gemm16<4, false, false, Pl<T>::in, Pl<T>::in>(lo, Ks + 16 * w * LD, LD, Ks, LD, 0, 64);
+        if (w >= 2) gemm16<4, false, false, Pl<T>::in, Pl<T>::in>(hi, Ks + 16 * w * LD, LD, Ks + 32 * LD, LD, 0, 64);
+    }
+    for (int i = tid; i < C * LD / 4; i += 128) reinterpret_cast<float4*>(Tm)[i] = make_float4(0.f, 0.f, 0.f, 0.f);
+#pragma unroll
+    for (int half = 0; half < 2; half++)
+#pragma unroll
+        for (int n = 0; n < 4; n++)
+#pragma unroll
+            for (int r = 0; r < 2; r++) {
+                const int i = 16 * w + g + 8 * r, j = 32 * half + 8 * n + 2 * t;
+                float a[2];
+#pragma unroll
+                for (int c = 0; c < 2; c++) {
+                    const float kk = half ? hi[n][2 * r + c] : lo[n][2 * r + c];
+                    a[c] = j + c < i ? decay(s_g[i], s_g[j + c]) * kk * s_theta[j + c] : 0.f;
+                }
+                st2(Am + i * LD + j, a[0], a[1]);
+            }
+    __syncthreads();
+    if (tid < 64) {
+        const int b = tid & ~15, j = tid & 15;
+        float col[16];
+#pragma unroll
+        for (int i = 0; i < 16; i++) {
+            float s = i == j ? 1.f : 0.f;
+            const float* row = Am + (b + i) * LD + b;
+#pragma unroll
+            for (int l = 0; l < i; l++) s = l < j ? s : fmaf(-row[l], col[l], s);
+            col[i] = i < j ? 0.f : s;
+            Tm[(b + i) * LD + b + j] = col[i];
+        }
+    }
+    __syncthreads();
+    float* Z = Ks;
+    {   // 16 -> 32, both pairs of blocks at once
+        const int p = tid >> 6, r = (tid >> 2) & 15, c = (tid & 3) * 4, r0 = 32 * p + 16, c0 = 32 * p;
+        float z[4] = {0.f, 0.f, 0.f, 0.f};
+        for (int l = 0; l < 16; l++) {
+            const float a = Am[(r0 + r) * LD + c0 + l];
+            const float4 b = *reinterpret_cast<const float4*>(Tm + (c0 + l) * LD + c0 + c);
+            // columns of T behind row l are 0 and must stay out: 0 times a later token's NaN would be a NaN
+            z[0] = c > l ? z[0] : fmaf(a, b.x, z[0]);
+            z[1] = c + 1 > l ? z[1] : fmaf(a, b.y, z[1]);
+            z[2] = c + 2 > l ? z[2] : fmaf(a, b.z, z[2]);
+            z[3] = c + 3 > l ? z[3] : fmaf(a, b.w, z[3]);
+        }
+        *reinterpret_cast<float4*>(Z + (16 * p + r) * LD + c) = make_float4(z[0], z[1], z[2], z[3]);
+        __syncthreads();
+        float o[4] = {0.f, 0.f, 0.f, 0.f};
+        for (int l = 0; l <= r; l++) {
+            const float a = -Tm[(r0 + r) * LD + r0 + l];
+            const float4 b = *reinterpret_cast<const float4*>(Z + (16 * p + l) * LD + c);
+            o[0] = fmaf(a, b.x, o[0]); o[1] = fmaf(a, b.y, o[1]); o[2] = fmaf(a, b.z, o[2]); o[3] = fmaf(a, b.w, o[3]);
+        }
+        *reinterpret_cast<float4*>(Tm + (r0 + r) * LD + c0 + c) = make_float4(o[0], o[1], o[2], o[3]);
+        __syncthreads();
+    }
+    {   // 32 -> 64
+        const int r = tid >> 2, c = (tid & 3) * 8;
+        float z[8];
+#pragma unroll
+        for (int i = 0; i < 8; i++) z[i] = 0.f;
+        for (int l = c; l < 32; l++) {
+            const float a = Am[(32 + r) * LD + l];
+#pragma unroll
+            for (int i = 0; i < 8; i++) z[i] = c + i > l ? z[i] : fmaf(a, Tm[l * LD + c + i], z[i]);
+        }
+#pragma unroll
+        for (int i = 0; i < 8; i++) Z[r * LD + c + i] = z[i];
+        __syncthreads();
+#pragma unroll
+        for (int i = 0; i < 8; i++) z[i] = 0.f;
+        for (int l = 0; l <= r; l++) {
+            const float a = -Tm[(32 + r) * LD + 32 + l];
+#pragma unroll
+            for (int i = 0; i < 8; i++) z[i] = fmaf(a, Z[l * LD + c + i], z[i]);
+        }
+        __syncthreads();
+#pragma unroll
+        for (int i = 0; i < 8; i++) Tm[(32 + r) * LD + c + i] = z[i];
+    }
+    __syncthreads();
+    float* out = A.tmat + tile * C * C;
+    for (int i = tid; i < C * C / 4; i += 128)
+        reinterpret_cast<float4*>(out)[i] = *reinterpret_cast<const float4*>(Tm + (i >> 4) * LD + (i & 15) * 4);
+}
+
+// ── forward states: the recurrence over chunks for NS columns of V ──
+// Four warps; warp w owns tokens 16w.. in the products over tokens and state rows 16w.. (of each 64 of dk) in the update,
+// whose accumulators stay in registers from chunk to chunk.
+template <typename T, int DKP, int NS>
+__global__ void __launch_bounds__(128) gd_state_fwd_kernel(Args A)
+{
+    constexpr int LK = DKP + 4, LN = NS + 4, NT = NS / 8, MT = DKP / 64;
+    extern __shared__ float4 smem4[];
+    float* Ks = reinterpret_cast<float*>(smem4);            // [64][LK]
+    float *Ts = Ks + C * LK, *Ms = Ts + C * LD;             // [64][LD], [NS][LK]
+    float *Rs = Ms + NS * LK, *Us = Rs + C * LN;            // [64][LN] each
+    __shared__ float4 s_gate[C];
+    __shared__ float s_w[C];
+    const int nsl = A.dvp / NS, sl = blockIdx.x % nsl, p = blockIdx.x / nsl, h = p % A.hv, seq = p / A.hv;
+    const int n0 = sl * NS, tid = threadIdx.x, lane = tid & 31, w = tid >> 5, g = lane >> 2, t = lane & 3;
+    const int slot0 = first_slot(A, seq), count = chunk_count(A, seq);
+
+    float S[MT][NT][4];
+    const float* m0 = A.m0 ? A.m0 + ((long long)seq * A.hv + h) * A.dv * A.dk : nullptr;
+#pragma unroll
+    for (int m = 0; m < MT; m++)
+#pragma unroll
+        for (int n = 0; n < NT; n++)
+#pragma unroll
+            for (int i = 0; i < 4; i++) {
+                const int row = 64 * m + 16 * w + g + 8 * (i >> 1), col = n0 + 8 * n + 2 * t + (i & 1);   // dk, dv
+                S[m][n][i] = m0 && row < A.dk && col < A.dv ? m0[(long long)col * A.dk + row] : 0.f;
+                Ms[(col - n0) * LK + row] = S[m][n][i];
+            }
+    __syncthreads();
+    for (int c = 0; c < count; c++) {
+        const int slot = slot0 + c;
+        const Chunk ch = get_chunk(A, slot);
+        const long long tile = (long long)slot * A.hv + h;
+        const T* kp = (const T*)A.k + ch.b * A.kb + ch.t0 * A.kt + (h / A.share) * A.kh;
+        const T* vp = (const T*)A.v + ch.b * A.vb + ch.t0 * A.vt + h * A.vh + n0;
+#pragma unroll
+        for (int m = 0; m < MT; m++) load_tile<T, 64, 128>(Ks + 64 * m, LK, kp + 64 * m, A.kt, ch.len, A.dk - 64 * m);
+        load_own<64, 64, 128>(Ts, LD, A.tmat + tile * C * C, C);
+        load_tile<T, NS, 128>(Rs, LN, vp, A.vt, ch.len, A.dv - n0);
+        if (tid < C) {
+            const float4 x = A.gates[tile * C + tid];
+            s_gate[tid] = x;
+            s_w[tid] = x.w * A.theta_eff[tile * C + tid];
+        }
+        float* mc = A.m_chunk + (tile * A.dvp + n0) * DKP;
+        for (int i = tid; i < NS * DKP / 4; i += 128) {
+            const int r = i / (DKP / 4), cc = (i - r * (DKP / 4)) * 4;
+            *reinterpret_cast<float4*>(mc + (long long)r * DKP + cc) = *reinterpret_cast<const float4*>(Ms + r * LK + cc);
+        }
+        __syncthreads();
+        float acc[NT][4];
+        zero(acc);
+        gemm16<NT, false, false, Pl<T>::in, TWO>(acc, Ks + 16 * w * LK, LK, Ms, LK, 0, DKP);
+#pragma unroll
+        for (int n = 0; n < NT; n++)
+#pragma unroll
+            for (int r = 0; r < 2; r++) {
+                const int i = 16 * w + g + 8 * r;
+                float2* rp = reinterpret_cast<float2*>(Rs + i * LN + 8 * n + 2 * t);
+                const float2 v = *rp;
+                *rp = make_float2(v.x - s_gate[i].z * acc[n][2 * r], v.y - s_gate[i].z * acc[n][2 * r + 1]);
+            }
+        __syncthreads();
+        zero(acc);
+        gemm16<NT, false, true, TWO, TWO>(acc, Ts + 16 * w * LD, LD, Rs, LN, 0, 16 * (w + 1));
+        float* ep = A.e + tile * C * A.dvp + n0;
+#pragma unroll
+        for (int n = 0; n < NT; n++)
+#pragma unroll
+            for (int r = 0; r < 2; r++) {
+                const int i = 16 * w + g + 8 * r, col = 8 * n + 2 * t;
+                st2(ep + (long long)i * A.dvp + col, acc[n][2 * r], acc[n][2 * r + 1]);
+                st2(Us + i * LN + col, s_w[i] * acc[n][2 * r], s_w[i] * acc[n][2 * r + 1]);
+            }
+        __syncthreads();
+        const float gl = s_gate[C - 1].z;
+#pragma unroll
+        for (int m = 0; m < MT; m++) {
+#pragma unroll
+            for (int n = 0; n < NT; n++)
+#pragma unroll
+                for (int i = 0; i < 4; i++) S[m][n][i] *= gl;
+            gemm16<NT, true, true, Pl<T>::in, TWO>(S[m], Ks + 64 * m + 16 * w, LK, Us, LN, 0, C);
+#pragma unroll
+            for (int n = 0; n < NT; n++)
+#pragma unroll
+                for (int i = 0; i < 4; i++)
+                    Ms[(8 * n + 2 * t + (i & 1)) * LK + 64 * m + 16 * w + g + 8 * (i >> 1)] = S[m][n][i];
+        }
+        __syncthreads();
+    }
+    float* mf = A.m_final + ((long long)seq * A.hv + h) * A.dv * A.dk;
+    for (int i = tid; i < NS * A.dk; i += 128) {
+        const int r = i / A.dk, cc = i - r * A.dk;
+        if (n0 + r < A.dv) mf[(long long)(n0 + r) * A.dk + cc] = Ms[r * LK + cc];
+    }
+}
+
+// Row-major store of a 16 x 32 accumulator block into a contiguous [row, heads, d] output.
+template <typename T>
+__device__ __forceinline__ void store_rows(T* out, const float (&acc)[4][4], int r0, int rows, int c0, int d, long long row_stride)
+{
+    const int lane = threadIdx.x & 31, g = lane >> 2, t = lane & 3;
+    const bool pair = ((d | (int)(row_stride & 1)) & 1) == 0 && (reinterpret_cast<uintptr_t>(out) & (2 * sizeof(T) - 1)) == 0;
+#pragma unroll
+    for (int n = 0; n < 4; n++)
+#pragma unroll
+        for (int r = 0; r < 2; r++) {
+            const int i = r0 + g + 8 * r, col = c0 + 8 * n + 2 * t;
+            if (i >= rows) continue;
+            T* p = out + i * row_stride + col;
+            if (pair) {
+                if (col < d) st2(p, acc[n][2 * r], acc[n][2 * r + 1]);
+            } else {
+                if (col < d) p[0] = from_f<T>(acc[n][2 * r]);
+                if (col + 1 < d) p[1] = from_f<T>(acc[n][2 * r + 1]);
+            }
+        }
+}
+
+// ── forward outputs ──
+// Eight warps: warp = 16 tokens x 32 of the tile's 64 columns.
+template <typename T>
+__global__ void __launch_bounds__(256) gd_out_fwd_kernel(Args A)
+{
+    extern __shared__ float4 smem4[];
+    float* Qs = reinterpret_cast<float*>(smem4);
+    float *Ks = Qs + C * LD, *Ms = Ks + C * LD;
+    __shared__ float4 s_gate[C];
+    __shared__ float s_theta[C];
+    const int slot = blockIdx.x / A.hv, h = blockIdx.x - slot * A.hv, n0 = blockIdx.y * 64;
+    const Chunk ch = get_chunk(A, slot);
+    if (ch.len <= 0) return;
+    const long long tile = (long long)slot * A.hv + h;
+    const int tid = threadIdx.x, lane = tid & 31, w = tid >> 5, rb = w & 3, hf = w >> 2, g = lane >> 2, t = lane & 3;
+    if (tid < C) { s_gate[tid] = A.gates[tile * C + tid]; s_theta[tid] = A.theta_eff[tile * C + tid]; }
+    const T* kp = (const T*)A.k + ch.b * A.kb + ch.t0 * A.kt + (h / A.share) * A.kh;
+    const T* qp = (const T*)A.q + ch.b * A.qb + ch.t0 * A.qt + (h / A.share) * A.qh;
+    constexpr int IN = Pl<T>::in, QP = Pl<T>::in == EXACT ? EXACT : Pl<T>::out, OUT = Pl<T>::out;
+    float att[4][4], y[4][4];
+    zero(att);
+    zero(y);
+    const bool need = 32 * hf <= 16 * rb + 15;
+    for (int c0 = 0; c0 < A.dk; c0 += 64) {
+        if (c0) __syncthreads();
+        load_tile<T, 64, 256>(Qs, LD, qp + c0, A.qt, ch.len, A.dk - c0);
+        load_tile<T, 64, 256>(Ks, LD, kp + c0, A.kt, ch.len, A.dk - c0);
+        load_own<64, 64, 256>(Ms, LD, A.m_chunk + (tile * A.dvp + n0) * A.dkp + c0, A.dkp);
+        __syncthreads();
+        if (need) gemm16<4, false, false, IN, IN>(att, Qs + 16 * rb * LD, LD, Ks + 32 * hf * LD, LD, 0, 64);
+        gemm16<4, false, false, QP, OUT>(y, Qs + 16 * rb * LD, LD, Ms + 32 * hf * LD, LD, 0, 64);
+    }
+    __syncthreads();
+    float *Pt = Ks, *Us = Ms;
+#pragma unroll
+    for (int n = 0; n < 4; n++)
+#pragma unroll
+        for (int i4 = 0; i4 < 4; i4++) {
+            const int i = 16 * rb + g + 8 * (i4 >> 1), j = 32 * hf + 8 * n + 2 * t + (i4 & 1);
+            const float4 gi = s_gate[i], gj = s_gate[j];
+            Pt[j * LD + i] = j <= i ? decay(make_float2(gi.x, gi.y), make_float2(gj.x, gj.y)) * A.scale * att[n][i4] : 0.f;
+            y[n][i4] *= A.scale * gi.z;
+        }
+    {
+        const float* ep = A.e + tile * C * A.dvp + n0;
+#pragma unroll
+        for (int i = 0; i < 4; i++) {
+            const int at = tid + i * 256, r = at >> 4, c = (at & 15) * 4;
+            float4 v = *reinterpret_cast<const float4*>(ep + (long long)r * A.dvp + c);
+            const float th = s_theta[r];
+            *reinterpret_cast<float4*>(Us + r * LD + c) = make_float4(v.x * th, v.y * th, v.z * th, v.w * th);
+        }
+    }
+    __syncthreads();
+    gemm16<4, true, true, OUT, OUT>(y, Pt + 16 * rb, LD, Us + 32 * hf, LD, 0, 16 * (rb + 1));
+    T* out = (T*)A.y + (ch.row0(A) * A.hv + h) * A.dv;
+    store_rows<T>(out, y, 16 * rb, ch.len, n0 + 32 * hf, A.dv, (long long)A.hv * A.dv);
+}
+
+// ── backward, what needs no state gradient: F = P^T dY ──
+template <typename T>
+__global__ void __launch_bounds__(256) gd_pre_bwd_kernel(Args A)
+{
+    extern __shared__ float4 smem4[];
+    float* Qs = reinterpret_cast<float*>(smem4);
+    float *Ks = Qs + C * LD, *Ys = Ks + C * LD;
+    __shared__ float4 s_gate[C];
+    const int slot = blockIdx.x / A.hv, h = blockIdx.x - slot * A.hv, n0 = blockIdx.y * 64;
+    const Chunk ch = get_chunk(A, slot);
+    if (ch.len <= 0) return;
+    const long long tile = (long long)slot * A.hv + h;
+    const int tid = threadIdx.x, lane = tid & 31, w = tid >> 5, rb = w & 3, hf = w >> 2, g = lane >> 2, t = lane & 3;
+    if (tid < C) s_gate[tid] = A.gates[tile * C + tid];
+    const T* kp = (const T*)A.k + ch.b * A.kb + ch.t0 * A.kt + (h / A.share) * A.kh;
+    const T* qp = (const T*)A.q + ch.b * A.qb + ch.t0 * A.qt + (h / A.share) * A.qh;
+    constexpr int IN = Pl<T>::in;
+    load_tile<T, 64, 256>(Ys, LD, (const T*)A.dy + ch.b * A.yb + ch.t0 * A.yt + h * A.yh + n0, A.yt, ch.len, A.dv - n0);
+    float att[4][4];                              // rows: j, columns: i >= j
+    zero(att);
+    const bool need = 32 * hf + 31 >= 16 * rb;
+    for (int c0 = 0; c0 < A.dk; c0 += 64) {
+        if (c0) __syncthreads();
+        load_tile<T, 64, 256>(Qs, LD, qp + c0, A.qt, ch.len, A.dk - c0);
+        load_tile<T, 64, 256>(Ks, LD, kp + c0, A.kt, ch.len, A.dk - c0);
+        __syncthreads();
+        if (need) gemm16<4, false, false, IN, IN>(att, Ks + 16 * rb * LD, LD, Qs + 32 * hf * LD, LD, 0, 64);
+    }
+    __syncthreads();
+    float* Ps = Ks;                               // [i][j]
+#pragma unroll
+    for (int n = 0; n < 4; n++)
+#pragma unroll
+        for (int i4 = 0; i4 < 4; i4++) {
+            const int j = 16 * rb + g + 8 * (i4 >> 1), i = 32 * hf + 8 * n + 2 * t + (i4 & 1);
+            const float4 gi = s_gate[i], gj = s_gate[j];
+            Ps[i * LD + j] = j <= i ? decay(make_float2(gi.x, gi.y), make_float2(gj.x, gj.y)) * A.scale * att[n][i4] : 0.f;
+        }
+    __syncthreads();
+    float f[4][4];
+    zero(f);
+    gemm16<4, true, true, TWO, IN>(f, Ps + 16 * rb, LD, Ys + 32 * hf, LD, 16 * rb, C);
+    float* fp = A.f + tile * C * A.dvp + n0 + 32 * hf;
+#pragma unroll
+    for (int n = 0; n < 4; n++)
+#pragma unroll
+        for (int r = 0; r < 2; r++)
+            st2(fp + (long long)(16 * rb + g + 8 * r) * A.dvp + 8 * n + 2 * t, f[n][2 * r], f[n][2 * r + 1]);
+}
+
+// ── backward states: the gradient of the state behind each chunk, last chunk first ──
+template <typename T, int DKP, int NS>
+__global__ void __launch_bounds__(128) gd_state_bwd_kernel(Args A)
+{
+    constexpr int LK = DKP + 4, LN = NS + 4, NT = NS / 8, MT = DKP / 64;
+    extern __shared__ float4 smem4[];
+    float* Ks = reinterpret_cast<float*>(smem4);
+    float *Qs = Ks + C * LK, *Ts = Qs + C * LK, *Ds = Ts + C * LD;
+    float *Rs = Ds + NS * LK, *Us = Rs + C * LN, *Ys = Us + C * LN;
+    __shared__ float4 s_gate[C];
+    __shared__ float s_theta[C];
+    const int nsl = A.dvp / NS, sl = blockIdx.x % nsl, p = blockIdx.x / nsl, h = p % A.hv, seq = p / A.hv;
+    const int n0 = sl * NS, tid = threadIdx.x, lane = tid & 31, w = tid >> 5, g = lane >> 2, t = lane & 3;
+    const int slot0 = first_slot(A, seq), count = chunk_count(A, seq);
+
+    float S[MT][NT][4];
+    const float* dm = A.d_m_final ? A.d_m_final + ((long long)seq * A.hv + h) * A.dv * A.dk : nullptr;
+#pragma unroll
+    for (int m = 0; m < MT; m++)
+#pragma unroll
+        for (int n = 0; n < NT; n++)
+#pragma unroll
+            for (int i = 0; i < 4; i++) {
+                const int row = 64 * m + 16 * w + g + 8 * (i >> 1), col = n0 + 8 * n + 2 * t + (i & 1);
+                S[m][n][i] = dm && row < A.dk && col < A.dv ? dm[(long long)col * A.dk + row] : 0.f;
+                Ds[(col - n0) * LK + row] = S[m][n][i];
+            }
+    __syncthreads();
+    for (int c = count - 1; c >= 0; c--) {
+        const int slot = slot0 + c;
+        const Chunk ch = get_chunk(A, slot);
+        const long long tile = (long long)slot * A.hv + h;
+        const T* kp = (const T*)A.k + ch.b * A.kb + ch.t0 * A.kt + (h / A.share) * A.kh;
+        const T* qp = (const T*)A.q + ch.b * A.qb + ch.t0 * A.qt + (h / A.share) * A.qh;
+        const T* yp = (const T*)A.dy + ch.b * A.yb + ch.t0 * A.yt + h * A.yh + n0;
+#pragma unroll
+        for (int m = 0; m < MT; m++) {
+            load_tile<T, 64, 128>(Ks + 64 * m, LK, kp + 64 * m, A.kt, ch.len, A.dk - 64 * m);
+            load_tile<T, 64, 128>(Qs + 64 * m, LK, qp + 64 * m, A.qt, ch.len, A.dk - 64 * m);
+        }
+        load_own<64, 64, 128>(Ts, LD, A.tmat + tile * C * C, C);
+        load_own<64, NS, 128>(Rs, LN, A.f + tile * C * A.dvp + n0, A.dvp);
+        load_tile<T, NS, 128>(Ys, LN, yp, A.yt, ch.len, A.dv - n0);
+        if (tid < C) { s_gate[tid] = A.gates[tile * C + tid]; s_theta[tid] = A.theta_eff[tile * C + tid]; }
+        float* dc = A.d_chunk + (tile * A.dvp + n0) * DKP;
+        for (int i = tid; i < NS * DKP / 4; i += 128) {
+            const int r = i / (DKP / 4), cc = (i - r * (DKP / 4)) * 4;
+            *reinterpret_cast<float4*>(dc + (long long)r * DKP + cc) = *reinterpret_cast<const float4*>(Ds + r * LK + cc);
+        }
+        __syncthreads();
+        float acc[NT][4];
+        zero(acc);
+        gemm16<NT, false, false, Pl<T>::in, TWO>(acc, Ks + 16 * w * LK, LK, Ds, LK, 0, DKP);
+#pragma unroll
+        for (int n = 0; n < NT; n++)
+#pragma unroll
+            for (int r = 0; r < 2; r++) {
+                const int i = 16 * w + g + 8 * r;
+                float2* rp = reinterpret_cast<float2*>(Rs + i * LN + 8 * n + 2 * t);
+                const float2 f = *rp;
+                const float wi = s_gate[i].w, th = s_theta[i];
+                *rp = make_float2(th * (f.x + wi * acc[n][2 * r]), th * (f.y + wi * acc[n][2 * r + 1]));
+            }
+        __syncthreads();
+        zero(acc);
+        gemm16<NT, true, true, TWO, TWO>(acc, Ts + 16 * w, LD, Rs, LN, 16 * w, C);
+        float* xp = A.x + tile * C * A.dvp + n0;
+        T* dv = (T*)A.d_v + (ch.row0(A) * A.hv + h) * A.dv;
+#pragma unroll
+        for (int n = 0; n < NT; n++)
+#pragma unroll
+            for (int r = 0; r < 2; r++) {
+                const int i = 16 * w + g + 8 * r, col = 8 * n + 2 * t;
+                const float a = acc[n][2 * r], b = acc[n][2 * r + 1], eg = -s_gate[i].z, ys = -eg * A.scale;
+                st2(xp + (long long)i * A.dvp + col, a, b);
+                st2(Us + i * LN + col, eg * a, eg * b);
+                float2* y = reinterpret_cast<float2*>(Ys + i * LN + col);
+                *y = make_float2(ys * y->x, ys * y->y);
+                if (i < ch.len) {
+                    const bool none = fabsf(s_theta[i]) <= THETA_TINY;     // theta was 0: so is the gradient of v
+                    T* o = dv + (long long)i * A.hv * A.dv + n0 + col;
+                    if (n0 + col < A.dv) o[0] = from_f<T>(none ? 0.f : a);
+                    if (n0 + col + 1 < A.dv) o[1] = from_f<T>(none ? 0.f : b);
+                }
+            }
+        __syncthreads();
+        const float gl = s_gate[C - 1].z;
+#pragma unroll
+        for (int m = 0; m < MT; m++) {
+#pragma unroll
+            for (int n = 0; n < NT; n++)
+#pragma unroll
+                for (int i = 0; i < 4; i++) S[m][n][i] *= gl;
+            gemm16<NT, true, true, Pl<T>::in, TWO>(S[m], Ks + 64 * m + 16 * w, LK, Us, LN, 0, C);
+            gemm16<NT, true, true, Pl<T>::in, TWO>(S[m], Qs + 64 * m + 16 * w, LK, Ys, LN, 0, C);
+#pragma unroll
+            for (int n = 0; n < NT; n++)
+#pragma unroll
+                for (int i = 0; i < 4; i++)
+                    Ds[(8 * n + 2 * t + (i & 1)) * LK + 64 * m + 16 * w + g + 8 * (i >> 1)] = S[m][n][i];
+        }
+        __syncthreads();
+    }
+    if (A.d_m0) {
+        float* o = A.d_m0 + ((long long)seq * A.hv + h) * A.dv * A.dk;
+        for (int i = tid; i < NS * A.dk; i += 128) {
+            const int r = i / A.dk, cc = i - r * A.dk;
+            if (n0 + r < A.dv) o[(long long)(n0 + r) * A.dk + cc] = Ds[r * LK + cc];
+        }
+    }
+}
+
+// ── backward outputs: d_q, d_k, d_theta and the gradient of G, for 64 columns of dk ──
+//   Mq_ij = scale e^{G_i - G_j} (dy_i.e_j) theta_j (j <= i),  Mb_ij = -e^{G_i - G_j} (x_i.e_j) theta_j (j < i)
+//   d_q = scale e^G dY M_0 + Mq K;  k as a query: -e^G X M_0 + Mb K;  k as a key: theta e^{G_L - G} E D + Mq^T Q + Mb^T K
+//   gradient of G_i: q_i.dq_i + k_i.(query part) - k_i.(key part), and <D, M_L> for the last one.
+// The tiles of dY, X and E make way for those of Q and K: 104 KB, two CTAs per SM.
+template <typename T>
+__global__ void __launch_bounds__(256, 2) gd_out_bwd_kernel(Args A)
+{
+    extern __shared__ float4 smem4[];
+    float* Ys = reinterpret_cast<float*>(smem4);
+    float *Xs = Ys + C * LD, *Es = Xs + C * LD, *Ms = Es + C * LD, *Mq = Ms + C * LD, *Mb = Mq + C * LD;
+    __shared__ float4 s_gate[C];
+    __shared__ float s_theta[C], s_row[2][C], s_red[8];
+    const int slot = blockIdx.x / A.hv, h = blockIdx.x - slot * A.hv, kt = blockIdx.y, k0 = kt * 64;
+    const Chunk ch = get_chunk(A, slot);
+    if (ch.len <= 0) return;
+    const long long tile = (long long)slot * A.hv + h;
+    const int tid = threadIdx.x, lane = tid & 31, w = tid >> 5, rb = w & 3, hf = w >> 2, g = lane >> 2, t = lane & 3;
+    constexpr int IN = Pl<T>::in;
+    if (tid < C) { s_gate[tid] = A.gates[tile * C + tid]; s_theta[tid] = A.theta_eff[tile * C + tid]; }
+    const T* yp = (const T*)A.dy + ch.b * A.yb + ch.t0 * A.yt + h * A.yh;
+    const int ndv = A.dvp / 64;
+    const bool need = 32 * hf <= 16 * rb + 15;
+    auto load_yxe = [&](int n0) {
+        load_tile<T, 64, 256>(Ys, LD, yp + n0, A.yt, ch.len, A.dv - n0);
+        load_own<64, 64, 256>(Xs, LD, A.x + tile * C * A.dvp + n0, A.dvp);
+        load_own<64, 64, 256>(Es, LD, A.e + tile * C * A.dvp + n0, A.dvp);
+    };
+    float dp[4][4], xe[4][4], xdot = 0.f;
+    zero(dp);
+    zero(xe);
+    for (int n = 0; n < ndv; n++) {
+        if (n) __syncthreads();
+        load_yxe(64 * n);
+        __syncthreads();
+        if (need) {
+            gemm16<4, false, false, IN, TWO>(dp, Ys + 16 * rb * LD, LD, Es + 32 * hf * LD, LD, 0, 64);
+            gemm16<4, false, false, TWO, TWO>(xe, Xs + 16 * rb * LD, LD, Es + 32 * hf * LD, LD, 0, 64);
+        }
+        if (kt == 0) {
+            const float *xr = Xs + (tid >> 2) * LD + (tid & 3), *er = Es + (tid >> 2) * LD + (tid & 3);
+#pragma unroll
+            for (int i = 0; i < 64; i += 4) xdot = fmaf(xr[i], er[i], xdot);
+        }
+    }
+    if (kt == 0) {
+        xdot += __shfl_xor_sync(0xffffffffu, xdot, 1);
+        xdot += __shfl_xor_sync(0xffffffffu, xdot, 2);
+        const int r = tid >> 2;
+        if ((tid & 3) == 0 && r < ch.len) A.d_theta[(ch.row0(A) + r) * A.hv + h] = xdot / s_theta[r];
+    }
+#pragma unroll
+    for (int n = 0; n < 4; n++)
+#pragma unroll
+        for (int i4 = 0; i4 < 4; i4++) {
+            const int i = 16 * rb + g + 8 * (i4 >> 1), j = 32 * hf + 8 * n + 2 * t + (i4 & 1);
+            const float4 gi = s_gate[i], gj = s_gate[j];
+            const float d = j <= i ? decay(make_float2(gi.x, gi.y), make_float2(gj.x, gj.y)) * s_theta[j] : 0.f;
+            Mq[j * LD + i] = j <= i ? A.scale * d * dp[n][i4] : 0.f;
+            Mb[j * LD + i] = j < i ? -d * xe[n][i4] : 0.f;
+        }
+    float dq[4][4], kq[4][4], ks[4][4], gsum = 0.f;
+    zero(dq);
+    zero(kq);
+    zero(ks);
+    for (int n = 0; n < ndv; n++) {
+        __syncthreads();
+        if (ndv > 1) load_yxe(64 * n);
+        const long long at = (tile * A.dvp + 64 * n) * A.dkp + k0;
+        load_own<64, 64, 256>(Ms, LD, A.m_chunk + at, A.dkp);
+        __syncthreads();
+        gemm16<4, false, true, IN, TWO>(dq, Ys + 16 * rb * LD, LD, Ms + 32 * hf, LD, 0, 64);
+        gemm16<4, false, true, TWO, TWO>(kq, Xs + 16 * rb * LD, LD, Ms + 32 * hf, LD, 0, 64);
+        __syncthreads();
+        const float* dc = A.d_chunk + at;
+        float s = 0.f;
+#pragma unroll
+        for (int i = 0; i < 4; i++) {
+            const int at4 = tid + i * 256, r = at4 >> 4, c = (at4 & 15) * 4;
+            const float4 v = *reinterpret_cast<const float4*>(dc + (long long)r * A.dkp + c);
+            float4* m = reinterpret_cast<float4*>(Ms + r * LD + c);
+            s += v.x * m->x + v.y * m->y + v.z * m->z + v.w * m->w;
+            *m = v;
+        }
+        gsum = fmaf(s_gate[C - 1].z, s, gsum);
+        __syncthreads();
+        gemm16<4, false, true, TWO, TWO>(ks, Es + 16 * rb * LD, LD, Ms + 32 * hf, LD, 0, 64);
+    }
+    __syncthreads();
+    float *Qs = Ys, *Ks = Xs;
+    load_tile<T, 64, 256>(Qs, LD, (const T*)A.q + ch.b * A.qb + ch.t0 * A.qt + (h / A.share) * A.qh + k0, A.qt, ch.len, A.dk - k0);
+    load_tile<T, 64, 256>(Ks, LD, (const T*)A.k + ch.b * A.kb + ch.t0 * A.kt + (h / A.share) * A.kh + k0, A.kt, ch.len, A.dk - k0);
+    __syncthreads();
+#pragma unroll
+    for (int n = 0; n < 4; n++)
+#pragma unroll
+        for (int i4 = 0; i4 < 4; i4++) {
+            const int i = 16 * rb + g + 8 * (i4 >> 1), col = 32 * hf + 8 * n + 2 * t + (i4 & 1);
+            dq[n][i4] *= A.scale * s_gate[i].z;
+            kq[n][i4] *= -s_gate[i].z;
+            ks[n][i4] *= s_theta[i] * s_gate[i].w;
+            gsum = fmaf(Ks[i * LD + col], ks[n][i4], gsum);
+        }
+    gemm16<4, true, true, TWO, IN>(dq, Mq + 16 * rb, LD, Ks + 32 * hf, LD, 0, 16 * (rb + 1));
+    gemm16<4, true, true, TWO, IN>(kq, Mb + 16 * rb, LD, Ks + 32 * hf, LD, 0, 16 * (rb + 1));
+    gemm16<4, false, true, TWO, IN>(ks, Mq + 16 * rb * LD, LD, Qs + 32 * hf, LD, 16 * rb, C);
+    gemm16<4, false, true, TWO, IN>(ks, Mb + 16 * rb * LD, LD, Ks + 32 * hf, LD, 16 * rb, C);
+    float row[2] = {0.f, 0.f};
+#pragma unroll
+    for (int n = 0; n < 4; n++)
+#pragma unroll
+        for (int i4 = 0; i4 < 4; i4++) {
+            const int i = 16 * rb + g + 8 * (i4 >> 1), col = 32 * hf + 8 * n + 2 * t + (i4 & 1);
+            row[i4 >> 1] += Qs[i * LD + col] * dq[n][i4] + Ks[i * LD + col] * (kq[n][i4] - ks[n][i4]);
+            kq[n][i4] += ks[n][i4];
+        }
+#pragma unroll
+    for (int r = 0; r < 2; r++) {
+        row[r] += __shfl_xor_sync(0xffffffffu, row[r], 1);
+        row[r] += __shfl_xor_sync(0xffffffffu, row[r], 2);
+        if (t == 0) s_row[hf][16 * rb + g + 8 * r] = row[r];
+    }
+    gsum = warp_sum(gsum);
+    if (lane == 0) s_red[w] = gsum;
+    __syncthreads();
+    const long long part = (long long)kt * A.slots * A.hv + tile;
+    if (tid < C) A.dg_part[part * C + tid] = s_row[0][tid] + s_row[1][tid];
+    if (tid == 0) {
+        float s = 0.f;
+        for (int i = 0; i < 8; i++) s += s_red[i];
+        A.dgl_part[part] = s;
+    }
+    if (A.share == 1) {
+        const long long at = (ch.row0(A) * A.hk + h) * A.dk, st = (long long)A.hk * A.dk;
+        store_rows<T>((T*)A.d_q + at, dq, 16 * rb, ch.len, k0 + 32 * hf, A.dk, st);
+        store_rows<T>((T*)A.d_k + at, kq, 16 * rb, ch.len, k0 + 32 * hf, A.dk, st);
+    } else {
+        const long long at = (ch.row0(A) * A.hv + h) * A.dk, st = (long long)A.hv * A.dk;
+        store_rows<float>(A.dq_part + at, dq, 16 * rb, ch.len, k0 + 32 * hf, A.dk, st);
+        store_rows<float>(A.dk_part + at, kq, 16 * rb, ch.len, k0 + 32 * hf, A.dk, st);
+    }
+}
+
+// Gradient of log_retain: sums of the gradient of G from each token to the chunk's end. One warp per chunk and head.
+__global__ void __launch_bounds__(128) gd_gate_bwd_kernel(Args A)
+{
+    const long long tile = (long long)blockIdx.x * 4 + (threadIdx.x >> 5);
+    if (tile >= (long long)A.slots * A.hv) return;
+    const int slot = (int)(tile / A.hv), h = (int)(tile - (long long)slot * A.hv), lane = threadIdx.x & 31;
+    const Chunk ch = get_chunk(A, slot);
+    if (ch.len <= 0) return;
+    double a = 0., b = 0.;
+    for (int kt = 0; kt < A.dkp / 64; kt++) {
+        const long long part = (long long)kt * A.slots * A.hv + tile;
+        a += A.dg_part[part * C + 2 * lane];
+        b += A.dg_part[part * C + 2 * lane + 1];
+        if (lane == 31) b += A.dgl_part[part];       // rows behind the chunk's last token are 0
+    }
+    double s = a + b;
+    for (int o = 1; o < 32; o <<= 1) { const double y = __shfl_down_sync(0xffffffffu, s, o); if (lane + o < 32) s += y; }
+    float* out = A.d_g + (ch.row0(A) + 2 * lane) * A.hv + h;
+    if (2 * lane < ch.len) out[0] = (float)s;
+    if (2 * lane + 1 < ch.len) out[A.hv] = (float)(s - a);
+}
+
+// Gradients of shared keys and queries: the value heads of a group, added in their order.
+template <typename T>
+__global__ void __launch_bounds__(256) gd_group_kernel(Args A, long long n)
+{
+    for (long long i = (long long)blockIdx.x * 256 + threadIdx.x; i < n; i += (long long)gridDim.x * 256) {
+        const long long rh = i / A.dk;                    // row * hk + key head
+        const int c = (int)(i - rh * A.dk);
+        const long long at = rh * A.share * A.dk + c;
+        float q = 0.f, k = 0.f;
+        for (int s = 0; s < A.share; s++) { q += A.dq_part[at + (long long)s * A.dk]; k += A.dk_part[at + (long long)s * A.dk]; }
+        ((T*)A.d_q)[i] = from_f<T>(q);
+        ((T*)A.d_k)[i] = from_f<T>(k);
+    }
+}
+
+// ── recurrent step ──
+// Bound by the state: read once, written once. Eight lanes hold a row of M (dk / 8 numbers each, in groups of four so
+// that a row's 128-byte pieces are whole); a CTA holds `rows` rows of one head. Sequences that name the same slot are
+// stepped one after the other, in their order, by the CTA of the first: a slot behaves as if they came in as further tokens.
+template <typename T, int NV, bool VEC>
+__global__ void __launch_bounds__(256) gd_step_kernel(Args A, float* M, const int* slots, int pool, int rows)
+{
+    const int per = (A.dv + rows - 1) / rows;
+    const int part = blockIdx.x % per, p = blockIdx.x / per, h = p % A.hv, first = p / A.hv;
+    const int lane8 = threadIdx.x & 7, grp = threadIdx.x >> 3;
+    int slot = first;
+    if (slots) {
+        slot = slots[first];
+        if (slot < 0 || slot >= pool) return;             // no sequence in this place
+        int seen = 0;
+        for (int i = threadIdx.x; i < first; i += 256) seen |= slots[i] == slot;
+        if (__syncthreads_or(seen)) return;
+    }
+    constexpr int RP = 4;                                 // rows a thread holds at a time
+    for (int r0 = part * rows; r0 < min(A.dv, (part + 1) * rows); r0 += 32 * RP) {
+        float4 m[RP][NV];
+        float* base = M + ((long long)slot * A.hv + h) * A.dv * A.dk;
+#pragma unroll
+        for (int r = 0; r < RP; r++) {
+            const int row = r0 + grp + 32 * r;
+            const bool on = row < min(A.dv, (part + 1) * rows);
+#pragma unroll
+            for (int v = 0; v < NV; v++) {
+                const int c = 4 * lane8 + 32 * v;
+                float4 x = make_float4(0.f, 0.f, 0.f, 0.f);
+                if (on) {
+                    const float* s = base + (long long)row * A.dk + c;
+                    if (VEC) { if (c < A.dk) x = *reinterpret_cast<const float4*>(s); }
+                    else {
+                        if (c < A.dk) x.x = s[0];
+                        if (c + 1 < A.dk) x.y = s[1];
+                        if (c + 2 < A.dk) x.z = s[2];
+                        if (c + 3 < A.dk) x.w = s[3];
+                    }
+                }
+                m[r][v] = x;
+            }
+        }
+        for (int b = first; b < A.batch; b++) {
+            if (b != first && (!slots || slots[b] != slot)) { if (!slots) break; continue; }
+            for (int tok = 0; tok < A.seq; tok++) {
+                const T* kp = (const T*)A.k + b * A.kb + tok * A.kt + (h / A.share) * A.kh;
+                const T* qp = (const T*)A.q + b * A.qb + tok * A.qt + (h / A.share) * A.qh;
+                const T* vp = (const T*)A.v + b * A.vb + tok * A.vt + h * A.vh;
+                const long long ga = b * A.gb + tok * A.gt + h * A.gh;
+                const float rt = expf(A.g[ga]), th = A.theta[ga];
+                float kf[NV][4], qf[NV][4];
+#pragma unroll
+                for (int v = 0; v < NV; v++)
+#pragma unroll
+                    for (int i = 0; i < 4; i++) {
+                        const int c = 4 * lane8 + 32 * v + i;
+                        kf[v][i] = c < A.dk ? to_f(kp[c]) : 0.f;
+                        qf[v][i] = c < A.dk ? to_f(qp[c]) : 0.f;
+                    }
+#pragma unroll
+                for (int r = 0; r < RP; r++) {
+                    const int row = r0 + grp + 32 * r;
+                    const bool on = row < min(A.dv, (part + 1) * rows);
+                    const float val = on ? to_f(vp[row]) : 0.f;
+                    float s = 0.f;
+#pragma unroll
+                    for (int v = 0; v < NV; v++) {
+                        m[r][v].x *= rt; m[r][v].y *= rt; m[r][v].z *= rt; m[r][v].w *= rt;
+                        s = fmaf(m[r][v].x, kf[v][0], s); s = fmaf(m[r][v].y, kf[v][1], s);
+                        s = fmaf(m[r][v].z, kf[v][2], s); s = fmaf(m[r][v].w, kf[v][3], s);
+                    }
+                    s += __shfl_xor_sync(0xffffffffu, s, 1);
+                    s += __shfl_xor_sync(0xffffffffu, s, 2);
+                    s += __shfl_xor_sync(0xffffffffu, s, 4);
+                    const float u = th * (val - s);
+                    float y = 0.f;
+#pragma unroll
+                    for (int v = 0; v < NV; v++) {
+                        m[r][v].x = fmaf(u, kf[v][0], m[r][v].x); m[r][v].y = fmaf(u, kf[v][1], m[r][v].y);
+                        m[r][v].z = fmaf(u, kf[v][2], m[r][v].z); m[r][v].w = fmaf(u, kf[v][3], m[r][v].w);
+                        y = fmaf(m[r][v].x, qf[v][0], y); y = fmaf(m[r][v].y, qf[v][1], y);
+                        y = fmaf(m[r][v].z, qf[v][2], y); y = fmaf(m[r][v].w, qf[v][3], y);
+                    }
+                    y += __shfl_xor_sync(0xffffffffu, y, 1);
+                    y += __shfl_xor_sync(0xffffffffu, y, 2);
+                    y += __shfl_xor_sync(0xffffffffu, y, 4);
+                    if (on && lane8 == 0)
+                        ((T*)A.y)[(((long long)b * A.seq + tok) * A.hv + h) * A.dv + row] = from_f<T>(A.scale * y);
+                }
+            }
+        }
+#pragma unroll
+        for (int r = 0; r < RP; r++) {
+            const int row = r0 + grp + 32 * r;
+            if (row >= min(A.dv, (part + 1) * rows)) continue;
+#pragma unroll
+            for (int v = 0; v < NV; v++) {
+                const int c = 4 * lane8 + 32 * v;
+                float* s = base + (long long)row * A.dk + c;
+                if (VEC) { if (c < A.dk) *reinterpret_cast<float4*>(s) = m[r][v]; }
+                else {
+                    if (c < A.dk) s[0] = m[r][v].x;
+                    if (c + 1 < A.dk) s[1] = m[r][v].y;
+                    if (c + 2 < A.dk) s[2] = m[r][v].z;
+                    if (c + 3 < A.dk) s[3] = m[r][v].w;
+                }
+            }
+        }
+    }
+}
+
+// ── host ──
+static bool fill(const char* where, const nlh_gated_delta_desc* d, Args& A)
+{
+    A = Args{};
+    const char* bad = nullptr;
+    if (!d) bad = "NULL descriptor";
+    else if (d->batch < 0 || d->seq < 0 || d->heads_k <= 0 || d->heads_v <= 0 || d->n_seqs < 0) bad = "bad dimensions";
+    else if (d->heads_v % d->heads_k != 0) bad = "heads_v is no multiple of heads_k";
+    else if (d->dk < 1 || d->dk > 128 || d->dv < 1 || d->dv > 128) bad = "dk and dv must be in 1..128";
+    else if (d->n_seqs > 0 && d->batch != 1) bad = "a packed batch has batch = 1";
+    else if ((long long)d->batch * d->seq >= (1LL << 31)) bad = "batch * seq must stay below 2^31";
+    if (bad) { record_status(NLH_ERR_INVALID_ARG, where, bad); return false; }
+    A.batch = d->batch; A.seq = d->seq; A.hk = d->heads_k; A.hv = d->heads_v; A.share = d->heads_v / d->heads_k;
+    A.dk = d->dk; A.dv = d->dv; A.n_seqs = d->n_seqs;
+    A.dkp = (d->dk + 63) / 64 * 64; A.dvp = (d->dv + 63) / 64 * 64;
+    A.kb = d->k_batch; A.kt = d->k_token; A.kh = d->k_head;
+    A.vb = d->v_batch; A.vt = d->v_token; A.vh = d->v_head;
+    A.qb = d->q_batch; A.qt = d->q_token; A.qh = d->q_head;
+    A.gb = d->gate_batch; A.gt = d->gate_token; A.gh = d->gate_head;
+    A.yb = d->dy_batch; A.yt = d->dy_token; A.yh = d->dy_head;
+    A.scale = d->scale;
+    A.nc = (d->seq + C - 1) / C;
+    const long long slots = d->n_seqs > 0 ? (long long)d->seq / C + d->n_seqs : (long long)d->batch * A.nc;
+    if (slots * d->heads_v >= (1LL << 31)) { record_status(NLH_ERR_INVALID_ARG, where, "too many chunks"); return false; }
+    A.slots = (int)slots;
+    return true;
+}
+
+// Places the private buffers that forward hands on to backward behind `base`; returns their bytes.
+static int64_t place_saved(Args& A, char* base)
+{
+    const int64_t tiles = (int64_t)A.slots * A.hv;
+    int64_t at = 0;
+    auto take = [&](int64_t bytes) { char* p = base + at; at += (bytes + 255) & ~(int64_t)255; return (void*)p; };
+    A.tmat = (float*)take(tiles * C * C * 4);
+    A.gates = (float4*)take(tiles * C * 16);
+    A.theta_eff = (float*)take(tiles * C * 4);
+    A.e = (float*)take(tiles * C * A.dvp * 4);
+    A.m_chunk = (float*)take(tiles * A.dvp * A.dkp * 4);
+    if (A.n_seqs > 0) {
+        A.map = (int4*)take((int64_t)A.slots * 16);
+        A.start = (int*)take((int64_t)(A.n_seqs + 1) * 4);
+        A.off = (int*)take((int64_t)(A.n_seqs + 1) * 4);
+    }
+    return at;
+}
+static int64_t place_bwd(Args& A, char* base)
+{
+    const int64_t tiles = (int64_t)A.slots * A.hv, nk = A.dkp / 64;
+    int64_t at = 0;
+    auto take = [&](int64_t bytes) { char* p = base + at; at += (bytes + 255) & ~(int64_t)255; return (void*)p; };
+    A.f = (float*)take(tiles * C * A.dvp * 4);
+    A.x = (float*)take(tiles * C * A.dvp * 4);
+    A.d_chunk = (float*)take(tiles * A.dvp * A.dkp * 4);
+    A.dg_part = (float*)take(nk * tiles * C * 4);
+    A.dgl_part = (float*)take(nk * tiles * 4);
+    if (A.share > 1) {
+        A.dk_part = (float*)take((int64_t)A.batch * A.seq * A.hv * A.dk * 4);
+        A.dq_part = (float*)take((int64_t)A.batch * A.seq * A.hv * A.dk * 4);
+    }
+    return at;
+}
+
+template <typename K> static bool allow_smem(K kernel, int bytes, const char* where)
+{
+    const cudaError_t e = cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, bytes);
+    if (e == cudaSuccess) return true;
+    record_status(NLH_ERR_CUDA, where, cudaGetErrorString(e));
+    return false;
+}
+
+constexpr int TILE_BYTES = C * LD * 4;
+constexpr int state_fwd_smem(int dkp, int ns) { return 4 * (C * (dkp + 4) + C * LD + ns * (dkp + 4) + 2 * C * (ns + 4)); }
+constexpr int state_bwd_smem(int dkp, int ns) { return 4 * (2 * C * (dkp + 4) + C * LD + ns * (dkp + 4) + 3 * C * (ns + 4)); }
+
+template <typename T, int DKP>
+static bool launch_states(const Args& A, bool backward, cudaStream_t st, const char* where)
+{
+    const int seqs = A.n_seqs > 0 ? A.n_seqs : A.batch;
+    const long long grid = (long long)seqs * A.hv * (A.dvp / 32);
+    if (grid == 0) return true;
+    if (grid >= (1LL << 31)) { record_status(NLH_ERR_INVALID_ARG, where, "too many sequences"); return false; }
+    if (backward) {
+        constexpr int bytes = state_bwd_smem(DKP, 32);
+        if (!allow_smem(gd_state_bwd_kernel<T, DKP, 32>, bytes, where)) return false;
+        gd_state_bwd_kernel<T, DKP, 32><<<(unsigned)grid, 128, bytes, st>>>(A);
+    } else {
+        constexpr int bytes = state_fwd_smem(DKP, 32);
+        if (!allow_smem(gd_state_fwd_kernel<T, DKP, 32>, bytes, where)) return false;
+        gd_state_fwd_kernel<T, DKP, 32><<<(unsigned)grid, 128, bytes, st>>>(A);
+    }
+    return check_launch(where);
+}
+
+template <typename T> static bool run_forward(Args& A, cudaStream_t st, const char* where)
+{
+    if (A.n_seqs > 0) {
+        gd_map_kernel<<<1, 1024, 0, st>>>(A);
+        if (!check_launch(where)) return false;
+    }
+    const unsigned tiles = (unsigned)((long long)A.slots * A.hv);
+    if (tiles) {
+        if (!allow_smem(gd_prep_kernel<T>, 3 * TILE_BYTES, where)) return false;
+        gd_prep_kernel<T><<<tiles, 128, 3 * TILE_BYTES, st>>>(A);
+        if (!check_launch(where)) return false;
+    }
+    if (!(A.dkp == 64 ? launch_states<T, 64>(A, false, st, where) : launch_states<T, 128>(A, false, st, where))) return false;
+    if (tiles) {
+        if (!allow_smem(gd_out_fwd_kernel<T>, 3 * TILE_BYTES, where)) return false;
+        gd_out_fwd_kernel<T><<<dim3(tiles, A.dvp / 64), 256, 3 * TILE_BYTES, st>>>(A);
+        if (!check_launch(where)) return false;
+    }
+    return true;
+}
+
+template <typename T> static bool run_backward(Args& A, cudaStream_t st, const char* where)
+{
+    const unsigned tiles = (unsigned)((long long)A.slots * A.hv);
+    if (tiles) {
+        if (!allow_smem(gd_pre_bwd_kernel<T>, 3 * TILE_BYTES, where)) return false;
+        gd_pre_bwd_kernel<T><<<dim3(tiles, A.dvp / 64), 256, 3 * TILE_BYTES, st>>>(A);
+        if (!check_launch(where)) return false;
+    }
+    if (!(A.dkp == 64 ? launch_states<T, 64>(A, true, st, where) : launch_states<T, 128>(A, true, st, where))) return false;
+    if (!tiles) return true;
+    if (!allow_smem(gd_out_bwd_kernel<T>, 6 * TILE_BYTES, where)) return false;
+    gd_out_bwd_kernel<T><<<dim3(tiles, A.dkp / 64), 256, 6 * TILE_BYTES, st>>>(A);
+    if (!check_launch(where)) return false;
+    gd_gate_bwd_kernel<<<(tiles + 3) / 4, 128, 0, st>>>(A);
+    if (!check_launch(where)) return false;
+    if (A.share > 1) {
+        // rows outside the sequences of a packed batch have no partial sums: their gradients are the caller's zeros
+        const long long n = (long long)A.batch * A.seq * A.hk * A.dk;
+        const long long need = (n + 255) / 256;
+        gd_group_kernel<T><<<(unsigned)(need < 148 * 16 ? need : 148 * 16), 256, 0, st>>>(A, n);
+        if (!check_launch(where)) return false;
+    }
+    return true;
+}
+
+}  // namespace gd
+}  // namespace nlh
+
+using namespace nlh;
+using namespace nlh::gd;
+
+extern "C" {
+
+int64_t nlh_gated_delta_saved_bytes(const nlh_gated_delta_desc* desc)
+{
+    Args A;
+    if (!fill("nlh_gated_delta_saved_bytes", desc, A)) return -1;
+    return place_saved(A, nullptr);
+}
+
+int64_t nlh_gated_delta_backward_bytes(const nlh_gated_delta_desc* desc)
+{
+    Args A;
+    if (!fill("nlh_gated_delta_backward_bytes", desc, A)) return -1;
+    return place_bwd(A, nullptr);
+}
+
+static bool gd_inputs(const char* where, Args& A, const nlh_gated_delta_desc* desc, const void* k, const void* v, const void* q,
+                      const float* log_retain, const float* theta, const int32_t* seq_starts)
+{
+    if (!fill(where, desc, A)) return false;
+    const bool tokens = (long long)A.batch * A.seq > 0;
+    if ((tokens && (!k || !v || !q || !log_retain || !theta)) || (A.n_seqs > 0) != (seq_starts != nullptr)) {
+        record_status(NLH_ERR_INVALID_ARG, where, "NULL pointer, or seq_starts without n_seqs");
+        return false;
+    }
+    A.k = k; A.v = v; A.q = q; A.g = log_retain; A.theta = theta; A.starts = seq_starts;
+    return true;
+}
+
+int32_t nlh_gated_delta_forward(const nlh_gated_delta_desc* desc, const void* k, const void* v, const void* q,
+    const float* log_retain, const float* theta, const float* m_initial, const int32_t* seq_starts, void* y, float* m_final,
+    void* saved, int64_t saved_bytes)
+{
+    const char* where = "nlh_gated_delta_forward";
+    Args A;
+    if (!gd_inputs(where, A, desc, k, v, q, log_retain, theta, seq_starts)) return NLH_ERR_INVALID_ARG;
+    const bool tokens = (long long)A.batch * A.seq > 0;
+    if ((tokens && !y) || (!m_final && (A.n_seqs > 0 || A.batch > 0)) || ((uintptr_t)saved & 15) || saved_bytes < place_saved(A, (char*)saved) || (tokens && !saved)) {
+        record_status(NLH_ERR_INVALID_ARG, where, "NULL output, or a saved buffer that is too small or not 16-byte aligned");
+        return NLH_ERR_INVALID_ARG;
+    }
+    A.m0 = m_initial; A.y = y; A.m_final = m_final;
+    const bool ok = desc->is_bf16 ? run_forward<__nv_bfloat16>(A, current_stream(), where) : run_forward<float>(A, current_stream(), where);
+    return ok ? NLH_OK : NLH_ERR_CUDA;
+}
+
+int32_t nlh_gated_delta_backward(const nlh_gated_delta_desc* desc, const void* k, const void* v, const void* q,
+    const float* log_retain, const float* theta, const int32_t* seq_starts, const void* saved, int64_t saved_bytes,
+    const void* d_y, const float* d_m_final, void* d_k, void* d_v, void* d_q, float* d_log_retain, float* d_theta,
+    float* d_m_initial, void* workspace, int64_t workspace_bytes)
+{
+    const char* where = "nlh_gated_delta_backward";
+    Args A;
+    if (!gd_inputs(where, A, desc, k, v, q, log_retain, theta, seq_starts)) return NLH_ERR_INVALID_ARG;
+    const bool tokens = (long long)A.batch * A.seq > 0;
+    if ((tokens && (!d_y || !d_k || !d_v || !d_q || !d_log_retain || !d_theta || !saved || !workspace)) ||
+        (((uintptr_t)saved | (uintptr_t)workspace) & 15) || saved_bytes < place_saved(A, (char*)saved) ||
+        workspace_bytes < place_bwd(A, (char*)workspace)) {
+        record_status(NLH_ERR_INVALID_ARG, where, "NULL pointer, or a buffer that is too small or not 16-byte aligned");
+        return NLH_ERR_INVALID_ARG;
+    }
+    A.dy = d_y; A.d_m_final = d_m_final; A.d_k = d_k; A.d_v = d_v; A.d_q = d_q;
+    A.d_g = d_log_retain; A.d_theta = d_theta; A.d_m0 = d_m_initial;
+    const bool ok = desc->is_bf16 ? run_backward<__nv_bfloat16>(A, current_stream(), where) : run_backward<float>(A, current_stream(), where);
+    return ok ? NLH_OK : NLH_ERR_CUDA;
+}
+
+int32_t nlh_gated_delta_step(const nlh_gated_delta_desc* desc, const void* k, const void* v, const void* q,
+    const float* log_retain, const float* theta, float* m, const int32_t* slots, int32_t n_slots, void* y)
+{
+    const char* where = "nlh_gated_delta_step";
+    Args A;
+    if (!gd_inputs(where, A, desc, k, v, q, log_retain, theta, nullptr)) return NLH_ERR_INVALID_ARG;
+    if ((long long)A.batch * A.seq == 0) return NLH_OK;
+    if (!m || !y || n_slots < (slots ? 0 : A.batch)) {
+        record_status(NLH_ERR_INVALID_ARG, where, "NULL pointer, or fewer states than sequences");
+        return NLH_ERR_INVALID_ARG;
+    }
+    A.y = y;
+    // 128 rows a CTA (one round of its threads) while that gives every SM two CTAs, else 32
+    const long long heads = (long long)A.batch * A.hv;
+    const int rows = heads * ((A.dv + 127) / 128) >= 2 * 148 ? 128 : 32;
+    const long long grid = heads * ((A.dv + rows - 1) / rows);
+    if (grid >= (1LL << 31)) { record_status(NLH_ERR_INVALID_ARG, where, "too many sequences"); return NLH_ERR_INVALID_ARG; }
+    cudaStream_t st = current_stream();
+    const bool vec = (A.dk & 3) == 0 && aligned16(m);
+#define NLH_GD_STEP(T, NV) (vec ? gd_step_kernel<T, NV, true><<<(unsigned)grid, 256, 0, st>>>(A, m, slots, n_slots, rows) \
+                                : gd_step_kernel<T, NV, false><<<(unsigned)grid, 256, 0, st>>>(A, m, slots, n_slots, rows))
+    if (desc->is_bf16) { if (A.dk <= 64) NLH_GD_STEP(__nv_bfloat16, 2); else NLH_GD_STEP(__nv_bfloat16, 4); }
+    else { if (A.dk <= 64) NLH_GD_STEP(float, 2); else NLH_GD_STEP(float, 4); }
+#undef NLH_GD_STEP
+    return check_launch(where) ? NLH_OK : NLH_ERR_CUDA;
+}
+
+}  // extern "C"

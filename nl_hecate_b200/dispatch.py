@@ -351,6 +351,160 @@ def titans_frozen_stream_backward(k, v, q, alpha, theta, eta, ms, d_y, chunk, wa
                 d_s_initial=ds0)
 
 
+# ── gated delta rule (additive API) ────────────────────────────────────────
+# k, q [B, S, Hk, dk], v [B, S, Hv, dv], log_retain, theta [B, S, Hv] fp32, any strides with a contiguous last
+# axis; Hk divides Hv. States m [B, Hv, dv, dk] fp32 (y = M q). A packed batch has B = 1 and seq_starts [n + 1] int32.
+
+class _on_device:
+    """The library launches on the current device's stream: calls on tensors of another device run under a guard."""
+
+    def __init__(self, t):
+        self.guard = None
+        if t.device.index != torch._C._cuda_getDevice():
+            self.guard = torch.cuda.device(t.device)
+
+    def __enter__(self):
+        if self.guard is not None:
+            self.guard.__enter__()
+
+    def __exit__(self, *exc):
+        if self.guard is not None:
+            self.guard.__exit__(*exc)
+        return False
+
+
+def _same_device(where, first, **others):
+    if not first.is_cuda:
+        raise ValueError(f"{where}: need CUDA tensors")
+    for n, t in others.items():
+        if t is not None and t.device != first.device:
+            raise ValueError(f"{where}.{n}: on {t.device}, the other tensors on {first.device}")
+
+
+def _need(where, name, t, dtype, shape):
+    """A contiguous tensor of this type and shape."""
+    if t.dtype != dtype or tuple(t.shape) != tuple(shape) or not t.is_contiguous():
+        raise ValueError(f"{where}.{name}: need a contiguous {dtype} tensor of shape {tuple(shape)}, "
+                         f"got {t.dtype} {tuple(t.shape)}")
+
+
+def _gated_delta_desc(where, k, v, q, log_retain, theta, scale, n_seqs, d_y=None):
+    if k.dim() != 4 or v.dim() != 4 or log_retain.dim() != 3:
+        raise ValueError(f"{where}: need k, q, v of [batch, seq, heads, d] and gates of [batch, seq, heads]")
+    b, s, hk, dk = k.shape
+    hv, dv = v.shape[2], v.shape[3]
+    if q.shape != k.shape or v.shape[:2] != k.shape[:2] or log_retain.shape != v.shape[:3] or theta.shape != v.shape[:3]:
+        raise ValueError(f"{where}: shapes do not fit: k {tuple(k.shape)}, q {tuple(q.shape)}, v {tuple(v.shape)}, "
+                         f"log_retain {tuple(log_retain.shape)}, theta {tuple(theta.shape)}")
+    if k.dtype not in (torch.float32, torch.bfloat16) or q.dtype != k.dtype or v.dtype != k.dtype:
+        raise ValueError(f"{where}: k, v and q must all be float32 or all bfloat16")
+    if log_retain.dtype != torch.float32 or theta.dtype != torch.float32:
+        raise ValueError(f"{where}: log_retain and theta must be float32")
+    for t in (k, v, q) if d_y is None else (k, v, q, d_y):
+        if t.stride(3) != 1 and t.shape[3] > 1:
+            raise ValueError(f"{where}: the last axis must be contiguous")
+    if log_retain.stride() != theta.stride():
+        raise ValueError(f"{where}: log_retain and theta must have the same strides")
+    if n_seqs and b != 1:
+        raise ValueError(f"{where}: a packed batch has batch 1")
+    dy = (0, 0, 0) if d_y is None else d_y.stride()[:3]
+    return ffi.GatedDeltaDesc(b, s, hk, hv, dk, dv, n_seqs, int(k.dtype == torch.bfloat16), *k.stride()[:3], *v.stride()[:3],
+                              *q.stride()[:3], *log_retain.stride(), *dy, scale)
+
+
+def _same_strides(a, b):
+    return (a, b) if a.stride() == b.stride() else (a.contiguous(), b.contiguous())
+
+
+def _starts_of(where, seq_starts):
+    if seq_starts is None:
+        return 0
+    if seq_starts.dim() != 1 or seq_starts.numel() < 2:
+        raise ValueError(f"{where}.seq_starts: need [sequences + 1] starts")
+    _need(where, "seq_starts", seq_starts, torch.int32, seq_starts.shape)
+    return seq_starts.numel() - 1
+
+
+def gated_delta_forward(k, v, q, log_retain, theta, m0=None, seq_starts=None, scale=1.0, want_saved=True):
+    """Gated delta rule over whole sequences (nlh_gated_delta_forward): returns (y like v, m_final
+    [sequences, Hv, dv, dk], saved). ``saved`` is what gated_delta_backward needs, None with want_saved=False.
+    In a packed batch the rows of y outside the sequences are zeros."""
+    where = "gated_delta_forward"
+    _same_device(where, k, v=v, q=q, log_retain=log_retain, theta=theta, m0=m0, seq_starts=seq_starts)
+    log_retain, theta = _same_strides(log_retain, theta)
+    n_seqs = _starts_of(where, seq_starts)
+    desc = _gated_delta_desc(where, k, v, q, log_retain, theta, scale, n_seqs)
+    b, s, hv, dv = v.shape
+    state = (n_seqs or b, hv, dv, k.shape[3])
+    if m0 is not None:
+        _need(where, "m0", m0, torch.float32, state)
+    with _on_device(k):
+        ref = C.byref(desc)
+        nbytes = ffi.lib().nlh_gated_delta_saved_bytes(ref)
+        if nbytes < 0:
+            ffi.check(ffi.lib().nlh_last_status(), where)
+        saved = torch.empty(max(nbytes, 1), dtype=torch.uint8, device=k.device)
+        y = (torch.zeros if n_seqs else torch.empty)(b, s, hv, dv, dtype=v.dtype, device=k.device)
+        m = torch.empty(state, dtype=torch.float32, device=k.device)
+        call("nlh_gated_delta_forward", desc=ref, k=k.data_ptr(), v=v.data_ptr(), q=q.data_ptr(),
+             log_retain=log_retain.data_ptr(), theta=theta.data_ptr(), m_initial=m0, seq_starts=seq_starts, y=y, m_final=m,
+             saved=saved, saved_bytes=nbytes)
+    return y, m, (saved if want_saved else None)
+
+
+def gated_delta_backward(k, v, q, log_retain, theta, saved, d_y, d_m_final=None, seq_starts=None, scale=1.0,
+                         want_initial=True):
+    """Gradients of gated_delta_forward, which has returned ``saved`` for the same inputs and scale:
+    dict(d_k, d_v, d_q, d_log_retain, d_theta, d_m_initial). d_y like v in type, any strides; d_m_final (gradient
+    of m_final) may be None. Keys shared by several value heads get the sum of their gradients."""
+    where = "gated_delta_backward"
+    _same_device(where, k, v=v, q=q, log_retain=log_retain, theta=theta, saved=saved, d_y=d_y, d_m_final=d_m_final,
+                 seq_starts=seq_starts)
+    log_retain, theta = _same_strides(log_retain, theta)
+    if d_y.shape != v.shape or d_y.dtype != v.dtype:
+        raise ValueError(f"{where}.d_y: need {v.dtype} {tuple(v.shape)}, got {d_y.dtype} {tuple(d_y.shape)}")
+    n_seqs = _starts_of(where, seq_starts)
+    desc = _gated_delta_desc(where, k, v, q, log_retain, theta, scale, n_seqs, d_y)
+    b, s, hv, dv = v.shape
+    state = (n_seqs or b, hv, dv, k.shape[3])
+    if d_m_final is not None:
+        _need(where, "d_m_final", d_m_final, torch.float32, state)
+    with _on_device(k):
+        ref = C.byref(desc)
+        lib = ffi.lib()
+        nbytes = lib.nlh_gated_delta_backward_bytes(ref)
+        if nbytes < 0:
+            ffi.check(lib.nlh_last_status(), where)
+        make = torch.zeros if n_seqs else torch.empty      # rows outside the sequences are not written
+        new = lambda t, dt=None: make(t.shape, dtype=dt or t.dtype, device=k.device)
+        work = make(max(nbytes, 1), dtype=torch.uint8, device=k.device)
+        g = dict(d_k=new(k), d_v=new(v), d_q=new(q), d_log_retain=new(theta), d_theta=new(theta))
+        g["d_m_initial"] = torch.empty(state, dtype=torch.float32, device=k.device) if want_initial else None
+        call("nlh_gated_delta_backward", desc=ref, k=k.data_ptr(), v=v.data_ptr(), q=q.data_ptr(),
+             log_retain=log_retain.data_ptr(), theta=theta.data_ptr(), seq_starts=seq_starts, saved=saved,
+             saved_bytes=saved.numel(), d_y=d_y.data_ptr(), d_m_final=d_m_final, workspace=work, workspace_bytes=nbytes, **g)
+    return g
+
+
+def gated_delta_step(k, v, q, log_retain, theta, m, slots=None, scale=1.0):
+    """One token (or a few) for each sequence on its stored state m [n_slots, Hv, dv, dk], updated in place
+    (nlh_gated_delta_step). slots [B] int32: the state of each sequence (None: sequence i has state i); one outside
+    [0, n_slots) marks an unused place of the batch, whose rows of y are zeros. Returns y like v."""
+    where = "gated_delta_step"
+    _same_device(where, k, v=v, q=q, log_retain=log_retain, theta=theta, m=m, slots=slots)
+    log_retain, theta = _same_strides(log_retain, theta)
+    desc = _gated_delta_desc(where, k, v, q, log_retain, theta, scale, 0)
+    _need(where, "m", m, torch.float32, (m.shape[0], v.shape[2], v.shape[3], k.shape[3]))
+    if slots is not None:
+        _need(where, "slots", slots, torch.int32, (k.shape[0],))
+    with _on_device(k):
+        y = (torch.empty if slots is None else torch.zeros)(v.shape, dtype=v.dtype, device=k.device)
+        call("nlh_gated_delta_step", desc=C.byref(desc), k=k.data_ptr(), v=v.data_ptr(), q=q.data_ptr(),
+             log_retain=log_retain.data_ptr(), theta=theta.data_ptr(), m=m, slots=slots, n_slots=m.shape[0], y=y)
+    torch.autograd.graph.increment_version(m)    # written past autograd
+    return y
+
+
 # ── SWA ────────────────────────────────────────────────────────────────────
 # q,k,v,out: [B,S,H*hd] bf16; attn_weights [B,H,S,n_p+W] bf16; grads f32.
 

@@ -30,6 +30,13 @@ class AdamWTensorDesc(C.Structure):
                 ("has_clamp", C.c_int32), ("active", C.c_int32)]
 
 
+class GatedDeltaDesc(C.Structure):
+    """Mirror of ``nlh_gated_delta_desc`` (include/nlh_ffi.h)."""
+    _fields_ = ([(n, C.c_int32) for n in ("batch", "seq", "heads_k", "heads_v", "dk", "dv", "n_seqs", "is_bf16")]
+                + [(f"{t}_{a}", C.c_int64) for t in ("k", "v", "q", "gate", "dy") for a in ("batch", "token", "head")]
+                + [("scale", C.c_float)])
+
+
 def _ctype(decl: str):
     decl = decl.strip()
     if decl == "void":
