@@ -515,6 +515,37 @@ int32_t nlh_copy_rows(const float* src, int64_t src_stride, float* dst, int32_t 
 /* dst [cols, rows] <- src [rows, cols] transposed. */
 int32_t nlh_transpose(const float* src, float* dst, int32_t rows, int32_t cols);
 
+/* ── Embedding lookup with scaling, gradient by sorted tokens (additive, no counterpart in the reference) ──
+ * Beside embedding_gather_cuda / embedding_scatter_add_cuda above. out[t] = scale * w[ids[t]], w [vocab, d] and out [n, d] both
+ * fp32 or both bf16; an id outside [0, vocab) gives a row of zeros and takes no part in the gradient. Backward: d_w [vocab, d] fp32,
+ * accumulate != 0: d_w[r] += scale * sum of the rows of d_out [n, d] (fp32 or bf16) with id r; 0: d_w is overwritten, zeros in
+ * rows without a token. Sums are in fp32 and in one order that n, ids and d fix: the same call gives the same bits. workspace
+ * (nlh_embedding_backward_bytes, 16-byte aligned) is the caller's. */
+int32_t nlh_embedding_forward(const void* w, int32_t w_is_bf16, const int32_t* ids, void* out, int32_t n, int32_t vocab,
+    int32_t d, float scale);
+int64_t nlh_embedding_backward_bytes(int32_t n, int32_t vocab, int32_t d);
+int32_t nlh_embedding_backward(const void* d_out, int32_t d_out_is_bf16, const int32_t* ids, float* d_w, int32_t n,
+    int32_t vocab, int32_t d, float scale, int32_t accumulate, void* workspace, int64_t workspace_bytes);
+
+/* ── Distillation from a teacher's top logits (additive, no counterpart in the reference) ──────
+ * Beside the cross-entropy above. logits [n, vocab] fp32 or bf16, rows row_stride elements apart; teacher_ids [n, k] and
+ * teacher_logits [n, k] (fp32 or bf16), k <= 1024: p = softmax(teacher / temperature) over a row's valid entries (an id outside
+ * [0, vocab) or a logit of -infinity marks an unused one; an id may occur more than once). target_ids [n] as in the
+ * cross-entropy. With n_hard rows that have a target and n_soft rows that have a teacher entry:
+ *   loss[0] = hard_weight / n_hard sum (lse(z) - z_target)
+ *           + soft_weight temperature^2 / n_soft sum_rows sum_k p_k (log p_k - z_k / temperature + lse(z / temperature)).
+ * A weight of 0 or NULL ids leave a term out. The backward writes d loss / d logits * grad_scale[0] (NULL = 1) in the logits'
+ * type, zeros in rows without a term; d_logits may be logits itself. saved (nlh_distill_saved_bytes, 16-byte
+ * aligned, the caller's) carries the rows' log-sum-exps; the backward's other arguments are the forward's. */
+int64_t nlh_distill_saved_bytes(int32_t n, int32_t vocab);
+int32_t nlh_distill_forward(const void* logits, int32_t logits_is_bf16, int64_t row_stride, const int32_t* target_ids,
+    const int32_t* teacher_ids, const void* teacher_logits, int32_t teacher_is_bf16, float* loss, void* saved,
+    int64_t saved_bytes, int32_t n, int32_t vocab, int32_t k, float temperature, float hard_weight, float soft_weight);
+int32_t nlh_distill_backward(const void* logits, int32_t logits_is_bf16, int64_t row_stride, const int32_t* target_ids,
+    const int32_t* teacher_ids, const void* teacher_logits, int32_t teacher_is_bf16, const void* saved, int64_t saved_bytes,
+    const float* grad_scale, void* d_logits, int64_t d_row_stride, int32_t n, int32_t vocab, int32_t k, float temperature,
+    float hard_weight, float soft_weight);
+
 /* ── Gated delta rule (additive, no counterpart in the reference) ──────────────────────────────
  *   M_t = e^{g_t} M_{t-1} + u_t k_t^T,  u_t = theta_t (v_t - e^{g_t} M_{t-1} k_t),  y_t = scale M_t q_t
  * beside the Delta rule above (core/src/delta_rule.rs), which takes its error before the decay. M [dv, dk]

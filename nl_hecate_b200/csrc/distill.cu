@@ -1,0 +1,544 @@
+// Distillation from a teacher's top logits: loss and gradient.
+//
+// A row of student logits z [vocab] comes with k teacher entries (id, logit t) and, optionally, a target id:
+//   p = softmax(t / tau) over the row's valid entries,
+//   loss = hard_weight mean(lse(z) - z_target) + soft_weight tau^2 mean(sum_k p_k (log p_k - z_k / tau + lse(z / tau))),
+//   dz_j = hard_weight / n_hard (softmax(z)_j - [j = target]) + soft_weight tau / n_soft (softmax(z / tau)_j - p_j),
+// each mean over the rows that have a target / a teacher entry. Both log-sum-exps come out of one pass over the row with a
+// running maximum, and the gradient out of one more: z is read twice and dz written once, which bounds the pair by HBM.
+// The exponentials are next (two an element; 16 a cycle and SM): at tau = 2 the one of z is the square of the one of z / tau.
+// Sums over rows and over entries of one id have one order; no atomics.
+#include <cuda_bf16.h>
+#include <math_constants.h>
+
+#include "nlh_common.cuh"
+#include "../../include/nlh_ffi.h"
+
+namespace nlh {
+namespace distill {
+
+constexpr int THREADS = 256;
+constexpr int MAX_K = 1024;
+constexpr float LOG2E = 1.4426950408889634f;
+
+struct Args {
+    const void* z;
+    long long z_row, d_row;              // elements between rows of logits and of d_logits
+    const int *targets, *ids;
+    const void* t;
+    void* d;
+    const float* grad;
+    int n, vocab, k, t_bf16, splits, per_split;
+    float tau, hard_w, soft_w;
+    bool hard, soft;                     // which terms exist
+    // saved
+    float *lse_h, *lse_s, *ce, *kl;      // [n]
+    int* flags;                          // [n] bit 0: has a target, bit 1: has a teacher entry
+    float* stats;                        // {-, hard_weight / n_hard, soft_weight tau / n_soft, -}
+    float* loss;
+    float4* part;                        // [n, splits] {max, sum e^(z - max), sum e^((z - max) / tau), -}
+};
+
+__device__ __forceinline__ float ld(const float* p) { return *p; }
+__device__ __forceinline__ float ld(const __nv_bfloat16* p) { return __bfloat162float(*p); }
+__device__ __forceinline__ float ex2(float x)
+{
+    float y;
+    asm("ex2.approx.ftz.f32 %0, %1;" : "=f"(y) : "f"(x));
+    return y;
+}
+
+// Which exponentials a row needs. ONE: e^(z c) alone (a single term, or tau = 1); SQUARE: tau = 2; BOTH: any other tau.
+enum Mode { ONE = 0, SQUARE = 1, BOTH = 2 };
+
+template <typename T> struct Vec { static constexpr int N = 16 / sizeof(T); };
+template <typename T> __device__ __forceinline__ void unpack(const uint4& u, float* f);
+template <> __device__ __forceinline__ void unpack<float>(const uint4& u, float* f)
+{
+    f[0] = __uint_as_float(u.x); f[1] = __uint_as_float(u.y); f[2] = __uint_as_float(u.z); f[3] = __uint_as_float(u.w);
+}
+template <> __device__ __forceinline__ void unpack<__nv_bfloat16>(const uint4& u, float* f)
+{
+    const unsigned w[4] = {u.x, u.y, u.z, u.w};
+#pragma unroll
+    for (int i = 0; i < 4; i++) { f[2 * i] = __uint_as_float(w[i] << 16); f[2 * i + 1] = __uint_as_float(w[i] & 0xffff0000u); }
+}
+template <typename T> __device__ __forceinline__ uint4 pack(const float* f);
+template <> __device__ __forceinline__ uint4 pack<float>(const float* f)
+{
+    return make_uint4(__float_as_uint(f[0]), __float_as_uint(f[1]), __float_as_uint(f[2]), __float_as_uint(f[3]));
+}
+template <> __device__ __forceinline__ uint4 pack<__nv_bfloat16>(const float* f)
+{
+    unsigned w[4];
+#pragma unroll
+    for (int i = 0; i < 4; i++) {
+        const __nv_bfloat162 b = __floats2bfloat162_rn(f[2 * i], f[2 * i + 1]);
+        w[i] = *reinterpret_cast<const unsigned*>(&b);
+    }
+    return make_uint4(w[0], w[1], w[2], w[3]);
+}
+
+struct Stat { float m, h, s; };          // maximum, sum e^(z - m), sum e^((z - m) / tau)
+
+template <int MODE>
+__device__ __forceinline__ void add_one(float x, float cs, float ns, float ch, float nh, float& h, float& s)
+{
+    const float e = ex2(fmaf(x, cs, ns));
+    s += e;
+    if (MODE == SQUARE) h = fmaf(e, e, h);
+    if (MODE == BOTH) h += ex2(fmaf(x, ch, nh));
+}
+template <int MODE, int N>
+__device__ __forceinline__ void add_block(Stat& a, const float* f, float cs, float ch)
+{
+    float lm = f[0];
+#pragma unroll
+    for (int i = 1; i < N; i++) lm = fmaxf(lm, f[i]);
+    const float m = fmaxf(a.m, lm);
+    if (m == -CUDART_INF_F) {
+        // nothing but -infinity so far; a NaN, which fmaxf passes over, must not be lost
+#pragma unroll
+        for (int i = 0; i < N; i++) if (f[i] != f[i]) { a.h = f[i]; a.s = f[i]; }
+        return;
+    }
+    const float ns = -m * cs, nh = -m * ch;
+    if (m > a.m) {
+        a.s *= ex2((a.m - m) * cs);
+        if (MODE != ONE) a.h *= ex2((a.m - m) * ch);
+        a.m = m;
+    }
+    float h[2] = {0.f, 0.f}, s[2] = {0.f, 0.f};
+#pragma unroll
+    for (int i = 0; i < N; i++) add_one<MODE>(f[i], cs, ns, ch, nh, h[i & 1], s[i & 1]);
+    a.h += h[0] + h[1];
+    a.s += s[0] + s[1];
+}
+template <int MODE>
+__device__ __forceinline__ Stat merge(const Stat& a, const Stat& b, float cs, float ch)
+{
+    Stat o;
+    o.m = fmaxf(a.m, b.m);
+    if (o.m == -CUDART_INF_F) { o.h = a.h + b.h; o.s = a.s + b.s; return o; }
+    o.s = a.s * ex2((a.m - o.m) * cs) + b.s * ex2((b.m - o.m) * cs);
+    o.h = MODE == ONE ? o.s : a.h * ex2((a.m - o.m) * ch) + b.h * ex2((b.m - o.m) * ch);
+    return o;
+}
+
+// max / sum over the block; every thread gets the same value
+__device__ __forceinline__ float block_max(float v, float* red)
+{
+#pragma unroll
+    for (int o = 16; o > 0; o >>= 1) v = fmaxf(v, __shfl_xor_sync(0xffffffffu, v, o));
+    if ((threadIdx.x & 31) == 0) red[threadIdx.x >> 5] = v;
+    __syncthreads();
+    v = red[0];
+    for (int w = 1; w < THREADS / 32; w++) v = fmaxf(v, red[w]);
+    __syncthreads();
+    return v;
+}
+
+// Statistics of columns [j0, j1) of a row: aligned 16-byte loads with four in flight, scalars at the ragged ends.
+template <typename T, int MODE>
+__device__ Stat row_stat(const T* row, int j0, int j1, float cs, float ch, Stat* red)
+{
+    constexpr int N = Vec<T>::N;
+    Stat a = {-CUDART_INF_F, 0.f, 0.f};
+    const int lead = min(j1 - j0, (int)(((16 - ((uintptr_t)(row + j0) & 15)) & 15) / sizeof(T)));
+    const int nvec = (j1 - j0 - lead) / N, tail = j0 + lead + nvec * N;
+    const uint4* r4 = reinterpret_cast<const uint4*>(row + j0 + lead);
+    for (int i = threadIdx.x; i < nvec; i += 4 * THREADS) {
+        uint4 u[4];
+#pragma unroll
+        for (int q = 0; q < 4; q++) if (i + q * THREADS < nvec) u[q] = __ldg(r4 + i + q * THREADS);
+#pragma unroll
+        for (int q = 0; q < 4; q++) {
+            if (i + q * THREADS < nvec) {
+                float f[N];
+                unpack<T>(u[q], f);
+                add_block<MODE, N>(a, f, cs, ch);
+            }
+        }
+    }
+    if (threadIdx.x < lead) { const float x = ld(row + j0 + threadIdx.x); add_block<MODE, 1>(a, &x, cs, ch); }
+    if (threadIdx.x < j1 - tail) { const float x = ld(row + tail + threadIdx.x); add_block<MODE, 1>(a, &x, cs, ch); }
+#pragma unroll
+    for (int o = 16; o > 0; o >>= 1) {
+        Stat b;
+        b.m = __shfl_xor_sync(0xffffffffu, a.m, o);
+        b.h = __shfl_xor_sync(0xffffffffu, a.h, o);
+        b.s = __shfl_xor_sync(0xffffffffu, a.s, o);
+        a = merge<MODE>(a, b, cs, ch);
+    }
+    if ((threadIdx.x & 31) == 0) red[threadIdx.x >> 5] = a;
+    __syncthreads();
+    a = red[0];
+    for (int w = 1; w < THREADS / 32; w++) a = merge<MODE>(a, red[w], cs, ch);
+    __syncthreads();
+    return a;
+}
+
+__device__ __forceinline__ float teacher(const Args& A, long long at)
+{
+    return A.t_bf16 ? ld((const __nv_bfloat16*)A.t + at) : ((const float*)A.t)[at];
+}
+// Entry i of a row: its id if it counts, -1 if not (an id outside the vocabulary, a logit of -infinity).
+__device__ __forceinline__ int entry(const Args& A, long long row, int i, float& t)
+{
+    const int id = A.ids[row * A.k + i];
+    t = teacher(A, row * A.k + i) / A.tau;
+    return id >= 0 && id < A.vocab && t != -CUDART_INF_F ? id : -1;
+}
+__device__ __forceinline__ bool has_target(const Args& A, int row)
+{
+    return A.hard && A.targets[row] >= 0 && A.targets[row] < A.vocab;
+}
+
+// The row's values from its statistics: log-sum-exps, cross-entropy, divergence.
+template <typename T>
+__device__ void finish_row(const Args& A, int row, const Stat& a, bool target, float* red)
+{
+    const T* z = (const T*)A.z + (long long)row * A.z_row;
+    const float lse_s = A.soft ? a.m / A.tau + logf(a.s) : 0.f;
+    const float lse_h = A.hard ? (A.soft && A.tau != 1.f ? a.m + logf(a.h) : a.m + logf(a.s)) : 0.f;
+    float kl = 0.f;
+    bool any = false;
+    if (A.soft) {
+        float top = -CUDART_INF_F;
+        bool mine = false;
+        for (int i = threadIdx.x; i < A.k; i += THREADS) {
+            float t;
+            if (entry(A, row, i, t) >= 0) { top = t != t ? t : fmaxf(top, t); mine = true; }
+        }
+        any = __syncthreads_or(mine);
+        if (any) {
+            top = block_max(top, red);
+            float sum = 0.f, cross = 0.f;         // sum e^(t - top); sum e^(t - top) (t - top - (z - m) / tau)
+            for (int i = threadIdx.x; i < A.k; i += THREADS) {
+                float t;
+                const int id = entry(A, row, i, t);
+                if (id < 0) continue;
+                const float e = expf(t - top);
+                sum += e;
+                if (e != 0.f) cross += e * ((t - top) - (ld(z + id) - a.m) / A.tau);
+            }
+            sum = block_sum(sum, red);
+            cross = block_sum(cross, red);
+            kl = cross / sum + logf(a.s) - logf(sum);
+        }
+    }
+    if (threadIdx.x == 0) {
+        A.lse_h[row] = lse_h;
+        A.lse_s[row] = lse_s;
+        A.ce[row] = target ? lse_h - ld(z + A.targets[row]) : 0.f;
+        A.kl[row] = kl;
+        A.flags[row] = (target ? 1 : 0) | (any ? 2 : 0);
+    }
+}
+
+template <typename T, int MODE>
+__global__ void __launch_bounds__(THREADS) fwd_kernel(Args A, float cs, float ch)
+{
+    __shared__ Stat s_stat[THREADS / 32];
+    __shared__ float red[32];
+    const int row = blockIdx.x / A.splits, sp = blockIdx.x - row * A.splits;
+    const bool target = has_target(A, row);
+    if (!A.soft && !target) {                     // no term: the row is not read
+        if (sp == 0 && threadIdx.x == 0) {
+            A.lse_h[row] = A.lse_s[row] = A.ce[row] = A.kl[row] = 0.f;
+            A.flags[row] = 0;
+        }
+        return;
+    }
+    const int j0 = sp * A.per_split, j1 = min(A.vocab, j0 + A.per_split);
+    const Stat a = row_stat<T, MODE>((const T*)A.z + (long long)row * A.z_row, j0, j1, cs, ch, s_stat);
+    if (A.splits > 1) {
+        if (threadIdx.x == 0) A.part[(long long)row * A.splits + sp] = make_float4(a.m, a.h, a.s, 0.f);
+        return;
+    }
+    finish_row<T>(A, row, a, target, red);
+}
+template <typename T, int MODE>
+__global__ void __launch_bounds__(THREADS) join_kernel(Args A, float cs, float ch)
+{
+    __shared__ float red[32];
+    const int row = blockIdx.x;
+    const bool target = has_target(A, row);
+    if (!A.soft && !target) return;
+    Stat a = {-CUDART_INF_F, 0.f, 0.f};
+    for (int i = 0; i < A.splits; i++) {
+        const float4 p = A.part[(long long)row * A.splits + i];
+        a = merge<MODE>(a, Stat{p.x, p.y, p.z}, cs, ch);
+    }
+    finish_row<T>(A, row, a, target, red);
+}
+
+// Means over the rows. One CTA, one order: thread i adds rows i, i + 1024, ... in 64 bits.
+__global__ void __launch_bounds__(1024) mean_kernel(Args A)
+{
+    __shared__ double s_d[2][32];
+    __shared__ int s_i[2][32];
+    double ce = 0., kl = 0.;
+    int nh = 0, ns = 0;
+#pragma unroll 8
+    for (int i = threadIdx.x; i < A.n; i += 1024) {
+        const int f = A.flags[i];
+        ce += A.ce[i];
+        kl += A.kl[i];
+        nh += f & 1;
+        ns += f >> 1;
+    }
+    for (int o = 16; o > 0; o >>= 1) {
+        ce += __shfl_xor_sync(0xffffffffu, ce, o);
+        kl += __shfl_xor_sync(0xffffffffu, kl, o);
+        nh += __shfl_xor_sync(0xffffffffu, nh, o);
+        ns += __shfl_xor_sync(0xffffffffu, ns, o);
+    }
+    const int w = threadIdx.x >> 5;
+    if ((threadIdx.x & 31) == 0) { s_d[0][w] = ce; s_d[1][w] = kl; s_i[0][w] = nh; s_i[1][w] = ns; }
+    __syncthreads();
+    if (threadIdx.x == 0) {
+        ce = kl = 0.;
+        nh = ns = 0;
+        for (int i = 0; i < 32; i++) { ce += s_d[0][i]; kl += s_d[1][i]; nh += s_i[0][i]; ns += s_i[1][i]; }
+        const double h = A.hard ? (double)A.hard_w / max(nh, 1) : 0., s = A.soft ? (double)A.soft_w / max(ns, 1) : 0.;
+        *A.loss = (float)((A.hard ? h * ce : 0.) + (A.soft ? s * A.tau * A.tau * kl : 0.));
+        A.stats[1] = (float)h;
+        A.stats[2] = (float)(s * A.tau);
+    }
+}
+
+template <int MODE>
+__device__ __forceinline__ float grad_at(float x, float cs, float os, float gs, float ch, float oh, float gh)
+{
+    // os, oh: -lse in base-2 units. ONE: a single softmax times gs
+    const float e = ex2(fmaf(x, cs, os));
+    if (MODE == ONE) return gs * e;
+    return fmaf(gs, e, gh * ex2(fmaf(x, ch, oh)));
+}
+
+// d_logits may be logits: a thread reads its elements before it writes them, and the elements of the entries, which are
+// written once more at the end with their p taken off, are read before anything is written.
+template <typename T, int MODE>
+__global__ void __launch_bounds__(THREADS) bwd_kernel(Args A, float cs, float ch)
+{
+    __shared__ int s_id[MAX_K + 1];
+    __shared__ float s_w[MAX_K + 1], s_z[MAX_K + 1], red[32];
+    constexpr int N = Vec<T>::N;
+    const int row = blockIdx.x / A.splits, sp = blockIdx.x - row * A.splits;
+    const int j0 = sp * A.per_split, j1 = min(A.vocab, j0 + A.per_split);
+    const T* z = (const T*)A.z + (long long)row * A.z_row;
+    T* d = (T*)A.d + (long long)row * A.d_row;
+    const int flags = A.flags[row];
+    const float g = A.grad ? *A.grad : 1.f;
+    float gh = flags & 1 ? g * A.stats[1] : 0.f, gs = flags & 2 ? g * A.stats[2] : 0.f;
+    const float wh = gh, ws = gs;                 // what a target / an entry's p takes off
+
+    const int lead = min(j1 - j0, (int)(((16 - ((uintptr_t)(z + j0) & 15)) & 15) / sizeof(T)));
+    const int nvec = (((uintptr_t)z ^ (uintptr_t)d) & 15) ? 0 : (j1 - j0 - lead) / N;      // 16-byte stores where both rows align
+    const int body = j0 + lead, tail = body + nvec * N;
+    if (flags == 0) {
+        const uint4 zero = make_uint4(0, 0, 0, 0);
+        for (int i = threadIdx.x; i < nvec; i += THREADS) reinterpret_cast<uint4*>(d + body)[i] = zero;
+        if (threadIdx.x < lead) d[j0 + threadIdx.x] = T(0.f);
+        for (int j = tail + threadIdx.x; j < j1; j += THREADS) d[j] = T(0.f);
+        return;
+    }
+    // entries of this CTA's columns, and the target as one more
+    float top = -CUDART_INF_F, sum = 0.f;
+    if (flags & 2) {
+        for (int i = threadIdx.x; i < A.k; i += THREADS) {
+            float t;
+            const int id = entry(A, row, i, t);
+            s_id[i] = id;
+            s_w[i] = t;
+            if (id >= 0) top = t != t ? t : fmaxf(top, t);
+        }
+        top = block_max(top, red);
+        for (int i = threadIdx.x; i < A.k; i += THREADS) {
+            const float e = s_id[i] >= 0 ? expf(s_w[i] - top) : 0.f;
+            s_w[i] = e;
+            sum += e;
+        }
+        sum = block_sum(sum, red);
+    }
+    const int k = flags & 2 ? A.k : 0;
+    for (int i = threadIdx.x; i < k; i += THREADS) {
+        const int id = s_id[i];
+        const bool here = id >= j0 && id < j1;
+        s_id[i] = here ? id : -1;
+        s_w[i] = ws * (s_w[i] / sum);
+        s_z[i] = here ? ld(z + id) : 0.f;
+    }
+    if (threadIdx.x == 0) {
+        const int id = flags & 1 ? A.targets[row] : -1;
+        const bool here = id >= j0 && id < j1;
+        s_id[k] = here ? id : -1;
+        s_w[k] = wh;
+        s_z[k] = here ? ld(z + id) : 0.f;
+    }
+    float os = -A.lse_s[row] * LOG2E, oh = -A.lse_h[row] * LOG2E;
+    if (MODE == ONE) {                            // one softmax: of the only term, or of both at tau = 1
+        if (!A.soft) os = oh;
+        gs = gs + gh;
+    }
+    __syncthreads();
+    const uint4* r4 = reinterpret_cast<const uint4*>(z + body);
+    uint4* d4 = reinterpret_cast<uint4*>(d + body);
+    for (int i = threadIdx.x; i < nvec; i += 4 * THREADS) {
+        uint4 u[4];
+#pragma unroll
+        for (int q = 0; q < 4; q++) if (i + q * THREADS < nvec) u[q] = r4[i + q * THREADS];
+#pragma unroll
+        for (int q = 0; q < 4; q++) {
+            if (i + q * THREADS < nvec) {
+                float f[N];
+                unpack<T>(u[q], f);
+#pragma unroll
+                for (int e = 0; e < N; e++) f[e] = grad_at<MODE>(f[e], cs, os, gs, ch, oh, gh);
+                d4[i + q * THREADS] = pack<T>(f);
+            }
+        }
+    }
+    if (threadIdx.x < lead) d[j0 + threadIdx.x] = T(grad_at<MODE>(ld(z + j0 + threadIdx.x), cs, os, gs, ch, oh, gh));
+    for (int j = tail + threadIdx.x; j < j1; j += THREADS) d[j] = T(grad_at<MODE>(ld(z + j), cs, os, gs, ch, oh, gh));
+    __syncthreads();
+    // an id that several entries name is written by the first of them, with all their p in the entries' order
+    for (int i = threadIdx.x; i <= k; i += THREADS) {
+        const int id = s_id[i];
+        if (id < 0) continue;
+        float w = 0.f;
+        bool first = true;
+        for (int j = 0; j <= k; j++)
+            if (s_id[j] == id) { first &= j >= i; w += s_w[j]; }
+        if (first) d[id] = T(grad_at<MODE>(s_z[i], cs, os, gs, ch, oh, gh) - w);
+    }
+}
+
+// ── host ──
+static int64_t place(Args& A, char* base)
+{
+    int64_t at = 0;
+    auto take = [&](int64_t bytes) { char* p = base + at; at += (bytes + 255) & ~(int64_t)255; return (void*)p; };
+    A.lse_h = (float*)take((int64_t)A.n * 4);
+    A.lse_s = (float*)take((int64_t)A.n * 4);
+    A.ce = (float*)take((int64_t)A.n * 4);
+    A.kl = (float*)take((int64_t)A.n * 4);
+    A.flags = (int*)take((int64_t)A.n * 4);
+    A.stats = (float*)take(16);
+    A.part = A.splits > 1 ? (float4*)take((int64_t)A.n * A.splits * 16) : nullptr;
+    return at;
+}
+// Few rows: each is divided over CTAs until every SM has two, in pieces of 4096 columns at least.
+static void divide(Args& A)
+{
+    const int most = (A.vocab + 4095) / 4096, want = A.n > 0 ? (2 * 148 + A.n - 1) / A.n : 1;
+    A.splits = A.n >= 148 ? 1 : (want < most ? want : most);
+    if (A.splits < 1) A.splits = 1;
+    A.per_split = ((A.vocab + A.splits - 1) / A.splits + 7) & ~7;
+    A.splits = (A.vocab + A.per_split - 1) / A.per_split;
+}
+static bool fill(const char* where, Args& A, const void* logits, int64_t row_stride, const int32_t* targets, const int32_t* teacher_ids,
+                 const void* teacher_logits, int32_t teacher_is_bf16, int32_t n, int32_t vocab, int32_t k, float temperature,
+                 float hard_weight, float soft_weight)
+{
+    A = Args{};
+    const char* bad = nullptr;
+    A.hard = targets != nullptr && hard_weight != 0.f;
+    A.soft = teacher_ids != nullptr && soft_weight != 0.f;
+    if (n < 0 || vocab <= 0 || k < 0 || k > MAX_K || row_stride < vocab) bad = "bad dimensions (k is at most 1024)";
+    else if (!(temperature > 0.f) || temperature > 1e6f || temperature < 1e-6f) bad = "the temperature must be in [1e-6, 1e6]";
+    else if (n > 0 && (!logits || (A.soft && k > 0 && !teacher_logits))) bad = "NULL pointer";
+    if (bad) { record_status(NLH_ERR_INVALID_ARG, where, bad); return false; }
+    A.z = logits; A.z_row = row_stride; A.targets = targets; A.ids = teacher_ids; A.t = teacher_logits; A.t_bf16 = teacher_is_bf16;
+    A.n = n; A.vocab = vocab; A.k = A.soft ? k : 0; A.tau = temperature; A.hard_w = hard_weight; A.soft_w = soft_weight;
+    divide(A);
+    return true;
+}
+static int mode_of(const Args& A) { return !(A.hard && A.soft) || A.tau == 1.f ? ONE : A.tau == 2.f ? SQUARE : BOTH; }
+
+template <typename T, int MODE> static bool forward(const Args& A, const char* where)
+{
+    cudaStream_t st = current_stream();
+    const float cs = LOG2E / (A.soft ? A.tau : 1.f), ch = LOG2E;
+    fwd_kernel<T, MODE><<<(unsigned)((long long)A.n * A.splits), THREADS, 0, st>>>(A, cs, ch);
+    if (!check_launch(where)) return false;
+    if (A.splits > 1) {
+        join_kernel<T, MODE><<<A.n, THREADS, 0, st>>>(A, cs, ch);
+        if (!check_launch(where)) return false;
+    }
+    return true;
+}
+template <typename T> static bool forward_mode(const Args& A, const char* where)
+{
+    switch (mode_of(A)) {
+    case ONE: return forward<T, ONE>(A, where);
+    case SQUARE: return forward<T, SQUARE>(A, where);
+    default: return forward<T, BOTH>(A, where);
+    }
+}
+template <typename T> static bool backward(const Args& A, const char* where)
+{
+    cudaStream_t st = current_stream();
+    const float cs = LOG2E / (A.soft ? A.tau : 1.f), ch = LOG2E;
+    const unsigned grid = (unsigned)((long long)A.n * A.splits);
+    if (mode_of(A) == ONE) bwd_kernel<T, ONE><<<grid, THREADS, 0, st>>>(A, cs, ch);
+    else bwd_kernel<T, BOTH><<<grid, THREADS, 0, st>>>(A, cs, ch);
+    return check_launch(where);
+}
+
+}  // namespace distill
+}  // namespace nlh
+
+using namespace nlh;
+
+extern "C" {
+
+int64_t nlh_distill_saved_bytes(int32_t n, int32_t vocab)
+{
+    if (n < 0 || vocab <= 0) return -1;
+    distill::Args A{};
+    A.n = n; A.vocab = vocab;
+    distill::divide(A);
+    return distill::place(A, nullptr);
+}
+
+int32_t nlh_distill_forward(const void* logits, int32_t logits_is_bf16, int64_t row_stride, const int32_t* target_ids,
+    const int32_t* teacher_ids, const void* teacher_logits, int32_t teacher_is_bf16, float* loss, void* saved, int64_t saved_bytes,
+    int32_t n, int32_t vocab, int32_t k, float temperature, float hard_weight, float soft_weight)
+{
+    const char* where = "nlh_distill_forward";
+    distill::Args A;
+    if (!distill::fill(where, A, logits, row_stride, target_ids, teacher_ids, teacher_logits, teacher_is_bf16, n, vocab, k, temperature,
+                       hard_weight, soft_weight)) return NLH_ERR_INVALID_ARG;
+    if (!loss || !saved || !aligned16(saved) || saved_bytes < distill::place(A, (char*)saved)) {
+        record_status(NLH_ERR_INVALID_ARG, where, "NULL output, or a saved buffer that is too small or not 16-byte aligned");
+        return NLH_ERR_INVALID_ARG;
+    }
+    A.loss = loss;
+    if (n > 0 && !(logits_is_bf16 ? distill::forward_mode<__nv_bfloat16>(A, where) : distill::forward_mode<float>(A, where)))
+        return NLH_ERR_CUDA;
+    distill::mean_kernel<<<1, 1024, 0, current_stream()>>>(A);
+    if (!check_launch(where)) return NLH_ERR_CUDA;
+    return NLH_OK;
+}
+
+int32_t nlh_distill_backward(const void* logits, int32_t logits_is_bf16, int64_t row_stride, const int32_t* target_ids,
+    const int32_t* teacher_ids, const void* teacher_logits, int32_t teacher_is_bf16, const void* saved, int64_t saved_bytes,
+    const float* grad_scale, void* d_logits, int64_t d_row_stride, int32_t n, int32_t vocab, int32_t k, float temperature,
+    float hard_weight, float soft_weight)
+{
+    const char* where = "nlh_distill_backward";
+    distill::Args A;
+    if (!distill::fill(where, A, logits, row_stride, target_ids, teacher_ids, teacher_logits, teacher_is_bf16, n, vocab, k, temperature,
+                       hard_weight, soft_weight)) return NLH_ERR_INVALID_ARG;
+    if (!saved || !aligned16(saved) || saved_bytes < distill::place(A, (char*)saved) || d_row_stride < vocab || (n > 0 && !d_logits)) {
+        record_status(NLH_ERR_INVALID_ARG, where, "NULL pointer, a bad stride, or a saved buffer that is too small or not 16-byte aligned");
+        return NLH_ERR_INVALID_ARG;
+    }
+    if (n == 0) return NLH_OK;
+    A.d = d_logits; A.d_row = d_row_stride; A.grad = grad_scale;
+    return (logits_is_bf16 ? distill::backward<__nv_bfloat16>(A, where) : distill::backward<float>(A, where)) ? NLH_OK : NLH_ERR_CUDA;
+}
+
+}  // extern "C"

@@ -1,0 +1,498 @@
+// Embedding lookup with scaling, and its gradient by sorted tokens.
+//
+//   out_t = scale w[id_t],   d_w[r] (+)= scale sum over {t : id_t = r} of d_out_t, in ascending t, in fp32.
+//
+// The gradient's rows meet wherever an id repeats, and in text a few ids are much of it. Instead of atomics (whose
+// order, and so whose sum, changes from run to run, and which queue up on the hot rows) the tokens are sorted by id with a
+// stable radix sort, every sum then has one order, and every row of d_w is touched once, by one writer:
+//   sort    : least significant digit first, 9 bits a pass: a histogram per 2048 tokens, then ranks from it
+//   reduce  : a run of sorted tokens per group of lanes; an id that lies inside the run is written at once, the pieces of one
+//             that crosses runs go to a buffer
+//   join    : those pieces, added in order by the run in which the id begins
+// Up to SMALL tokens one launch does it all: a CTA per token looks for its id in the whole list, and the first token of an id
+// adds up its rows.
+// Bound by HBM: d_out is read once, the touched rows of d_w once and written once.
+#include <cuda_bf16.h>
+
+#include "nlh_common.cuh"
+#include "../../include/nlh_ffi.h"
+
+namespace nlh {
+namespace emb {
+
+constexpr int BITS = 9, BINS = 1 << BITS;
+constexpr int SORT_THREADS = 256, SORT_ITEMS = 8, SORT_TILE = SORT_THREADS * SORT_ITEMS;
+constexpr int SMALL = 2048;
+constexpr int THREADS = 128;
+
+template <typename T> struct Vec { static constexpr int N = 16 / sizeof(T); };
+template <typename T, int N> __device__ __forceinline__ void load(const T* p, float* f);
+template <> __device__ __forceinline__ void load<float, 4>(const float* p, float* f)
+{
+    const float4 v = *reinterpret_cast<const float4*>(p);
+    f[0] = v.x; f[1] = v.y; f[2] = v.z; f[3] = v.w;
+}
+template <> __device__ __forceinline__ void load<__nv_bfloat16, 8>(const __nv_bfloat16* p, float* f)
+{
+    const uint4 u = *reinterpret_cast<const uint4*>(p);
+    const unsigned w[4] = {u.x, u.y, u.z, u.w};
+#pragma unroll
+    for (int i = 0; i < 4; i++) { f[2 * i] = __uint_as_float(w[i] << 16); f[2 * i + 1] = __uint_as_float(w[i] & 0xffff0000u); }
+}
+template <> __device__ __forceinline__ void load<float, 1>(const float* p, float* f) { f[0] = *p; }
+template <> __device__ __forceinline__ void load<__nv_bfloat16, 1>(const __nv_bfloat16* p, float* f) { f[0] = __bfloat162float(*p); }
+// N floats to / from fp32 memory
+template <int N> __device__ __forceinline__ void store_f32(float* p, const float* f)
+{
+    if (N == 1) { p[0] = f[0]; return; }
+#pragma unroll
+    for (int i = 0; i < N; i += 4) *reinterpret_cast<float4*>(p + i) = make_float4(f[i], f[i + 1], f[i + 2], f[i + 3]);
+}
+template <int N> __device__ __forceinline__ void load_f32(const float* p, float* f)
+{
+    if (N == 1) { f[0] = p[0]; return; }
+#pragma unroll
+    for (int i = 0; i < N; i += 4) {
+        const float4 v = *reinterpret_cast<const float4*>(p + i);
+        f[i] = v.x; f[i + 1] = v.y; f[i + 2] = v.z; f[i + 3] = v.w;
+    }
+}
+__device__ __forceinline__ void put(float* p, float x) { *p = x; }
+__device__ __forceinline__ void put(__nv_bfloat16* p, float x) { *p = __float2bfloat16(x); }
+
+// ── lookup ──
+// `lanes` lanes share a row (a power of two, 32 at most), N elements each and step.
+template <typename T, int N>
+__global__ void __launch_bounds__(256) lookup_kernel(const T* __restrict__ w, const int* __restrict__ ids, T* __restrict__ out, int n,
+                                                     int vocab, int d, int lanes, float scale)
+{
+    const int per = 256 / lanes, lane = threadIdx.x & (lanes - 1);
+    for (long long t = (long long)blockIdx.x * per + threadIdx.x / lanes; t < n; t += (long long)gridDim.x * per) {
+        const int id = ids[t];
+        const bool ok = id >= 0 && id < vocab;
+        const T* src = w + (long long)(ok ? id : 0) * d;
+        T* dst = out + t * d;
+#pragma unroll 4
+        for (int c = lane * N; c < d; c += lanes * N) {
+            float f[N];
+            if (ok) load<T, N>(src + c, f);
+#pragma unroll
+            for (int i = 0; i < N; i++) f[i] = ok ? f[i] * scale : 0.f;
+            if (N == 1) put(dst + c, f[0]);
+            else if (sizeof(T) == 4) store_f32<N>((float*)(dst + c), f);
+            else {
+                unsigned u[4];
+#pragma unroll
+                for (int i = 0; i < 4; i++) {
+                    const __nv_bfloat162 b = __floats2bfloat162_rn(f[(2 * i) % N], f[(2 * i + 1) % N]);
+                    u[i] = *reinterpret_cast<const unsigned*>(&b);
+                }
+                *reinterpret_cast<uint4*>(dst + c) = make_uint4(u[0], u[1], u[2], u[3]);
+            }
+        }
+    }
+}
+
+// ── sort ──
+// Key of a token: its id, or vocab (behind all others) where the id is none.
+__device__ __forceinline__ int key_of(const int* ids, const int2* in, int i, int vocab, int& pos)
+{
+    if (in) { const int2 x = in[i]; pos = x.y; return x.x; }
+    pos = i;
+    const int id = ids[i];
+    return id >= 0 && id < vocab ? id : vocab;
+}
+// hist [BINS, blocks]: tokens of each digit in each tile
+__global__ void __launch_bounds__(SORT_THREADS) hist_kernel(const int* ids, const int2* in, int* hist, int n, int vocab, int shift, int blocks)
+{
+    __shared__ int s[BINS];
+    for (int i = threadIdx.x; i < BINS; i += SORT_THREADS) s[i] = 0;
+    __syncthreads();
+    for (int j = 0; j < SORT_ITEMS; j++) {
+        const int i = blockIdx.x * SORT_TILE + j * SORT_THREADS + threadIdx.x;
+        int pos;
+        if (i < n) atomicAdd(&s[(key_of(ids, in, i, vocab, pos) >> shift) & (BINS - 1)], 1);
+    }
+    __syncthreads();
+    for (int i = threadIdx.x; i < BINS; i += SORT_THREADS) hist[(long long)i * blocks + blockIdx.x] = s[i];
+}
+// One warp per digit: counts -> sums over the tiles before; the digit's total behind them in `total`.
+__global__ void __launch_bounds__(256) scan_kernel(int* hist, int* total, int blocks)
+{
+    const int digit = blockIdx.x * 8 + (threadIdx.x >> 5), lane = threadIdx.x & 31;
+    int* h = hist + (long long)digit * blocks;
+    int carry = 0;
+    for (int b = 0; b < blocks; b += 32) {
+        const int c = b + lane < blocks ? h[b + lane] : 0;
+        int s = c;
+        for (int o = 1; o < 32; o <<= 1) { const int y = __shfl_up_sync(0xffffffffu, s, o); if (lane >= o) s += y; }
+        if (b + lane < blocks) h[b + lane] = carry + s - c;
+        carry += __shfl_sync(0xffffffffu, s, 31);
+    }
+    if (lane == 0) total[digit] = carry;
+}
+// Every token to its place: tokens of smaller digits, of this digit in the tiles before, in the warps before, in this warp before.
+__global__ void __launch_bounds__(SORT_THREADS) scatter_kernel(const int* ids, const int2* in, int2* out, const int* hist, const int* total,
+                                                               int n, int vocab, int shift, int blocks)
+{
+    constexpr int WARPS = SORT_THREADS / 32, SEG = SORT_TILE / WARPS;
+    __shared__ int s_cnt[WARPS][BINS], s_scan[WARPS];
+    const int lane = threadIdx.x & 31, w = threadIdx.x >> 5;
+    for (int i = threadIdx.x; i < WARPS * BINS; i += SORT_THREADS) (&s_cnt[0][0])[i] = 0;
+    __syncthreads();
+    int key[SORT_ITEMS], pos[SORT_ITEMS], rank[SORT_ITEMS];
+#pragma unroll
+    for (int j = 0; j < SORT_ITEMS; j++) {
+        const int i = blockIdx.x * SORT_TILE + w * SEG + j * 32 + lane;
+        key[j] = -1;
+        if (i < n) key[j] = key_of(ids, in, i, vocab, pos[j]);
+    }
+#pragma unroll
+    for (int j = 0; j < SORT_ITEMS; j++) {
+        const int digit = key[j] < 0 ? -1 : (key[j] >> shift) & (BINS - 1);
+        const unsigned same = __match_any_sync(0xffffffffu, digit);
+        int before = 0;
+        if (digit >= 0) before = s_cnt[w][digit];
+        __syncwarp();
+        if (digit >= 0) {
+            rank[j] = before + __popc(same & ((1u << lane) - 1));
+            if (lane == __ffs(same) - 1) s_cnt[w][digit] = before + __popc(same);
+        }
+        __syncwarp();
+    }
+    __syncthreads();
+    // digits 2 threadIdx.x, 2 threadIdx.x + 1: where this tile's first token of the digit goes, then each warp's
+    int tot[2], first[2];
+#pragma unroll
+    for (int e = 0; e < 2; e++) {
+        const int digit = 2 * threadIdx.x + e;
+        if (total) { tot[e] = total[digit]; first[e] = hist[(long long)digit * blocks + blockIdx.x]; }
+        else {
+            tot[e] = first[e] = 0;
+            for (int b = 0; b < blocks; b++) {
+                const int c = hist[(long long)digit * blocks + b];
+                if (b < blockIdx.x) first[e] += c;
+                tot[e] += c;
+            }
+        }
+    }
+    int s = tot[0] + tot[1];
+    for (int o = 1; o < 32; o <<= 1) { const int y = __shfl_up_sync(0xffffffffu, s, o); if (lane >= o) s += y; }
+    if (lane == 31) s_scan[w] = s;
+    __syncthreads();
+    for (int j = 0; j < w; j++) s += s_scan[j];
+#pragma unroll
+    for (int e = 0; e < 2; e++) {
+        const int digit = 2 * threadIdx.x + e;
+        int at = s - tot[0] - tot[1] + (e ? tot[0] : 0) + first[e];
+        for (int j = 0; j < WARPS; j++) { const int c = s_cnt[j][digit]; s_cnt[j][digit] = at; at += c; }
+    }
+    __syncthreads();
+#pragma unroll
+    for (int j = 0; j < SORT_ITEMS; j++)
+        if (key[j] >= 0) out[s_cnt[w][(key[j] >> shift) & (BINS - 1)] + rank[j]] = make_int2(key[j], pos[j]);
+}
+
+// ── reduce ──
+// A group of `lanes` lanes takes `run` sorted tokens (and columns blockIdx.y * lanes * N ..). part [runs, 2, d]: the piece of an id
+// that began before the run, and of one that goes on behind it.
+template <typename T, int N, bool ADD>
+__global__ void __launch_bounds__(THREADS) reduce_kernel(const T* __restrict__ dy, const int2* __restrict__ sorted, float* __restrict__ dw,
+                                                         float* __restrict__ part, int n, int vocab, int d, int lanes, int run, float scale)
+{
+    const int per = THREADS / lanes, lane = threadIdx.x & (lanes - 1);
+    const int r = blockIdx.x * per + threadIdx.x / lanes, c = (blockIdx.y * lanes + lane) * N;
+    const long long b = (long long)r * run;
+    if (b >= n || c >= d) return;
+    const int e = (int)min((long long)n, b + run);
+    const int prev = b > 0 ? sorted[b - 1].x : -1, next = e < n ? sorted[e].x : -1;
+    float acc[N];
+#pragma unroll
+    for (int i = 0; i < N; i++) acc[i] = 0.f;
+    int cur = sorted[b].x;
+    bool head = cur == prev;
+    auto flush = [&](bool tail) {
+        if (cur >= vocab) return;
+        if (head || tail) {
+            store_f32<N>(part + ((long long)r * 2 + (head ? 0 : 1)) * d + c, acc);
+        } else {
+            float o[N];
+            float* p = dw + (long long)cur * d + c;
+            if (ADD) load_f32<N>(p, o);
+#pragma unroll
+            for (int i = 0; i < N; i++) o[i] = ADD ? fmaf(scale, acc[i], o[i]) : scale * acc[i];
+            store_f32<N>(p, o);
+        }
+    };
+    constexpr int U = 8;
+    for (int i = (int)b; i < e; i += U) {
+        float f[U][N];
+        int key[U];
+#pragma unroll
+        for (int u = 0; u < U; u++) {
+            key[u] = vocab;
+            if (i + u < e) {
+                const int2 s = sorted[i + u];
+                key[u] = s.x;
+                if (s.x < vocab) load<T, N>(dy + (long long)s.y * d + c, f[u]);
+            }
+        }
+#pragma unroll
+        for (int u = 0; u < U; u++) {
+            if (i + u >= e) break;
+            if (key[u] != cur) {
+                flush(false);
+                cur = key[u];
+                head = false;
+#pragma unroll
+                for (int x = 0; x < N; x++) acc[x] = 0.f;
+            }
+            if (cur < vocab) {
+#pragma unroll
+                for (int x = 0; x < N; x++) acc[x] += f[u][x];
+            }
+        }
+    }
+    flush(cur == next);
+}
+// Ids that cross runs: the run in which one begins adds its pieces up.
+template <int N, bool ADD>
+__global__ void __launch_bounds__(THREADS) join_kernel(const int2* __restrict__ sorted, float* __restrict__ dw, const float* __restrict__ part,
+                                                       int n, int vocab, int d, int lanes, int run, float scale)
+{
+    const int per = THREADS / lanes, lane = threadIdx.x & (lanes - 1);
+    const int r = blockIdx.x * per + threadIdx.x / lanes, c = (blockIdx.y * lanes + lane) * N;
+    const long long b = (long long)r * run, e = b + run;
+    if (e >= n || c >= d) return;
+    const int key = sorted[e - 1].x;
+    if (key >= vocab || sorted[e].x != key) return;                    // nothing goes on behind this run
+    if (b > 0 && sorted[b].x == key && sorted[b - 1].x == key) return;  // it began before it
+    float acc[N];
+    load_f32<N>(part + ((long long)r * 2 + 1) * d + c, acc);
+    constexpr int U = 8;
+    for (long long q = r + 1; q * run < n; q += U) {
+        float f[U][N];
+        bool on[U];
+#pragma unroll
+        for (int u = 0; u < U; u++) {
+            on[u] = (q + u) * run < n && sorted[(q + u) * run].x == key;    // sorted: run q + u begins with the id or is behind it
+            if (on[u]) load_f32<N>(part + (q + u) * 2 * d + c, f[u]);
+        }
+#pragma unroll
+        for (int u = 0; u < U; u++)
+            if (on[u]) {
+#pragma unroll
+                for (int i = 0; i < N; i++) acc[i] += f[u][i];
+            }
+        if (!on[U - 1]) break;
+    }
+    float o[N];
+    float* p = dw + (long long)key * d + c;
+    if (ADD) load_f32<N>(p, o);
+#pragma unroll
+    for (int i = 0; i < N; i++) o[i] = ADD ? fmaf(scale, acc[i], o[i]) : scale * acc[i];
+    store_f32<N>(p, o);
+}
+
+// ── few tokens ──
+// A CTA per token. Groups of `lanes` lanes take stretches of the id's tokens, joined in order.
+template <typename T, int N, bool ADD>
+__global__ void __launch_bounds__(THREADS) small_kernel(const T* __restrict__ dy, const int* __restrict__ ids, float* __restrict__ dw, int n,
+                                                        int vocab, int d, int lanes, float scale)
+{
+    __shared__ int s_list[SMALL], s_warp[THREADS / 32];
+    __shared__ float s_acc[THREADS * N];
+    const int t = blockIdx.x, id = ids[t], w = threadIdx.x >> 5, wl = threadIdx.x & 31;
+    if (id < 0 || id >= vocab) return;
+    bool seen = false;
+    for (int i = threadIdx.x; i < t; i += THREADS) seen |= ids[i] == id;
+    if (__syncthreads_or(seen)) return;
+    int count = 0;
+    for (int base = t; base < n; base += THREADS) {
+        const bool hit = base + threadIdx.x < n && ids[base + threadIdx.x] == id;
+        const unsigned m = __ballot_sync(0xffffffffu, hit);
+        if (wl == 0) s_warp[w] = __popc(m);
+        __syncthreads();
+        int at = count;
+        for (int j = 0; j < w; j++) at += s_warp[j];
+        if (hit) s_list[at + __popc(m & ((1u << wl) - 1))] = base + threadIdx.x;
+        for (int j = 0; j < THREADS / 32; j++) count += s_warp[j];
+        __syncthreads();
+    }
+    const int per = THREADS / lanes, lane = threadIdx.x & (lanes - 1), grp = threadIdx.x / lanes;
+    const int stretch = (count + per - 1) / per, i0 = grp * stretch, i1 = min(count, i0 + stretch);
+    for (int c0 = 0; c0 < d; c0 += lanes * N) {
+        const int c = c0 + lane * N;
+        float acc[N];
+#pragma unroll
+        for (int i = 0; i < N; i++) acc[i] = 0.f;
+        if (c < d) {
+#pragma unroll 8
+            for (int i = i0; i < i1; i++) {
+                float f[N];
+                load<T, N>(dy + (long long)s_list[i] * d + c, f);
+#pragma unroll
+                for (int x = 0; x < N; x++) acc[x] += f[x];
+            }
+        }
+        if (per > 1) {
+#pragma unroll
+            for (int i = 0; i < N; i++) s_acc[i * THREADS + threadIdx.x] = acc[i];
+            __syncthreads();
+            if (grp == 0) {
+                for (int j = 1; j < per; j++)
+#pragma unroll
+                    for (int i = 0; i < N; i++) acc[i] += s_acc[i * THREADS + j * lanes + lane];
+            }
+            __syncthreads();
+        }
+        if (grp == 0 && c < d) {
+            float o[N];
+            float* p = dw + (long long)id * d + c;
+            if (ADD) load_f32<N>(p, o);
+#pragma unroll
+            for (int i = 0; i < N; i++) o[i] = ADD ? fmaf(scale, acc[i], o[i]) : scale * acc[i];
+            store_f32<N>(p, o);
+        }
+    }
+}
+
+// ── host ──
+struct Plan {
+    int passes, blocks, run, runs;
+    int2 *a, *b;
+    int *hist, *total;
+    float* part;
+};
+static int64_t place(Plan& P, char* base, int n, int vocab, int d)
+{
+    P = Plan{};
+    if (n <= SMALL) return 0;
+    int bits = 1;
+    while (bits < 31 && (vocab >> bits) != 0) bits++;          // keys 0 .. vocab
+    P.passes = (bits + BITS - 1) / BITS;
+    P.blocks = (int)(((int64_t)n + SORT_TILE - 1) / SORT_TILE);
+    // runs of 32 sorted tokens give every SM a few even at SMALL tokens; longer ones shorten the join of a hot id where there are plenty
+    P.run = n <= (1 << 18) ? 32 : 128;
+    P.runs = (int)(((int64_t)n + P.run - 1) / P.run);
+    int64_t at = 0;
+    auto take = [&](int64_t bytes) { char* p = base + at; at += (bytes + 255) & ~(int64_t)255; return (void*)p; };
+    P.a = (int2*)take((int64_t)n * 8);
+    P.b = (int2*)take((int64_t)n * 8);
+    P.hist = (int*)take((int64_t)BINS * P.blocks * 4);
+    P.total = (int*)take(BINS * 4);
+    P.part = (float*)take((int64_t)P.runs * 2 * d * 4);
+    return at;
+}
+static int lanes_for(int d, int per, int most)
+{
+    int l = 1;
+    while (l < most && l * per < d) l <<= 1;
+    return l;
+}
+
+template <typename T, int N, bool ADD>
+static bool backward(const T* dy, const int* ids, float* dw, int n, int vocab, int d, float scale, char* ws, const char* where)
+{
+    cudaStream_t st = current_stream();
+    Plan P;
+    place(P, ws, n, vocab, d);
+    const int lanes = lanes_for(d, N, THREADS);
+    if (n <= SMALL) {
+        small_kernel<T, N, ADD><<<n, THREADS, 0, st>>>(dy, ids, dw, n, vocab, d, lanes, scale);
+        return check_launch(where);
+    }
+    const int2* in = nullptr;
+    int2* out = P.a;
+    for (int p = 0; p < P.passes; p++) {
+        hist_kernel<<<P.blocks, SORT_THREADS, 0, st>>>(ids, in, P.hist, n, vocab, p * BITS, P.blocks);
+        if (!check_launch(where)) return false;
+        // a scatter CTA adds up the histograms itself while they are few: one launch less
+        const bool scan = P.blocks > 64;
+        if (scan) {
+            scan_kernel<<<BINS / 8, 256, 0, st>>>(P.hist, P.total, P.blocks);
+            if (!check_launch(where)) return false;
+        }
+        scatter_kernel<<<P.blocks, SORT_THREADS, 0, st>>>(ids, in, out, P.hist, scan ? P.total : nullptr, n, vocab, p * BITS, P.blocks);
+        if (!check_launch(where)) return false;
+        in = out;
+        out = out == P.a ? P.b : P.a;
+    }
+    const int per = THREADS / lanes;
+    const dim3 grid((P.runs + per - 1) / per, (d + lanes * N - 1) / (lanes * N));
+    reduce_kernel<T, N, ADD><<<grid, THREADS, 0, st>>>(dy, in, dw, P.part, n, vocab, d, lanes, P.run, scale);
+    if (!check_launch(where)) return false;
+    join_kernel<N, ADD><<<grid, THREADS, 0, st>>>(in, dw, P.part, n, vocab, d, lanes, P.run, scale);
+    return check_launch(where);
+}
+
+template <typename T, int N> static bool lookup(const T* w, const int* ids, T* out, int n, int vocab, int d, float scale, const char* where)
+{
+    const int lanes = lanes_for(d, N, 32), per = 256 / lanes;
+    const long long need = ((long long)n + per - 1) / per;
+    lookup_kernel<T, N><<<(unsigned)(need < 148 * 32 ? need : 148 * 32), 256, 0, current_stream()>>>(w, ids, out, n, vocab, d, lanes, scale);
+    return check_launch(where);
+}
+
+}  // namespace emb
+}  // namespace nlh
+
+using namespace nlh;
+
+extern "C" {
+
+int32_t nlh_embedding_forward(const void* w, int32_t w_is_bf16, const int32_t* ids, void* out, int32_t n, int32_t vocab, int32_t d,
+    float scale)
+{
+    const char* where = "nlh_embedding_forward";
+    if (n < 0 || vocab <= 0 || d <= 0 || (n > 0 && (!w || !ids || !out))) {
+        record_status(NLH_ERR_INVALID_ARG, where, "bad dimensions or NULL pointer");
+        return NLH_ERR_INVALID_ARG;
+    }
+    if (n == 0) return NLH_OK;
+    const bool vec = aligned16(w) && aligned16(out);
+    bool ok;
+    if (w_is_bf16) {
+        typedef __nv_bfloat16 T;
+        ok = vec && d % 8 == 0 ? emb::lookup<T, 8>((const T*)w, ids, (T*)out, n, vocab, d, scale, where)
+                               : emb::lookup<T, 1>((const T*)w, ids, (T*)out, n, vocab, d, scale, where);
+    } else {
+        ok = vec && d % 4 == 0 ? emb::lookup<float, 4>((const float*)w, ids, (float*)out, n, vocab, d, scale, where)
+                               : emb::lookup<float, 1>((const float*)w, ids, (float*)out, n, vocab, d, scale, where);
+    }
+    return ok ? NLH_OK : NLH_ERR_CUDA;
+}
+
+int64_t nlh_embedding_backward_bytes(int32_t n, int32_t vocab, int32_t d)
+{
+    if (n < 0 || vocab <= 0 || d <= 0) return -1;
+    emb::Plan P;
+    return emb::place(P, nullptr, n, vocab, d);
+}
+
+int32_t nlh_embedding_backward(const void* d_out, int32_t d_out_is_bf16, const int32_t* ids, float* d_w, int32_t n, int32_t vocab,
+    int32_t d, float scale, int32_t accumulate, void* workspace, int64_t workspace_bytes)
+{
+    const char* where = "nlh_embedding_backward";
+    const int64_t need = nlh_embedding_backward_bytes(n, vocab, d);
+    if (need < 0 || !d_w || (n > 0 && (!d_out || !ids)) || (need > 0 && (!workspace || !aligned16(workspace))) || workspace_bytes < need) {
+        record_status(NLH_ERR_INVALID_ARG, where, "bad dimensions, NULL pointer, or a workspace that is too small or not 16-byte aligned");
+        return NLH_ERR_INVALID_ARG;
+    }
+    if (!accumulate) {      // rows without a token
+        const cudaError_t e = cudaMemsetAsync(d_w, 0, (size_t)vocab * d * 4, current_stream());
+        if (e != cudaSuccess) { record_status(NLH_ERR_CUDA, where, cudaGetErrorString(e)); return NLH_ERR_CUDA; }
+    }
+    if (n == 0) return NLH_OK;
+    const bool vec = aligned16(d_out) && aligned16(d_w);
+    char* ws = (char*)workspace;
+    bool ok;
+#define NLH_EMB(T, N) (accumulate ? emb::backward<T, N, true>((const T*)d_out, ids, d_w, n, vocab, d, scale, ws, where) \
+                                  : emb::backward<T, N, false>((const T*)d_out, ids, d_w, n, vocab, d, scale, ws, where))
+    if (d_out_is_bf16) ok = vec && d % 8 == 0 ? NLH_EMB(__nv_bfloat16, 8) : NLH_EMB(__nv_bfloat16, 1);
+    else ok = vec && d % 4 == 0 ? NLH_EMB(float, 4) : NLH_EMB(float, 1);
+#undef NLH_EMB
+    return ok ? NLH_OK : NLH_ERR_CUDA;
+}
+
+}  // extern "C"

@@ -505,6 +505,111 @@ def gated_delta_step(k, v, q, log_retain, theta, m, slots=None, scale=1.0):
     return y
 
 
+# ── embedding with scaling, gradient by sorted tokens (additive API) ───────
+def _ids32(where, name, ids, numel=None):
+    if ids.dtype != torch.int32 or not ids.is_contiguous() or (numel is not None and ids.numel() != numel):
+        raise ValueError(f"{where}.{name}: need contiguous int32 ids" + ("" if numel is None else f", {numel} of them"))
+
+
+def embedding_forward(w, ids, scale=1.0):
+    """scale * w[ids] (nlh_embedding_forward): w [vocab, d] fp32 or bf16, ids int32 of any shape; returns [*ids.shape, d]
+    in w's type. An id outside [0, vocab) gives a row of zeros."""
+    where = "embedding_forward"
+    _same_device(where, w, ids=ids)
+    if w.dim() != 2 or w.dtype not in (torch.float32, torch.bfloat16) or not w.is_contiguous():
+        raise ValueError(f"{where}.w: need a contiguous fp32 or bf16 [vocab, d]")
+    _ids32(where, "ids", ids)
+    with _on_device(w):
+        out = torch.empty(*ids.shape, w.shape[1], dtype=w.dtype, device=w.device)
+        call("nlh_embedding_forward", w=w, w_is_bf16=int(w.dtype == torch.bfloat16), ids=ids, out=out, n=ids.numel(),
+             vocab=w.shape[0], d=w.shape[1], scale=scale)
+    return out
+
+
+def embedding_backward(d_out, ids, d_w, scale=1.0, accumulate=True):
+    """Gradient of embedding_forward (nlh_embedding_backward): d_w [vocab, d] fp32 += scale * the sums of d_out's rows
+    by id, or = with accumulate=False. The same inputs give the same bits. Returns d_w."""
+    where = "embedding_backward"
+    _same_device(where, d_w, d_out=d_out, ids=ids)
+    if d_w.dim() != 2:
+        raise ValueError(f"{where}.d_w: need [vocab, d]")
+    _need(where, "d_w", d_w, torch.float32, d_w.shape)
+    vocab, d = d_w.shape
+    if d_out.dtype not in (torch.float32, torch.bfloat16) or d_out.shape != (*ids.shape, d) or not d_out.is_contiguous():
+        raise ValueError(f"{where}.d_out: need a contiguous fp32 or bf16 {(*ids.shape, d)}, got {d_out.dtype} {tuple(d_out.shape)}")
+    _ids32(where, "ids", ids)
+    with _on_device(d_w):
+        n = ids.numel()
+        nbytes = ffi.lib().nlh_embedding_backward_bytes(n, vocab, d)
+        work = torch.empty(nbytes, dtype=torch.uint8, device=d_w.device) if nbytes > 0 else None
+        call("nlh_embedding_backward", d_out=d_out, d_out_is_bf16=int(d_out.dtype == torch.bfloat16), ids=ids, d_w=d_w, n=n,
+             vocab=vocab, d=d, scale=scale, accumulate=int(accumulate), workspace=work, workspace_bytes=max(nbytes, 0))
+    torch.autograd.graph.increment_version(d_w)      # written past autograd
+    return d_w
+
+
+# ── distillation from a teacher's top logits (additive API) ────────────────
+class DistillSaved:
+    """What distill_backward needs of its forward: the forward's arguments and the rows' statistics."""
+    __slots__ = ("buffer", "shape", "dtype", "args")
+
+
+def distill_forward(logits, teacher_ids, teacher_logits, targets=None, temperature=1.0, soft_weight=1.0, hard_weight=0.0):
+    """Distillation loss (nlh_distill_forward) of student logits [n, vocab] (fp32 or bf16, rows may be strided) from
+    a teacher's top entries teacher_ids [n, k] int32 (outside [0, vocab): unused) and teacher_logits [n, k]:
+    soft_weight * temperature^2 * mean KL(teacher || student at the temperature) + hard_weight * mean cross-entropy with
+    targets [n] int32 (outside [0, vocab): none). Returns (loss, saved)."""
+    where = "distill_forward"
+    _same_device(where, logits, teacher_ids=teacher_ids, teacher_logits=teacher_logits, targets=targets)
+    if logits.dim() != 2 or logits.dtype not in (torch.float32, torch.bfloat16) or (logits.shape[1] > 1 and logits.stride(1) != 1):
+        raise ValueError(f"{where}.logits: need fp32 or bf16 [n, vocab] with contiguous rows")
+    n, vocab = logits.shape
+    if teacher_ids.dim() != 2 or teacher_ids.shape[0] != n or teacher_logits.shape != teacher_ids.shape:
+        raise ValueError(f"{where}: teacher_ids {tuple(teacher_ids.shape)} and teacher_logits {tuple(teacher_logits.shape)} "
+                         f"must both be [{n}, k]")
+    _ids32(where, "teacher_ids", teacher_ids)
+    if teacher_logits.dtype not in (torch.float32, torch.bfloat16) or not teacher_logits.is_contiguous():
+        raise ValueError(f"{where}.teacher_logits: need contiguous fp32 or bf16")
+    if targets is not None:
+        _ids32(where, "targets", targets, n)
+    row_stride = logits.stride(0) if n > 1 else vocab
+    with _on_device(logits):
+        nbytes = ffi.lib().nlh_distill_saved_bytes(n, vocab)
+        s = DistillSaved()
+        s.buffer = torch.empty(max(nbytes, 16), dtype=torch.uint8, device=logits.device)
+        s.shape, s.dtype = logits.shape, logits.dtype
+        s.args = dict(logits_is_bf16=int(logits.dtype == torch.bfloat16), row_stride=row_stride, target_ids=targets,
+                      teacher_ids=teacher_ids, teacher_logits=teacher_logits,
+                      teacher_is_bf16=int(teacher_logits.dtype == torch.bfloat16), saved=s.buffer, saved_bytes=s.buffer.numel(),
+                      n=n, vocab=vocab, k=teacher_ids.shape[1], temperature=temperature, hard_weight=hard_weight,
+                      soft_weight=soft_weight)
+        loss = torch.empty((), dtype=torch.float32, device=logits.device)
+        call("nlh_distill_forward", logits=logits.data_ptr(), loss=loss, **s.args)
+    return loss, s
+
+
+def distill_backward(logits, saved, grad=None, out=None):
+    """Gradient of distill_forward with respect to logits, times the fp32 scalar tensor ``grad``. out (default: a new
+    tensor) may be logits itself. The tensors given to the forward must not have changed."""
+    where = "distill_backward"
+    _same_device(where, logits, grad=grad, out=out, saved=saved.buffer)
+    if logits.shape != saved.shape or logits.dtype != saved.dtype:
+        raise ValueError(f"{where}.logits: not what distill_forward was given")
+    n, vocab = logits.shape
+    if out is None:
+        out = torch.empty(n, vocab, dtype=logits.dtype, device=logits.device)
+    elif out.shape != logits.shape or out.dtype != logits.dtype or (vocab > 1 and out.stride(1) != 1):
+        raise ValueError(f"{where}.out: need {logits.dtype} {tuple(logits.shape)} with contiguous rows")
+    if grad is not None and (grad.dtype != torch.float32 or grad.numel() != 1):
+        raise ValueError(f"{where}.grad: need one fp32 value")
+    stride = lambda t: t.stride(0) if n > 1 else vocab
+    with _on_device(logits):
+        call("nlh_distill_backward", logits=logits.data_ptr(), grad_scale=None if grad is None else grad.data_ptr(),
+             d_logits=out.data_ptr(), d_row_stride=stride(out), **{**saved.args, "row_stride": stride(logits)})
+    torch.autograd.graph.increment_version(out)      # written past autograd
+    return out
+
+
 # ── SWA ────────────────────────────────────────────────────────────────────
 # q,k,v,out: [B,S,H*hd] bf16; attn_weights [B,H,S,n_p+W] bf16; grads f32.
 
