@@ -584,7 +584,7 @@ int32_t nlh_gated_delta_backward(const nlh_gated_delta_desc* desc, const void* k
     float* d_m_initial, void* workspace, int64_t workspace_bytes);
 /* Recurrent form: seq tokens (one, or a few) for each of batch sequences on stored states m [n_slots, heads_v, dv, dk],
  * updated in place. slots [batch] on the device gives each sequence's state; NULL: sequence i has state i. A slot outside
- * [0, n_slots) is skipped and its rows of y are not written. A slot named more than once is stepped in the order of the batch. */
+ * [0, n_slots) is no sequence: its rows of y are zeros. A slot named more than once is stepped in the order of the batch. */
 int32_t nlh_gated_delta_step(const nlh_gated_delta_desc* desc, const void* k, const void* v, const void* q,
     const float* log_retain, const float* theta, float* m, const int32_t* slots, int32_t n_slots, void* y);
 

@@ -204,21 +204,31 @@ __global__ void __launch_bounds__(128) gd_prep_kernel(Args A)
         reinterpret_cast<float4*>(out)[i] = *reinterpret_cast<const float4*>(Tm + (i >> 4) * LD + (i & 15) * 4);
 }
 
-// ── forward states: the recurrence over chunks for NS columns of V ──
-// Four warps; warp w owns tokens 16w.. in the products over tokens and state rows 16w.. (of each 64 of dk) in the update,
-// whose accumulators stay in registers from chunk to chunk.
+// ── forward states: the recurrence over chunks for NS = 32 columns of V ──
+// Eight warps: warp = 16 rows (tokens; state rows of each 64 of dk in the update) x 16 columns. The state stays in the
+// update's accumulators from chunk to chunk. While a chunk is computed the next one's K, T, V and gates are on their
+// way in registers; K has two buffers, because it is read until the chunk's end. Three barriers a chunk. Bound by that chain:
+// three products of 64 x 32 x 64 that wait for one another. 64 columns a CTA would halve the reads of K and T, which
+// come from L2, but leave half the CTAs to hide the chain behind.
+template <int DKP, int NS> struct StateSmem {
+    // LS: pairs between rows of a split [token][column] matrix
+    static constexpr int LK = DKP + 4, LS = NS + 2, BYTES = 4 * (2 * C * LK + C * LD) + 8 * (NS * LK + 2 * C * LS);
+};
+struct GateRow { float4 g; float theta; };
+
 template <typename T, int DKP, int NS>
-__global__ void __launch_bounds__(128) gd_state_fwd_kernel(Args A)
+__global__ void __launch_bounds__(256, DKP == 64 ? 2 : 1) gd_state_fwd_kernel(Args A)
 {
-    constexpr int LK = DKP + 4, LN = NS + 4, NT = NS / 8, MT = DKP / 64;
+    constexpr int LK = DKP + 4, LS = NS + 2, MT = DKP / 64, NT = NS / 16, H = NS / 2;
     extern __shared__ float4 smem4[];
-    float* Ks = reinterpret_cast<float*>(smem4);            // [64][LK]
-    float *Ts = Ks + C * LK, *Ms = Ts + C * LD;             // [64][LD], [NS][LK]
-    float *Rs = Ms + NS * LK, *Us = Rs + C * LN;            // [64][LN] each
-    __shared__ float4 s_gate[C];
-    __shared__ float s_w[C];
+    float* Kb = reinterpret_cast<float*>(smem4);                        // [2][64][LK]
+    float* Ts = Kb + 2 * C * LK;                                        // [64][LD]
+    float2* Ms = reinterpret_cast<float2*>(Ts + C * LD);                // [NS][LK] pairs
+    float2 *Rs = Ms + NS * LK, *Us = Rs + C * LS;                       // [64][LS] pairs
+    __shared__ float4 s_gate[2][C];
+    __shared__ float s_w[2][C];
     const int nsl = A.dvp / NS, sl = blockIdx.x % nsl, p = blockIdx.x / nsl, h = p % A.hv, seq = p / A.hv;
-    const int n0 = sl * NS, tid = threadIdx.x, lane = tid & 31, w = tid >> 5, g = lane >> 2, t = lane & 3;
+    const int n0 = sl * NS, tid = threadIdx.x, lane = tid & 31, w = tid >> 5, rb = w & 3, hf = w >> 2, g = lane >> 2, t = lane & 3;
     const int slot0 = first_slot(A, seq), count = chunk_count(A, seq);
 
     float S[MT][NT][4];
@@ -229,78 +239,112 @@ __global__ void __launch_bounds__(128) gd_state_fwd_kernel(Args A)
         for (int n = 0; n < NT; n++)
 #pragma unroll
             for (int i = 0; i < 4; i++) {
-                const int row = 64 * m + 16 * w + g + 8 * (i >> 1), col = n0 + 8 * n + 2 * t + (i & 1);   // dk, dv
-                S[m][n][i] = m0 && row < A.dk && col < A.dv ? m0[(long long)col * A.dk + row] : 0.f;
-                Ms[(col - n0) * LK + row] = S[m][n][i];
+                const int row = 64 * m + 16 * rb + g + 8 * (i >> 1), col = H * hf + 8 * n + 2 * t + (i & 1);   // dk, dv
+                S[m][n][i] = m0 && row < A.dk && n0 + col < A.dv ? m0[(long long)(n0 + col) * A.dk + row] : 0.f;
+                Ms[col * LK + row] = split_pair(S[m][n][i]);
             }
-    __syncthreads();
-    for (int c = 0; c < count; c++) {
+    Prefetch<T, DKP, 256> pk;
+    Prefetch<float, 64, 256> pt;
+    GateRow pg;
+    Pair<T> pv[NT][2];
+    const bool vpair = ((reinterpret_cast<uintptr_t>((const T*)A.v + n0) | (uintptr_t)((A.vb | A.vt | A.vh) * (long long)sizeof(T))) &
+                        (2 * sizeof(T) - 1)) == 0 && (A.dv & 1) == 0;
+    auto fetch = [&](int c) {
         const int slot = slot0 + c;
         const Chunk ch = get_chunk(A, slot);
         const long long tile = (long long)slot * A.hv + h;
-        const T* kp = (const T*)A.k + ch.b * A.kb + ch.t0 * A.kt + (h / A.share) * A.kh;
+        pk.load((const T*)A.k + ch.b * A.kb + ch.t0 * A.kt + (h / A.share) * A.kh, A.kt, ch.len, A.dk);
+        pt.load(A.tmat + tile * C * C, C, C, C);
+        if (tid < C) { ldg(pg.g, reinterpret_cast<const float*>(A.gates + tile * C + tid)); ldg(pg.theta, A.theta_eff + tile * C + tid); }
         const T* vp = (const T*)A.v + ch.b * A.vb + ch.t0 * A.vt + h * A.vh + n0;
-#pragma unroll
-        for (int m = 0; m < MT; m++) load_tile<T, 64, 128>(Ks + 64 * m, LK, kp + 64 * m, A.kt, ch.len, A.dk - 64 * m);
-        load_own<64, 64, 128>(Ts, LD, A.tmat + tile * C * C, C);
-        load_tile<T, NS, 128>(Rs, LN, vp, A.vt, ch.len, A.dv - n0);
-        if (tid < C) {
-            const float4 x = A.gates[tile * C + tid];
-            s_gate[tid] = x;
-            s_w[tid] = x.w * A.theta_eff[tile * C + tid];
-        }
-        float* mc = A.m_chunk + (tile * A.dvp + n0) * DKP;
-        for (int i = tid; i < NS * DKP / 4; i += 128) {
-            const int r = i / (DKP / 4), cc = (i - r * (DKP / 4)) * 4;
-            *reinterpret_cast<float4*>(mc + (long long)r * DKP + cc) = *reinterpret_cast<const float4*>(Ms + r * LK + cc);
-        }
-        __syncthreads();
-        float acc[NT][4];
-        zero(acc);
-        gemm16<NT, false, false, Pl<T>::in, TWO>(acc, Ks + 16 * w * LK, LK, Ms, LK, 0, DKP);
 #pragma unroll
         for (int n = 0; n < NT; n++)
 #pragma unroll
             for (int r = 0; r < 2; r++) {
-                const int i = 16 * w + g + 8 * r;
-                float2* rp = reinterpret_cast<float2*>(Rs + i * LN + 8 * n + 2 * t);
-                const float2 v = *rp;
-                *rp = make_float2(v.x - s_gate[i].z * acc[n][2 * r], v.y - s_gate[i].z * acc[n][2 * r + 1]);
+                const int row = 16 * rb + g + 8 * r, col = H * hf + 8 * n + 2 * t;
+                pv[n][r].load(vp + row * A.vt + col, row < ch.len && n0 + col < A.dv, row < ch.len && n0 + col + 1 < A.dv, vpair);
+            }
+    };
+    auto commit = [&](int buf) {
+        pk.store(Kb + buf * C * LK, LK);
+        pt.store(Ts, LD);
+        if (tid < C) { s_gate[buf][tid] = pg.g; s_w[buf][tid] = pg.g.w * pg.theta; }
+    };
+    if (count > 0) { fetch(0); commit(0); }
+    __syncthreads();
+    for (int c = 0; c < count; c++) {
+        const int buf = c & 1;
+        const long long tile = (long long)(slot0 + c) * A.hv + h;
+        const float* Ks = Kb + buf * C * LK;
+        Pair<T> v[NT][2];
+#pragma unroll
+        for (int n = 0; n < NT; n++)
+#pragma unroll
+            for (int r = 0; r < 2; r++) v[n][r] = pv[n][r];
+        float* mc = A.m_chunk + (tile * A.dvp + n0) * DKP;
+#pragma unroll
+        for (int m = 0; m < MT; m++)
+#pragma unroll
+            for (int n = 0; n < NT; n++)
+#pragma unroll
+                for (int i = 0; i < 4; i++)
+                    mc[(H * hf + 8 * n + 2 * t + (i & 1)) * DKP + 64 * m + 16 * rb + g + 8 * (i >> 1)] = S[m][n][i];
+        if (c + 1 < count) fetch(c + 1);
+        float acc[NT][4];
+        zero(acc);
+        gemm16s<NT, false, false, Pl<T>::in>(acc, Ks + 16 * rb * LK, LK, Ms + H * hf * LK, LK, 0, DKP);
+#pragma unroll
+        for (int n = 0; n < NT; n++)
+#pragma unroll
+            for (int r = 0; r < 2; r++) {
+                const int row = 16 * rb + g + 8 * r;
+                const float2 x = v[n][r].get();
+                float2* o = Rs + row * LS + H * hf + 8 * n + 2 * t;
+                o[0] = split_pair(x.x - s_gate[buf][row].z * acc[n][2 * r]);
+                o[1] = split_pair(x.y - s_gate[buf][row].z * acc[n][2 * r + 1]);
             }
         __syncthreads();
         zero(acc);
-        gemm16<NT, false, true, TWO, TWO>(acc, Ts + 16 * w * LD, LD, Rs, LN, 0, 16 * (w + 1));
+        gemm16s<NT, false, true, TWO>(acc, Ts + 16 * rb * LD, LD, Rs + H * hf, LS, 0, 16 * (rb + 1));
         float* ep = A.e + tile * C * A.dvp + n0;
 #pragma unroll
         for (int n = 0; n < NT; n++)
 #pragma unroll
             for (int r = 0; r < 2; r++) {
-                const int i = 16 * w + g + 8 * r, col = 8 * n + 2 * t;
-                st2(ep + (long long)i * A.dvp + col, acc[n][2 * r], acc[n][2 * r + 1]);
-                st2(Us + i * LN + col, s_w[i] * acc[n][2 * r], s_w[i] * acc[n][2 * r + 1]);
+                const int row = 16 * rb + g + 8 * r, col = H * hf + 8 * n + 2 * t;
+                const float a = acc[n][2 * r], b = acc[n][2 * r + 1], wt = s_w[buf][row];
+                st2(ep + (long long)row * A.dvp + col, a, b);
+                Us[row * LS + col] = split_pair(wt * a);
+                Us[row * LS + col + 1] = split_pair(wt * b);
             }
         __syncthreads();
-        const float gl = s_gate[C - 1].z;
+        const float gl = s_gate[buf][C - 1].z;
 #pragma unroll
         for (int m = 0; m < MT; m++) {
 #pragma unroll
             for (int n = 0; n < NT; n++)
 #pragma unroll
                 for (int i = 0; i < 4; i++) S[m][n][i] *= gl;
-            gemm16<NT, true, true, Pl<T>::in, TWO>(S[m], Ks + 64 * m + 16 * w, LK, Us, LN, 0, C);
+            gemm16s<NT, true, true, Pl<T>::in>(S[m], Ks + 64 * m + 16 * rb, LK, Us + H * hf, LS, 0, C);
 #pragma unroll
             for (int n = 0; n < NT; n++)
 #pragma unroll
                 for (int i = 0; i < 4; i++)
-                    Ms[(8 * n + 2 * t + (i & 1)) * LK + 64 * m + 16 * w + g + 8 * (i >> 1)] = S[m][n][i];
+                    Ms[(H * hf + 8 * n + 2 * t + (i & 1)) * LK + 64 * m + 16 * rb + g + 8 * (i >> 1)] = split_pair(S[m][n][i]);
         }
+        if (c + 1 < count) commit(buf ^ 1);
         __syncthreads();
     }
     float* mf = A.m_final + ((long long)seq * A.hv + h) * A.dv * A.dk;
-    for (int i = tid; i < NS * A.dk; i += 128) {
-        const int r = i / A.dk, cc = i - r * A.dk;
-        if (n0 + r < A.dv) mf[(long long)(n0 + r) * A.dk + cc] = Ms[r * LK + cc];
-    }
+#pragma unroll
+    for (int m = 0; m < MT; m++)
+#pragma unroll
+        for (int n = 0; n < NT; n++)
+#pragma unroll
+            for (int i = 0; i < 4; i++) {
+                const int row = 64 * m + 16 * rb + g + 8 * (i >> 1), col = n0 + H * hf + 8 * n + 2 * t + (i & 1);
+                if (row < A.dk && col < A.dv) mf[(long long)col * A.dk + row] = S[m][n][i];
+            }
 }
 
 // Row-major store of a 16 x 32 accumulator block into a contiguous [row, heads, d] output.
@@ -384,13 +428,13 @@ __global__ void __launch_bounds__(256) gd_out_fwd_kernel(Args A)
     store_rows<T>(out, y, 16 * rb, ch.len, n0 + 32 * hf, A.dv, (long long)A.hv * A.dv);
 }
 
-// ── backward, what needs no state gradient: F = P^T dY ──
+// ── backward, what needs no state gradient: F = P^T dY, and N = scale (e^G Q)^T dY into the place of D ──
 template <typename T>
 __global__ void __launch_bounds__(256) gd_pre_bwd_kernel(Args A)
 {
     extern __shared__ float4 smem4[];
     float* Qs = reinterpret_cast<float*>(smem4);
-    float *Ks = Qs + C * LD, *Ys = Ks + C * LD;
+    float *Ks = Qs + C * LD, *Ys = Ks + C * LD, *Yg = Ys + C * LD;
     __shared__ float4 s_gate[C];
     const int slot = blockIdx.x / A.hv, h = blockIdx.x - slot * A.hv, n0 = blockIdx.y * 64;
     const Chunk ch = get_chunk(A, slot);
@@ -402,6 +446,8 @@ __global__ void __launch_bounds__(256) gd_pre_bwd_kernel(Args A)
     const T* qp = (const T*)A.q + ch.b * A.qb + ch.t0 * A.qt + (h / A.share) * A.qh;
     constexpr int IN = Pl<T>::in;
     load_tile<T, 64, 256>(Ys, LD, (const T*)A.dy + ch.b * A.yb + ch.t0 * A.yt + h * A.yh + n0, A.yt, ch.len, A.dv - n0);
+    __syncthreads();
+    for (int i = tid; i < C * C; i += 256) Yg[(i >> 6) * LD + (i & 63)] = A.scale * s_gate[i >> 6].z * Ys[(i >> 6) * LD + (i & 63)];
     float att[4][4];                              // rows: j, columns: i >= j
     zero(att);
     const bool need = 32 * hf + 31 >= 16 * rb;
@@ -411,6 +457,15 @@ __global__ void __launch_bounds__(256) gd_pre_bwd_kernel(Args A)
         load_tile<T, 64, 256>(Ks, LD, kp + c0, A.kt, ch.len, A.dk - c0);
         __syncthreads();
         if (need) gemm16<4, false, false, IN, IN>(att, Ks + 16 * rb * LD, LD, Qs + 32 * hf * LD, LD, 0, 64);
+        float nn[4][4];                           // rows: dv, columns: dk
+        zero(nn);
+        gemm16<4, true, true, TWO, IN>(nn, Yg + 16 * rb, LD, Qs + 32 * hf, LD, 0, C);
+        float* np = A.d_chunk + (tile * A.dvp + n0) * A.dkp + c0 + 32 * hf;
+#pragma unroll
+        for (int n = 0; n < 4; n++)
+#pragma unroll
+            for (int r = 0; r < 2; r++)
+                st2(np + (16 * rb + g + 8 * r) * A.dkp + 8 * n + 2 * t, nn[n][2 * r], nn[n][2 * r + 1]);
     }
     __syncthreads();
     float* Ps = Ks;                               // [i][j]
@@ -434,19 +489,22 @@ __global__ void __launch_bounds__(256) gd_pre_bwd_kernel(Args A)
             st2(fp + (long long)(16 * rb + g + 8 * r) * A.dvp + 8 * n + 2 * t, f[n][2 * r], f[n][2 * r + 1]);
 }
 
-// ── backward states: the gradient of the state behind each chunk, last chunk first ──
+// ── backward states: the gradient D of the state behind each chunk, last chunk first ──
+//   F = P^T dY + e^{G_L - G} K D,  X = T^T (theta F),  D <- e^{G_L} D + N - (e^G K)^T X,  N = scale (e^G Q)^T dY.
+// The forward kernel's structure. N is in D's place in d_chunk when a chunk is reached, and is read a chunk ahead.
 template <typename T, int DKP, int NS>
-__global__ void __launch_bounds__(128) gd_state_bwd_kernel(Args A)
+__global__ void __launch_bounds__(256, DKP == 64 ? 2 : 1) gd_state_bwd_kernel(Args A)
 {
-    constexpr int LK = DKP + 4, LN = NS + 4, NT = NS / 8, MT = DKP / 64;
+    constexpr int LK = DKP + 4, LS = NS + 2, MT = DKP / 64, NT = NS / 16, H = NS / 2;
     extern __shared__ float4 smem4[];
-    float* Ks = reinterpret_cast<float*>(smem4);
-    float *Qs = Ks + C * LK, *Ts = Qs + C * LK, *Ds = Ts + C * LD;
-    float *Rs = Ds + NS * LK, *Us = Rs + C * LN, *Ys = Us + C * LN;
-    __shared__ float4 s_gate[C];
-    __shared__ float s_theta[C];
+    float* Kb = reinterpret_cast<float*>(smem4);
+    float* Ts = Kb + 2 * C * LK;
+    float2* Ds = reinterpret_cast<float2*>(Ts + C * LD);
+    float2 *Rs = Ds + NS * LK, *Us = Rs + C * LS;
+    __shared__ float4 s_gate[2][C];
+    __shared__ float s_theta[2][C];
     const int nsl = A.dvp / NS, sl = blockIdx.x % nsl, p = blockIdx.x / nsl, h = p % A.hv, seq = p / A.hv;
-    const int n0 = sl * NS, tid = threadIdx.x, lane = tid & 31, w = tid >> 5, g = lane >> 2, t = lane & 3;
+    const int n0 = sl * NS, tid = threadIdx.x, lane = tid & 31, w = tid >> 5, rb = w & 3, hf = w >> 2, g = lane >> 2, t = lane & 3;
     const int slot0 = first_slot(A, seq), count = chunk_count(A, seq);
 
     float S[MT][NT][4];
@@ -457,92 +515,125 @@ __global__ void __launch_bounds__(128) gd_state_bwd_kernel(Args A)
         for (int n = 0; n < NT; n++)
 #pragma unroll
             for (int i = 0; i < 4; i++) {
-                const int row = 64 * m + 16 * w + g + 8 * (i >> 1), col = n0 + 8 * n + 2 * t + (i & 1);
-                S[m][n][i] = dm && row < A.dk && col < A.dv ? dm[(long long)col * A.dk + row] : 0.f;
-                Ds[(col - n0) * LK + row] = S[m][n][i];
+                const int row = 64 * m + 16 * rb + g + 8 * (i >> 1), col = H * hf + 8 * n + 2 * t + (i & 1);
+                S[m][n][i] = dm && row < A.dk && n0 + col < A.dv ? dm[(long long)(n0 + col) * A.dk + row] : 0.f;
+                Ds[col * LK + row] = split_pair(S[m][n][i]);
             }
-    __syncthreads();
-    for (int c = count - 1; c >= 0; c--) {
+    Prefetch<T, DKP, 256> pk;
+    Prefetch<float, 64, 256> pt;
+    GateRow pg;
+    float pf[NT][4], pn[MT][NT][4];
+    auto fetch = [&](int c) {
         const int slot = slot0 + c;
         const Chunk ch = get_chunk(A, slot);
         const long long tile = (long long)slot * A.hv + h;
-        const T* kp = (const T*)A.k + ch.b * A.kb + ch.t0 * A.kt + (h / A.share) * A.kh;
-        const T* qp = (const T*)A.q + ch.b * A.qb + ch.t0 * A.qt + (h / A.share) * A.qh;
-        const T* yp = (const T*)A.dy + ch.b * A.yb + ch.t0 * A.yt + h * A.yh + n0;
-#pragma unroll
-        for (int m = 0; m < MT; m++) {
-            load_tile<T, 64, 128>(Ks + 64 * m, LK, kp + 64 * m, A.kt, ch.len, A.dk - 64 * m);
-            load_tile<T, 64, 128>(Qs + 64 * m, LK, qp + 64 * m, A.qt, ch.len, A.dk - 64 * m);
-        }
-        load_own<64, 64, 128>(Ts, LD, A.tmat + tile * C * C, C);
-        load_own<64, NS, 128>(Rs, LN, A.f + tile * C * A.dvp + n0, A.dvp);
-        load_tile<T, NS, 128>(Ys, LN, yp, A.yt, ch.len, A.dv - n0);
-        if (tid < C) { s_gate[tid] = A.gates[tile * C + tid]; s_theta[tid] = A.theta_eff[tile * C + tid]; }
-        float* dc = A.d_chunk + (tile * A.dvp + n0) * DKP;
-        for (int i = tid; i < NS * DKP / 4; i += 128) {
-            const int r = i / (DKP / 4), cc = (i - r * (DKP / 4)) * 4;
-            *reinterpret_cast<float4*>(dc + (long long)r * DKP + cc) = *reinterpret_cast<const float4*>(Ds + r * LK + cc);
-        }
-        __syncthreads();
-        float acc[NT][4];
-        zero(acc);
-        gemm16<NT, false, false, Pl<T>::in, TWO>(acc, Ks + 16 * w * LK, LK, Ds, LK, 0, DKP);
+        pk.load((const T*)A.k + ch.b * A.kb + ch.t0 * A.kt + (h / A.share) * A.kh, A.kt, ch.len, A.dk);
+        pt.load(A.tmat + tile * C * C, C, C, C);
+        if (tid < C) { ldg(pg.g, reinterpret_cast<const float*>(A.gates + tile * C + tid)); ldg(pg.theta, A.theta_eff + tile * C + tid); }
+        const float* fp = A.f + tile * C * A.dvp + n0;
+        const float* np = A.d_chunk + (tile * A.dvp + n0) * DKP;
 #pragma unroll
         for (int n = 0; n < NT; n++)
 #pragma unroll
-            for (int r = 0; r < 2; r++) {
-                const int i = 16 * w + g + 8 * r;
-                float2* rp = reinterpret_cast<float2*>(Rs + i * LN + 8 * n + 2 * t);
-                const float2 f = *rp;
-                const float wi = s_gate[i].w, th = s_theta[i];
-                *rp = make_float2(th * (f.x + wi * acc[n][2 * r]), th * (f.y + wi * acc[n][2 * r + 1]));
+            for (int i = 0; i < 4; i++) {
+                const int row = 16 * rb + g + 8 * (i >> 1), col = H * hf + 8 * n + 2 * t + (i & 1);
+                if (!(i & 1)) {
+                    float2 x;
+                    ldg(x, fp + (long long)row * A.dvp + col);
+                    pf[n][i] = x.x;
+                    pf[n][i + 1] = x.y;
+                }
+#pragma unroll
+                for (int m = 0; m < MT; m++) ldg(pn[m][n][i], np + col * DKP + 64 * m + row);
+            }
+    };
+    auto commit = [&](int buf) {
+        pk.store(Kb + buf * C * LK, LK);
+        pt.store(Ts, LD);
+        if (tid < C) { s_gate[buf][tid] = pg.g; s_theta[buf][tid] = pg.theta; }
+    };
+    if (count > 0) { fetch(count - 1); commit(0); }
+    __syncthreads();
+    for (int c = count - 1; c >= 0; c--) {
+        const int buf = (count - 1 - c) & 1, slot = slot0 + c;
+        const Chunk ch = get_chunk(A, slot);
+        const long long tile = (long long)slot * A.hv + h;
+        const float* Ks = Kb + buf * C * LK;
+        float f[NT][4], nn[MT][NT][4];
+        float* dc = A.d_chunk + (tile * A.dvp + n0) * DKP;
+#pragma unroll
+        for (int n = 0; n < NT; n++)
+#pragma unroll
+            for (int i = 0; i < 4; i++) {
+                f[n][i] = pf[n][i];
+#pragma unroll
+                for (int m = 0; m < MT; m++) {
+                    nn[m][n][i] = pn[m][n][i];
+                    dc[(H * hf + 8 * n + 2 * t + (i & 1)) * DKP + 64 * m + 16 * rb + g + 8 * (i >> 1)] = S[m][n][i];
+                }
+            }
+        if (c > 0) fetch(c - 1);
+        float acc[NT][4];
+        zero(acc);
+        gemm16s<NT, false, false, Pl<T>::in>(acc, Ks + 16 * rb * LK, LK, Ds + H * hf * LK, LK, 0, DKP);
+#pragma unroll
+        for (int n = 0; n < NT; n++)
+#pragma unroll
+            for (int i = 0; i < 4; i++) {
+                const int row = 16 * rb + g + 8 * (i >> 1);
+                Rs[row * LS + H * hf + 8 * n + 2 * t + (i & 1)] =
+                    split_pair(s_theta[buf][row] * (f[n][i] + s_gate[buf][row].w * acc[n][i]));
             }
         __syncthreads();
         zero(acc);
-        gemm16<NT, true, true, TWO, TWO>(acc, Ts + 16 * w, LD, Rs, LN, 16 * w, C);
+        gemm16s<NT, true, true, TWO>(acc, Ts + 16 * rb, LD, Rs + H * hf, LS, 16 * rb, C);
         float* xp = A.x + tile * C * A.dvp + n0;
-        T* dv = (T*)A.d_v + (ch.row0(A) * A.hv + h) * A.dv;
+        T* dv = (T*)A.d_v + (ch.row0(A) * A.hv + h) * A.dv + n0;
 #pragma unroll
         for (int n = 0; n < NT; n++)
 #pragma unroll
             for (int r = 0; r < 2; r++) {
-                const int i = 16 * w + g + 8 * r, col = 8 * n + 2 * t;
-                const float a = acc[n][2 * r], b = acc[n][2 * r + 1], eg = -s_gate[i].z, ys = -eg * A.scale;
-                st2(xp + (long long)i * A.dvp + col, a, b);
-                st2(Us + i * LN + col, eg * a, eg * b);
-                float2* y = reinterpret_cast<float2*>(Ys + i * LN + col);
-                *y = make_float2(ys * y->x, ys * y->y);
-                if (i < ch.len) {
-                    const bool none = fabsf(s_theta[i]) <= THETA_TINY;     // theta was 0: so is the gradient of v
-                    T* o = dv + (long long)i * A.hv * A.dv + n0 + col;
+                const int row = 16 * rb + g + 8 * r, col = H * hf + 8 * n + 2 * t;
+                const float a = acc[n][2 * r], b = acc[n][2 * r + 1], eg = -s_gate[buf][row].z;
+                st2(xp + (long long)row * A.dvp + col, a, b);
+                Us[row * LS + col] = split_pair(eg * a);
+                Us[row * LS + col + 1] = split_pair(eg * b);
+                if (row < ch.len) {
+                    const bool none = fabsf(s_theta[buf][row]) <= THETA_TINY;     // theta was 0: so is the gradient of v
+                    T* o = dv + (long long)row * A.hv * A.dv + col;
                     if (n0 + col < A.dv) o[0] = from_f<T>(none ? 0.f : a);
                     if (n0 + col + 1 < A.dv) o[1] = from_f<T>(none ? 0.f : b);
                 }
             }
         __syncthreads();
-        const float gl = s_gate[C - 1].z;
+        const float gl = s_gate[buf][C - 1].z;
 #pragma unroll
         for (int m = 0; m < MT; m++) {
 #pragma unroll
             for (int n = 0; n < NT; n++)
 #pragma unroll
-                for (int i = 0; i < 4; i++) S[m][n][i] *= gl;
-            gemm16<NT, true, true, Pl<T>::in, TWO>(S[m], Ks + 64 * m + 16 * w, LK, Us, LN, 0, C);
-            gemm16<NT, true, true, Pl<T>::in, TWO>(S[m], Qs + 64 * m + 16 * w, LK, Ys, LN, 0, C);
+                for (int i = 0; i < 4; i++) S[m][n][i] = fmaf(gl, S[m][n][i], nn[m][n][i]);
+            gemm16s<NT, true, true, Pl<T>::in>(S[m], Ks + 64 * m + 16 * rb, LK, Us + H * hf, LS, 0, C);
 #pragma unroll
             for (int n = 0; n < NT; n++)
 #pragma unroll
                 for (int i = 0; i < 4; i++)
-                    Ds[(8 * n + 2 * t + (i & 1)) * LK + 64 * m + 16 * w + g + 8 * (i >> 1)] = S[m][n][i];
+                    Ds[(H * hf + 8 * n + 2 * t + (i & 1)) * LK + 64 * m + 16 * rb + g + 8 * (i >> 1)] = split_pair(S[m][n][i]);
         }
+        if (c > 0) commit(buf ^ 1);
         __syncthreads();
     }
     if (A.d_m0) {
         float* o = A.d_m0 + ((long long)seq * A.hv + h) * A.dv * A.dk;
-        for (int i = tid; i < NS * A.dk; i += 128) {
-            const int r = i / A.dk, cc = i - r * A.dk;
-            if (n0 + r < A.dv) o[(long long)(n0 + r) * A.dk + cc] = Ds[r * LK + cc];
-        }
+#pragma unroll
+        for (int m = 0; m < MT; m++)
+#pragma unroll
+            for (int n = 0; n < NT; n++)
+#pragma unroll
+                for (int i = 0; i < 4; i++) {
+                    const int row = 64 * m + 16 * rb + g + 8 * (i >> 1), col = n0 + H * hf + 8 * n + 2 * t + (i & 1);
+                    if (row < A.dk && col < A.dv) o[(long long)col * A.dk + row] = S[m][n][i];
+                }
     }
 }
 
@@ -736,13 +827,24 @@ __global__ void __launch_bounds__(256) gd_step_kernel(Args A, float* M, const in
     const int per = (A.dv + rows - 1) / rows;
     const int part = blockIdx.x % per, p = blockIdx.x / per, h = p % A.hv, first = p / A.hv;
     const int lane8 = threadIdx.x & 7, grp = threadIdx.x >> 3;
-    int slot = first;
+    int slot = first, last = first + 1;                   // sequences first .. last - 1 may be of this slot
     if (slots) {
         slot = slots[first];
-        if (slot < 0 || slot >= pool) return;             // no sequence in this place
-        int seen = 0;
-        for (int i = threadIdx.x; i < first; i += 256) seen |= slots[i] == slot;
+        if (slot < 0 || slot >= pool) {                   // no sequence in this place
+            for (int i = threadIdx.x; i < A.seq * rows; i += 256) {
+                const int tok = i / rows, row = part * rows + i - tok * rows;
+                if (row < A.dv) ((T*)A.y)[(((long long)first * A.seq + tok) * A.hv + h) * A.dv + row] = from_f<T>(0.f);
+            }
+            return;
+        }
+        bool seen = false, again = false;
+        for (int i = threadIdx.x; i < A.batch; i += 256) {
+            const bool same = slots[i] == slot;
+            seen |= same && i < first;
+            again |= same && i > first;
+        }
         if (__syncthreads_or(seen)) return;
+        if (__syncthreads_or(again)) last = A.batch;
     }
     constexpr int RP = 4;                                 // rows a thread holds at a time
     for (int r0 = part * rows; r0 < min(A.dv, (part + 1) * rows); r0 += 32 * RP) {
@@ -769,8 +871,8 @@ __global__ void __launch_bounds__(256) gd_step_kernel(Args A, float* M, const in
                 m[r][v] = x;
             }
         }
-        for (int b = first; b < A.batch; b++) {
-            if (b != first && (!slots || slots[b] != slot)) { if (!slots) break; continue; }
+        for (int b = first; b < last; b++) {
+            if (b != first && slots[b] != slot) continue;
             for (int tok = 0; tok < A.seq; tok++) {
                 const T* kp = (const T*)A.k + b * A.kb + tok * A.kt + (h / A.share) * A.kh;
                 const T* qp = (const T*)A.q + b * A.qb + tok * A.qt + (h / A.share) * A.qh;
@@ -910,26 +1012,28 @@ template <typename K> static bool allow_smem(K kernel, int bytes, const char* wh
 }
 
 constexpr int TILE_BYTES = C * LD * 4;
-constexpr int state_fwd_smem(int dkp, int ns) { return 4 * (C * (dkp + 4) + C * LD + ns * (dkp + 4) + 2 * C * (ns + 4)); }
-constexpr int state_bwd_smem(int dkp, int ns) { return 4 * (2 * C * (dkp + 4) + C * LD + ns * (dkp + 4) + 3 * C * (ns + 4)); }
 
-template <typename T, int DKP>
-static bool launch_states(const Args& A, bool backward, cudaStream_t st, const char* where)
+template <typename T, int DKP, int NS>
+static bool launch_states_ns(const Args& A, long long heads, bool backward, cudaStream_t st, const char* where)
 {
-    const int seqs = A.n_seqs > 0 ? A.n_seqs : A.batch;
-    const long long grid = (long long)seqs * A.hv * (A.dvp / 32);
-    if (grid == 0) return true;
+    const long long grid = heads * (A.dvp / NS);
     if (grid >= (1LL << 31)) { record_status(NLH_ERR_INVALID_ARG, where, "too many sequences"); return false; }
+    constexpr int bytes = StateSmem<DKP, NS>::BYTES;
     if (backward) {
-        constexpr int bytes = state_bwd_smem(DKP, 32);
-        if (!allow_smem(gd_state_bwd_kernel<T, DKP, 32>, bytes, where)) return false;
-        gd_state_bwd_kernel<T, DKP, 32><<<(unsigned)grid, 128, bytes, st>>>(A);
+        if (!allow_smem(gd_state_bwd_kernel<T, DKP, NS>, bytes, where)) return false;
+        gd_state_bwd_kernel<T, DKP, NS><<<(unsigned)grid, 256, bytes, st>>>(A);
     } else {
-        constexpr int bytes = state_fwd_smem(DKP, 32);
-        if (!allow_smem(gd_state_fwd_kernel<T, DKP, 32>, bytes, where)) return false;
-        gd_state_fwd_kernel<T, DKP, 32><<<(unsigned)grid, 128, bytes, st>>>(A);
+        if (!allow_smem(gd_state_fwd_kernel<T, DKP, NS>, bytes, where)) return false;
+        gd_state_fwd_kernel<T, DKP, NS><<<(unsigned)grid, 256, bytes, st>>>(A);
     }
     return check_launch(where);
+}
+template <typename T, int DKP> static bool launch_states(const Args& A, bool backward, cudaStream_t st, const char* where)
+{
+    const long long heads = (long long)(A.n_seqs > 0 ? A.n_seqs : A.batch) * A.hv;
+    if (heads == 0) return true;
+    if (heads * (A.dvp / 32) < 2 * 148) return launch_states_ns<T, DKP, 16>(A, heads, backward, st, where);
+    return launch_states_ns<T, DKP, 32>(A, heads, backward, st, where);
 }
 
 template <typename T> static bool run_forward(Args& A, cudaStream_t st, const char* where)
@@ -957,8 +1061,8 @@ template <typename T> static bool run_backward(Args& A, cudaStream_t st, const c
 {
     const unsigned tiles = (unsigned)((long long)A.slots * A.hv);
     if (tiles) {
-        if (!allow_smem(gd_pre_bwd_kernel<T>, 3 * TILE_BYTES, where)) return false;
-        gd_pre_bwd_kernel<T><<<dim3(tiles, A.dvp / 64), 256, 3 * TILE_BYTES, st>>>(A);
+        if (!allow_smem(gd_pre_bwd_kernel<T>, 4 * TILE_BYTES, where)) return false;
+        gd_pre_bwd_kernel<T><<<dim3(tiles, A.dvp / 64), 256, 4 * TILE_BYTES, st>>>(A);
         if (!check_launch(where)) return false;
     }
     if (!(A.dkp == 64 ? launch_states<T, 64>(A, true, st, where) : launch_states<T, 128>(A, true, st, where))) return false;

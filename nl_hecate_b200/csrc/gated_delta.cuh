@@ -213,6 +213,142 @@ __device__ __forceinline__ void gemm16(float (&acc)[NT][4], const float* A, int 
         }
     }
 }
+// The same with B split beforehand into pairs (hi, lo): a matrix that several warps read is split once, by who writes it.
+// B[n][k] rows are 4 (mod 16) pairs apart, B[k][n] rows 2 (mod 8), for 8-byte reads without bank conflicts.
+template <int NT, bool AK, bool BK, int PA>
+__device__ __forceinline__ void gemm16s(float (&acc)[NT][4], const float* A, int lda, const float2* B, int ldb, int k0, int k1)
+{
+    const int lane = threadIdx.x & 31, g = lane >> 2, t = lane & 3;
+    constexpr bool PAIR = AK || BK;
+#pragma unroll 4
+    for (int k = k0; k < k1; k += 8) {
+        float af[4];
+        if (AK) {
+            const float* p = A + (k + 2 * t) * lda + g;
+            af[0] = p[0]; af[1] = p[8]; af[2] = p[lda]; af[3] = p[lda + 8];
+        } else if (PAIR) {
+            const float2 x = *reinterpret_cast<const float2*>(A + g * lda + k + 2 * t);
+            const float2 y = *reinterpret_cast<const float2*>(A + (g + 8) * lda + k + 2 * t);
+            af[0] = x.x; af[2] = x.y; af[1] = y.x; af[3] = y.y;
+        } else {
+            const float* p = A + g * lda + k + t;
+            af[0] = p[0]; af[1] = p[8 * lda]; af[2] = p[4]; af[3] = p[8 * lda + 4];
+        }
+        unsigned ah[4], al[4];
+#pragma unroll
+        for (int i = 0; i < 4; i++) split<PA>(af[i], ah[i], al[i]);
+#pragma unroll
+        for (int n = 0; n < NT; n++) {
+            float2 b0, b1;
+            if (BK) {
+                const float2* p = B + (k + 2 * t) * ldb + n * 8 + g;
+                b0 = p[0]; b1 = p[ldb];
+            } else if (PAIR) {
+                const float2* p = B + (n * 8 + g) * ldb + k + 2 * t;
+                b0 = p[0]; b1 = p[1];
+            } else {
+                const float2* p = B + (n * 8 + g) * ldb + k + t;
+                b0 = p[0]; b1 = p[4];
+            }
+            float s[4] = {0.f, 0.f, 0.f, 0.f};
+            if (PA == TWO) mma_tf32(s, al, __float_as_uint(b0.x), __float_as_uint(b1.x));
+            mma_tf32(s, ah, __float_as_uint(b0.y), __float_as_uint(b1.y));
+            mma_tf32(s, ah, __float_as_uint(b0.x), __float_as_uint(b1.x));
+#pragma unroll
+            for (int i = 0; i < 4; i++) acc[n][i] += s[i];
+        }
+    }
+}
+__device__ __forceinline__ float2 split_pair(float x)
+{
+    const float h = round_tf32(x);
+    return make_float2(h, __fsub_rn(x, h));
+}
+
+// A tile on its way from global to shared memory, in registers: loaded while the chunk before it is computed. Rows that do
+// not allow vector loads are read when they are stored instead.
+template <typename T> struct Raw { typedef float4 type; };
+template <> struct Raw<__nv_bfloat16> { typedef uint2 type; };
+__device__ __forceinline__ float4 widen(float4 v) { return v; }
+__device__ __forceinline__ float4 widen(uint2 u)
+{
+    const float2 a = __bfloat1622float2(*reinterpret_cast<const __nv_bfloat162*>(&u.x));
+    const float2 b = __bfloat1622float2(*reinterpret_cast<const __nv_bfloat162*>(&u.y));
+    return make_float4(a.x, a.y, b.x, b.y);
+}
+// Loads that stay where they are written: left to itself the compiler moves them down to their first use.
+__device__ __forceinline__ void ldg(float4& v, const float* p)
+{
+    asm volatile("ld.global.v4.f32 {%0, %1, %2, %3}, [%4];\n" : "=f"(v.x), "=f"(v.y), "=f"(v.z), "=f"(v.w) : "l"(p));
+}
+__device__ __forceinline__ void ldg(uint2& v, const __nv_bfloat16* p)
+{
+    asm volatile("ld.global.v2.u32 {%0, %1}, [%2];\n" : "=r"(v.x), "=r"(v.y) : "l"(p));
+}
+__device__ __forceinline__ void ldg(float& v, const float* p) { asm volatile("ld.global.f32 %0, [%1];\n" : "=f"(v) : "l"(p)); }
+__device__ __forceinline__ void ldg(float2& v, const float* p)
+{
+    asm volatile("ld.global.v2.f32 {%0, %1}, [%2];\n" : "=f"(v.x), "=f"(v.y) : "l"(p));
+}
+__device__ __forceinline__ void ldg(unsigned& v, const __nv_bfloat16* p) { asm volatile("ld.global.u32 %0, [%1];\n" : "=r"(v) : "l"(p)); }
+
+// Two neighbouring columns of a strided matrix, as they came; `pair` says that one load may take both.
+template <typename T> struct Pair;
+template <> struct Pair<float> {
+    float2 r;
+    __device__ __forceinline__ void load(const float* p, bool a, bool b, bool pair)
+    {
+        r = make_float2(0.f, 0.f);
+        if (pair) { if (a) ldg(r, p); }
+        else { if (a) r.x = p[0]; if (b) r.y = p[1]; }
+    }
+    __device__ __forceinline__ float2 get() const { return r; }
+};
+template <> struct Pair<__nv_bfloat16> {
+    unsigned r;
+    __device__ __forceinline__ void load(const __nv_bfloat16* p, bool a, bool b, bool pair)
+    {
+        r = 0;
+        if (pair) { if (a) ldg(r, p); }
+        else {
+            const unsigned short *u = reinterpret_cast<const unsigned short*>(p);
+            r = (a ? (unsigned)u[0] : 0u) | (b ? (unsigned)u[1] << 16 : 0u);
+        }
+    }
+    __device__ __forceinline__ float2 get() const { return make_float2(__uint_as_float(r << 16), __uint_as_float(r & 0xffff0000u)); }
+};
+
+template <typename T, int COLS, int THREADS> struct Prefetch {
+    typedef typename Raw<T>::type R;
+    static constexpr int PER_ROW = COLS / 4, N = C * PER_ROW / THREADS;
+    R r[N];
+    const T* base;
+    long long stride;
+    int rows, cols;
+    bool vec;
+    __device__ __forceinline__ void load(const T* b, long long st, int nr, int nc)
+    {
+        base = b; stride = st; rows = nr; cols = nc;
+        vec = ((reinterpret_cast<uintptr_t>(b) | (uintptr_t)(st * (long long)sizeof(T))) & (4 * sizeof(T) - 1)) == 0 && (nc & 3) == 0;
+        if (!vec) return;
+#pragma unroll
+        for (int i = 0; i < N; i++) {
+            const int at = threadIdx.x + i * THREADS, row = at / PER_ROW, c = (at - row * PER_ROW) * 4;
+            r[i] = R{};
+            if (row < rows && c < cols) ldg(r[i], base + row * stride + c);
+        }
+    }
+    __device__ __forceinline__ void store(float* dst, int ld) const
+    {
+        if (!vec) { load_tile<T, COLS, THREADS>(dst, ld, base, stride, rows, cols); return; }
+#pragma unroll
+        for (int i = 0; i < N; i++) {
+            const int at = threadIdx.x + i * THREADS, row = at / PER_ROW, c = (at - row * PER_ROW) * 4;
+            *reinterpret_cast<float4*>(dst + row * ld + c) = widen(r[i]);
+        }
+    }
+};
+
 template <int NT> __device__ __forceinline__ void zero(float (&acc)[NT][4])
 {
 #pragma unroll

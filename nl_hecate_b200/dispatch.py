@@ -498,7 +498,7 @@ def gated_delta_step(k, v, q, log_retain, theta, m, slots=None, scale=1.0):
     if slots is not None:
         _need(where, "slots", slots, torch.int32, (k.shape[0],))
     with _on_device(k):
-        y = (torch.empty if slots is None else torch.zeros)(v.shape, dtype=v.dtype, device=k.device)
+        y = torch.empty(v.shape, dtype=v.dtype, device=k.device)
         call("nlh_gated_delta_step", desc=C.byref(desc), k=k.data_ptr(), v=v.data_ptr(), q=q.data_ptr(),
              log_retain=log_retain.data_ptr(), theta=theta.data_ptr(), m=m, slots=slots, n_slots=m.shape[0], y=y)
     torch.autograd.graph.increment_version(m)    # written past autograd
