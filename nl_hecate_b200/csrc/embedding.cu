@@ -57,6 +57,23 @@ template <int N> __device__ __forceinline__ void load_f32(const float* p, float*
         f[i] = v.x; f[i + 1] = v.y; f[i + 2] = v.z; f[i + 3] = v.w;
     }
 }
+// One writer per row of d_w: a reduction without an answer, which no load waits for, has no other to race with.
+template <int N, bool ADD> __device__ __forceinline__ void add_row(float* p, const float* acc, float scale)
+{
+    if (!ADD) {
+        float o[N];
+#pragma unroll
+        for (int i = 0; i < N; i++) o[i] = scale * acc[i];
+        store_f32<N>(p, o);
+    } else if (N == 1) {
+        atomicAdd(p, scale * acc[0]);
+    } else {
+#pragma unroll
+        for (int i = 0; i < N; i += 4)
+            atomicAdd(reinterpret_cast<float4*>(p + i), make_float4(scale * acc[i], scale * acc[(i + 1) % N], scale * acc[(i + 2) % N],
+                                                                  scale * acc[(i + 3) % N]));
+    }
+}
 __device__ __forceinline__ void put(float* p, float x) { *p = x; }
 __device__ __forceinline__ void put(__nv_bfloat16* p, float x) { *p = __float2bfloat16(x); }
 
@@ -200,39 +217,42 @@ template <typename T, int N, bool ADD>
 __global__ void __launch_bounds__(THREADS) reduce_kernel(const T* __restrict__ dy, const int2* __restrict__ sorted, float* __restrict__ dw,
                                                          float* __restrict__ part, int n, int vocab, int d, int lanes, int run, float scale)
 {
-    const int per = THREADS / lanes, lane = threadIdx.x & (lanes - 1);
-    const int r = blockIdx.x * per + threadIdx.x / lanes, c = (blockIdx.y * lanes + lane) * N;
+    const int per = THREADS / lanes, lane = threadIdx.x & (lanes - 1), grp = threadIdx.x / lanes;
+    const int r = blockIdx.x * per + grp, c = (blockIdx.y * lanes + lane) * N;
+    extern __shared__ int2 s_all[];               // [per][run + 2]: the tokens of each run, the one before and the one behind
+    for (int i = threadIdx.x; i < per * (run + 2); i += THREADS) {
+        const int q = i / (run + 2);
+        const long long at = ((long long)blockIdx.x * per + q) * run + (i - q * (run + 2)) - 1;
+        s_all[i] = at >= 0 && at < n ? sorted[at] : make_int2(-1, 0);
+    }
+    __syncthreads();
+    const int2* mine = s_all + grp * (run + 2) + 1;
     const long long b = (long long)r * run;
     if (b >= n || c >= d) return;
-    const int e = (int)min((long long)n, b + run);
-    const int prev = b > 0 ? sorted[b - 1].x : -1, next = e < n ? sorted[e].x : -1;
+    const int e = (int)min((long long)run, n - b);
+    const int prev = mine[-1].x, next = mine[e].x;
     float acc[N];
 #pragma unroll
     for (int i = 0; i < N; i++) acc[i] = 0.f;
-    int cur = sorted[b].x;
+    int cur = mine[0].x;
     bool head = cur == prev;
     auto flush = [&](bool tail) {
         if (cur >= vocab) return;
         if (head || tail) {
             store_f32<N>(part + ((long long)r * 2 + (head ? 0 : 1)) * d + c, acc);
         } else {
-            float o[N];
-            float* p = dw + (long long)cur * d + c;
-            if (ADD) load_f32<N>(p, o);
-#pragma unroll
-            for (int i = 0; i < N; i++) o[i] = ADD ? fmaf(scale, acc[i], o[i]) : scale * acc[i];
-            store_f32<N>(p, o);
+            add_row<N, ADD>(dw + (long long)cur * d + c, acc, scale);
         }
     };
     constexpr int U = 8;
-    for (int i = (int)b; i < e; i += U) {
+    for (int i = 0; i < e; i += U) {
         float f[U][N];
         int key[U];
 #pragma unroll
         for (int u = 0; u < U; u++) {
             key[u] = vocab;
             if (i + u < e) {
-                const int2 s = sorted[i + u];
+                const int2 s = mine[i + u];
                 key[u] = s.x;
                 if (s.x < vocab) load<T, N>(dy + (long long)s.y * d + c, f[u]);
             }
@@ -255,43 +275,48 @@ __global__ void __launch_bounds__(THREADS) reduce_kernel(const T* __restrict__ d
     }
     flush(cur == next);
 }
-// Ids that cross runs: the run in which one begins adds its pieces up.
+// Ids that cross runs: the run in which one begins adds its pieces up. A CTA per run and 32 N columns; most have nothing to do.
+// Its eight warps look 256 runs ahead at once for the last one that begins with the id, take a stretch of the pieces each and
+// join their sums in order. (One warp walking the pieces of the most frequent id of a text of 32768 tokens took 51 us.)
 template <int N, bool ADD>
-__global__ void __launch_bounds__(THREADS) join_kernel(const int2* __restrict__ sorted, float* __restrict__ dw, const float* __restrict__ part,
-                                                       int n, int vocab, int d, int lanes, int run, float scale)
+__global__ void __launch_bounds__(256) join_kernel(const int2* __restrict__ sorted, float* __restrict__ dw, const float* __restrict__ part,
+                                                   int n, int vocab, int d, int run, float scale)
 {
-    const int per = THREADS / lanes, lane = threadIdx.x & (lanes - 1);
-    const int r = blockIdx.x * per + threadIdx.x / lanes, c = (blockIdx.y * lanes + lane) * N;
-    const long long b = (long long)r * run, e = b + run;
-    if (e >= n || c >= d) return;
+    __shared__ float s_acc[8][32 * N];
+    const int lane = threadIdx.x & 31, w = threadIdx.x >> 5, c = (blockIdx.y * 32 + lane) * N;
+    const long long r = blockIdx.x, b = r * run, e = b + run;
+    if (e >= n) return;
     const int key = sorted[e - 1].x;
     if (key >= vocab || sorted[e].x != key) return;                    // nothing goes on behind this run
     if (b > 0 && sorted[b].x == key && sorted[b - 1].x == key) return;  // it began before it
-    float acc[N];
-    load_f32<N>(part + ((long long)r * 2 + 1) * d + c, acc);
-    constexpr int U = 8;
-    for (long long q = r + 1; q * run < n; q += U) {
-        float f[U][N];
-        bool on[U];
-#pragma unroll
-        for (int u = 0; u < U; u++) {
-            on[u] = (q + u) * run < n && sorted[(q + u) * run].x == key;    // sorted: run q + u begins with the id or is behind it
-            if (on[u]) load_f32<N>(part + (q + u) * 2 * d + c, f[u]);
-        }
-#pragma unroll
-        for (int u = 0; u < U; u++)
-            if (on[u]) {
-#pragma unroll
-                for (int i = 0; i < N; i++) acc[i] += f[u][i];
-            }
-        if (!on[U - 1]) break;
+    long long pieces = 0;                                              // runs behind r that begin with the id
+    for (;;) {
+        const long long q = r + 1 + pieces + threadIdx.x;
+        const int more = __syncthreads_count(q * run < n && sorted[q * run].x == key);    // sorted: they are the first ones
+        pieces += more;
+        if (more < 256) break;
     }
-    float o[N];
-    float* p = dw + (long long)key * d + c;
-    if (ADD) load_f32<N>(p, o);
+    const long long each = (pieces + 8) / 8, i0 = w * each, i1 = min(pieces + 1, i0 + each);   // piece 0 is run r's own
+    float acc[N];
 #pragma unroll
-    for (int i = 0; i < N; i++) o[i] = ADD ? fmaf(scale, acc[i], o[i]) : scale * acc[i];
-    store_f32<N>(p, o);
+    for (int i = 0; i < N; i++) acc[i] = 0.f;
+    if (c < d) {
+#pragma unroll 8
+        for (long long i = i0; i < i1; i++) {
+            float f[N];
+            load_f32<N>(part + ((r + i) * 2 + (i == 0)) * d + c, f);
+#pragma unroll
+            for (int x = 0; x < N; x++) acc[x] += f[x];
+        }
+    }
+#pragma unroll
+    for (int i = 0; i < N; i++) s_acc[w][i * 32 + lane] = acc[i];
+    __syncthreads();
+    if (w != 0 || c >= d) return;
+    for (int j = 1; j < 8; j++)
+#pragma unroll
+        for (int i = 0; i < N; i++) acc[i] += s_acc[j][i * 32 + lane];
+    add_row<N, ADD>(dw + (long long)key * d + c, acc, scale);
 }
 
 // ── few tokens ──
@@ -346,14 +371,7 @@ __global__ void __launch_bounds__(THREADS) small_kernel(const T* __restrict__ dy
             }
             __syncthreads();
         }
-        if (grp == 0 && c < d) {
-            float o[N];
-            float* p = dw + (long long)id * d + c;
-            if (ADD) load_f32<N>(p, o);
-#pragma unroll
-            for (int i = 0; i < N; i++) o[i] = ADD ? fmaf(scale, acc[i], o[i]) : scale * acc[i];
-            store_f32<N>(p, o);
-        }
+        if (grp == 0 && c < d) add_row<N, ADD>(dw + (long long)id * d + c, acc, scale);
     }
 }
 
@@ -397,7 +415,7 @@ static bool backward(const T* dy, const int* ids, float* dw, int n, int vocab, i
     cudaStream_t st = current_stream();
     Plan P;
     place(P, ws, n, vocab, d);
-    const int lanes = lanes_for(d, N, THREADS);
+    const int lanes = max(4, lanes_for(d, N, THREADS));         // four at least: the tokens of all runs of a CTA fit 48 KB
     if (n <= SMALL) {
         small_kernel<T, N, ADD><<<n, THREADS, 0, st>>>(dy, ids, dw, n, vocab, d, lanes, scale);
         return check_launch(where);
@@ -420,9 +438,9 @@ static bool backward(const T* dy, const int* ids, float* dw, int n, int vocab, i
     }
     const int per = THREADS / lanes;
     const dim3 grid((P.runs + per - 1) / per, (d + lanes * N - 1) / (lanes * N));
-    reduce_kernel<T, N, ADD><<<grid, THREADS, 0, st>>>(dy, in, dw, P.part, n, vocab, d, lanes, P.run, scale);
+    reduce_kernel<T, N, ADD><<<grid, THREADS, per * (P.run + 2) * sizeof(int2), st>>>(dy, in, dw, P.part, n, vocab, d, lanes, P.run, scale);
     if (!check_launch(where)) return false;
-    join_kernel<N, ADD><<<grid, THREADS, 0, st>>>(in, dw, P.part, n, vocab, d, lanes, P.run, scale);
+    join_kernel<N, ADD><<<dim3(P.runs, (d + 32 * N - 1) / (32 * N)), 256, 0, st>>>(in, dw, P.part, n, vocab, d, P.run, scale);
     return check_launch(where);
 }
 
