@@ -17,7 +17,6 @@
 namespace nlh {
 namespace distill {
 
-constexpr int THREADS = 256;
 constexpr int MAX_K = 1024;
 constexpr float LOG2E = 1.4426950408889634f;
 
@@ -32,8 +31,8 @@ struct Args {
     float tau, hard_w, soft_w;
     bool hard, soft;                     // which terms exist
     // saved
-    float *lse_h, *lse_s, *ce, *kl;      // [n]
-    int* flags;                          // [n] bit 0: has a target, bit 1: has a teacher entry
+    float2* lse;                         // [n] log-sum-exp of z, of z / tau
+    float2* row;                         // [n] cross-entropy, divergence; -infinity (which neither can be) where a row has none
     float* stats;                        // {-, hard_weight / n_hard, soft_weight tau / n_soft, -}
     float* loss;
     float4* part;                        // [n, splits] {max, sum e^(z - max), sum e^((z - max) / tau), -}
@@ -89,28 +88,61 @@ __device__ __forceinline__ void add_one(float x, float cs, float ns, float ch, f
     if (MODE == SQUARE) h = fmaf(e, e, h);
     if (MODE == BOTH) h += ex2(fmaf(x, ch, nh));
 }
-template <int MODE, int N>
-__device__ __forceinline__ void add_block(Stat& a, const float* f, float cs, float ch)
+template <int MODE> __device__ __forceinline__ void raise(Stat& a, float m, float cs, float ch)
 {
-    float lm = f[0];
-#pragma unroll
-    for (int i = 1; i < N; i++) lm = fmaxf(lm, f[i]);
-    const float m = fmaxf(a.m, lm);
-    if (m == -CUDART_INF_F) {
-        // nothing but -infinity so far; a NaN, which fmaxf passes over, must not be lost
-#pragma unroll
-        for (int i = 0; i < N; i++) if (f[i] != f[i]) { a.h = f[i]; a.s = f[i]; }
-        return;
-    }
-    const float ns = -m * cs, nh = -m * ch;
     if (m > a.m) {
         a.s *= ex2((a.m - m) * cs);
         if (MODE != ONE) a.h *= ex2((a.m - m) * ch);
         a.m = m;
     }
+}
+template <int MODE> __device__ __forceinline__ void add_scalar(Stat& a, float x, float cs, float ch)
+{
+    const float m = fmaxf(a.m, x);
+    if (m == -CUDART_INF_F) {
+        if (x != x) a.h = a.s = x;                // nothing but -infinity so far; a NaN, which fmaxf passes over, must not be lost
+        return;
+    }
+    raise<MODE>(a, m, cs, ch);
+    add_one<MODE>(x, cs, -m * cs, ch, -m * ch, a.h, a.s);
+}
+__device__ __forceinline__ float max_of(const uint4& u, const float*)
+{
+    return fmaxf(fmaxf(__uint_as_float(u.x), __uint_as_float(u.y)), fmaxf(__uint_as_float(u.z), __uint_as_float(u.w)));
+}
+__device__ __forceinline__ float max_of(const uint4& u, const __nv_bfloat16*)
+{
+    const __nv_bfloat162* p = reinterpret_cast<const __nv_bfloat162*>(&u);
+    const __nv_bfloat162 m = __hmax2(__hmax2(p[0], p[1]), __hmax2(p[2], p[3]));
+    return fmaxf(__low2float(m), __high2float(m));
+}
+// V 16-byte vectors at once: one step of the running maximum, in the elements' own type, then their exponentials.
+template <typename T, int MODE, int V>
+__device__ __forceinline__ void add_vectors(Stat& a, const uint4* u, float cs, float ch)
+{
+    constexpr int N = Vec<T>::N;
+    float m = a.m;
+#pragma unroll
+    for (int v = 0; v < V; v++) m = fmaxf(m, max_of(u[v], (const T*)nullptr));
+    if (m == -CUDART_INF_F) {
+#pragma unroll
+        for (int v = 0; v < V; v++) {
+            float f[N];
+            unpack<T>(u[v], f);
+            for (int i = 0; i < N; i++) add_scalar<MODE>(a, f[i], cs, ch);
+        }
+        return;
+    }
+    raise<MODE>(a, m, cs, ch);
+    const float ns = -m * cs, nh = -m * ch;
     float h[2] = {0.f, 0.f}, s[2] = {0.f, 0.f};
 #pragma unroll
-    for (int i = 0; i < N; i++) add_one<MODE>(f[i], cs, ns, ch, nh, h[i & 1], s[i & 1]);
+    for (int v = 0; v < V; v++) {
+        float f[N];
+        unpack<T>(u[v], f);
+#pragma unroll
+        for (int i = 0; i < N; i++) add_one<MODE>(f[i], cs, ns, ch, nh, h[i & 1], s[i & 1]);
+    }
     a.h += h[0] + h[1];
     a.s += s[0] + s[1];
 }
@@ -125,43 +157,28 @@ __device__ __forceinline__ Stat merge(const Stat& a, const Stat& b, float cs, fl
     return o;
 }
 
-// max / sum over the block; every thread gets the same value
-__device__ __forceinline__ float block_max(float v, float* red)
-{
-#pragma unroll
-    for (int o = 16; o > 0; o >>= 1) v = fmaxf(v, __shfl_xor_sync(0xffffffffu, v, o));
-    if ((threadIdx.x & 31) == 0) red[threadIdx.x >> 5] = v;
-    __syncthreads();
-    v = red[0];
-    for (int w = 1; w < THREADS / 32; w++) v = fmaxf(v, red[w]);
-    __syncthreads();
-    return v;
-}
-
-// Statistics of columns [j0, j1) of a row: aligned 16-byte loads with four in flight, scalars at the ragged ends.
-template <typename T, int MODE>
-__device__ Stat row_stat(const T* row, int j0, int j1, float cs, float ch, Stat* red)
+// Statistics of columns [j0, j1) of a row by the first TH threads: aligned 16-byte loads, four in flight, scalars at the ragged
+// ends; one value per warp into red.
+template <typename T, int MODE, int TH>
+__device__ void row_stat(const T* row, int j0, int j1, float cs, float ch, Stat* red)
 {
     constexpr int N = Vec<T>::N;
     Stat a = {-CUDART_INF_F, 0.f, 0.f};
     const int lead = min(j1 - j0, (int)(((16 - ((uintptr_t)(row + j0) & 15)) & 15) / sizeof(T)));
     const int nvec = (j1 - j0 - lead) / N, tail = j0 + lead + nvec * N;
     const uint4* r4 = reinterpret_cast<const uint4*>(row + j0 + lead);
-    for (int i = threadIdx.x; i < nvec; i += 4 * THREADS) {
+    for (int i = threadIdx.x; i < nvec; i += 4 * TH) {
         uint4 u[4];
 #pragma unroll
-        for (int q = 0; q < 4; q++) if (i + q * THREADS < nvec) u[q] = __ldg(r4 + i + q * THREADS);
+        for (int q = 0; q < 4; q++) if (i + q * TH < nvec) u[q] = __ldg(r4 + i + q * TH);
+        if (i + 3 * TH < nvec) add_vectors<T, MODE, 4>(a, u, cs, ch);
+        else {
 #pragma unroll
-        for (int q = 0; q < 4; q++) {
-            if (i + q * THREADS < nvec) {
-                float f[N];
-                unpack<T>(u[q], f);
-                add_block<MODE, N>(a, f, cs, ch);
-            }
+            for (int q = 0; q < 3; q++) if (i + q * TH < nvec) add_vectors<T, MODE, 1>(a, u + q, cs, ch);
         }
     }
-    if (threadIdx.x < lead) { const float x = ld(row + j0 + threadIdx.x); add_block<MODE, 1>(a, &x, cs, ch); }
-    if (threadIdx.x < j1 - tail) { const float x = ld(row + tail + threadIdx.x); add_block<MODE, 1>(a, &x, cs, ch); }
+    if (threadIdx.x < lead) add_scalar<MODE>(a, ld(row + j0 + threadIdx.x), cs, ch);
+    if (threadIdx.x < j1 - tail) add_scalar<MODE>(a, ld(row + tail + threadIdx.x), cs, ch);
 #pragma unroll
     for (int o = 16; o > 0; o >>= 1) {
         Stat b;
@@ -171,11 +188,6 @@ __device__ Stat row_stat(const T* row, int j0, int j1, float cs, float ch, Stat*
         a = merge<MODE>(a, b, cs, ch);
     }
     if ((threadIdx.x & 31) == 0) red[threadIdx.x >> 5] = a;
-    __syncthreads();
-    a = red[0];
-    for (int w = 1; w < THREADS / 32; w++) a = merge<MODE>(a, red[w], cs, ch);
-    __syncthreads();
-    return a;
 }
 
 __device__ __forceinline__ float teacher(const Args& A, long long at)
@@ -193,84 +205,93 @@ __device__ __forceinline__ bool has_target(const Args& A, int row)
 {
     return A.hard && A.targets[row] >= 0 && A.targets[row] < A.vocab;
 }
-
-// The row's values from its statistics: log-sum-exps, cross-entropy, divergence.
-template <typename T>
-__device__ void finish_row(const Args& A, int row, const Stat& a, bool target, float* red)
+__device__ __forceinline__ float warp_max(float v)
+{
+#pragma unroll
+    for (int o = 16; o > 0; o >>= 1) v = fmaxf(v, __shfl_xor_sync(0xffffffffu, v, o));
+    return v;
+}
+// One warp: sum_k p_k (log p_k - z_k / tau) of a row; -infinity where it has no entry.
+template <typename T> __device__ float teacher_cross(const Args& A, int row, const T* z)
+{
+    const int lane = threadIdx.x & 31;
+    float top = -CUDART_INF_F;
+    bool mine = false;
+    for (int i = lane; i < A.k; i += 32) {
+        float t;
+        if (entry(A, row, i, t) >= 0) { top = t != t ? t : fmaxf(top, t); mine = true; }
+    }
+    if (!__any_sync(0xffffffffu, mine)) return -CUDART_INF_F;
+    top = warp_max(top);
+    float sum = 0.f, cross = 0.f;                 // sum e^(t - top); sum e^(t - top) (t - top - z / tau)
+    for (int i = lane; i < A.k; i += 32) {
+        float t;
+        const int id = entry(A, row, i, t);
+        if (id < 0) continue;
+        const float e = expf(t - top);
+        sum += e;
+        if (e != 0.f) cross += e * ((t - top) - ld(z + id) / A.tau);
+    }
+    sum = warp_sum(sum);
+    cross = warp_sum(cross);
+    return cross / sum - logf(sum);
+}
+// One thread: the row's values from its statistics.
+template <typename T> __device__ void finish_row(const Args& A, int row, const Stat& a, bool target, float cross)
 {
     const T* z = (const T*)A.z + (long long)row * A.z_row;
     const float lse_s = A.soft ? a.m / A.tau + logf(a.s) : 0.f;
     const float lse_h = A.hard ? (A.soft && A.tau != 1.f ? a.m + logf(a.h) : a.m + logf(a.s)) : 0.f;
-    float kl = 0.f;
-    bool any = false;
-    if (A.soft) {
-        float top = -CUDART_INF_F;
-        bool mine = false;
-        for (int i = threadIdx.x; i < A.k; i += THREADS) {
-            float t;
-            if (entry(A, row, i, t) >= 0) { top = t != t ? t : fmaxf(top, t); mine = true; }
-        }
-        any = __syncthreads_or(mine);
-        if (any) {
-            top = block_max(top, red);
-            float sum = 0.f, cross = 0.f;         // sum e^(t - top); sum e^(t - top) (t - top - (z - m) / tau)
-            for (int i = threadIdx.x; i < A.k; i += THREADS) {
-                float t;
-                const int id = entry(A, row, i, t);
-                if (id < 0) continue;
-                const float e = expf(t - top);
-                sum += e;
-                if (e != 0.f) cross += e * ((t - top) - (ld(z + id) - a.m) / A.tau);
-            }
-            sum = block_sum(sum, red);
-            cross = block_sum(cross, red);
-            kl = cross / sum + logf(a.s) - logf(sum);
-        }
-    }
-    if (threadIdx.x == 0) {
-        A.lse_h[row] = lse_h;
-        A.lse_s[row] = lse_s;
-        A.ce[row] = target ? lse_h - ld(z + A.targets[row]) : 0.f;
-        A.kl[row] = kl;
-        A.flags[row] = (target ? 1 : 0) | (any ? 2 : 0);
-    }
+    A.lse[row] = make_float2(lse_h, lse_s);
+    A.row[row] = make_float2(target ? lse_h - ld(z + A.targets[row]) : -CUDART_INF_F, cross != -CUDART_INF_F ? cross + lse_s : cross);
 }
 
-template <typename T, int MODE>
-__global__ void __launch_bounds__(THREADS) fwd_kernel(Args A, float cs, float ch)
+// TH threads read the row; one more warp reads the teacher's entries meanwhile.
+template <typename T, int MODE, int TH>
+__global__ void __launch_bounds__(TH + 32, TH == 128 ? 10 : 5) fwd_kernel(Args A, float cs, float ch)
 {
-    __shared__ Stat s_stat[THREADS / 32];
-    __shared__ float red[32];
+    __shared__ Stat s_stat[TH / 32];
+    __shared__ float s_cross;
     const int row = blockIdx.x / A.splits, sp = blockIdx.x - row * A.splits;
     const bool target = has_target(A, row);
     if (!A.soft && !target) {                     // no term: the row is not read
         if (sp == 0 && threadIdx.x == 0) {
-            A.lse_h[row] = A.lse_s[row] = A.ce[row] = A.kl[row] = 0.f;
-            A.flags[row] = 0;
+            A.lse[row] = make_float2(0.f, 0.f);
+            A.row[row] = make_float2(-CUDART_INF_F, -CUDART_INF_F);
         }
         return;
     }
-    const int j0 = sp * A.per_split, j1 = min(A.vocab, j0 + A.per_split);
-    const Stat a = row_stat<T, MODE>((const T*)A.z + (long long)row * A.z_row, j0, j1, cs, ch, s_stat);
-    if (A.splits > 1) {
-        if (threadIdx.x == 0) A.part[(long long)row * A.splits + sp] = make_float4(a.m, a.h, a.s, 0.f);
-        return;
+    const T* z = (const T*)A.z + (long long)row * A.z_row;
+    if (threadIdx.x < TH) {
+        const int j0 = sp * A.per_split, j1 = min(A.vocab, j0 + A.per_split);
+        row_stat<T, MODE, TH>(z, j0, j1, cs, ch, s_stat);
+    } else {
+        const float x = A.soft && A.splits == 1 ? teacher_cross<T>(A, row, z) : -CUDART_INF_F;
+        if (threadIdx.x == TH) s_cross = x;
     }
-    finish_row<T>(A, row, a, target, red);
+    __syncthreads();
+    if (threadIdx.x == 0) {
+        Stat a = s_stat[0];
+        for (int w = 1; w < TH / 32; w++) a = merge<MODE>(a, s_stat[w], cs, ch);
+        if (A.splits > 1) A.part[(long long)row * A.splits + sp] = make_float4(a.m, a.h, a.s, 0.f);
+        else finish_row<T>(A, row, a, target, s_cross);
+    }
 }
 template <typename T, int MODE>
-__global__ void __launch_bounds__(THREADS) join_kernel(Args A, float cs, float ch)
+__global__ void __launch_bounds__(32) join_kernel(Args A, float cs, float ch)
 {
-    __shared__ float red[32];
     const int row = blockIdx.x;
     const bool target = has_target(A, row);
     if (!A.soft && !target) return;
+    const float cross = A.soft ? teacher_cross<T>(A, row, (const T*)A.z + (long long)row * A.z_row) : -CUDART_INF_F;
+    if (threadIdx.x != 0) return;
     Stat a = {-CUDART_INF_F, 0.f, 0.f};
+#pragma unroll 8
     for (int i = 0; i < A.splits; i++) {
         const float4 p = A.part[(long long)row * A.splits + i];
         a = merge<MODE>(a, Stat{p.x, p.y, p.z}, cs, ch);
     }
-    finish_row<T>(A, row, a, target, red);
+    finish_row<T>(A, row, a, target, cross);
 }
 
 // Means over the rows. One CTA, one order: thread i adds rows i, i + 1024, ... in 64 bits.
@@ -280,13 +301,11 @@ __global__ void __launch_bounds__(1024) mean_kernel(Args A)
     __shared__ int s_i[2][32];
     double ce = 0., kl = 0.;
     int nh = 0, ns = 0;
-#pragma unroll 8
+#pragma unroll 16
     for (int i = threadIdx.x; i < A.n; i += 1024) {
-        const int f = A.flags[i];
-        ce += A.ce[i];
-        kl += A.kl[i];
-        nh += f & 1;
-        ns += f >> 1;
+        const float2 x = A.row[i];
+        if (x.x != -CUDART_INF_F) { ce += x.x; nh++; }
+        if (x.y != -CUDART_INF_F) { kl += x.y; ns++; }
     }
     for (int o = 16; o > 0; o >>= 1) {
         ce += __shfl_xor_sync(0xffffffffu, ce, o);
@@ -308,103 +327,109 @@ __global__ void __launch_bounds__(1024) mean_kernel(Args A)
     }
 }
 
+// ONE: a single softmax times gs. SQUARE: e^(z - lse_h) = (e^(z / 2 - lse_s))^2 e^(2 lse_s - lse_h), gh holds the last factor
+// (between 1 and vocab). os, oh: -lse in base-2 units.
 template <int MODE>
 __device__ __forceinline__ float grad_at(float x, float cs, float os, float gs, float ch, float oh, float gh)
 {
-    // os, oh: -lse in base-2 units. ONE: a single softmax times gs
     const float e = ex2(fmaf(x, cs, os));
     if (MODE == ONE) return gs * e;
+    if (MODE == SQUARE) return e * fmaf(gh, e, gs);
     return fmaf(gs, e, gh * ex2(fmaf(x, ch, oh)));
 }
 
-// d_logits may be logits: a thread reads its elements before it writes them, and the elements of the entries, which are
-// written once more at the end with their p taken off, are read before anything is written.
-template <typename T, int MODE>
-__global__ void __launch_bounds__(THREADS) bwd_kernel(Args A, float cs, float ch)
+// Barrier that the two kinds of warps reach at different places: the entries' elements have been read.
+template <int TH> __device__ __forceinline__ void entries_read() { asm volatile("bar.sync 1, %0;\n" ::"n"(TH + 32) : "memory"); }
+
+// TH threads write the row; one more warp has the entries. d_logits may be logits: a thread reads its elements before it writes
+// them, and the elements of the entries, which are written once more at the end with their p taken off, are read before
+// anything is written.
+template <typename T, int MODE, int TH>
+__global__ void __launch_bounds__(TH + 32, TH == 128 ? 12 : 7) bwd_kernel(Args A, float cs, float ch)
 {
     __shared__ int s_id[MAX_K + 1];
-    __shared__ float s_w[MAX_K + 1], s_z[MAX_K + 1], red[32];
+    __shared__ float s_w[MAX_K + 1], s_z[MAX_K + 1];
     constexpr int N = Vec<T>::N;
     const int row = blockIdx.x / A.splits, sp = blockIdx.x - row * A.splits;
     const int j0 = sp * A.per_split, j1 = min(A.vocab, j0 + A.per_split);
     const T* z = (const T*)A.z + (long long)row * A.z_row;
     T* d = (T*)A.d + (long long)row * A.d_row;
-    const int flags = A.flags[row];
+    const float2 rv = A.row[row], lse = A.lse[row];
+    const bool hard = rv.x != -CUDART_INF_F, soft = rv.y != -CUDART_INF_F;
     const float g = A.grad ? *A.grad : 1.f;
-    float gh = flags & 1 ? g * A.stats[1] : 0.f, gs = flags & 2 ? g * A.stats[2] : 0.f;
-    const float wh = gh, ws = gs;                 // what a target / an entry's p takes off
+    const float wh = hard ? g * A.stats[1] : 0.f, ws = soft ? g * A.stats[2] : 0.f;    // what the target / an entry's p takes off
 
     const int lead = min(j1 - j0, (int)(((16 - ((uintptr_t)(z + j0) & 15)) & 15) / sizeof(T)));
     const int nvec = (((uintptr_t)z ^ (uintptr_t)d) & 15) ? 0 : (j1 - j0 - lead) / N;      // 16-byte stores where both rows align
     const int body = j0 + lead, tail = body + nvec * N;
-    if (flags == 0) {
+    if (!hard && !soft) {
         const uint4 zero = make_uint4(0, 0, 0, 0);
-        for (int i = threadIdx.x; i < nvec; i += THREADS) reinterpret_cast<uint4*>(d + body)[i] = zero;
+        for (int i = threadIdx.x; i < nvec; i += TH + 32) reinterpret_cast<uint4*>(d + body)[i] = zero;
         if (threadIdx.x < lead) d[j0 + threadIdx.x] = T(0.f);
-        for (int j = tail + threadIdx.x; j < j1; j += THREADS) d[j] = T(0.f);
+        for (int j = tail + threadIdx.x; j < j1; j += TH + 32) d[j] = T(0.f);
         return;
     }
-    // entries of this CTA's columns, and the target as one more
-    float top = -CUDART_INF_F, sum = 0.f;
-    if (flags & 2) {
-        for (int i = threadIdx.x; i < A.k; i += THREADS) {
+    float gs = ws, gh = wh, os = -lse.y * LOG2E, oh = -lse.x * LOG2E;
+    if (MODE == ONE) {                            // one softmax: of the only term, or of both at tau = 1
+        if (!A.soft) os = oh;
+        gs = ws + wh;
+    }
+    if (MODE == SQUARE) gh *= ex2(oh - 2.f * os);
+    const int k = soft ? A.k : 0;
+    const uint4* r4 = reinterpret_cast<const uint4*>(z + body);
+    uint4* d4 = reinterpret_cast<uint4*>(d + body);
+    if (threadIdx.x < TH) {
+        uint4 u[4];
+#pragma unroll
+        for (int q = 0; q < 4; q++) if (threadIdx.x + q * TH < nvec) u[q] = r4[threadIdx.x + q * TH];
+        entries_read<TH>();
+        for (int i = threadIdx.x; i < nvec; i += 4 * TH) {
+#pragma unroll
+            for (int q = 0; q < 4; q++) {
+                if (i + q * TH < nvec) {
+                    float f[N];
+                    unpack<T>(u[q], f);
+#pragma unroll
+                    for (int e = 0; e < N; e++) f[e] = grad_at<MODE>(f[e], cs, os, gs, ch, oh, gh);
+                    d4[i + q * TH] = pack<T>(f);
+                }
+                if (i + (q + 4) * TH < nvec) u[q] = r4[i + (q + 4) * TH];
+            }
+        }
+        if (threadIdx.x < lead) d[j0 + threadIdx.x] = T(grad_at<MODE>(ld(z + j0 + threadIdx.x), cs, os, gs, ch, oh, gh));
+        for (int j = tail + threadIdx.x; j < j1; j += TH) d[j] = T(grad_at<MODE>(ld(z + j), cs, os, gs, ch, oh, gh));
+    } else {
+        const int lane = threadIdx.x - TH;
+        float top = -CUDART_INF_F, sum = 0.f;
+        for (int i = lane; i < k; i += 32) {
             float t;
             const int id = entry(A, row, i, t);
-            s_id[i] = id;
-            s_w[i] = t;
+            const bool here = id >= j0 && id < j1;
+            s_id[i] = here ? id : -1;
+            s_z[i] = here ? ld(z + id) : 0.f;
+            s_w[i] = id >= 0 ? t : -CUDART_INF_F;
             if (id >= 0) top = t != t ? t : fmaxf(top, t);
         }
-        top = block_max(top, red);
-        for (int i = threadIdx.x; i < A.k; i += THREADS) {
-            const float e = s_id[i] >= 0 ? expf(s_w[i] - top) : 0.f;
+        if (lane == 0) {                          // the target is one more entry
+            const int id = hard ? A.targets[row] : -1;
+            const bool here = id >= j0 && id < j1;
+            s_id[k] = here ? id : -1;
+            s_w[k] = wh;
+            s_z[k] = here ? ld(z + id) : 0.f;
+        }
+        entries_read<TH>();
+        top = warp_max(top);
+        for (int i = lane; i < k; i += 32) {
+            const float e = expf(s_w[i] - top);   // 0 for an entry that does not count
             s_w[i] = e;
             sum += e;
         }
-        sum = block_sum(sum, red);
+        sum = warp_sum(sum);
+        for (int i = lane; i < k; i += 32) s_w[i] = ws * (s_w[i] / sum);
     }
-    const int k = flags & 2 ? A.k : 0;
-    for (int i = threadIdx.x; i < k; i += THREADS) {
-        const int id = s_id[i];
-        const bool here = id >= j0 && id < j1;
-        s_id[i] = here ? id : -1;
-        s_w[i] = ws * (s_w[i] / sum);
-        s_z[i] = here ? ld(z + id) : 0.f;
-    }
-    if (threadIdx.x == 0) {
-        const int id = flags & 1 ? A.targets[row] : -1;
-        const bool here = id >= j0 && id < j1;
-        s_id[k] = here ? id : -1;
-        s_w[k] = wh;
-        s_z[k] = here ? ld(z + id) : 0.f;
-    }
-    float os = -A.lse_s[row] * LOG2E, oh = -A.lse_h[row] * LOG2E;
-    if (MODE == ONE) {                            // one softmax: of the only term, or of both at tau = 1
-        if (!A.soft) os = oh;
-        gs = gs + gh;
-    }
-    __syncthreads();
-    const uint4* r4 = reinterpret_cast<const uint4*>(z + body);
-    uint4* d4 = reinterpret_cast<uint4*>(d + body);
-    for (int i = threadIdx.x; i < nvec; i += 4 * THREADS) {
-        uint4 u[4];
-#pragma unroll
-        for (int q = 0; q < 4; q++) if (i + q * THREADS < nvec) u[q] = r4[i + q * THREADS];
-#pragma unroll
-        for (int q = 0; q < 4; q++) {
-            if (i + q * THREADS < nvec) {
-                float f[N];
-                unpack<T>(u[q], f);
-#pragma unroll
-                for (int e = 0; e < N; e++) f[e] = grad_at<MODE>(f[e], cs, os, gs, ch, oh, gh);
-                d4[i + q * THREADS] = pack<T>(f);
-            }
-        }
-    }
-    if (threadIdx.x < lead) d[j0 + threadIdx.x] = T(grad_at<MODE>(ld(z + j0 + threadIdx.x), cs, os, gs, ch, oh, gh));
-    for (int j = tail + threadIdx.x; j < j1; j += THREADS) d[j] = T(grad_at<MODE>(ld(z + j), cs, os, gs, ch, oh, gh));
     __syncthreads();
     // an id that several entries name is written by the first of them, with all their p in the entries' order
-    for (int i = threadIdx.x; i <= k; i += THREADS) {
+    for (int i = threadIdx.x; i <= k; i += TH + 32) {
         const int id = s_id[i];
         if (id < 0) continue;
         float w = 0.f;
@@ -420,11 +445,8 @@ static int64_t place(Args& A, char* base)
 {
     int64_t at = 0;
     auto take = [&](int64_t bytes) { char* p = base + at; at += (bytes + 255) & ~(int64_t)255; return (void*)p; };
-    A.lse_h = (float*)take((int64_t)A.n * 4);
-    A.lse_s = (float*)take((int64_t)A.n * 4);
-    A.ce = (float*)take((int64_t)A.n * 4);
-    A.kl = (float*)take((int64_t)A.n * 4);
-    A.flags = (int*)take((int64_t)A.n * 4);
+    A.lse = (float2*)take((int64_t)A.n * 8);
+    A.row = (float2*)take((int64_t)A.n * 8);
     A.stats = (float*)take(16);
     A.part = A.splits > 1 ? (float4*)take((int64_t)A.n * A.splits * 16) : nullptr;
     return at;
@@ -457,34 +479,39 @@ static bool fill(const char* where, Args& A, const void* logits, int64_t row_str
 }
 static int mode_of(const Args& A) { return !(A.hard && A.soft) || A.tau == 1.f ? ONE : A.tau == 2.f ? SQUARE : BOTH; }
 
-template <typename T, int MODE> static bool forward(const Args& A, const char* where)
+// Threads per row: enough rows must be in flight to fill the memory, and the last ones must not take long.
+static int threads_of(const Args& A) { return A.vocab <= 16384 ? 128 : 256; }
+
+template <typename T, int MODE, int TH> static bool forward(const Args& A, const char* where)
 {
     cudaStream_t st = current_stream();
     const float cs = LOG2E / (A.soft ? A.tau : 1.f), ch = LOG2E;
-    fwd_kernel<T, MODE><<<(unsigned)((long long)A.n * A.splits), THREADS, 0, st>>>(A, cs, ch);
+    fwd_kernel<T, MODE, TH><<<(unsigned)((long long)A.n * A.splits), TH + 32, 0, st>>>(A, cs, ch);
     if (!check_launch(where)) return false;
     if (A.splits > 1) {
-        join_kernel<T, MODE><<<A.n, THREADS, 0, st>>>(A, cs, ch);
+        join_kernel<T, MODE><<<A.n, 32, 0, st>>>(A, cs, ch);
         if (!check_launch(where)) return false;
     }
     return true;
 }
-template <typename T> static bool forward_mode(const Args& A, const char* where)
+template <typename T, int MODE, int TH> static bool backward(const Args& A, const char* where)
+{
+    const float cs = LOG2E / (A.soft ? A.tau : 1.f), ch = LOG2E;
+    bwd_kernel<T, MODE, TH><<<(unsigned)((long long)A.n * A.splits), TH + 32, 0, current_stream()>>>(A, cs, ch);
+    return check_launch(where);
+}
+template <typename T, int MODE> static bool launch_mode(const Args& A, bool bwd, const char* where)
+{
+    if (threads_of(A) == 128) return bwd ? backward<T, MODE, 128>(A, where) : forward<T, MODE, 128>(A, where);
+    return bwd ? backward<T, MODE, 256>(A, where) : forward<T, MODE, 256>(A, where);
+}
+template <typename T> static bool launch(const Args& A, bool bwd, const char* where)
 {
     switch (mode_of(A)) {
-    case ONE: return forward<T, ONE>(A, where);
-    case SQUARE: return forward<T, SQUARE>(A, where);
-    default: return forward<T, BOTH>(A, where);
+    case ONE: return launch_mode<T, ONE>(A, bwd, where);
+    case SQUARE: return launch_mode<T, SQUARE>(A, bwd, where);
+    default: return launch_mode<T, BOTH>(A, bwd, where);
     }
-}
-template <typename T> static bool backward(const Args& A, const char* where)
-{
-    cudaStream_t st = current_stream();
-    const float cs = LOG2E / (A.soft ? A.tau : 1.f), ch = LOG2E;
-    const unsigned grid = (unsigned)((long long)A.n * A.splits);
-    if (mode_of(A) == ONE) bwd_kernel<T, ONE><<<grid, THREADS, 0, st>>>(A, cs, ch);
-    else bwd_kernel<T, BOTH><<<grid, THREADS, 0, st>>>(A, cs, ch);
-    return check_launch(where);
 }
 
 }  // namespace distill
@@ -516,7 +543,7 @@ int32_t nlh_distill_forward(const void* logits, int32_t logits_is_bf16, int64_t 
         return NLH_ERR_INVALID_ARG;
     }
     A.loss = loss;
-    if (n > 0 && !(logits_is_bf16 ? distill::forward_mode<__nv_bfloat16>(A, where) : distill::forward_mode<float>(A, where)))
+    if (n > 0 && !(logits_is_bf16 ? distill::launch<__nv_bfloat16>(A, false, where) : distill::launch<float>(A, false, where)))
         return NLH_ERR_CUDA;
     distill::mean_kernel<<<1, 1024, 0, current_stream()>>>(A);
     if (!check_launch(where)) return NLH_ERR_CUDA;
@@ -538,7 +565,7 @@ int32_t nlh_distill_backward(const void* logits, int32_t logits_is_bf16, int64_t
     }
     if (n == 0) return NLH_OK;
     A.d = d_logits; A.d_row = d_row_stride; A.grad = grad_scale;
-    return (logits_is_bf16 ? distill::backward<__nv_bfloat16>(A, where) : distill::backward<float>(A, where)) ? NLH_OK : NLH_ERR_CUDA;
+    return (logits_is_bf16 ? distill::launch<__nv_bfloat16>(A, true, where) : distill::launch<float>(A, true, where)) ? NLH_OK : NLH_ERR_CUDA;
 }
 
 }  // extern "C"
