@@ -28,7 +28,7 @@ struct Args {
     void* d;
     const float* grad;
     int n, vocab, k, t_bf16, splits, per_split;
-    float tau, hard_w, soft_w;
+    float tau, inv_tau, hard_w, soft_w;
     bool hard, soft;                     // which terms exist
     // saved
     float2* lse;                         // [n] log-sum-exp of z, of z / tau
@@ -45,6 +45,38 @@ __device__ __forceinline__ float ex2(float x)
     float y;
     asm("ex2.approx.ftz.f32 %0, %1;" : "=f"(y) : "f"(x));
     return y;
+}
+
+// Two fp32 operations in one instruction: the kernels are bound by instruction issue next to the exponentials.
+typedef unsigned long long f2;
+__device__ __forceinline__ f2 pair(float a, float b)
+{
+    f2 r;
+    asm("mov.b64 %0, {%1, %2};" : "=l"(r) : "f"(a), "f"(b));
+    return r;
+}
+__device__ __forceinline__ float2 both(f2 v)
+{
+    float2 r;
+    asm("mov.b64 {%0, %1}, %2;" : "=f"(r.x), "=f"(r.y) : "l"(v));
+    return r;
+}
+__device__ __forceinline__ f2 fma2(f2 a, f2 b, f2 c)
+{
+    f2 r;
+    asm("fma.rn.f32x2 %0, %1, %2, %3;" : "=l"(r) : "l"(a), "l"(b), "l"(c));
+    return r;
+}
+__device__ __forceinline__ f2 add2(f2 a, f2 b)
+{
+    f2 r;
+    asm("add.rn.f32x2 %0, %1, %2;" : "=l"(r) : "l"(a), "l"(b));
+    return r;
+}
+__device__ __forceinline__ f2 ex2_2(f2 v)
+{
+    const float2 x = both(v);
+    return pair(ex2(x.x), ex2(x.y));
 }
 
 // Which exponentials a row needs. ONE: e^(z c) alone (a single term, or tau = 1); SQUARE: tau = 2; BOTH: any other tau.
@@ -134,17 +166,22 @@ __device__ __forceinline__ void add_vectors(Stat& a, const uint4* u, float cs, f
         return;
     }
     raise<MODE>(a, m, cs, ch);
-    const float ns = -m * cs, nh = -m * ch;
-    float h[2] = {0.f, 0.f}, s[2] = {0.f, 0.f};
+    const f2 c2 = pair(cs, cs), n2 = pair(-m * cs, -m * cs), ch2 = pair(ch, ch), nh2 = pair(-m * ch, -m * ch);
+    f2 h = pair(0.f, 0.f), s = pair(0.f, 0.f);
 #pragma unroll
     for (int v = 0; v < V; v++) {
         float f[N];
         unpack<T>(u[v], f);
 #pragma unroll
-        for (int i = 0; i < N; i++) add_one<MODE>(f[i], cs, ns, ch, nh, h[i & 1], s[i & 1]);
+        for (int i = 0; i < N; i += 2) {
+            const f2 x = pair(f[i], f[i + 1]), e = ex2_2(fma2(x, c2, n2));
+            s = add2(s, e);
+            if (MODE == SQUARE) h = fma2(e, e, h);
+            if (MODE == BOTH) h = add2(h, ex2_2(fma2(x, ch2, nh2)));
+        }
     }
-    a.h += h[0] + h[1];
-    a.s += s[0] + s[1];
+    a.h += both(h).x + both(h).y;
+    a.s += both(s).x + both(s).y;
 }
 template <int MODE>
 __device__ __forceinline__ Stat merge(const Stat& a, const Stat& b, float cs, float ch)
@@ -157,17 +194,24 @@ __device__ __forceinline__ Stat merge(const Stat& a, const Stat& b, float cs, fl
     return o;
 }
 
-// Statistics of columns [j0, j1) of a row by the first TH threads: aligned 16-byte loads, four in flight, scalars at the ragged
-// ends; one value per warp into red.
+__device__ __forceinline__ float warp_max(float v)
+{
+#pragma unroll
+    for (int o = 16; o > 0; o >>= 1) v = fmaxf(v, __shfl_xor_sync(0xffffffffu, v, o));
+    return v;
+}
+
+// Statistics of columns [j0, j1) of a row by TH threads: aligned 16-byte loads, four in flight, scalars at the ragged ends.
+// The calling warp's share.
 template <typename T, int MODE, int TH>
-__device__ void row_stat(const T* row, int j0, int j1, float cs, float ch, Stat* red)
+__device__ __forceinline__ Stat row_stat(const T* row, int j0, int j1, float cs, float ch, int tid)
 {
     constexpr int N = Vec<T>::N;
     Stat a = {-CUDART_INF_F, 0.f, 0.f};
     const int lead = min(j1 - j0, (int)(((16 - ((uintptr_t)(row + j0) & 15)) & 15) / sizeof(T)));
     const int nvec = (j1 - j0 - lead) / N, tail = j0 + lead + nvec * N;
     const uint4* r4 = reinterpret_cast<const uint4*>(row + j0 + lead);
-    for (int i = threadIdx.x; i < nvec; i += 4 * TH) {
+    for (int i = tid; i < nvec; i += 4 * TH) {
         uint4 u[4];
 #pragma unroll
         for (int q = 0; q < 4; q++) if (i + q * TH < nvec) u[q] = __ldg(r4 + i + q * TH);
@@ -177,17 +221,13 @@ __device__ void row_stat(const T* row, int j0, int j1, float cs, float ch, Stat*
             for (int q = 0; q < 3; q++) if (i + q * TH < nvec) add_vectors<T, MODE, 1>(a, u + q, cs, ch);
         }
     }
-    if (threadIdx.x < lead) add_scalar<MODE>(a, ld(row + j0 + threadIdx.x), cs, ch);
-    if (threadIdx.x < j1 - tail) add_scalar<MODE>(a, ld(row + tail + threadIdx.x), cs, ch);
-#pragma unroll
-    for (int o = 16; o > 0; o >>= 1) {
-        Stat b;
-        b.m = __shfl_xor_sync(0xffffffffu, a.m, o);
-        b.h = __shfl_xor_sync(0xffffffffu, a.h, o);
-        b.s = __shfl_xor_sync(0xffffffffu, a.s, o);
-        a = merge<MODE>(a, b, cs, ch);
-    }
-    if ((threadIdx.x & 31) == 0) red[threadIdx.x >> 5] = a;
+    if (tid < lead) add_scalar<MODE>(a, ld(row + j0 + tid), cs, ch);
+    if (tid < j1 - tail) add_scalar<MODE>(a, ld(row + tail + tid), cs, ch);
+    const float m = warp_max(a.m);
+    if (m != -CUDART_INF_F) raise<MODE>(a, m, cs, ch);
+    a.s = warp_sum(a.s);
+    if (MODE != ONE) a.h = warp_sum(a.h);
+    return a;
 }
 
 __device__ __forceinline__ float teacher(const Args& A, long long at)
@@ -198,18 +238,12 @@ __device__ __forceinline__ float teacher(const Args& A, long long at)
 __device__ __forceinline__ int entry(const Args& A, long long row, int i, float& t)
 {
     const int id = A.ids[row * A.k + i];
-    t = teacher(A, row * A.k + i) / A.tau;
+    t = teacher(A, row * A.k + i) * A.inv_tau;
     return id >= 0 && id < A.vocab && t != -CUDART_INF_F ? id : -1;
 }
 __device__ __forceinline__ bool has_target(const Args& A, int row)
 {
     return A.hard && A.targets[row] >= 0 && A.targets[row] < A.vocab;
-}
-__device__ __forceinline__ float warp_max(float v)
-{
-#pragma unroll
-    for (int o = 16; o > 0; o >>= 1) v = fmaxf(v, __shfl_xor_sync(0xffffffffu, v, o));
-    return v;
 }
 // One warp: sum_k p_k (log p_k - z_k / tau) of a row; -infinity where it has no entry.
 template <typename T> __device__ float teacher_cross(const Args& A, int row, const T* z)
@@ -230,28 +264,27 @@ template <typename T> __device__ float teacher_cross(const Args& A, int row, con
         if (id < 0) continue;
         const float e = expf(t - top);
         sum += e;
-        if (e != 0.f) cross += e * ((t - top) - ld(z + id) / A.tau);
+        if (e != 0.f) cross += e * ((t - top) - ld(z + id) * A.inv_tau);
     }
     sum = warp_sum(sum);
     cross = warp_sum(cross);
     return cross / sum - logf(sum);
 }
-// One thread: the row's values from its statistics.
-template <typename T> __device__ void finish_row(const Args& A, int row, const Stat& a, bool target, float cross)
+// One thread: the row's values from its statistics; zt is the target's logit.
+__device__ __forceinline__ void finish_row(const Args& A, int row, const Stat& a, bool target, float zt, float cross)
 {
-    const T* z = (const T*)A.z + (long long)row * A.z_row;
-    const float lse_s = A.soft ? a.m / A.tau + logf(a.s) : 0.f;
+    const float lse_s = A.soft ? a.m * A.inv_tau + logf(a.s) : 0.f;
     const float lse_h = A.hard ? (A.soft && A.tau != 1.f ? a.m + logf(a.h) : a.m + logf(a.s)) : 0.f;
     A.lse[row] = make_float2(lse_h, lse_s);
-    A.row[row] = make_float2(target ? lse_h - ld(z + A.targets[row]) : -CUDART_INF_F, cross != -CUDART_INF_F ? cross + lse_s : cross);
+    A.row[row] = make_float2(target ? lse_h - zt : -CUDART_INF_F, cross != -CUDART_INF_F ? cross + lse_s : cross);
 }
 
 // TH threads read the row; one more warp reads the teacher's entries meanwhile.
 template <typename T, int MODE, int TH>
-__global__ void __launch_bounds__(TH + 32, TH == 128 ? 10 : 5) fwd_kernel(Args A, float cs, float ch)
+__global__ void __launch_bounds__(TH + 32, TH == 128 ? 8 : 6) fwd_kernel(Args A, float cs, float ch)
 {
     __shared__ Stat s_stat[TH / 32];
-    __shared__ float s_cross;
+    __shared__ float s_cross, s_target;
     const int row = blockIdx.x / A.splits, sp = blockIdx.x - row * A.splits;
     const bool target = has_target(A, row);
     if (!A.soft && !target) {                     // no term: the row is not read
@@ -264,8 +297,10 @@ __global__ void __launch_bounds__(TH + 32, TH == 128 ? 10 : 5) fwd_kernel(Args A
     const T* z = (const T*)A.z + (long long)row * A.z_row;
     if (threadIdx.x < TH) {
         const int j0 = sp * A.per_split, j1 = min(A.vocab, j0 + A.per_split);
-        row_stat<T, MODE, TH>(z, j0, j1, cs, ch, s_stat);
+        const Stat a = row_stat<T, MODE, TH>(z, j0, j1, cs, ch, threadIdx.x);
+        if ((threadIdx.x & 31) == 0) s_stat[threadIdx.x >> 5] = a;
     } else {
+        if (threadIdx.x == TH) s_target = target && A.splits == 1 ? ld(z + A.targets[row]) : 0.f;
         const float x = A.soft && A.splits == 1 ? teacher_cross<T>(A, row, z) : -CUDART_INF_F;
         if (threadIdx.x == TH) s_cross = x;
     }
@@ -274,8 +309,28 @@ __global__ void __launch_bounds__(TH + 32, TH == 128 ? 10 : 5) fwd_kernel(Args A
         Stat a = s_stat[0];
         for (int w = 1; w < TH / 32; w++) a = merge<MODE>(a, s_stat[w], cs, ch);
         if (A.splits > 1) A.part[(long long)row * A.splits + sp] = make_float4(a.m, a.h, a.s, 0.f);
-        else finish_row<T>(A, row, a, target, s_cross);
+        else finish_row(A, row, a, target, s_target, s_cross);
     }
+}
+// A warp per row, four rows a CTA.
+template <typename T, int MODE>
+__global__ void __launch_bounds__(128, 12) fwd_warp_kernel(Args A, float cs, float ch)
+{
+    const int row = blockIdx.x * 4 + (threadIdx.x >> 5), lane = threadIdx.x & 31;
+    if (row >= A.n) return;
+    const bool target = has_target(A, row);
+    if (!A.soft && !target) {
+        if (lane == 0) {
+            A.lse[row] = make_float2(0.f, 0.f);
+            A.row[row] = make_float2(-CUDART_INF_F, -CUDART_INF_F);
+        }
+        return;
+    }
+    const T* z = (const T*)A.z + (long long)row * A.z_row;
+    const float zt = target ? ld(z + A.targets[row]) : 0.f;
+    const float cross = A.soft ? teacher_cross<T>(A, row, z) : -CUDART_INF_F;
+    const Stat a = row_stat<T, MODE, 32>(z, 0, A.vocab, cs, ch, lane);
+    if (lane == 0) finish_row(A, row, a, target, zt, cross);
 }
 template <typename T, int MODE>
 __global__ void __launch_bounds__(32) join_kernel(Args A, float cs, float ch)
@@ -283,7 +338,9 @@ __global__ void __launch_bounds__(32) join_kernel(Args A, float cs, float ch)
     const int row = blockIdx.x;
     const bool target = has_target(A, row);
     if (!A.soft && !target) return;
-    const float cross = A.soft ? teacher_cross<T>(A, row, (const T*)A.z + (long long)row * A.z_row) : -CUDART_INF_F;
+    const T* z = (const T*)A.z + (long long)row * A.z_row;
+    const float zt = target ? ld(z + A.targets[row]) : 0.f;
+    const float cross = A.soft ? teacher_cross<T>(A, row, z) : -CUDART_INF_F;
     if (threadIdx.x != 0) return;
     Stat a = {-CUDART_INF_F, 0.f, 0.f};
 #pragma unroll 8
@@ -291,7 +348,7 @@ __global__ void __launch_bounds__(32) join_kernel(Args A, float cs, float ch)
         const float4 p = A.part[(long long)row * A.splits + i];
         a = merge<MODE>(a, Stat{p.x, p.y, p.z}, cs, ch);
     }
-    finish_row<T>(A, row, a, target, cross);
+    finish_row(A, row, a, target, zt, cross);
 }
 
 // Means over the rows. One CTA, one order: thread i adds rows i, i + 1024, ... in 64 bits.
@@ -338,6 +395,146 @@ __device__ __forceinline__ float grad_at(float x, float cs, float os, float gs, 
     return fmaf(gs, e, gh * ex2(fmaf(x, ch, oh)));
 }
 
+// What a row's gradient is made of.
+struct RowGrad {
+    bool hard, soft;
+    float wh, ws;                        // what the target / an entry's p takes off
+    float os, oh, gs, gh;                // see grad_at
+};
+template <int MODE> __device__ __forceinline__ RowGrad row_grad(const Args& A, int row)
+{
+    RowGrad r;
+    const float2 rv = A.row[row], lse = A.lse[row];
+    const float g = A.grad ? *A.grad : 1.f, sh = A.stats[1], ss = A.stats[2];
+    r.hard = rv.x != -CUDART_INF_F;
+    r.soft = rv.y != -CUDART_INF_F;
+    r.wh = r.hard ? g * sh : 0.f;
+    r.ws = r.soft ? g * ss : 0.f;
+    r.gs = r.ws; r.gh = r.wh; r.os = -lse.y * LOG2E; r.oh = -lse.x * LOG2E;
+    if (MODE == ONE) {                   // one softmax: of the only term, or of both at tau = 1
+        if (!A.soft) r.os = r.oh;
+        r.gs = r.ws + r.wh;
+    }
+    if (MODE == SQUARE) r.gh *= ex2(r.oh - 2.f * r.os);
+    return r;
+}
+template <int MODE> __device__ __forceinline__ float grad_of(float x, const RowGrad& r, float cs, float ch)
+{
+    return grad_at<MODE>(x, cs, r.os, r.gs, ch, r.oh, r.gh);
+}
+
+// Columns [j0, j1) of a row by TH threads.
+template <typename T> struct Span {
+    int j0, j1, lead, nvec, body, tail;
+    __device__ __forceinline__ Span(const T* z, const T* d, int a, int b) : j0(a), j1(b)
+    {
+        lead = min(j1 - j0, (int)(((16 - ((uintptr_t)(z + j0) & 15)) & 15) / sizeof(T)));
+        nvec = (((uintptr_t)z ^ (uintptr_t)d) & 15) ? 0 : (j1 - j0 - lead) / Vec<T>::N;    // 16-byte stores where both rows align
+        body = j0 + lead;
+        tail = body + nvec * Vec<T>::N;
+    }
+};
+template <typename T, int TH> __device__ __forceinline__ void load_first(uint4 (&u)[4], const T* z, const Span<T>& s, int tid)
+{
+    const uint4* r4 = reinterpret_cast<const uint4*>(z + s.body);
+#pragma unroll
+    for (int q = 0; q < 4; q++) if (tid + q * TH < s.nvec) u[q] = r4[tid + q * TH];
+}
+template <typename T, int MODE, int TH>
+__device__ __forceinline__ void write_row(const T* z, T* d, const Span<T>& s, uint4 (&u)[4], const RowGrad& r, float cs, float ch, int tid)
+{
+    constexpr int N = Vec<T>::N;
+    const uint4* r4 = reinterpret_cast<const uint4*>(z + s.body);
+    uint4* d4 = reinterpret_cast<uint4*>(d + s.body);
+    for (int i = tid; i < s.nvec; i += 4 * TH) {
+        if (i != tid) {
+#pragma unroll
+            for (int q = 0; q < 4; q++) if (i + q * TH < s.nvec) u[q] = r4[i + q * TH];
+        }
+#pragma unroll
+        for (int q = 0; q < 4; q++) {
+            if (i + q * TH < s.nvec) {
+                float f[N];
+                unpack<T>(u[q], f);
+#pragma unroll
+                for (int e = 0; e < N; e++) f[e] = grad_of<MODE>(f[e], r, cs, ch);
+                d4[i + q * TH] = pack<T>(f);
+            }
+        }
+    }
+    if (tid < s.lead) d[s.j0 + tid] = T(grad_of<MODE>(ld(z + s.j0 + tid), r, cs, ch));
+    for (int j = s.tail + tid; j < s.j1; j += TH) d[j] = T(grad_of<MODE>(ld(z + j), r, cs, ch));
+}
+template <typename T, int TH> __device__ __forceinline__ void zero_row(T* d, const Span<T>& s, int tid)
+{
+    for (int i = tid; i < s.nvec; i += TH) reinterpret_cast<uint4*>(d + s.body)[i] = make_uint4(0, 0, 0, 0);
+    if (tid < s.lead) d[s.j0 + tid] = T(0.f);
+    for (int j = s.tail + tid; j < s.j1; j += TH) d[j] = T(0.f);
+}
+
+// The row's entries in shared memory by one warp: ids inside [j0, j1), logits z there, and (in weigh) p times its weight; the
+// target is one more entry.
+struct Entries { int* id; float *w, *z; };
+template <typename T> __device__ __forceinline__ float read_entries(const Args& A, const Entries& E, int row, const T* z, int j0, int j1, int k,
+                                                                    const RowGrad& r)
+{
+    const int lane = threadIdx.x & 31;
+    float top = -CUDART_INF_F;
+    for (int i = lane; i < k; i += 32) {
+        float t;
+        const int id = entry(A, row, i, t);
+        const bool here = id >= j0 && id < j1;
+        E.id[i] = here ? id : -1;
+        E.z[i] = here ? ld(z + id) : 0.f;
+        E.w[i] = id >= 0 ? t : -CUDART_INF_F;
+        if (id >= 0) top = t != t ? t : fmaxf(top, t);
+    }
+    if (lane == 0) {
+        const int id = r.hard ? A.targets[row] : -1;
+        const bool here = id >= j0 && id < j1;
+        E.id[k] = here ? id : -1;
+        for (int i = k + 1; i & 3; i++) E.id[i] = -1;
+        E.w[k] = r.wh;
+        E.z[k] = here ? ld(z + id) : 0.f;
+    }
+    return top;
+}
+__device__ __forceinline__ void weigh(const Entries& E, int k, float top, float ws)
+{
+    const int lane = threadIdx.x & 31;
+    float sum = 0.f;
+    top = warp_max(top);
+    for (int i = lane; i < k; i += 32) {
+        const float e = expf(E.w[i] - top);       // 0 for an entry that does not count
+        E.w[i] = e;
+        sum += e;
+    }
+    const float wn = ws / warp_sum(sum);
+    for (int i = lane; i < k; i += 32) E.w[i] *= wn;
+}
+// An id that several entries name is written by the first of them, with all their p in the entries' order.
+template <typename T, int MODE, int TH>
+__device__ __forceinline__ void write_entries(const Entries& E, int k, T* d, const RowGrad& r, float cs, float ch, int tid)
+{
+    for (int i = tid; i <= k; i += TH) {
+        const int id = E.id[i];
+        if (id < 0) continue;
+        float w = E.w[i];
+        bool first = true;
+        int same = 0;
+        for (int j = 0; j <= k; j += 4) {
+            const int4 o = *reinterpret_cast<const int4*>(E.id + j);
+            same += (o.x == id) + (o.y == id) + (o.z == id) + (o.w == id);
+        }
+        if (same > 1) {
+            w = 0.f;
+            for (int j = 0; j <= k; j++)
+                if (E.id[j] == id) { first &= j >= i; w += E.w[j]; }
+        }
+        if (first) d[id] = T(grad_of<MODE>(E.z[i], r, cs, ch) - w);
+    }
+}
+
 // Barrier that the two kinds of warps reach at different places: the entries' elements have been read.
 template <int TH> __device__ __forceinline__ void entries_read() { asm volatile("bar.sync 1, %0;\n" ::"n"(TH + 32) : "memory"); }
 
@@ -345,101 +542,32 @@ template <int TH> __device__ __forceinline__ void entries_read() { asm volatile(
 // them, and the elements of the entries, which are written once more at the end with their p taken off, are read before
 // anything is written.
 template <typename T, int MODE, int TH>
-__global__ void __launch_bounds__(TH + 32, TH == 128 ? 12 : 7) bwd_kernel(Args A, float cs, float ch)
+__global__ void __launch_bounds__(TH + 32, TH == 128 ? 12 : 5) bwd_kernel(Args A, float cs, float ch)
 {
-    __shared__ int s_id[MAX_K + 1];
+    __shared__ __align__(16) int s_id[MAX_K + 4];
     __shared__ float s_w[MAX_K + 1], s_z[MAX_K + 1];
-    constexpr int N = Vec<T>::N;
+    const Entries E = {s_id, s_w, s_z};
     const int row = blockIdx.x / A.splits, sp = blockIdx.x - row * A.splits;
     const int j0 = sp * A.per_split, j1 = min(A.vocab, j0 + A.per_split);
     const T* z = (const T*)A.z + (long long)row * A.z_row;
     T* d = (T*)A.d + (long long)row * A.d_row;
-    const float2 rv = A.row[row], lse = A.lse[row];
-    const bool hard = rv.x != -CUDART_INF_F, soft = rv.y != -CUDART_INF_F;
-    const float g = A.grad ? *A.grad : 1.f;
-    const float wh = hard ? g * A.stats[1] : 0.f, ws = soft ? g * A.stats[2] : 0.f;    // what the target / an entry's p takes off
-
-    const int lead = min(j1 - j0, (int)(((16 - ((uintptr_t)(z + j0) & 15)) & 15) / sizeof(T)));
-    const int nvec = (((uintptr_t)z ^ (uintptr_t)d) & 15) ? 0 : (j1 - j0 - lead) / N;      // 16-byte stores where both rows align
-    const int body = j0 + lead, tail = body + nvec * N;
-    if (!hard && !soft) {
-        const uint4 zero = make_uint4(0, 0, 0, 0);
-        for (int i = threadIdx.x; i < nvec; i += TH + 32) reinterpret_cast<uint4*>(d + body)[i] = zero;
-        if (threadIdx.x < lead) d[j0 + threadIdx.x] = T(0.f);
-        for (int j = tail + threadIdx.x; j < j1; j += TH + 32) d[j] = T(0.f);
-        return;
-    }
-    float gs = ws, gh = wh, os = -lse.y * LOG2E, oh = -lse.x * LOG2E;
-    if (MODE == ONE) {                            // one softmax: of the only term, or of both at tau = 1
-        if (!A.soft) os = oh;
-        gs = ws + wh;
-    }
-    if (MODE == SQUARE) gh *= ex2(oh - 2.f * os);
-    const int k = soft ? A.k : 0;
-    const uint4* r4 = reinterpret_cast<const uint4*>(z + body);
-    uint4* d4 = reinterpret_cast<uint4*>(d + body);
+    const Span<T> s(z, d, j0, j1);
+    uint4 u[4];                                   // on their way while the row's statistics come in
+    if (threadIdx.x < TH) load_first<T, TH>(u, z, s, threadIdx.x);
+    const RowGrad r = row_grad<MODE>(A, row);
+    if (!r.hard && !r.soft) { zero_row<T, TH + 32>(d, s, threadIdx.x); return; }
+    const int k = r.soft ? A.k : 0;
     if (threadIdx.x < TH) {
-        uint4 u[4];
-#pragma unroll
-        for (int q = 0; q < 4; q++) if (threadIdx.x + q * TH < nvec) u[q] = r4[threadIdx.x + q * TH];
         entries_read<TH>();
-        for (int i = threadIdx.x; i < nvec; i += 4 * TH) {
-#pragma unroll
-            for (int q = 0; q < 4; q++) {
-                if (i + q * TH < nvec) {
-                    float f[N];
-                    unpack<T>(u[q], f);
-#pragma unroll
-                    for (int e = 0; e < N; e++) f[e] = grad_at<MODE>(f[e], cs, os, gs, ch, oh, gh);
-                    d4[i + q * TH] = pack<T>(f);
-                }
-                if (i + (q + 4) * TH < nvec) u[q] = r4[i + (q + 4) * TH];
-            }
-        }
-        if (threadIdx.x < lead) d[j0 + threadIdx.x] = T(grad_at<MODE>(ld(z + j0 + threadIdx.x), cs, os, gs, ch, oh, gh));
-        for (int j = tail + threadIdx.x; j < j1; j += TH) d[j] = T(grad_at<MODE>(ld(z + j), cs, os, gs, ch, oh, gh));
+        write_row<T, MODE, TH>(z, d, s, u, r, cs, ch, threadIdx.x);
     } else {
-        const int lane = threadIdx.x - TH;
-        float top = -CUDART_INF_F, sum = 0.f;
-        for (int i = lane; i < k; i += 32) {
-            float t;
-            const int id = entry(A, row, i, t);
-            const bool here = id >= j0 && id < j1;
-            s_id[i] = here ? id : -1;
-            s_z[i] = here ? ld(z + id) : 0.f;
-            s_w[i] = id >= 0 ? t : -CUDART_INF_F;
-            if (id >= 0) top = t != t ? t : fmaxf(top, t);
-        }
-        if (lane == 0) {                          // the target is one more entry
-            const int id = hard ? A.targets[row] : -1;
-            const bool here = id >= j0 && id < j1;
-            s_id[k] = here ? id : -1;
-            s_w[k] = wh;
-            s_z[k] = here ? ld(z + id) : 0.f;
-        }
+        const float top = read_entries<T>(A, E, row, z, j0, j1, k, r);
         entries_read<TH>();
-        top = warp_max(top);
-        for (int i = lane; i < k; i += 32) {
-            const float e = expf(s_w[i] - top);   // 0 for an entry that does not count
-            s_w[i] = e;
-            sum += e;
-        }
-        sum = warp_sum(sum);
-        for (int i = lane; i < k; i += 32) s_w[i] = ws * (s_w[i] / sum);
+        weigh(E, k, top, r.ws);
     }
     __syncthreads();
-    // an id that several entries name is written by the first of them, with all their p in the entries' order
-    for (int i = threadIdx.x; i <= k; i += TH + 32) {
-        const int id = s_id[i];
-        if (id < 0) continue;
-        float w = 0.f;
-        bool first = true;
-        for (int j = 0; j <= k; j++)
-            if (s_id[j] == id) { first &= j >= i; w += s_w[j]; }
-        if (first) d[id] = T(grad_at<MODE>(s_z[i], cs, os, gs, ch, oh, gh) - w);
-    }
+    write_entries<T, MODE, TH + 32>(E, k, d, r, cs, ch, threadIdx.x);
 }
-
 // ── host ──
 static int64_t place(Args& A, char* base)
 {
@@ -473,37 +601,42 @@ static bool fill(const char* where, Args& A, const void* logits, int64_t row_str
     else if (n > 0 && (!logits || (A.soft && k > 0 && !teacher_logits))) bad = "NULL pointer";
     if (bad) { record_status(NLH_ERR_INVALID_ARG, where, bad); return false; }
     A.z = logits; A.z_row = row_stride; A.targets = targets; A.ids = teacher_ids; A.t = teacher_logits; A.t_bf16 = teacher_is_bf16;
-    A.n = n; A.vocab = vocab; A.k = A.soft ? k : 0; A.tau = temperature; A.hard_w = hard_weight; A.soft_w = soft_weight;
+    A.n = n; A.vocab = vocab; A.k = A.soft ? k : 0; A.tau = temperature; A.inv_tau = 1.f / temperature; A.hard_w = hard_weight; A.soft_w = soft_weight;
     divide(A);
     return true;
 }
 static int mode_of(const Args& A) { return !(A.hard && A.soft) || A.tau == 1.f ? ONE : A.tau == 2.f ? SQUARE : BOTH; }
 
-// Threads per row: enough rows must be in flight to fill the memory, and the last ones must not take long.
-static int threads_of(const Args& A) { return A.vocab <= 16384 ? 128 : 256; }
+// Who reads a row in the forward: with many short rows a warp, which waits at no barrier (32768 x 8192 bf16 at tau 2: 110 us
+// against 132), else a CTA (8192 x 16000: 63 us against 65). The backward writes as well, and is faster with a CTA at every size
+// (32768 x 8192: 196 us against 216).
+static bool warp_rows(const Args& A) { return A.vocab <= 12288 && A.n >= 4096; }
 
-template <typename T, int MODE, int TH> static bool forward(const Args& A, const char* where)
+template <typename T, int MODE, int TH> static bool forward(const Args& A, float cs, const char* where)
 {
     cudaStream_t st = current_stream();
-    const float cs = LOG2E / (A.soft ? A.tau : 1.f), ch = LOG2E;
-    fwd_kernel<T, MODE, TH><<<(unsigned)((long long)A.n * A.splits), TH + 32, 0, st>>>(A, cs, ch);
+    fwd_kernel<T, MODE, TH><<<(unsigned)((long long)A.n * A.splits), TH + 32, 0, st>>>(A, cs, LOG2E);
     if (!check_launch(where)) return false;
     if (A.splits > 1) {
-        join_kernel<T, MODE><<<A.n, 32, 0, st>>>(A, cs, ch);
+        join_kernel<T, MODE><<<A.n, 32, 0, st>>>(A, cs, LOG2E);
         if (!check_launch(where)) return false;
     }
     return true;
 }
-template <typename T, int MODE, int TH> static bool backward(const Args& A, const char* where)
+template <typename T, int MODE, int TH> static bool backward(const Args& A, float cs, const char* where)
 {
-    const float cs = LOG2E / (A.soft ? A.tau : 1.f), ch = LOG2E;
-    bwd_kernel<T, MODE, TH><<<(unsigned)((long long)A.n * A.splits), TH + 32, 0, current_stream()>>>(A, cs, ch);
+    bwd_kernel<T, MODE, TH><<<(unsigned)((long long)A.n * A.splits), TH + 32, 0, current_stream()>>>(A, cs, LOG2E);
     return check_launch(where);
 }
 template <typename T, int MODE> static bool launch_mode(const Args& A, bool bwd, const char* where)
 {
-    if (threads_of(A) == 128) return bwd ? backward<T, MODE, 128>(A, where) : forward<T, MODE, 128>(A, where);
-    return bwd ? backward<T, MODE, 256>(A, where) : forward<T, MODE, 256>(A, where);
+    const float cs = LOG2E / (A.soft ? A.tau : 1.f);
+    if (!bwd && warp_rows(A)) {
+        fwd_warp_kernel<T, MODE><<<(unsigned)(((long long)A.n + 3) / 4), 128, 0, current_stream()>>>(A, cs, LOG2E);
+        return check_launch(where);
+    }
+    if (A.vocab <= 16384) return bwd ? backward<T, MODE, 128>(A, cs, where) : forward<T, MODE, 128>(A, cs, where);
+    return bwd ? backward<T, MODE, 256>(A, cs, where) : forward<T, MODE, 256>(A, cs, where);
 }
 template <typename T> static bool launch(const Args& A, bool bwd, const char* where)
 {
