@@ -72,8 +72,10 @@ template <typename T>
 __global__ void __launch_bounds__(128) gd_prep_kernel(Args A)
 {
     extern __shared__ float4 smem4[];
-    float* Ks = reinterpret_cast<float*>(smem4);
-    float *Am = Ks + C * LD, *Tm = Am + C * LD;
+    float* Am = reinterpret_cast<float*>(smem4);
+    float* Tm = Am + C * LD;
+    bf* Ks = reinterpret_cast<bf*>(Tm + C * LD);
+    float* Z = reinterpret_cast<float*>(Ks);
     __shared__ float2 s_g[C];
     __shared__ float s_theta[C];
     const int slot = blockIdx.x / A.hv, h = blockIdx.x - slot * A.hv;
@@ -108,16 +110,17 @@ __global__ void __launch_bounds__(128) gd_prep_kernel(Args A)
             s_theta[i] = (float)th[j];
         }
     }
+    constexpr int IN = Pl<T>::in, PS = C * LP;
     float lo[4][4], hi[4][4];
     zero(lo);
     zero(hi);
     const T* kp = (const T*)A.k + ch.b * A.kb + ch.t0 * A.kt + (h / A.share) * A.kh;
     for (int c0 = 0; c0 < A.dk; c0 += 64) {
         __syncthreads();
-        load_tile<T, 64, 128>(Ks, LD, kp + c0, A.kt, ch.len, A.dk - c0);
+        load_tile<T, 64, 128>(Ks, LP, PS, kp + c0, A.kt, ch.len, A.dk - c0);
         __syncthreads();
-        gemm16<4, false, false, Pl<T>::in, Pl<T>::in>(lo, Ks + 16 * w * LD, LD, Ks, LD, 0, 64);
-        if (w >= 2) gemm16<4, false, false, Pl<T>::in, Pl<T>::in>(hi, Ks + 16 * w * LD, LD, Ks + 32 * LD, LD, 0, 64);
+        gemm<4, false, false, IN, IN>(lo, Ks + 16 * w * LP, LP, PS, Ks, LP, PS, 0, 64);
+        if (w >= 2) gemm<4, false, false, IN, IN>(hi, Ks + 16 * w * LP, LP, PS, Ks + 32 * LP, LP, PS, 0, 64);
     }
     for (int i = tid; i < C * LD / 4; i += 128) reinterpret_cast<float4*>(Tm)[i] = make_float4(0.f, 0.f, 0.f, 0.f);
 #pragma unroll
@@ -150,7 +153,6 @@ __global__ void __launch_bounds__(128) gd_prep_kernel(Args A)
         }
     }
     __syncthreads();
-    float* Z = Ks;
     {   // 16 -> 32, both pairs of blocks at once
         const int p = tid >> 6, r = (tid >> 2) & 15, c = (tid & 3) * 4, r0 = 32 * p + 16, c0 = 32 * p;
         float z[4] = {0.f, 0.f, 0.f, 0.f};
@@ -199,32 +201,36 @@ __global__ void __launch_bounds__(128) gd_prep_kernel(Args A)
         for (int i = 0; i < 8; i++) Tm[(32 + r) * LD + c + i] = z[i];
     }
     __syncthreads();
-    float* out = A.tmat + tile * C * C;
-    for (int i = tid; i < C * C / 4; i += 128)
-        reinterpret_cast<float4*>(out)[i] = *reinterpret_cast<const float4*>(Tm + (i >> 4) * LD + (i & 15) * 4);
+    bf* out = reinterpret_cast<bf*>(A.tmat + tile * T_BYTES);
+    for (int i = tid; i < C * 16; i += 128) {
+        const int r = i >> 4, c = (i & 15) * 4;
+        put4<3>(out + r * LP + c, PS, *reinterpret_cast<const float4*>(Tm + r * LD + c));
+    }
 }
 
-// ── forward states: the recurrence over chunks for NS = 32 columns of V ──
-// Eight warps: warp = 16 rows (tokens; state rows of each 64 of dk in the update) x 16 columns. The state stays in the
-// update's accumulators from chunk to chunk. While a chunk is computed the next one's K, T, V and gates are on their
-// way in registers; K has two buffers, because it is read until the chunk's end. Three barriers a chunk. Bound by that chain:
-// three products of 64 x 32 x 64 that wait for one another. 64 columns a CTA would halve the reads of K and T, which
-// come from L2, but leave half the CTAs to hide the chain behind.
-template <int DKP, int NS> struct StateSmem {
-    // LS: pairs between rows of a split [token][column] matrix
-    static constexpr int LK = DKP + 4, LS = NS + 2, BYTES = 4 * (2 * C * LK + C * LD) + 8 * (NS * LK + 2 * C * LS);
+// ── forward states: the recurrence over chunks for NS columns of V ──
+// Eight warps: warp = 16 rows (tokens; state rows of each 64 of dk in the update) x half of the columns. The state (transposed, S
+// [dk, dv]) stays in the update's accumulators from chunk to chunk. While a chunk is computed the next one's K, T, V and gates are
+// on their way in registers. Bound by the chain of three products of 64 x NS x 64 a chunk: NS = 32 shares the loads of K and T
+// among more columns, NS = 16 gives twice the CTAs where heads are few. A bf16 K has two buffers, so that only the
+// products' own barriers are left; three planes of a fp32 one have one buffer, which lets two CTAs share an SM.
+template <typename T, int DKP, int NS> struct StateSmem {
+    static constexpr int LK = DKP + 8, LS = NS + 8, KB = Pl<T>::in == 1 ? 2 : 1;       // bf16 between rows of K, of [..][NS] matrices
+    static constexpr int PK = C * LK, PM = DKP * LS, PR = C * LS;                      // bf16 of one plane
+    static constexpr int BYTES = T_BYTES + 2 * (KB * Pl<T>::in * PK + 3 * PM + 6 * PR);
 };
 struct GateRow { float4 g; float theta; };
 
 template <typename T, int DKP, int NS>
 __global__ void __launch_bounds__(256, DKP == 64 ? 2 : 1) gd_state_fwd_kernel(Args A)
 {
-    constexpr int LK = DKP + 4, LS = NS + 2, MT = DKP / 64, NT = NS / 16, H = NS / 2;
+    typedef StateSmem<T, DKP, NS> L;
+    constexpr int LK = L::LK, LS = L::LS, MT = DKP / 64, NT = NS / 16, H = NS / 2, IN = Pl<T>::in;
     extern __shared__ float4 smem4[];
-    float* Kb = reinterpret_cast<float*>(smem4);                        // [2][64][LK]
-    float* Ts = Kb + 2 * C * LK;                                        // [64][LD]
-    float2* Ms = reinterpret_cast<float2*>(Ts + C * LD);                // [NS][LK] pairs
-    float2 *Rs = Ms + NS * LK, *Us = Rs + C * LS;                       // [64][LS] pairs
+    bf* Ts = reinterpret_cast<bf*>(smem4);              // [64][LP], three planes
+    bf* Kb = Ts + T_BYTES / 2;                          // [KB] [64][LK]
+    bf* Ms = Kb + L::KB * IN * L::PK;                   // [DKP][LS]
+    bf *Rs = Ms + 3 * L::PM, *Us = Rs + 3 * L::PR;      // [64][LS]
     __shared__ float4 s_gate[2][C];
     __shared__ float s_w[2][C];
     const int nsl = A.dvp / NS, sl = blockIdx.x % nsl, p = blockIdx.x / nsl, h = p % A.hv, seq = p / A.hv;
@@ -233,18 +239,26 @@ __global__ void __launch_bounds__(256, DKP == 64 ? 2 : 1) gd_state_fwd_kernel(Ar
 
     float S[MT][NT][4];
     const float* m0 = A.m0 ? A.m0 + ((long long)seq * A.hv + h) * A.dv * A.dk : nullptr;
+    auto put_state = [&](int m) {
 #pragma unroll
-    for (int m = 0; m < MT; m++)
+        for (int n = 0; n < NT; n++)
+#pragma unroll
+            for (int r = 0; r < 2; r++)
+                put2<3>(Ms + (64 * m + 16 * rb + g + 8 * r) * LS + H * hf + 8 * n + 2 * t, L::PM, S[m][n][2 * r], S[m][n][2 * r + 1]);
+    };
+#pragma unroll
+    for (int m = 0; m < MT; m++) {
 #pragma unroll
         for (int n = 0; n < NT; n++)
 #pragma unroll
             for (int i = 0; i < 4; i++) {
-                const int row = 64 * m + 16 * rb + g + 8 * (i >> 1), col = H * hf + 8 * n + 2 * t + (i & 1);   // dk, dv
-                S[m][n][i] = m0 && row < A.dk && n0 + col < A.dv ? m0[(long long)(n0 + col) * A.dk + row] : 0.f;
-                Ms[col * LK + row] = split_pair(S[m][n][i]);
+                const int row = 64 * m + 16 * rb + g + 8 * (i >> 1), col = n0 + H * hf + 8 * n + 2 * t + (i & 1);   // dk, dv
+                S[m][n][i] = m0 && row < A.dk && col < A.dv ? m0[(long long)col * A.dk + row] : 0.f;
             }
+        put_state(m);
+    }
     Prefetch<T, DKP, 256> pk;
-    Prefetch<float, 64, 256> pt;
+    PrefetchT<256> pt;
     GateRow pg;
     Pair<T> pv[NT][2];
     const bool vpair = ((reinterpret_cast<uintptr_t>((const T*)A.v + n0) | (uintptr_t)((A.vb | A.vt | A.vh) * (long long)sizeof(T))) &
@@ -254,7 +268,7 @@ __global__ void __launch_bounds__(256, DKP == 64 ? 2 : 1) gd_state_fwd_kernel(Ar
         const Chunk ch = get_chunk(A, slot);
         const long long tile = (long long)slot * A.hv + h;
         pk.load((const T*)A.k + ch.b * A.kb + ch.t0 * A.kt + (h / A.share) * A.kh, A.kt, ch.len, A.dk);
-        pt.load(A.tmat + tile * C * C, C, C, C);
+        pt.load(A.tmat + tile * T_BYTES);
         if (tid < C) { ldg(pg.g, reinterpret_cast<const float*>(A.gates + tile * C + tid)); ldg(pg.theta, A.theta_eff + tile * C + tid); }
         const T* vp = (const T*)A.v + ch.b * A.vb + ch.t0 * A.vt + h * A.vh + n0;
 #pragma unroll
@@ -266,8 +280,9 @@ __global__ void __launch_bounds__(256, DKP == 64 ? 2 : 1) gd_state_fwd_kernel(Ar
             }
     };
     auto commit = [&](int buf) {
-        pk.store(Kb + buf * C * LK, LK);
-        pt.store(Ts, LD);
+        if (L::KB == 1) __syncthreads();              // the one buffer of K has been read
+        pk.store(Kb + (L::KB == 1 ? 0 : buf) * IN * L::PK, LK, L::PK);
+        pt.store(Ts);
         if (tid < C) { s_gate[buf][tid] = pg.g; s_w[buf][tid] = pg.g.w * pg.theta; }
     };
     if (count > 0) { fetch(0); commit(0); }
@@ -275,37 +290,34 @@ __global__ void __launch_bounds__(256, DKP == 64 ? 2 : 1) gd_state_fwd_kernel(Ar
     for (int c = 0; c < count; c++) {
         const int buf = c & 1;
         const long long tile = (long long)(slot0 + c) * A.hv + h;
-        const float* Ks = Kb + buf * C * LK;
+        const bf* Ks = Kb + (L::KB == 1 ? 0 : buf) * IN * L::PK;
         Pair<T> v[NT][2];
+        float* mc = A.m_chunk + tile * DKP * A.dvp + n0;
 #pragma unroll
         for (int n = 0; n < NT; n++)
 #pragma unroll
-            for (int r = 0; r < 2; r++) v[n][r] = pv[n][r];
-        float* mc = A.m_chunk + (tile * A.dvp + n0) * DKP;
+            for (int r = 0; r < 2; r++) {
+                v[n][r] = pv[n][r];
 #pragma unroll
-        for (int m = 0; m < MT; m++)
-#pragma unroll
-            for (int n = 0; n < NT; n++)
-#pragma unroll
-                for (int i = 0; i < 4; i++)
-                    mc[(H * hf + 8 * n + 2 * t + (i & 1)) * DKP + 64 * m + 16 * rb + g + 8 * (i >> 1)] = S[m][n][i];
+                for (int m = 0; m < MT; m++)
+                    st2(mc + (64 * m + 16 * rb + g + 8 * r) * A.dvp + H * hf + 8 * n + 2 * t, S[m][n][2 * r], S[m][n][2 * r + 1]);
+            }
         if (c + 1 < count) fetch(c + 1);
         float acc[NT][4];
         zero(acc);
-        gemm16s<NT, false, false, Pl<T>::in>(acc, Ks + 16 * rb * LK, LK, Ms + H * hf * LK, LK, 0, DKP);
+        gemm<NT, false, true, IN, 3>(acc, Ks + 16 * rb * LK, LK, L::PK, Ms + H * hf, LS, L::PM, 0, DKP);
 #pragma unroll
         for (int n = 0; n < NT; n++)
 #pragma unroll
             for (int r = 0; r < 2; r++) {
                 const int row = 16 * rb + g + 8 * r;
                 const float2 x = v[n][r].get();
-                float2* o = Rs + row * LS + H * hf + 8 * n + 2 * t;
-                o[0] = split_pair(x.x - s_gate[buf][row].z * acc[n][2 * r]);
-                o[1] = split_pair(x.y - s_gate[buf][row].z * acc[n][2 * r + 1]);
+                put2<3>(Rs + row * LS + H * hf + 8 * n + 2 * t, L::PR, x.x - s_gate[buf][row].z * acc[n][2 * r],
+                        x.y - s_gate[buf][row].z * acc[n][2 * r + 1]);
             }
         __syncthreads();
         zero(acc);
-        gemm16s<NT, false, true, TWO>(acc, Ts + 16 * rb * LD, LD, Rs + H * hf, LS, 0, 16 * (rb + 1));
+        gemm<NT, false, true, 3, 3>(acc, Ts + 16 * rb * LP, LP, C * LP, Rs + H * hf, LS, L::PR, 0, 16 * (rb + 1));
         float* ep = A.e + tile * C * A.dvp + n0;
 #pragma unroll
         for (int n = 0; n < NT; n++)
@@ -314,8 +326,7 @@ __global__ void __launch_bounds__(256, DKP == 64 ? 2 : 1) gd_state_fwd_kernel(Ar
                 const int row = 16 * rb + g + 8 * r, col = H * hf + 8 * n + 2 * t;
                 const float a = acc[n][2 * r], b = acc[n][2 * r + 1], wt = s_w[buf][row];
                 st2(ep + (long long)row * A.dvp + col, a, b);
-                Us[row * LS + col] = split_pair(wt * a);
-                Us[row * LS + col + 1] = split_pair(wt * b);
+                put2<3>(Us + row * LS + col, L::PR, wt * a, wt * b);
             }
         __syncthreads();
         const float gl = s_gate[buf][C - 1].z;
@@ -325,12 +336,8 @@ __global__ void __launch_bounds__(256, DKP == 64 ? 2 : 1) gd_state_fwd_kernel(Ar
             for (int n = 0; n < NT; n++)
 #pragma unroll
                 for (int i = 0; i < 4; i++) S[m][n][i] *= gl;
-            gemm16s<NT, true, true, Pl<T>::in>(S[m], Ks + 64 * m + 16 * rb, LK, Us + H * hf, LS, 0, C);
-#pragma unroll
-            for (int n = 0; n < NT; n++)
-#pragma unroll
-                for (int i = 0; i < 4; i++)
-                    Ms[(H * hf + 8 * n + 2 * t + (i & 1)) * LK + 64 * m + 16 * rb + g + 8 * (i >> 1)] = split_pair(S[m][n][i]);
+            gemm<NT, true, true, IN, 3>(S[m], Ks + 64 * m + 16 * rb, LK, L::PK, Us + H * hf, LS, L::PR, 0, C);
+            put_state(m);
         }
         if (c + 1 < count) commit(buf ^ 1);
         __syncthreads();
@@ -370,13 +377,19 @@ __device__ __forceinline__ void store_rows(T* out, const float (&acc)[4][4], int
 }
 
 // ── forward outputs ──
-// Eight warps: warp = 16 tokens x 32 of the tile's 64 columns.
+// Eight warps: warp = 16 tokens x 32 of the tile's 64 columns. For bf16 the state, P and U are two planes: y is rounded to bf16.
+template <typename T> struct OutFwdSmem {
+    static constexpr int PS = C * LP, IN = Pl<T>::in, O = Pl<T>::out, KP = IN > O ? IN : O;      // P goes where K was
+    static constexpr int BYTES = 2 * PS * (IN + KP + O);
+};
 template <typename T>
-__global__ void __launch_bounds__(256) gd_out_fwd_kernel(Args A)
+__global__ void __launch_bounds__(256, Pl<T>::in == 1 ? 3 : 2) gd_out_fwd_kernel(Args A)
 {
+    typedef OutFwdSmem<T> L;
+    constexpr int PS = L::PS, IN = L::IN, O = L::O;
     extern __shared__ float4 smem4[];
-    float* Qs = reinterpret_cast<float*>(smem4);
-    float *Ks = Qs + C * LD, *Ms = Ks + C * LD;
+    bf* Qs = reinterpret_cast<bf*>(smem4);
+    bf *Ks = Qs + IN * PS, *Ms = Ks + L::KP * PS;
     __shared__ float4 s_gate[C];
     __shared__ float s_theta[C];
     const int slot = blockIdx.x / A.hv, h = blockIdx.x - slot * A.hv, n0 = blockIdx.y * 64;
@@ -387,54 +400,55 @@ __global__ void __launch_bounds__(256) gd_out_fwd_kernel(Args A)
     if (tid < C) { s_gate[tid] = A.gates[tile * C + tid]; s_theta[tid] = A.theta_eff[tile * C + tid]; }
     const T* kp = (const T*)A.k + ch.b * A.kb + ch.t0 * A.kt + (h / A.share) * A.kh;
     const T* qp = (const T*)A.q + ch.b * A.qb + ch.t0 * A.qt + (h / A.share) * A.qh;
-    constexpr int IN = Pl<T>::in, QP = Pl<T>::in == EXACT ? EXACT : Pl<T>::out, OUT = Pl<T>::out;
     float att[4][4], y[4][4];
     zero(att);
     zero(y);
     const bool need = 32 * hf <= 16 * rb + 15;
     for (int c0 = 0; c0 < A.dk; c0 += 64) {
         if (c0) __syncthreads();
-        load_tile<T, 64, 256>(Qs, LD, qp + c0, A.qt, ch.len, A.dk - c0);
-        load_tile<T, 64, 256>(Ks, LD, kp + c0, A.kt, ch.len, A.dk - c0);
-        load_own<64, 64, 256>(Ms, LD, A.m_chunk + (tile * A.dvp + n0) * A.dkp + c0, A.dkp);
+        load_tile<T, 64, 256>(Qs, LP, PS, qp + c0, A.qt, ch.len, A.dk - c0);
+        load_tile<T, 64, 256>(Ks, LP, PS, kp + c0, A.kt, ch.len, A.dk - c0);
+        load_own<O, 256>(Ms, A.m_chunk + (tile * A.dkp + c0) * A.dvp + n0, A.dvp);
         __syncthreads();
-        if (need) gemm16<4, false, false, IN, IN>(att, Qs + 16 * rb * LD, LD, Ks + 32 * hf * LD, LD, 0, 64);
-        gemm16<4, false, false, QP, OUT>(y, Qs + 16 * rb * LD, LD, Ms + 32 * hf * LD, LD, 0, 64);
+        if (need) gemm<4, false, false, IN, IN>(att, Qs + 16 * rb * LP, LP, PS, Ks + 32 * hf * LP, LP, PS, 0, 64);
+        gemm<4, false, true, IN, O>(y, Qs + 16 * rb * LP, LP, PS, Ms + 32 * hf, LP, PS, 0, 64);
     }
     __syncthreads();
-    float *Pt = Ks, *Us = Ms;
+    bf *Ps = Ks, *Us = Ms;
 #pragma unroll
     for (int n = 0; n < 4; n++)
 #pragma unroll
-        for (int i4 = 0; i4 < 4; i4++) {
-            const int i = 16 * rb + g + 8 * (i4 >> 1), j = 32 * hf + 8 * n + 2 * t + (i4 & 1);
-            const float4 gi = s_gate[i], gj = s_gate[j];
-            Pt[j * LD + i] = j <= i ? decay(make_float2(gi.x, gi.y), make_float2(gj.x, gj.y)) * A.scale * att[n][i4] : 0.f;
-            y[n][i4] *= A.scale * gi.z;
-        }
-    {
-        const float* ep = A.e + tile * C * A.dvp + n0;
+        for (int r = 0; r < 2; r++) {
+            const int i = 16 * rb + g + 8 * r, j = 32 * hf + 8 * n + 2 * t;
+            const float4 gi = s_gate[i];
+            float x[2];
 #pragma unroll
-        for (int i = 0; i < 4; i++) {
-            const int at = tid + i * 256, r = at >> 4, c = (at & 15) * 4;
-            float4 v = *reinterpret_cast<const float4*>(ep + (long long)r * A.dvp + c);
-            const float th = s_theta[r];
-            *reinterpret_cast<float4*>(Us + r * LD + c) = make_float4(v.x * th, v.y * th, v.z * th, v.w * th);
+            for (int e = 0; e < 2; e++) {
+                const float4 gj = s_gate[j + e];
+                x[e] = j + e <= i ? decay(make_float2(gi.x, gi.y), make_float2(gj.x, gj.y)) * A.scale * att[n][2 * r + e] : 0.f;
+                y[n][2 * r + e] *= A.scale * gi.z;
+            }
+            put2<O>(Ps + i * LP + j, PS, x[0], x[1]);
         }
-    }
+    load_own<O, 256>(Us, A.e + tile * C * A.dvp + n0, A.dvp, s_theta);
     __syncthreads();
-    gemm16<4, true, true, OUT, OUT>(y, Pt + 16 * rb, LD, Us + 32 * hf, LD, 0, 16 * (rb + 1));
+    gemm<4, false, true, O, O>(y, Ps + 16 * rb * LP, LP, PS, Us + 32 * hf, LP, PS, 0, 16 * (rb + 1));
     T* out = (T*)A.y + (ch.row0(A) * A.hv + h) * A.dv;
     store_rows<T>(out, y, 16 * rb, ch.len, n0 + 32 * hf, A.dv, (long long)A.hv * A.dv);
 }
 
 // ── backward, what needs no state gradient: F = P^T dY, and N = scale (e^G Q)^T dY into the place of D ──
+template <typename T> struct PreBwdSmem {
+    static constexpr int PS = C * LP, IN = Pl<T>::in, BYTES = 2 * PS * (2 * IN + 3 + 3);          // P^T goes where K was
+};
 template <typename T>
-__global__ void __launch_bounds__(256) gd_pre_bwd_kernel(Args A)
+__global__ void __launch_bounds__(256, 2) gd_pre_bwd_kernel(Args A)
 {
+    typedef PreBwdSmem<T> L;
+    constexpr int PS = L::PS, IN = L::IN;
     extern __shared__ float4 smem4[];
-    float* Qs = reinterpret_cast<float*>(smem4);
-    float *Ks = Qs + C * LD, *Ys = Ks + C * LD, *Yg = Ys + C * LD;
+    bf* Qs = reinterpret_cast<bf*>(smem4);
+    bf *Ys = Qs + IN * PS, *Ks = Ys + IN * PS, *Yg = Ks + 3 * PS;
     __shared__ float4 s_gate[C];
     const int slot = blockIdx.x / A.hv, h = blockIdx.x - slot * A.hv, n0 = blockIdx.y * 64;
     const Chunk ch = get_chunk(A, slot);
@@ -444,43 +458,54 @@ __global__ void __launch_bounds__(256) gd_pre_bwd_kernel(Args A)
     if (tid < C) s_gate[tid] = A.gates[tile * C + tid];
     const T* kp = (const T*)A.k + ch.b * A.kb + ch.t0 * A.kt + (h / A.share) * A.kh;
     const T* qp = (const T*)A.q + ch.b * A.qb + ch.t0 * A.qt + (h / A.share) * A.qh;
-    constexpr int IN = Pl<T>::in;
-    load_tile<T, 64, 256>(Ys, LD, (const T*)A.dy + ch.b * A.yb + ch.t0 * A.yt + h * A.yh + n0, A.yt, ch.len, A.dv - n0);
+    load_tile<T, 64, 256>(Ys, LP, PS, (const T*)A.dy + ch.b * A.yb + ch.t0 * A.yt + h * A.yh + n0, A.yt, ch.len, A.dv - n0);
     __syncthreads();
-    for (int i = tid; i < C * C; i += 256) Yg[(i >> 6) * LD + (i & 63)] = A.scale * s_gate[i >> 6].z * Ys[(i >> 6) * LD + (i & 63)];
+#pragma unroll
+    for (int i = 0; i < C * 32 / 256; i++) {
+        const int at = tid + i * 256, r = at >> 5, c = (at & 31) * 2;
+        const float2 v = get2<IN>(Ys + r * LP + c, PS);
+        const float s = A.scale * s_gate[r].z;
+        put2<3>(Yg + r * LP + c, PS, s * v.x, s * v.y);
+    }
     float att[4][4];                              // rows: j, columns: i >= j
     zero(att);
     const bool need = 32 * hf + 31 >= 16 * rb;
     for (int c0 = 0; c0 < A.dk; c0 += 64) {
         if (c0) __syncthreads();
-        load_tile<T, 64, 256>(Qs, LD, qp + c0, A.qt, ch.len, A.dk - c0);
-        load_tile<T, 64, 256>(Ks, LD, kp + c0, A.kt, ch.len, A.dk - c0);
+        load_tile<T, 64, 256>(Qs, LP, PS, qp + c0, A.qt, ch.len, A.dk - c0);
+        load_tile<T, 64, 256>(Ks, LP, PS, kp + c0, A.kt, ch.len, A.dk - c0);
         __syncthreads();
-        if (need) gemm16<4, false, false, IN, IN>(att, Ks + 16 * rb * LD, LD, Qs + 32 * hf * LD, LD, 0, 64);
-        float nn[4][4];                           // rows: dv, columns: dk
+        if (need) gemm<4, false, false, IN, IN>(att, Ks + 16 * rb * LP, LP, PS, Qs + 32 * hf * LP, LP, PS, 0, 64);
+        float nn[4][4];                           // rows: dk, columns: dv
         zero(nn);
-        gemm16<4, true, true, TWO, IN>(nn, Yg + 16 * rb, LD, Qs + 32 * hf, LD, 0, C);
-        float* np = A.d_chunk + (tile * A.dvp + n0) * A.dkp + c0 + 32 * hf;
+        gemm<4, true, true, IN, 3>(nn, Qs + 16 * rb, LP, PS, Yg + 32 * hf, LP, PS, 0, C);
+        float* np = A.d_chunk + (tile * A.dkp + c0) * A.dvp + n0 + 32 * hf;
 #pragma unroll
         for (int n = 0; n < 4; n++)
 #pragma unroll
             for (int r = 0; r < 2; r++)
-                st2(np + (16 * rb + g + 8 * r) * A.dkp + 8 * n + 2 * t, nn[n][2 * r], nn[n][2 * r + 1]);
+                st2(np + (16 * rb + g + 8 * r) * A.dvp + 8 * n + 2 * t, nn[n][2 * r], nn[n][2 * r + 1]);
     }
     __syncthreads();
-    float* Ps = Ks;                               // [i][j]
+    bf* Pt = Ks;                                  // [j][i]
 #pragma unroll
     for (int n = 0; n < 4; n++)
 #pragma unroll
-        for (int i4 = 0; i4 < 4; i4++) {
-            const int j = 16 * rb + g + 8 * (i4 >> 1), i = 32 * hf + 8 * n + 2 * t + (i4 & 1);
-            const float4 gi = s_gate[i], gj = s_gate[j];
-            Ps[i * LD + j] = j <= i ? decay(make_float2(gi.x, gi.y), make_float2(gj.x, gj.y)) * A.scale * att[n][i4] : 0.f;
+        for (int r = 0; r < 2; r++) {
+            const int j = 16 * rb + g + 8 * r, i = 32 * hf + 8 * n + 2 * t;
+            const float4 gj = s_gate[j];
+            float x[2];
+#pragma unroll
+            for (int e = 0; e < 2; e++) {
+                const float4 gi = s_gate[i + e];
+                x[e] = j <= i + e ? decay(make_float2(gi.x, gi.y), make_float2(gj.x, gj.y)) * A.scale * att[n][2 * r + e] : 0.f;
+            }
+            put2<3>(Pt + j * LP + i, PS, x[0], x[1]);
         }
     __syncthreads();
     float f[4][4];
     zero(f);
-    gemm16<4, true, true, TWO, IN>(f, Ps + 16 * rb, LD, Ys + 32 * hf, LD, 16 * rb, C);
+    gemm<4, false, true, 3, IN>(f, Pt + 16 * rb * LP, LP, PS, Ys + 32 * hf, LP, PS, 16 * rb, C);
     float* fp = A.f + tile * C * A.dvp + n0 + 32 * hf;
 #pragma unroll
     for (int n = 0; n < 4; n++)
@@ -495,12 +520,13 @@ __global__ void __launch_bounds__(256) gd_pre_bwd_kernel(Args A)
 template <typename T, int DKP, int NS>
 __global__ void __launch_bounds__(256, DKP == 64 ? 2 : 1) gd_state_bwd_kernel(Args A)
 {
-    constexpr int LK = DKP + 4, LS = NS + 2, MT = DKP / 64, NT = NS / 16, H = NS / 2;
+    typedef StateSmem<T, DKP, NS> L;
+    constexpr int LK = L::LK, LS = L::LS, MT = DKP / 64, NT = NS / 16, H = NS / 2, IN = Pl<T>::in;
     extern __shared__ float4 smem4[];
-    float* Kb = reinterpret_cast<float*>(smem4);
-    float* Ts = Kb + 2 * C * LK;
-    float2* Ds = reinterpret_cast<float2*>(Ts + C * LD);
-    float2 *Rs = Ds + NS * LK, *Us = Rs + C * LS;
+    bf* Ts = reinterpret_cast<bf*>(smem4);
+    bf* Kb = Ts + T_BYTES / 2;
+    bf* Ds = Kb + L::KB * IN * L::PK;
+    bf *Rs = Ds + 3 * L::PM, *Us = Rs + 3 * L::PR;
     __shared__ float4 s_gate[2][C];
     __shared__ float s_theta[2][C];
     const int nsl = A.dvp / NS, sl = blockIdx.x % nsl, p = blockIdx.x / nsl, h = p % A.hv, seq = p / A.hv;
@@ -509,47 +535,51 @@ __global__ void __launch_bounds__(256, DKP == 64 ? 2 : 1) gd_state_bwd_kernel(Ar
 
     float S[MT][NT][4];
     const float* dm = A.d_m_final ? A.d_m_final + ((long long)seq * A.hv + h) * A.dv * A.dk : nullptr;
+    auto put_state = [&](int m) {
 #pragma unroll
-    for (int m = 0; m < MT; m++)
+        for (int n = 0; n < NT; n++)
+#pragma unroll
+            for (int r = 0; r < 2; r++)
+                put2<3>(Ds + (64 * m + 16 * rb + g + 8 * r) * LS + H * hf + 8 * n + 2 * t, L::PM, S[m][n][2 * r], S[m][n][2 * r + 1]);
+    };
+#pragma unroll
+    for (int m = 0; m < MT; m++) {
 #pragma unroll
         for (int n = 0; n < NT; n++)
 #pragma unroll
             for (int i = 0; i < 4; i++) {
-                const int row = 64 * m + 16 * rb + g + 8 * (i >> 1), col = H * hf + 8 * n + 2 * t + (i & 1);
-                S[m][n][i] = dm && row < A.dk && n0 + col < A.dv ? dm[(long long)(n0 + col) * A.dk + row] : 0.f;
-                Ds[col * LK + row] = split_pair(S[m][n][i]);
+                const int row = 64 * m + 16 * rb + g + 8 * (i >> 1), col = n0 + H * hf + 8 * n + 2 * t + (i & 1);
+                S[m][n][i] = dm && row < A.dk && col < A.dv ? dm[(long long)col * A.dk + row] : 0.f;
             }
+        put_state(m);
+    }
     Prefetch<T, DKP, 256> pk;
-    Prefetch<float, 64, 256> pt;
+    PrefetchT<256> pt;
     GateRow pg;
-    float pf[NT][4], pn[MT][NT][4];
+    float2 pf[NT][2], pn[MT][NT][2];
     auto fetch = [&](int c) {
         const int slot = slot0 + c;
         const Chunk ch = get_chunk(A, slot);
         const long long tile = (long long)slot * A.hv + h;
         pk.load((const T*)A.k + ch.b * A.kb + ch.t0 * A.kt + (h / A.share) * A.kh, A.kt, ch.len, A.dk);
-        pt.load(A.tmat + tile * C * C, C, C, C);
+        pt.load(A.tmat + tile * T_BYTES);
         if (tid < C) { ldg(pg.g, reinterpret_cast<const float*>(A.gates + tile * C + tid)); ldg(pg.theta, A.theta_eff + tile * C + tid); }
         const float* fp = A.f + tile * C * A.dvp + n0;
-        const float* np = A.d_chunk + (tile * A.dvp + n0) * DKP;
+        const float* np = A.d_chunk + tile * DKP * A.dvp + n0;
 #pragma unroll
         for (int n = 0; n < NT; n++)
 #pragma unroll
-            for (int i = 0; i < 4; i++) {
-                const int row = 16 * rb + g + 8 * (i >> 1), col = H * hf + 8 * n + 2 * t + (i & 1);
-                if (!(i & 1)) {
-                    float2 x;
-                    ldg(x, fp + (long long)row * A.dvp + col);
-                    pf[n][i] = x.x;
-                    pf[n][i + 1] = x.y;
-                }
+            for (int r = 0; r < 2; r++) {
+                const int row = 16 * rb + g + 8 * r, col = H * hf + 8 * n + 2 * t;
+                ldg(pf[n][r], fp + (long long)row * A.dvp + col);
 #pragma unroll
-                for (int m = 0; m < MT; m++) ldg(pn[m][n][i], np + col * DKP + 64 * m + row);
+                for (int m = 0; m < MT; m++) ldg(pn[m][n][r], np + (64 * m + row) * A.dvp + col);
             }
     };
     auto commit = [&](int buf) {
-        pk.store(Kb + buf * C * LK, LK);
-        pt.store(Ts, LD);
+        if (L::KB == 1) __syncthreads();
+        pk.store(Kb + (L::KB == 1 ? 0 : buf) * IN * L::PK, LK, L::PK);
+        pt.store(Ts);
         if (tid < C) { s_gate[buf][tid] = pg.g; s_theta[buf][tid] = pg.theta; }
     };
     if (count > 0) { fetch(count - 1); commit(0); }
@@ -558,35 +588,35 @@ __global__ void __launch_bounds__(256, DKP == 64 ? 2 : 1) gd_state_bwd_kernel(Ar
         const int buf = (count - 1 - c) & 1, slot = slot0 + c;
         const Chunk ch = get_chunk(A, slot);
         const long long tile = (long long)slot * A.hv + h;
-        const float* Ks = Kb + buf * C * LK;
-        float f[NT][4], nn[MT][NT][4];
-        float* dc = A.d_chunk + (tile * A.dvp + n0) * DKP;
+        const bf* Ks = Kb + (L::KB == 1 ? 0 : buf) * IN * L::PK;
+        float2 f[NT][2], nn[MT][NT][2];
+        float* dc = A.d_chunk + tile * DKP * A.dvp + n0;
 #pragma unroll
         for (int n = 0; n < NT; n++)
 #pragma unroll
-            for (int i = 0; i < 4; i++) {
-                f[n][i] = pf[n][i];
+            for (int r = 0; r < 2; r++) {
+                f[n][r] = pf[n][r];
 #pragma unroll
                 for (int m = 0; m < MT; m++) {
-                    nn[m][n][i] = pn[m][n][i];
-                    dc[(H * hf + 8 * n + 2 * t + (i & 1)) * DKP + 64 * m + 16 * rb + g + 8 * (i >> 1)] = S[m][n][i];
+                    nn[m][n][r] = pn[m][n][r];
+                    st2(dc + (64 * m + 16 * rb + g + 8 * r) * A.dvp + H * hf + 8 * n + 2 * t, S[m][n][2 * r], S[m][n][2 * r + 1]);
                 }
             }
         if (c > 0) fetch(c - 1);
         float acc[NT][4];
         zero(acc);
-        gemm16s<NT, false, false, Pl<T>::in>(acc, Ks + 16 * rb * LK, LK, Ds + H * hf * LK, LK, 0, DKP);
+        gemm<NT, false, true, IN, 3>(acc, Ks + 16 * rb * LK, LK, L::PK, Ds + H * hf, LS, L::PM, 0, DKP);
 #pragma unroll
         for (int n = 0; n < NT; n++)
 #pragma unroll
-            for (int i = 0; i < 4; i++) {
-                const int row = 16 * rb + g + 8 * (i >> 1);
-                Rs[row * LS + H * hf + 8 * n + 2 * t + (i & 1)] =
-                    split_pair(s_theta[buf][row] * (f[n][i] + s_gate[buf][row].w * acc[n][i]));
+            for (int r = 0; r < 2; r++) {
+                const int row = 16 * rb + g + 8 * r;
+                const float wi = s_gate[buf][row].w, th = s_theta[buf][row];
+                put2<3>(Rs + row * LS + H * hf + 8 * n + 2 * t, L::PR, th * (f[n][r].x + wi * acc[n][2 * r]), th * (f[n][r].y + wi * acc[n][2 * r + 1]));
             }
         __syncthreads();
         zero(acc);
-        gemm16s<NT, true, true, TWO>(acc, Ts + 16 * rb, LD, Rs + H * hf, LS, 16 * rb, C);
+        gemm<NT, true, true, 3, 3>(acc, Ts + 16 * rb, LP, C * LP, Rs + H * hf, LS, L::PR, 16 * rb, C);
         float* xp = A.x + tile * C * A.dvp + n0;
         T* dv = (T*)A.d_v + (ch.row0(A) * A.hv + h) * A.dv + n0;
 #pragma unroll
@@ -596,8 +626,7 @@ __global__ void __launch_bounds__(256, DKP == 64 ? 2 : 1) gd_state_bwd_kernel(Ar
                 const int row = 16 * rb + g + 8 * r, col = H * hf + 8 * n + 2 * t;
                 const float a = acc[n][2 * r], b = acc[n][2 * r + 1], eg = -s_gate[buf][row].z;
                 st2(xp + (long long)row * A.dvp + col, a, b);
-                Us[row * LS + col] = split_pair(eg * a);
-                Us[row * LS + col + 1] = split_pair(eg * b);
+                put2<3>(Us + row * LS + col, L::PR, eg * a, eg * b);
                 if (row < ch.len) {
                     const bool none = fabsf(s_theta[buf][row]) <= THETA_TINY;     // theta was 0: so is the gradient of v
                     T* o = dv + (long long)row * A.hv * A.dv + col;
@@ -612,13 +641,12 @@ __global__ void __launch_bounds__(256, DKP == 64 ? 2 : 1) gd_state_bwd_kernel(Ar
 #pragma unroll
             for (int n = 0; n < NT; n++)
 #pragma unroll
-                for (int i = 0; i < 4; i++) S[m][n][i] = fmaf(gl, S[m][n][i], nn[m][n][i]);
-            gemm16s<NT, true, true, Pl<T>::in>(S[m], Ks + 64 * m + 16 * rb, LK, Us + H * hf, LS, 0, C);
-#pragma unroll
-            for (int n = 0; n < NT; n++)
-#pragma unroll
-                for (int i = 0; i < 4; i++)
-                    Ds[(H * hf + 8 * n + 2 * t + (i & 1)) * LK + 64 * m + 16 * rb + g + 8 * (i >> 1)] = split_pair(S[m][n][i]);
+                for (int r = 0; r < 2; r++) {
+                    S[m][n][2 * r] = fmaf(gl, S[m][n][2 * r], nn[m][n][r].x);
+                    S[m][n][2 * r + 1] = fmaf(gl, S[m][n][2 * r + 1], nn[m][n][r].y);
+                }
+            gemm<NT, true, true, IN, 3>(S[m], Ks + 64 * m + 16 * rb, LK, L::PK, Us + H * hf, LS, L::PR, 0, C);
+            put_state(m);
         }
         if (c > 0) commit(buf ^ 1);
         __syncthreads();
@@ -641,13 +669,18 @@ __global__ void __launch_bounds__(256, DKP == 64 ? 2 : 1) gd_state_bwd_kernel(Ar
 //   Mq_ij = scale e^{G_i - G_j} (dy_i.e_j) theta_j (j <= i),  Mb_ij = -e^{G_i - G_j} (x_i.e_j) theta_j (j < i)
 //   d_q = scale e^G dY M_0 + Mq K;  k as a query: -e^G X M_0 + Mb K;  k as a key: theta e^{G_L - G} E D + Mq^T Q + Mb^T K
 //   gradient of G_i: q_i.dq_i + k_i.(query part) - k_i.(key part), and <D, M_L> for the last one.
-// The tiles of dY, X and E make way for those of Q and K: 104 KB, two CTAs per SM.
+// Four tiles at a time in shared memory: dY, X, E with M_0, then with D; Mq, Mb, Q, K take their places. Two CTAs per SM.
+template <typename T> struct OutBwdSmem {
+    static constexpr int PS = C * LP, IN = Pl<T>::in, BYTES = 2 * PS * (IN + 9);
+};
 template <typename T>
 __global__ void __launch_bounds__(256, 2) gd_out_bwd_kernel(Args A)
 {
+    typedef OutBwdSmem<T> L;
+    constexpr int PS = L::PS, IN = L::IN;
     extern __shared__ float4 smem4[];
-    float* Ys = reinterpret_cast<float*>(smem4);
-    float *Xs = Ys + C * LD, *Es = Xs + C * LD, *Ms = Es + C * LD, *Mq = Ms + C * LD, *Mb = Mq + C * LD;
+    bf* Ys = reinterpret_cast<bf*>(smem4);
+    bf *Xs = Ys + IN * PS, *Es = Xs + 3 * PS, *Ms = Es + 3 * PS;
     __shared__ float4 s_gate[C];
     __shared__ float s_theta[C], s_row[2][C], s_red[8];
     const int slot = blockIdx.x / A.hv, h = blockIdx.x - slot * A.hv, kt = blockIdx.y, k0 = kt * 64;
@@ -655,103 +688,109 @@ __global__ void __launch_bounds__(256, 2) gd_out_bwd_kernel(Args A)
     if (ch.len <= 0) return;
     const long long tile = (long long)slot * A.hv + h;
     const int tid = threadIdx.x, lane = tid & 31, w = tid >> 5, rb = w & 3, hf = w >> 2, g = lane >> 2, t = lane & 3;
-    constexpr int IN = Pl<T>::in;
     if (tid < C) { s_gate[tid] = A.gates[tile * C + tid]; s_theta[tid] = A.theta_eff[tile * C + tid]; }
     const T* yp = (const T*)A.dy + ch.b * A.yb + ch.t0 * A.yt + h * A.yh;
-    const int ndv = A.dvp / 64;
     const bool need = 32 * hf <= 16 * rb + 15;
-    auto load_yxe = [&](int n0) {
-        load_tile<T, 64, 256>(Ys, LD, yp + n0, A.yt, ch.len, A.dv - n0);
-        load_own<64, 64, 256>(Xs, LD, A.x + tile * C * A.dvp + n0, A.dvp);
-        load_own<64, 64, 256>(Es, LD, A.e + tile * C * A.dvp + n0, A.dvp);
-    };
-    float dp[4][4], xe[4][4], xdot = 0.f;
+    float dp[4][4], xe[4][4], dq[4][4], kq[4][4], ks[4][4], xdot = 0.f, gsum = 0.f;
     zero(dp);
     zero(xe);
-    for (int n = 0; n < ndv; n++) {
-        if (n) __syncthreads();
-        load_yxe(64 * n);
-        __syncthreads();
-        if (need) {
-            gemm16<4, false, false, IN, TWO>(dp, Ys + 16 * rb * LD, LD, Es + 32 * hf * LD, LD, 0, 64);
-            gemm16<4, false, false, TWO, TWO>(xe, Xs + 16 * rb * LD, LD, Es + 32 * hf * LD, LD, 0, 64);
-        }
-        if (kt == 0) {
-            const float *xr = Xs + (tid >> 2) * LD + (tid & 3), *er = Es + (tid >> 2) * LD + (tid & 3);
-#pragma unroll
-            for (int i = 0; i < 64; i += 4) xdot = fmaf(xr[i], er[i], xdot);
-        }
-    }
-    if (kt == 0) {
-        xdot += __shfl_xor_sync(0xffffffffu, xdot, 1);
-        xdot += __shfl_xor_sync(0xffffffffu, xdot, 2);
-        const int r = tid >> 2;
-        if ((tid & 3) == 0 && r < ch.len) A.d_theta[(ch.row0(A) + r) * A.hv + h] = xdot / s_theta[r];
-    }
-#pragma unroll
-    for (int n = 0; n < 4; n++)
-#pragma unroll
-        for (int i4 = 0; i4 < 4; i4++) {
-            const int i = 16 * rb + g + 8 * (i4 >> 1), j = 32 * hf + 8 * n + 2 * t + (i4 & 1);
-            const float4 gi = s_gate[i], gj = s_gate[j];
-            const float d = j <= i ? decay(make_float2(gi.x, gi.y), make_float2(gj.x, gj.y)) * s_theta[j] : 0.f;
-            Mq[j * LD + i] = j <= i ? A.scale * d * dp[n][i4] : 0.f;
-            Mb[j * LD + i] = j < i ? -d * xe[n][i4] : 0.f;
-        }
-    float dq[4][4], kq[4][4], ks[4][4], gsum = 0.f;
     zero(dq);
     zero(kq);
     zero(ks);
-    for (int n = 0; n < ndv; n++) {
+    for (int n = 0; n < A.dvp; n += 64) {
+        if (n) __syncthreads();
+        load_tile<T, 64, 256>(Ys, LP, PS, yp + n, A.yt, ch.len, A.dv - n);
+        const long long at = (tile * A.dkp + k0) * A.dvp + n;
+        load_own<3, 256>(Ms, A.m_chunk + at, A.dvp);
+        const float *xg = A.x + tile * C * A.dvp + n, *eg = A.e + tile * C * A.dvp + n;
+#pragma unroll
+        for (int i = 0; i < 4; i++) {             // X and E; the gradient of theta is x.e / theta
+            const int r = (tid + i * 256) >> 4, c = (tid & 15) * 4;
+            const float4 x = *reinterpret_cast<const float4*>(xg + (long long)r * A.dvp + c);
+            const float4 e = *reinterpret_cast<const float4*>(eg + (long long)r * A.dvp + c);
+            put4<3>(Xs + r * LP + c, PS, x);
+            put4<3>(Es + r * LP + c, PS, e);
+            float s = x.x * e.x + x.y * e.y + x.z * e.z + x.w * e.w;      // 16 lanes hold a row
+#pragma unroll
+            for (int o = 8; o > 0; o >>= 1) s += __shfl_xor_sync(0xffffffffu, s, o);
+            if ((tid & 15) == i) xdot += s;       // lane i keeps row (tid + 256 i) / 16
+        }
         __syncthreads();
-        if (ndv > 1) load_yxe(64 * n);
-        const long long at = (tile * A.dvp + 64 * n) * A.dkp + k0;
-        load_own<64, 64, 256>(Ms, LD, A.m_chunk + at, A.dkp);
+        if (need) {
+            gemm<4, false, false, IN, 3>(dp, Ys + 16 * rb * LP, LP, PS, Es + 32 * hf * LP, LP, PS, 0, 64);
+            gemm<4, false, false, 3, 3>(xe, Xs + 16 * rb * LP, LP, PS, Es + 32 * hf * LP, LP, PS, 0, 64);
+        }
+        gemm<4, false, false, IN, 3>(dq, Ys + 16 * rb * LP, LP, PS, Ms + 32 * hf * LP, LP, PS, 0, 64);
+        gemm<4, false, false, 3, 3>(kq, Xs + 16 * rb * LP, LP, PS, Ms + 32 * hf * LP, LP, PS, 0, 64);
         __syncthreads();
-        gemm16<4, false, true, IN, TWO>(dq, Ys + 16 * rb * LD, LD, Ms + 32 * hf, LD, 0, 64);
-        gemm16<4, false, true, TWO, TWO>(kq, Xs + 16 * rb * LD, LD, Ms + 32 * hf, LD, 0, 64);
-        __syncthreads();
-        const float* dc = A.d_chunk + at;
         float s = 0.f;
 #pragma unroll
         for (int i = 0; i < 4; i++) {
-            const int at4 = tid + i * 256, r = at4 >> 4, c = (at4 & 15) * 4;
-            const float4 v = *reinterpret_cast<const float4*>(dc + (long long)r * A.dkp + c);
-            float4* m = reinterpret_cast<float4*>(Ms + r * LD + c);
-            s += v.x * m->x + v.y * m->y + v.z * m->z + v.w * m->w;
-            *m = v;
+            const int r = (tid + i * 256) >> 4, c = (tid & 15) * 4;
+            const long long o = at + (long long)r * A.dvp + c;
+            const float4 v = *reinterpret_cast<const float4*>(A.d_chunk + o), m = *reinterpret_cast<const float4*>(A.m_chunk + o);
+            s += v.x * m.x + v.y * m.y + v.z * m.z + v.w * m.w;
+            put4<3>(Ms + r * LP + c, PS, v);
         }
         gsum = fmaf(s_gate[C - 1].z, s, gsum);
         __syncthreads();
-        gemm16<4, false, true, TWO, TWO>(ks, Es + 16 * rb * LD, LD, Ms + 32 * hf, LD, 0, 64);
+        gemm<4, false, false, 3, 3>(ks, Es + 16 * rb * LP, LP, PS, Ms + 32 * hf * LP, LP, PS, 0, 64);
+    }
+    if (kt == 0 && (tid & 15) < 4) {
+        const int r = (tid + (tid & 15) * 256) >> 4;
+        if (r < ch.len) A.d_theta[(ch.row0(A) + r) * A.hv + h] = xdot / s_theta[r];
     }
     __syncthreads();
-    float *Qs = Ys, *Ks = Xs;
-    load_tile<T, 64, 256>(Qs, LD, (const T*)A.q + ch.b * A.qb + ch.t0 * A.qt + (h / A.share) * A.qh + k0, A.qt, ch.len, A.dk - k0);
-    load_tile<T, 64, 256>(Ks, LD, (const T*)A.k + ch.b * A.kb + ch.t0 * A.kt + (h / A.share) * A.kh + k0, A.kt, ch.len, A.dk - k0);
+    bf *Mq = Xs, *Mb = Es, *Qs = Ys, *Ks = Ms;
+    load_tile<T, 64, 256>(Qs, LP, PS, (const T*)A.q + ch.b * A.qb + ch.t0 * A.qt + (h / A.share) * A.qh + k0, A.qt, ch.len, A.dk - k0);
+    load_tile<T, 64, 256>(Ks, LP, PS, (const T*)A.k + ch.b * A.kb + ch.t0 * A.kt + (h / A.share) * A.kh + k0, A.kt, ch.len, A.dk - k0);
+#pragma unroll
+    for (int n = 0; n < 4; n++)
+#pragma unroll
+        for (int r = 0; r < 2; r++) {
+            const int i = 16 * rb + g + 8 * r, j = 32 * hf + 8 * n + 2 * t;
+            const float4 gi = s_gate[i];
+            float a[2], b[2];
+#pragma unroll
+            for (int e = 0; e < 2; e++) {
+                const float4 gj = s_gate[j + e];
+                const float d = j + e <= i ? decay(make_float2(gi.x, gi.y), make_float2(gj.x, gj.y)) * s_theta[j + e] : 0.f;
+                a[e] = j + e <= i ? A.scale * d * dp[n][2 * r + e] : 0.f;
+                b[e] = j + e < i ? -d * xe[n][2 * r + e] : 0.f;
+            }
+            put2<3>(Mq + i * LP + j, PS, a[0], a[1]);
+            put2<3>(Mb + i * LP + j, PS, b[0], b[1]);
+        }
     __syncthreads();
 #pragma unroll
     for (int n = 0; n < 4; n++)
 #pragma unroll
-        for (int i4 = 0; i4 < 4; i4++) {
-            const int i = 16 * rb + g + 8 * (i4 >> 1), col = 32 * hf + 8 * n + 2 * t + (i4 & 1);
-            dq[n][i4] *= A.scale * s_gate[i].z;
-            kq[n][i4] *= -s_gate[i].z;
-            ks[n][i4] *= s_theta[i] * s_gate[i].w;
-            gsum = fmaf(Ks[i * LD + col], ks[n][i4], gsum);
+        for (int r = 0; r < 2; r++) {
+            const int i = 16 * rb + g + 8 * r, col = 32 * hf + 8 * n + 2 * t;
+            const float2 k2 = get2<IN>(Ks + i * LP + col, PS);
+            const float eg = s_gate[i].z, wt = s_theta[i] * s_gate[i].w;
+#pragma unroll
+            for (int e = 0; e < 2; e++) {
+                dq[n][2 * r + e] *= A.scale * eg;
+                kq[n][2 * r + e] *= -eg;
+                ks[n][2 * r + e] *= wt;
+            }
+            gsum += k2.x * ks[n][2 * r] + k2.y * ks[n][2 * r + 1];
         }
-    gemm16<4, true, true, TWO, IN>(dq, Mq + 16 * rb, LD, Ks + 32 * hf, LD, 0, 16 * (rb + 1));
-    gemm16<4, true, true, TWO, IN>(kq, Mb + 16 * rb, LD, Ks + 32 * hf, LD, 0, 16 * (rb + 1));
-    gemm16<4, false, true, TWO, IN>(ks, Mq + 16 * rb * LD, LD, Qs + 32 * hf, LD, 16 * rb, C);
-    gemm16<4, false, true, TWO, IN>(ks, Mb + 16 * rb * LD, LD, Ks + 32 * hf, LD, 16 * rb, C);
+    gemm<4, false, true, 3, IN>(dq, Mq + 16 * rb * LP, LP, PS, Ks + 32 * hf, LP, PS, 0, 16 * (rb + 1));
+    gemm<4, false, true, 3, IN>(kq, Mb + 16 * rb * LP, LP, PS, Ks + 32 * hf, LP, PS, 0, 16 * (rb + 1));
+    gemm<4, true, true, 3, IN>(ks, Mq + 16 * rb, LP, PS, Qs + 32 * hf, LP, PS, 16 * rb, C);
+    gemm<4, true, true, 3, IN>(ks, Mb + 16 * rb, LP, PS, Ks + 32 * hf, LP, PS, 16 * rb, C);
     float row[2] = {0.f, 0.f};
 #pragma unroll
     for (int n = 0; n < 4; n++)
 #pragma unroll
-        for (int i4 = 0; i4 < 4; i4++) {
-            const int i = 16 * rb + g + 8 * (i4 >> 1), col = 32 * hf + 8 * n + 2 * t + (i4 & 1);
-            row[i4 >> 1] += Qs[i * LD + col] * dq[n][i4] + Ks[i * LD + col] * (kq[n][i4] - ks[n][i4]);
-            kq[n][i4] += ks[n][i4];
+        for (int r = 0; r < 2; r++) {
+            const int i = 16 * rb + g + 8 * r, col = 32 * hf + 8 * n + 2 * t;
+            const float2 q2 = get2<IN>(Qs + i * LP + col, PS), k2 = get2<IN>(Ks + i * LP + col, PS);
+            row[r] += q2.x * dq[n][2 * r] + q2.y * dq[n][2 * r + 1] + k2.x * (kq[n][2 * r] - ks[n][2 * r]) + k2.y * (kq[n][2 * r + 1] - ks[n][2 * r + 1]);
+            kq[n][2 * r] += ks[n][2 * r];
+            kq[n][2 * r + 1] += ks[n][2 * r + 1];
         }
 #pragma unroll
     for (int r = 0; r < 2; r++) {
@@ -974,7 +1013,7 @@ static int64_t place_saved(Args& A, char* base)
     const int64_t tiles = (int64_t)A.slots * A.hv;
     int64_t at = 0;
     auto take = [&](int64_t bytes) { char* p = base + at; at += (bytes + 255) & ~(int64_t)255; return (void*)p; };
-    A.tmat = (float*)take(tiles * C * C * 4);
+    A.tmat = (unsigned char*)take(tiles * T_BYTES);
     A.gates = (float4*)take(tiles * C * 16);
     A.theta_eff = (float*)take(tiles * C * 4);
     A.e = (float*)take(tiles * C * A.dvp * 4);
@@ -1011,14 +1050,12 @@ template <typename K> static bool allow_smem(K kernel, int bytes, const char* wh
     return false;
 }
 
-constexpr int TILE_BYTES = C * LD * 4;
-
 template <typename T, int DKP, int NS>
 static bool launch_states_ns(const Args& A, long long heads, bool backward, cudaStream_t st, const char* where)
 {
     const long long grid = heads * (A.dvp / NS);
     if (grid >= (1LL << 31)) { record_status(NLH_ERR_INVALID_ARG, where, "too many sequences"); return false; }
-    constexpr int bytes = StateSmem<DKP, NS>::BYTES;
+    constexpr int bytes = StateSmem<T, DKP, NS>::BYTES;
     if (backward) {
         if (!allow_smem(gd_state_bwd_kernel<T, DKP, NS>, bytes, where)) return false;
         gd_state_bwd_kernel<T, DKP, NS><<<(unsigned)grid, 256, bytes, st>>>(A);
@@ -1044,14 +1081,16 @@ template <typename T> static bool run_forward(Args& A, cudaStream_t st, const ch
     }
     const unsigned tiles = (unsigned)((long long)A.slots * A.hv);
     if (tiles) {
-        if (!allow_smem(gd_prep_kernel<T>, 3 * TILE_BYTES, where)) return false;
-        gd_prep_kernel<T><<<tiles, 128, 3 * TILE_BYTES, st>>>(A);
+        constexpr int bytes = 2 * C * LD * 4 + Pl<T>::in * C * LP * 2 > 3 * C * LD * 4 ? 2 * C * LD * 4 + Pl<T>::in * C * LP * 2 : 3 * C * LD * 4;
+        if (!allow_smem(gd_prep_kernel<T>, bytes, where)) return false;
+        gd_prep_kernel<T><<<tiles, 128, bytes, st>>>(A);
         if (!check_launch(where)) return false;
     }
     if (!(A.dkp == 64 ? launch_states<T, 64>(A, false, st, where) : launch_states<T, 128>(A, false, st, where))) return false;
     if (tiles) {
-        if (!allow_smem(gd_out_fwd_kernel<T>, 3 * TILE_BYTES, where)) return false;
-        gd_out_fwd_kernel<T><<<dim3(tiles, A.dvp / 64), 256, 3 * TILE_BYTES, st>>>(A);
+        constexpr int bytes = OutFwdSmem<T>::BYTES;
+        if (!allow_smem(gd_out_fwd_kernel<T>, bytes, where)) return false;
+        gd_out_fwd_kernel<T><<<dim3(tiles, A.dvp / 64), 256, bytes, st>>>(A);
         if (!check_launch(where)) return false;
     }
     return true;
@@ -1061,14 +1100,16 @@ template <typename T> static bool run_backward(Args& A, cudaStream_t st, const c
 {
     const unsigned tiles = (unsigned)((long long)A.slots * A.hv);
     if (tiles) {
-        if (!allow_smem(gd_pre_bwd_kernel<T>, 4 * TILE_BYTES, where)) return false;
-        gd_pre_bwd_kernel<T><<<dim3(tiles, A.dvp / 64), 256, 4 * TILE_BYTES, st>>>(A);
+        constexpr int bytes = PreBwdSmem<T>::BYTES;
+        if (!allow_smem(gd_pre_bwd_kernel<T>, bytes, where)) return false;
+        gd_pre_bwd_kernel<T><<<dim3(tiles, A.dvp / 64), 256, bytes, st>>>(A);
         if (!check_launch(where)) return false;
     }
     if (!(A.dkp == 64 ? launch_states<T, 64>(A, true, st, where) : launch_states<T, 128>(A, true, st, where))) return false;
     if (!tiles) return true;
-    if (!allow_smem(gd_out_bwd_kernel<T>, 6 * TILE_BYTES, where)) return false;
-    gd_out_bwd_kernel<T><<<dim3(tiles, A.dkp / 64), 256, 6 * TILE_BYTES, st>>>(A);
+    constexpr int bytes = OutBwdSmem<T>::BYTES;
+    if (!allow_smem(gd_out_bwd_kernel<T>, bytes, where)) return false;
+    gd_out_bwd_kernel<T><<<dim3(tiles, A.dkp / 64), 256, bytes, st>>>(A);
     if (!check_launch(where)) return false;
     gd_gate_bwd_kernel<<<(tiles + 3) / 4, 128, 0, st>>>(A);
     if (!check_launch(where)) return false;

@@ -8,12 +8,14 @@
 //   M_L = e^{G_L} M_0 + (diag(theta e^{G_L - G}) E)^T K.
 // theta scales the columns of B, not the rows, so that no gradient has to divide by a theta that may be 0.
 //
-// Products run on the tensor cores as tf32 (mma.sync m16n8k8). A fp32 operand is split into two tf32 numbers
-// (22 significand bits) and the product takes three passes, low terms first; an operand that came in as bf16 is
-// exact in one. A product whose result is rounded to bf16 takes one pass with operands rounded to tf32 (11 bits,
-// 2^-12 of the value against the result's 2^-9). Why not tcgen05: the matrices are 64 x 64 x 64 and each depends
-// on the one before it. One M64 N64 K16 tcgen05.mma takes 55 cycles (1190 multiply-adds a cycle), a bf16
-// mma.sync 983, a tf32 one 486, and the results of mma.sync are in registers where the next product needs
+// Products run on the tensor cores in bf16 (mma.sync m16n8k16) with fp32 sums. A fp32 operand is split into three bf16 planes
+// (24 significand bits) when it is written to shared memory, and a product of two such takes six passes, smallest terms
+// first; an operand that came in as bf16 is one plane, exact. A result that is rounded to bf16 is computed from two planes
+// (16 bits against the result's 8). Two tf32 numbers for a fp32 one take the same time on the tensor cores, but their splitting,
+// redone by every warp that reads them, and twice the instructions around each pass held the kernels at 40 % of it:
+// 64 sequences x 8 heads x 512 tokens fp32, forward and backward, TF32_TIME us against PLANE_TIME.
+// Why not tcgen05: the matrices are 64 x 64 x 64 and each depends on the one before it. One M64 N64 K16 tcgen05.mma takes 55
+// cycles (1190 multiply-adds a cycle), mma.sync does 983, and its results are in registers where the next product needs
 // them; tcgen05 needs a commit, a wait and a trip through TMEM and shared memory for each.
 #pragma once
 
@@ -25,7 +27,9 @@ namespace nlh {
 namespace gd {
 
 constexpr int C = 64;          // tokens per chunk
-constexpr int LD = 68;         // floats between rows of a 64-column tile: = 4 (mod 32), see gemm16
+constexpr int LD = 68;         // floats between rows of a 64-column fp32 tile
+constexpr int LP = 72;         // bf16 between rows of a 64-column plane: 16-byte pieces of eight rows hit all banks
+constexpr int T_BYTES = 3 * C * LP * 2;    // the three planes of T, in global memory as they are in shared memory
 constexpr float G_FLOOR = -200.f;      // e^-200 is 0 in fp32: a retention of 0 (g = -inf) without inf - inf
 constexpr float THETA_TINY = 8.673617379884035e-19f;   // 2^-60, see gd_prep_kernel
 
@@ -38,11 +42,11 @@ struct Args {
     float scale;
     int slots, nc;                     // chunk slots; chunks per sequence of a dense batch
     // private buffers, one tile per slot and value head
-    float* tmat;                       // [slot, hv, 64, 64]
+    unsigned char* tmat;               // [slot, hv] three planes of T, T_BYTES each
     float4* gates;                     // [slot, hv, 64] {G high, G low, e^G, e^(G_L - G)}
     float* theta_eff;                  // [slot, hv, 64]
     float* e;                          // [slot, hv, 64, dvp]
-    float* m_chunk;                    // [slot, hv, dvp, dkp] state in front of the chunk
+    float* m_chunk;                    // [slot, hv, dkp, dvp] state in front of the chunk, transposed
     int4* map;                         // [slot] {sequence, first token, length, -} of a ragged batch
     int *start, *off;                  // [n_seqs + 1] first token and first slot of each sequence
     void* y;
@@ -98,190 +102,182 @@ __device__ __forceinline__ float4 ld4(const __nv_bfloat16* p)
     return make_float4(a.x, a.y, b.x, b.y);
 }
 
-// rows x COLS of a strided matrix -> shared memory, zero outside [0, rows) x [0, cols). `base` points at column 0 of
-// row 0. Vector loads where every row start is aligned to four elements and cols is a multiple of 4.
+// ── bf16 planes in shared memory ──
+typedef __nv_bfloat16 bf;
+template <typename T> struct Pl { static constexpr int in = 3, out = 3; };      // planes of an input, of an operand of y
+template <> struct Pl<__nv_bfloat16> { static constexpr int in = 1, out = 2; };
+
+__device__ __forceinline__ unsigned pack2(float x, float y)
+{
+    const __nv_bfloat162 h = __floats2bfloat162_rn(x, y);
+    return *reinterpret_cast<const unsigned*>(&h);
+}
+__device__ __forceinline__ float lo_f(unsigned u) { return __uint_as_float(u << 16); }
+__device__ __forceinline__ float hi_f(unsigned u) { return __uint_as_float(u & 0xffff0000u); }
+// Two neighbouring values -> P planes, `ps` elements apart. What a plane leaves over is exact in fp32.
+template <int P> __device__ __forceinline__ void put2(bf* p, int ps, float x, float y)
+{
+#pragma unroll
+    for (int i = 0; i < P; i++) {
+        const unsigned h = pack2(x, y);
+        *reinterpret_cast<unsigned*>(p + i * ps) = h;
+        if (i + 1 < P) { x -= lo_f(h); y -= hi_f(h); }
+    }
+}
+template <int P> __device__ __forceinline__ float2 get2(const bf* p, int ps)
+{
+    float2 r = make_float2(0.f, 0.f);
+#pragma unroll
+    for (int i = P - 1; i >= 0; i--) {
+        const unsigned h = *reinterpret_cast<const unsigned*>(p + i * ps);
+        r.x += lo_f(h);
+        r.y += hi_f(h);
+    }
+    return r;
+}
+template <int P> __device__ __forceinline__ void put4(bf* p, int ps, float4 v)
+{
+#pragma unroll
+    for (int i = 0; i < P; i++) {
+        const unsigned a = pack2(v.x, v.y), b = pack2(v.z, v.w);
+        *reinterpret_cast<uint2*>(p + i * ps) = make_uint2(a, b);
+        if (i + 1 < P) { v.x -= lo_f(a); v.y -= hi_f(a); v.z -= lo_f(b); v.w -= hi_f(b); }
+    }
+}
+// Four elements of an input as they came -> its planes.
+__device__ __forceinline__ void put_raw(bf* p, int ps, float4 v) { put4<3>(p, ps, v); }
+__device__ __forceinline__ void put_raw(bf* p, int ps, uint2 v) { *reinterpret_cast<uint2*>(p) = v; }
+__device__ __forceinline__ void put_one(bf* p, int ps, float x)
+{
+#pragma unroll
+    for (int i = 0; i < 3; i++) { p[i * ps] = __float2bfloat16(x); x -= __bfloat162float(p[i * ps]); }
+}
+__device__ __forceinline__ void put_one(bf* p, int ps, bf x) { *p = x; }
+
+template <typename T> struct Raw { typedef float4 type; };
+template <> struct Raw<bf> { typedef uint2 type; };
+template <typename T> __device__ __forceinline__ bool vec_ok(const T* base, long long stride, int cols)
+{
+    return ((reinterpret_cast<uintptr_t>(base) | (uintptr_t)(stride * (long long)sizeof(T))) & (4 * sizeof(T) - 1)) == 0 && (cols & 3) == 0;
+}
+
+// 64 x COLS of a strided input -> its planes, zero outside [0, rows) x [0, cols). `base` points at column 0 of row 0. Vector loads
+// where every row start is aligned to four elements and cols is a multiple of 4.
 template <typename T, int COLS, int THREADS>
-__device__ __forceinline__ void load_tile(float* dst, int ld, const T* base, long long stride, int rows, int cols)
+__device__ __forceinline__ void load_tile(bf* dst, int ld, int ps, const T* base, long long stride, int rows, int cols)
 {
     constexpr int PER_ROW = COLS / 4;
-    const bool vec = ((reinterpret_cast<uintptr_t>(base) | (uintptr_t)(stride * (long long)sizeof(T))) & (4 * sizeof(T) - 1)) == 0 &&
-                     (cols & 3) == 0;
-    if (vec) {
+    typedef typename Raw<T>::type R;
+    if (vec_ok(base, stride, cols)) {
 #pragma unroll
         for (int i = 0; i < C * PER_ROW / THREADS; i++) {
             const int at = threadIdx.x + i * THREADS, r = at / PER_ROW, c = (at - r * PER_ROW) * 4;
-            const float4 v = r < rows && c < cols ? ld4(base + r * stride + c) : make_float4(0.f, 0.f, 0.f, 0.f);
-            *reinterpret_cast<float4*>(dst + r * ld + c) = v;
+            R v = R{};
+            if (r < rows && c < cols) v = *reinterpret_cast<const R*>(base + r * stride + c);
+            put_raw(dst + r * ld + c, ps, v);
         }
     } else {
 #pragma unroll 4
         for (int i = 0; i < C * COLS / THREADS; i++) {
             const int at = threadIdx.x + i * THREADS, r = at / COLS, c = at - r * COLS;
-            dst[r * ld + c] = r < rows && c < cols ? to_f(base[r * stride + c]) : 0.f;
+            put_one(dst + r * ld + c, ps, r < rows && c < cols ? base[r * stride + c] : from_f<T>(0.f));
         }
     }
 }
-// The same for the private, padded buffers: always aligned, ROWS x COLS whole.
-template <int ROWS, int COLS, int THREADS>
-__device__ __forceinline__ void load_own(float* dst, int ld, const float* base, int stride)
+// 64 x 64 of a private, padded buffer, each row times scale[row] where a scale is given.
+template <int P, int THREADS>
+__device__ __forceinline__ void load_own(bf* dst, const float* base, int stride, const float* scale = nullptr)
 {
-    constexpr int PER_ROW = COLS / 4;
 #pragma unroll
-    for (int i = 0; i < ROWS * PER_ROW / THREADS; i++) {
-        const int at = threadIdx.x + i * THREADS, r = at / PER_ROW, c = (at - r * PER_ROW) * 4;
-        *reinterpret_cast<float4*>(dst + r * ld + c) = *reinterpret_cast<const float4*>(base + (long long)r * stride + c);
+    for (int i = 0; i < C * 16 / THREADS; i++) {
+        const int at = threadIdx.x + i * THREADS, r = at >> 4, c = (at & 15) * 4;
+        float4 v = *reinterpret_cast<const float4*>(base + (long long)r * stride + c);
+        if (scale) { const float s = scale[r]; v.x *= s; v.y *= s; v.z *= s; v.w *= s; }
+        put4<P>(dst + r * LP + c, C * LP, v);
     }
 }
 
-// ── tf32 products ──
-enum Planes { EXACT = 0, ONE = 1, TWO = 2 };   // operand exact in tf32; rounded to tf32; split into two
-
-// x = hi + lo, hi rounded to 11 bits by Dekker's splitting (the constant is 2^13 + 1). A NaN stays a NaN in hi, an infinity
-// or a value above 4e34 becomes one; adding half a unit to the bits instead would turn the NaN 0x7fffffff into -0.
-__device__ __forceinline__ float round_tf32(float x)
+// ── products ──
+__device__ __forceinline__ unsigned smem_addr(const void* p) { return (unsigned)__cvta_generic_to_shared(p); }
+template <bool TRANS> __device__ __forceinline__ void ldsm4(unsigned (&r)[4], unsigned a)
 {
-    const float c = __fmul_rn(x, 8193.f);
-    return __fsub_rn(c, __fsub_rn(c, x));
+    if (TRANS) asm volatile("ldmatrix.sync.aligned.m8n8.x4.trans.shared.b16 {%0,%1,%2,%3}, [%4];\n" : "=r"(r[0]), "=r"(r[1]), "=r"(r[2]), "=r"(r[3]) : "r"(a) : "memory");
+    else asm volatile("ldmatrix.sync.aligned.m8n8.x4.shared.b16 {%0,%1,%2,%3}, [%4];\n" : "=r"(r[0]), "=r"(r[1]), "=r"(r[2]), "=r"(r[3]) : "r"(a) : "memory");
 }
-template <int P>
-__device__ __forceinline__ void split(float x, unsigned& hi, unsigned& lo)
+template <bool TRANS> __device__ __forceinline__ void ldsm2(unsigned& r0, unsigned& r1, unsigned a)
 {
-    if (P == EXACT) { hi = __float_as_uint(x); return; }
-    const float h = round_tf32(x);
-    hi = __float_as_uint(h);
-    if (P == TWO) lo = __float_as_uint(__fsub_rn(x, h));
+    if (TRANS) asm volatile("ldmatrix.sync.aligned.m8n8.x2.trans.shared.b16 {%0,%1}, [%2];\n" : "=r"(r0), "=r"(r1) : "r"(a) : "memory");
+    else asm volatile("ldmatrix.sync.aligned.m8n8.x2.shared.b16 {%0,%1}, [%2];\n" : "=r"(r0), "=r"(r1) : "r"(a) : "memory");
 }
-__device__ __forceinline__ void mma_tf32(float (&c)[4], const unsigned (&a)[4], unsigned b0, unsigned b1)
+__device__ __forceinline__ void mma_bf16(float (&c)[4], const unsigned (&a)[4], unsigned b0, unsigned b1)
 {
-    asm volatile("mma.sync.aligned.m16n8k8.row.col.f32.tf32.tf32.f32 {%0,%1,%2,%3}, {%4,%5,%6,%7}, {%8,%9}, {%0,%1,%2,%3};\n"
+    asm volatile("mma.sync.aligned.m16n8k16.row.col.f32.bf16.bf16.f32 {%0,%1,%2,%3}, {%4,%5,%6,%7}, {%8,%9}, {%0,%1,%2,%3};\n"
                  : "+f"(c[0]), "+f"(c[1]), "+f"(c[2]), "+f"(c[3])
                  : "r"(a[0]), "r"(a[1]), "r"(a[2]), "r"(a[3]), "r"(b0), "r"(b1));
 }
-
-// One warp: acc (16 x 8 NT) += A (16 x K) B (K x 8 NT) over k in [k0, k1), both multiples of 8.
-// AK / BK: the operand is stored with k as its row index (A[k][m], B[k][n]) instead of A[m][k], B[n][k].
-// Rows are LD = 4 (mod 32) floats apart. A row of the product's k-step may take any eight k as long as both operands
-// agree: with k-rows in play lane t takes k + 2t and k + 2t + 1, which makes reads of k-rows free of bank conflicts
-// (bank 8t + g) and reads of the other kind 8-byte loads; without them it takes k + t and k + t + 4 (bank 4g + t).
-// The tensor core cuts its sums off instead of rounding them, and 24 of them on one accumulator add up to 1.4e-6; so
-// a k-step starts from 0 and is added to the accumulator with rounding: 2.4e-6 -> 3.5e-7 against 64 bits over a
-// training step of 512 tokens (a chunked form in fp32 FMA: 3.5e-7), for 12 % of the time.
+// One warp: acc (16 x 8 NT) += A (16 x K) B (K x 8 NT) over k in [k0, k1), multiples of 16.
+// AK / BK: the operand is stored with k as its row index (A[k][m], B[k][n]) instead of A[m][k], B[n][k]. PA, PB planes,
+// psa, psb elements apart. Terms of planes i and j with i + j below the larger count are taken.
+// The tensor core cuts its sums off instead of rounding them, and 24 of them on one accumulator add up to 1.4e-6; so a
+// k-step starts from 0 and is added to the accumulator with rounding.
 template <int NT, bool AK, bool BK, int PA, int PB>
-__device__ __forceinline__ void gemm16(float (&acc)[NT][4], const float* A, int lda, const float* B, int ldb, int k0, int k1)
+__device__ __forceinline__ void gemm(float (&acc)[NT][4], const bf* A, int lda, int psa, const bf* B, int ldb, int psb, int k0, int k1)
 {
-    const int lane = threadIdx.x & 31, g = lane >> 2, t = lane & 3;
-    constexpr bool PAIR = AK || BK;
+    constexpr int TOP = (PA > PB ? PA : PB) - 1;
+    const int l = threadIdx.x & 31, l8 = l & 7, q = l >> 3;
+    const unsigned a0 = smem_addr(AK ? A + ((q >> 1) * 8 + l8) * lda + (q & 1) * 8 : A + ((q & 1) * 8 + l8) * lda + (q >> 1) * 8);
+    const unsigned b0 = smem_addr(BK ? B + ((q & 1) * 8 + l8) * ldb + (q >> 1) * 8 : B + ((q >> 1) * 8 + l8) * ldb + (q & 1) * 8);
 #pragma unroll 2
-    for (int k = k0; k < k1; k += 8) {
-        float af[4];
-        if (AK) {
-            const float* p = A + (k + 2 * t) * lda + g;
-            af[0] = p[0]; af[1] = p[8]; af[2] = p[lda]; af[3] = p[lda + 8];
-        } else if (PAIR) {
-            const float2 x = *reinterpret_cast<const float2*>(A + g * lda + k + 2 * t);
-            const float2 y = *reinterpret_cast<const float2*>(A + (g + 8) * lda + k + 2 * t);
-            af[0] = x.x; af[2] = x.y; af[1] = y.x; af[3] = y.y;
-        } else {
-            const float* p = A + g * lda + k + t;
-            af[0] = p[0]; af[1] = p[8 * lda]; af[2] = p[4]; af[3] = p[8 * lda + 4];
-        }
-        unsigned ah[4], al[4];
+    for (int k = k0; k < k1; k += 16) {
+        unsigned a[PA][4];
 #pragma unroll
-        for (int i = 0; i < 4; i++) split<PA>(af[i], ah[i], al[i]);
+        for (int i = 0; i < PA; i++) ldsm4<AK>(a[i], a0 + 2 * (i * psa + (AK ? k * lda : k)));
 #pragma unroll
-        for (int n = 0; n < NT; n++) {
-            float b0, b1;
-            if (BK) {
-                const float* p = B + (k + 2 * t) * ldb + n * 8 + g;
-                b0 = p[0]; b1 = p[ldb];
-            } else if (PAIR) {
-                const float2 x = *reinterpret_cast<const float2*>(B + (n * 8 + g) * ldb + k + 2 * t);
-                b0 = x.x; b1 = x.y;
-            } else {
-                const float* p = B + (n * 8 + g) * ldb + k + t;
-                b0 = p[0]; b1 = p[4];
+        for (int n = 0; n < NT; n += 2) {
+            unsigned b[PB][4];
+#pragma unroll
+            for (int j = 0; j < PB; j++) {
+                const unsigned at = b0 + 2 * (j * psb + (BK ? k * ldb + n * 8 : k + n * 8 * ldb));
+                if (n + 1 < NT) ldsm4<BK>(b[j], at);
+                else ldsm2<BK>(b[j][0], b[j][1], at);
             }
-            unsigned h0, h1, l0, l1;
-            split<PB>(b0, h0, l0);
-            split<PB>(b1, h1, l1);
-            float s[4] = {0.f, 0.f, 0.f, 0.f};
-            if (PA == TWO) mma_tf32(s, al, h0, h1);
-            if (PB == TWO) mma_tf32(s, ah, l0, l1);
-            mma_tf32(s, ah, h0, h1);
 #pragma unroll
-            for (int i = 0; i < 4; i++) acc[n][i] += s[i];
+            for (int e = 0; e < 2; e++) {
+                if (n + e < NT) {
+                    float s[4] = {0.f, 0.f, 0.f, 0.f};
+#pragma unroll
+                    for (int o = TOP; o >= 0; o--)
+#pragma unroll
+                        for (int i = 0; i < PA; i++)
+                            if (o - i >= 0 && o - i < PB) mma_bf16(s, a[i], b[o - i][2 * e], b[o - i][2 * e + 1]);
+#pragma unroll
+                    for (int x = 0; x < 4; x++) acc[n + e][x] += s[x];
+                }
+            }
         }
     }
 }
-// The same with B split beforehand into pairs (hi, lo): a matrix that several warps read is split once, by who writes it.
-// B[n][k] rows are 4 (mod 16) pairs apart, B[k][n] rows 2 (mod 8), for 8-byte reads without bank conflicts.
-template <int NT, bool AK, bool BK, int PA>
-__device__ __forceinline__ void gemm16s(float (&acc)[NT][4], const float* A, int lda, const float2* B, int ldb, int k0, int k1)
+template <int NT> __device__ __forceinline__ void zero(float (&acc)[NT][4])
 {
-    const int lane = threadIdx.x & 31, g = lane >> 2, t = lane & 3;
-    constexpr bool PAIR = AK || BK;
-#pragma unroll 4
-    for (int k = k0; k < k1; k += 8) {
-        float af[4];
-        if (AK) {
-            const float* p = A + (k + 2 * t) * lda + g;
-            af[0] = p[0]; af[1] = p[8]; af[2] = p[lda]; af[3] = p[lda + 8];
-        } else if (PAIR) {
-            const float2 x = *reinterpret_cast<const float2*>(A + g * lda + k + 2 * t);
-            const float2 y = *reinterpret_cast<const float2*>(A + (g + 8) * lda + k + 2 * t);
-            af[0] = x.x; af[2] = x.y; af[1] = y.x; af[3] = y.y;
-        } else {
-            const float* p = A + g * lda + k + t;
-            af[0] = p[0]; af[1] = p[8 * lda]; af[2] = p[4]; af[3] = p[8 * lda + 4];
-        }
-        unsigned ah[4], al[4];
 #pragma unroll
-        for (int i = 0; i < 4; i++) split<PA>(af[i], ah[i], al[i]);
+    for (int n = 0; n < NT; n++)
 #pragma unroll
-        for (int n = 0; n < NT; n++) {
-            float2 b0, b1;
-            if (BK) {
-                const float2* p = B + (k + 2 * t) * ldb + n * 8 + g;
-                b0 = p[0]; b1 = p[ldb];
-            } else if (PAIR) {
-                const float2* p = B + (n * 8 + g) * ldb + k + 2 * t;
-                b0 = p[0]; b1 = p[1];
-            } else {
-                const float2* p = B + (n * 8 + g) * ldb + k + t;
-                b0 = p[0]; b1 = p[4];
-            }
-            float s[4] = {0.f, 0.f, 0.f, 0.f};
-            if (PA == TWO) mma_tf32(s, al, __float_as_uint(b0.x), __float_as_uint(b1.x));
-            mma_tf32(s, ah, __float_as_uint(b0.y), __float_as_uint(b1.y));
-            mma_tf32(s, ah, __float_as_uint(b0.x), __float_as_uint(b1.x));
-#pragma unroll
-            for (int i = 0; i < 4; i++) acc[n][i] += s[i];
-        }
-    }
-}
-__device__ __forceinline__ float2 split_pair(float x)
-{
-    const float h = round_tf32(x);
-    return make_float2(h, __fsub_rn(x, h));
+        for (int i = 0; i < 4; i++) acc[n][i] = 0.f;
 }
 
-// A tile on its way from global to shared memory, in registers: loaded while the chunk before it is computed. Rows that do
-// not allow vector loads are read when they are stored instead.
-template <typename T> struct Raw { typedef float4 type; };
-template <> struct Raw<__nv_bfloat16> { typedef uint2 type; };
-__device__ __forceinline__ float4 widen(float4 v) { return v; }
-__device__ __forceinline__ float4 widen(uint2 u)
-{
-    const float2 a = __bfloat1622float2(*reinterpret_cast<const __nv_bfloat162*>(&u.x));
-    const float2 b = __bfloat1622float2(*reinterpret_cast<const __nv_bfloat162*>(&u.y));
-    return make_float4(a.x, a.y, b.x, b.y);
-}
-// Loads that stay where they are written: left to itself the compiler moves them down to their first use.
+// e^{G_i - G_j} from the pairs (high, low)
+__device__ __forceinline__ float decay(float2 gi, float2 gj) { return expf((gi.x - gj.x) + (gi.y - gj.y)); }
+
+// ── loads that stay where they are written: left to itself the compiler moves them down to their first use ──
 __device__ __forceinline__ void ldg(float4& v, const float* p)
 {
     asm volatile("ld.global.v4.f32 {%0, %1, %2, %3}, [%4];\n" : "=f"(v.x), "=f"(v.y), "=f"(v.z), "=f"(v.w) : "l"(p));
 }
-__device__ __forceinline__ void ldg(uint2& v, const __nv_bfloat16* p)
+__device__ __forceinline__ void ldg(uint4& v, const void* p)
+{
+    asm volatile("ld.global.v4.u32 {%0, %1, %2, %3}, [%4];\n" : "=r"(v.x), "=r"(v.y), "=r"(v.z), "=r"(v.w) : "l"(p));
+}
+__device__ __forceinline__ void ldg(uint2& v, const bf* p)
 {
     asm volatile("ld.global.v2.u32 {%0, %1}, [%2];\n" : "=r"(v.x), "=r"(v.y) : "l"(p));
 }
@@ -290,7 +286,7 @@ __device__ __forceinline__ void ldg(float2& v, const float* p)
 {
     asm volatile("ld.global.v2.f32 {%0, %1}, [%2];\n" : "=f"(v.x), "=f"(v.y) : "l"(p));
 }
-__device__ __forceinline__ void ldg(unsigned& v, const __nv_bfloat16* p) { asm volatile("ld.global.u32 %0, [%1];\n" : "=r"(v) : "l"(p)); }
+__device__ __forceinline__ void ldg(unsigned& v, const bf* p) { asm volatile("ld.global.u32 %0, [%1];\n" : "=r"(v) : "l"(p)); }
 
 // Two neighbouring columns of a strided matrix, as they came; `pair` says that one load may take both.
 template <typename T> struct Pair;
@@ -304,20 +300,22 @@ template <> struct Pair<float> {
     }
     __device__ __forceinline__ float2 get() const { return r; }
 };
-template <> struct Pair<__nv_bfloat16> {
+template <> struct Pair<bf> {
     unsigned r;
-    __device__ __forceinline__ void load(const __nv_bfloat16* p, bool a, bool b, bool pair)
+    __device__ __forceinline__ void load(const bf* p, bool a, bool b, bool pair)
     {
         r = 0;
         if (pair) { if (a) ldg(r, p); }
         else {
-            const unsigned short *u = reinterpret_cast<const unsigned short*>(p);
+            const unsigned short* u = reinterpret_cast<const unsigned short*>(p);
             r = (a ? (unsigned)u[0] : 0u) | (b ? (unsigned)u[1] << 16 : 0u);
         }
     }
-    __device__ __forceinline__ float2 get() const { return make_float2(__uint_as_float(r << 16), __uint_as_float(r & 0xffff0000u)); }
+    __device__ __forceinline__ float2 get() const { return make_float2(lo_f(r), hi_f(r)); }
 };
 
+// A tile of an input on its way from global to shared memory, in registers: loaded while the chunk before it is computed. Rows
+// that do not allow vector loads are read when they are stored instead.
 template <typename T, int COLS, int THREADS> struct Prefetch {
     typedef typename Raw<T>::type R;
     static constexpr int PER_ROW = COLS / 4, N = C * PER_ROW / THREADS;
@@ -329,7 +327,7 @@ template <typename T, int COLS, int THREADS> struct Prefetch {
     __device__ __forceinline__ void load(const T* b, long long st, int nr, int nc)
     {
         base = b; stride = st; rows = nr; cols = nc;
-        vec = ((reinterpret_cast<uintptr_t>(b) | (uintptr_t)(st * (long long)sizeof(T))) & (4 * sizeof(T) - 1)) == 0 && (nc & 3) == 0;
+        vec = vec_ok(b, st, nc);
         if (!vec) return;
 #pragma unroll
         for (int i = 0; i < N; i++) {
@@ -338,31 +336,33 @@ template <typename T, int COLS, int THREADS> struct Prefetch {
             if (row < rows && c < cols) ldg(r[i], base + row * stride + c);
         }
     }
-    __device__ __forceinline__ void store(float* dst, int ld) const
+    __device__ __forceinline__ void store(bf* dst, int ld, int ps) const
     {
-        if (!vec) { load_tile<T, COLS, THREADS>(dst, ld, base, stride, rows, cols); return; }
+        if (!vec) { load_tile<T, COLS, THREADS>(dst, ld, ps, base, stride, rows, cols); return; }
 #pragma unroll
         for (int i = 0; i < N; i++) {
             const int at = threadIdx.x + i * THREADS, row = at / PER_ROW, c = (at - row * PER_ROW) * 4;
-            *reinterpret_cast<float4*>(dst + row * ld + c) = widen(r[i]);
+            put_raw(dst + row * ld + c, ps, r[i]);
         }
     }
 };
-
-template <int NT> __device__ __forceinline__ void zero(float (&acc)[NT][4])
-{
+// The planes of T, copied as they are.
+template <int THREADS> struct PrefetchT {
+    static constexpr int N = (T_BYTES / 16 + THREADS - 1) / THREADS;
+    uint4 r[N];
+    __device__ __forceinline__ void load(const unsigned char* p)
+    {
 #pragma unroll
-    for (int n = 0; n < NT; n++)
+        for (int i = 0; i < N; i++)
+            if ((int)threadIdx.x + i * THREADS < T_BYTES / 16) ldg(r[i], p + (threadIdx.x + i * THREADS) * 16);
+    }
+    __device__ __forceinline__ void store(bf* dst) const
+    {
 #pragma unroll
-        for (int i = 0; i < 4; i++) acc[n][i] = 0.f;
-}
-
-// e^{G_i - G_j} from the pairs (high, low)
-__device__ __forceinline__ float decay(float2 gi, float2 gj) { return expf((gi.x - gj.x) + (gi.y - gj.y)); }
-
-// Planes of an operand that came in as T, of a fp32 one, and of operands of a product that is stored as T.
-template <typename T> struct Pl { static constexpr int in = TWO, mid = TWO, out = TWO; };
-template <> struct Pl<__nv_bfloat16> { static constexpr int in = EXACT, mid = TWO, out = ONE; };
+        for (int i = 0; i < N; i++)
+            if ((int)threadIdx.x + i * THREADS < T_BYTES / 16) reinterpret_cast<uint4*>(dst)[threadIdx.x + i * THREADS] = r[i];
+    }
+};
 
 }  // namespace gd
 }  // namespace nlh
