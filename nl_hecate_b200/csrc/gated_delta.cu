@@ -858,48 +858,41 @@ __global__ void __launch_bounds__(256) gd_group_kernel(Args A, long long n)
 
 // ── recurrent step ──
 // Bound by the state: read once, written once. Eight lanes hold a row of M (dk / 8 numbers each, in groups of four so
-// that a row's 128-byte pieces are whole); a CTA holds `rows` rows of one head. Sequences that name the same slot are
-// stepped one after the other, in their order, by the CTA of the first: a slot behaves as if they came in as further tokens.
+// that a row's 128-byte pieces are whole), a thread RP rows at a time; a CTA holds `rows` rows of one head. Small CTAs, so that
+// some of an SM's load while others store: 256 x 16 states of 128 x 128 take 99 us (5.4 TB/s) with 64 rows a CTA and three
+// CTAs per SM, 128 us with two, 180 us with 128 rows and two.
+// Sequences that name the same slot are stepped one after the other, in their order, by the CTA of the first: a slot behaves
+// as if they came in as further tokens.
 template <typename T, int NV, bool VEC>
-__global__ void __launch_bounds__(256) gd_step_kernel(Args A, float* M, const int* slots, int pool, int rows)
+__global__ void __launch_bounds__(256, 3) gd_step_kernel(Args A, float* M, const int* slots, int pool, int rows)
 {
+    constexpr int RP = 8 / NV;
     const int per = (A.dv + rows - 1) / rows;
     const int part = blockIdx.x % per, p = blockIdx.x / per, h = p % A.hv, first = p / A.hv;
-    const int lane8 = threadIdx.x & 7, grp = threadIdx.x >> 3;
-    int slot = first, last = first + 1;                   // sequences first .. last - 1 may be of this slot
-    if (slots) {
-        slot = slots[first];
-        if (slot < 0 || slot >= pool) {                   // no sequence in this place
-            for (int i = threadIdx.x; i < A.seq * rows; i += 256) {
-                const int tok = i / rows, row = part * rows + i - tok * rows;
-                if (row < A.dv) ((T*)A.y)[(((long long)first * A.seq + tok) * A.hv + h) * A.dv + row] = from_f<T>(0.f);
-            }
-            return;
+    const int lane8 = threadIdx.x & 7, grp = threadIdx.x >> 3, end = min(A.dv, (part + 1) * rows);
+    const int slot = slots ? slots[first] : first;
+    if (slot < 0 || slot >= pool) {                       // no sequence in this place
+        for (int i = threadIdx.x; i < A.seq * rows; i += 256) {
+            const int tok = i / rows, row = part * rows + i - tok * rows;
+            if (row < A.dv) ((T*)A.y)[(((long long)first * A.seq + tok) * A.hv + h) * A.dv + row] = from_f<T>(0.f);
         }
-        bool seen = false, again = false;
-        for (int i = threadIdx.x; i < A.batch; i += 256) {
-            const bool same = slots[i] == slot;
-            seen |= same && i < first;
-            again |= same && i > first;
-        }
-        if (__syncthreads_or(seen)) return;
-        if (__syncthreads_or(again)) last = A.batch;
+        return;
     }
-    constexpr int RP = 4;                                 // rows a thread holds at a time
-    for (int r0 = part * rows; r0 < min(A.dv, (part + 1) * rows); r0 += 32 * RP) {
+    int last = first + 1;                                 // sequences first .. last - 1 may be of this slot
+    bool looked = slots == nullptr;
+    for (int r0 = part * rows; r0 < end; r0 += 32 * RP) {
         float4 m[RP][NV];
         float* base = M + ((long long)slot * A.hv + h) * A.dv * A.dk;
 #pragma unroll
         for (int r = 0; r < RP; r++) {
             const int row = r0 + grp + 32 * r;
-            const bool on = row < min(A.dv, (part + 1) * rows);
 #pragma unroll
             for (int v = 0; v < NV; v++) {
                 const int c = 4 * lane8 + 32 * v;
                 float4 x = make_float4(0.f, 0.f, 0.f, 0.f);
-                if (on) {
+                if (row < end) {
                     const float* s = base + (long long)row * A.dk + c;
-                    if (VEC) { if (c < A.dk) x = *reinterpret_cast<const float4*>(s); }
+                    if (VEC) { if (c < A.dk) ldg(x, s); }
                     else {
                         if (c < A.dk) x.x = s[0];
                         if (c + 1 < A.dk) x.y = s[1];
@@ -909,6 +902,17 @@ __global__ void __launch_bounds__(256) gd_step_kernel(Args A, float* M, const in
                 }
                 m[r][v] = x;
             }
+        }
+        if (!looked) {                                    // while the rows are on their way: who else names this slot?
+            looked = true;
+            bool seen = false, again = false;
+            for (int i = threadIdx.x; i < A.batch; i += 256) {
+                const bool same = slots[i] == slot;
+                seen |= same && i < first;
+                again |= same && i > first;
+            }
+            if (__syncthreads_or(seen)) return;
+            if (__syncthreads_or(again)) last = A.batch;
         }
         for (int b = first; b < last; b++) {
             if (b != first && slots[b] != slot) continue;
@@ -920,18 +924,25 @@ __global__ void __launch_bounds__(256) gd_step_kernel(Args A, float* M, const in
                 const float rt = expf(A.g[ga]), th = A.theta[ga];
                 float kf[NV][4], qf[NV][4];
 #pragma unroll
-                for (int v = 0; v < NV; v++)
+                for (int v = 0; v < NV; v++) {
+                    const int c = 4 * lane8 + 32 * v;
+                    if (VEC) {
+                        float4 a = make_float4(0.f, 0.f, 0.f, 0.f), o = a;
+                        if (c < A.dk) { a = ld4(kp + c); o = ld4(qp + c); }
+                        kf[v][0] = a.x; kf[v][1] = a.y; kf[v][2] = a.z; kf[v][3] = a.w;
+                        qf[v][0] = o.x; qf[v][1] = o.y; qf[v][2] = o.z; qf[v][3] = o.w;
+                    } else {
 #pragma unroll
-                    for (int i = 0; i < 4; i++) {
-                        const int c = 4 * lane8 + 32 * v + i;
-                        kf[v][i] = c < A.dk ? to_f(kp[c]) : 0.f;
-                        qf[v][i] = c < A.dk ? to_f(qp[c]) : 0.f;
+                        for (int i = 0; i < 4; i++) {
+                            kf[v][i] = c + i < A.dk ? to_f(kp[c + i]) : 0.f;
+                            qf[v][i] = c + i < A.dk ? to_f(qp[c + i]) : 0.f;
+                        }
                     }
+                }
 #pragma unroll
                 for (int r = 0; r < RP; r++) {
                     const int row = r0 + grp + 32 * r;
-                    const bool on = row < min(A.dv, (part + 1) * rows);
-                    const float val = on ? to_f(vp[row]) : 0.f;
+                    const float val = row < end ? to_f(vp[row]) : 0.f;
                     float s = 0.f;
 #pragma unroll
                     for (int v = 0; v < NV; v++) {
@@ -954,7 +965,7 @@ __global__ void __launch_bounds__(256) gd_step_kernel(Args A, float* M, const in
                     y += __shfl_xor_sync(0xffffffffu, y, 1);
                     y += __shfl_xor_sync(0xffffffffu, y, 2);
                     y += __shfl_xor_sync(0xffffffffu, y, 4);
-                    if (on && lane8 == 0)
+                    if (row < end && lane8 == 0)
                         ((T*)A.y)[(((long long)b * A.seq + tok) * A.hv + h) * A.dv + row] = from_f<T>(A.scale * y);
                 }
             }
@@ -962,7 +973,7 @@ __global__ void __launch_bounds__(256) gd_step_kernel(Args A, float* M, const in
 #pragma unroll
         for (int r = 0; r < RP; r++) {
             const int row = r0 + grp + 32 * r;
-            if (row >= min(A.dv, (part + 1) * rows)) continue;
+            if (row >= end) continue;
 #pragma unroll
             for (int v = 0; v < NV; v++) {
                 const int c = 4 * lane8 + 32 * v;
@@ -1208,13 +1219,15 @@ int32_t nlh_gated_delta_step(const nlh_gated_delta_desc* desc, const void* k, co
         return NLH_ERR_INVALID_ARG;
     }
     A.y = y;
-    // 128 rows a CTA (one round of its threads) while that gives every SM two CTAs, else 32
+    // one round of a CTA's threads (64 rows of dk > 64, 128 shorter ones) while that gives every SM two CTAs, else 32 rows
     const long long heads = (long long)A.batch * A.hv;
-    const int rows = heads * ((A.dv + 127) / 128) >= 2 * 148 ? 128 : 32;
+    const int full = A.dk > 64 ? 64 : 128, rows = heads * ((A.dv + full - 1) / full) >= 2 * 148 ? full : 32;
     const long long grid = heads * ((A.dv + rows - 1) / rows);
     if (grid >= (1LL << 31)) { record_status(NLH_ERR_INVALID_ARG, where, "too many sequences"); return NLH_ERR_INVALID_ARG; }
     cudaStream_t st = current_stream();
-    const bool vec = (A.dk & 3) == 0 && aligned16(m);
+    const int es = desc->is_bf16 ? 2 : 4;
+    const bool vec = (A.dk & 3) == 0 && aligned16(m) && (((uintptr_t)k | (uintptr_t)q) & (4 * es - 1)) == 0 &&
+                     ((A.kb | A.kt | A.kh | A.qb | A.qt | A.qh) & 3) == 0;
 #define NLH_GD_STEP(T, NV) (vec ? gd_step_kernel<T, NV, true><<<(unsigned)grid, 256, 0, st>>>(A, m, slots, n_slots, rows) \
                                 : gd_step_kernel<T, NV, false><<<(unsigned)grid, 256, 0, st>>>(A, m, slots, n_slots, rows))
     if (desc->is_bf16) { if (A.dk <= 64) NLH_GD_STEP(__nv_bfloat16, 2); else NLH_GD_STEP(__nv_bfloat16, 4); }

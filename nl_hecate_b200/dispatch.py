@@ -12,6 +12,7 @@ if the CUDA library is missing or records an error: there is no CPU path here.
 from __future__ import annotations
 
 import ctypes as C
+import struct
 
 import numpy as np
 import torch
@@ -355,35 +356,54 @@ def titans_frozen_stream_backward(k, v, q, alpha, theta, eta, ms, d_y, chunk, wa
 # k, q [B, S, Hk, dk], v [B, S, Hv, dv], log_retain, theta [B, S, Hv] fp32, any strides with a contiguous last
 # axis; Hk divides Hv. States m [B, Hv, dv, dk] fp32 (y = M q). A packed batch has B = 1 and seq_starts [n + 1] int32.
 
-class _on_device:
-    """The library launches on the current device's stream: calls on tensors of another device run under a guard."""
-
-    def __init__(self, t):
-        self.guard = None
-        if t.device.index != torch._C._cuda_getDevice():
-            self.guard = torch.cuda.device(t.device)
-
-    def __enter__(self):
-        if self.guard is not None:
-            self.guard.__enter__()
-
-    def __exit__(self, *exc):
-        if self.guard is not None:
-            self.guard.__exit__(*exc)
-        return False
+_CURRENT_DEVICE = torch._C._cuda_getDevice
+_CURRENT_STREAM = torch._C._cuda_getCurrentRawStream
+_DESC = struct.Struct("8i15qf")          # nlh_gated_delta_desc (ffi.GatedDeltaDesc), packed in one call
 
 
-def _same_device(where, first, **others):
-    if not first.is_cuda:
+def _entry(name):
+    """The C function of a status-returning entry, for calls with positional arguments as in the header: these
+    operators run in microseconds, and call()'s keyword arguments would cost as much again."""
+    fn = getattr(ffi.lib(), name)
+
+    def run(device, *args):
+        if device != _CURRENT_DEVICE():                 # tensors of another device: its stream, under a guard
+            with torch.cuda.device(device):
+                return run(device, *args)
+        ffi.lib().nlh_set_stream(_CURRENT_STREAM(device))
+        rc = fn(*args)
+        if rc:
+            ffi.check(rc, name)
+
+    _ENTRIES[name] = run
+    return run
+
+
+_ENTRIES = {}
+
+
+def _run(name, device, *args):
+    return (_ENTRIES.get(name) or _entry(name))(device, *args)
+
+
+def _device_of(where, first, *others):
+    """Index of the one CUDA device that all these tensors (None apart) are on."""
+    d = first.get_device()
+    if d < 0:
         raise ValueError(f"{where}: need CUDA tensors")
-    for n, t in others.items():
-        if t is not None and t.device != first.device:
-            raise ValueError(f"{where}.{n}: on {t.device}, the other tensors on {first.device}")
+    for t in others:
+        if t is not None and t.get_device() != d:
+            raise ValueError(f"{where}: tensors on different devices ({first.device}, {t.device})")
+    return d
+
+
+def _ptr(t):
+    return None if t is None else t.data_ptr()
 
 
 def _need(where, name, t, dtype, shape):
     """A contiguous tensor of this type and shape."""
-    if t.dtype != dtype or tuple(t.shape) != tuple(shape) or not t.is_contiguous():
+    if t.dtype != dtype or t.shape != shape or not t.is_contiguous():
         raise ValueError(f"{where}.{name}: need a contiguous {dtype} tensor of shape {tuple(shape)}, "
                          f"got {t.dtype} {tuple(t.shape)}")
 
@@ -392,24 +412,22 @@ def _gated_delta_desc(where, k, v, q, log_retain, theta, scale, n_seqs, d_y=None
     if k.dim() != 4 or v.dim() != 4 or log_retain.dim() != 3:
         raise ValueError(f"{where}: need k, q, v of [batch, seq, heads, d] and gates of [batch, seq, heads]")
     b, s, hk, dk = k.shape
-    hv, dv = v.shape[2], v.shape[3]
-    if q.shape != k.shape or v.shape[:2] != k.shape[:2] or log_retain.shape != v.shape[:3] or theta.shape != v.shape[:3]:
+    bv, sv, hv, dv = v.shape
+    if q.shape != k.shape or bv != b or sv != s or log_retain.shape != (b, s, hv) or theta.shape != (b, s, hv):
         raise ValueError(f"{where}: shapes do not fit: k {tuple(k.shape)}, q {tuple(q.shape)}, v {tuple(v.shape)}, "
                          f"log_retain {tuple(log_retain.shape)}, theta {tuple(theta.shape)}")
-    if k.dtype not in (torch.float32, torch.bfloat16) or q.dtype != k.dtype or v.dtype != k.dtype:
+    dt = k.dtype
+    if (dt != torch.float32 and dt != torch.bfloat16) or q.dtype != dt or v.dtype != dt:
         raise ValueError(f"{where}: k, v and q must all be float32 or all bfloat16")
     if log_retain.dtype != torch.float32 or theta.dtype != torch.float32:
         raise ValueError(f"{where}: log_retain and theta must be float32")
-    for t in (k, v, q) if d_y is None else (k, v, q, d_y):
-        if t.stride(3) != 1 and t.shape[3] > 1:
-            raise ValueError(f"{where}: the last axis must be contiguous")
-    if log_retain.stride() != theta.stride():
-        raise ValueError(f"{where}: log_retain and theta must have the same strides")
+    ks, vs, qs, gs = k.stride(), v.stride(), q.stride(), log_retain.stride()
+    ys = (0, 0, 0, 1) if d_y is None else d_y.stride()
+    if (dk > 1 and (ks[3] != 1 or qs[3] != 1)) or (dv > 1 and (vs[3] != 1 or ys[3] != 1)):
+        raise ValueError(f"{where}: the last axis must be contiguous")
     if n_seqs and b != 1:
         raise ValueError(f"{where}: a packed batch has batch 1")
-    dy = (0, 0, 0) if d_y is None else d_y.stride()[:3]
-    return ffi.GatedDeltaDesc(b, s, hk, hv, dk, dv, n_seqs, int(k.dtype == torch.bfloat16), *k.stride()[:3], *v.stride()[:3],
-                              *q.stride()[:3], *log_retain.stride(), *dy, scale)
+    return _DESC.pack(b, s, hk, hv, dk, dv, n_seqs, dt == torch.bfloat16, *ks[:3], *vs[:3], *qs[:3], *gs, *ys[:3], scale)
 
 
 def _same_strides(a, b):
@@ -425,30 +443,31 @@ def _starts_of(where, seq_starts):
     return seq_starts.numel() - 1
 
 
+def _bytes(where, fn, *args):
+    n = fn(*args)
+    if n < 0:
+        ffi.check(ffi.lib().nlh_last_status() or 1, where)
+    return n
+
+
 def gated_delta_forward(k, v, q, log_retain, theta, m0=None, seq_starts=None, scale=1.0, want_saved=True):
     """Gated delta rule over whole sequences (nlh_gated_delta_forward): returns (y like v, m_final
     [sequences, Hv, dv, dk], saved). ``saved`` is what gated_delta_backward needs, None with want_saved=False.
     In a packed batch the rows of y outside the sequences are zeros."""
     where = "gated_delta_forward"
-    _same_device(where, k, v=v, q=q, log_retain=log_retain, theta=theta, m0=m0, seq_starts=seq_starts)
+    device = _device_of(where, k, v, q, log_retain, theta, m0, seq_starts)
     log_retain, theta = _same_strides(log_retain, theta)
     n_seqs = _starts_of(where, seq_starts)
     desc = _gated_delta_desc(where, k, v, q, log_retain, theta, scale, n_seqs)
-    b, s, hv, dv = v.shape
-    state = (n_seqs or b, hv, dv, k.shape[3])
+    state = (n_seqs or k.shape[0], v.shape[2], v.shape[3], k.shape[3])
     if m0 is not None:
         _need(where, "m0", m0, torch.float32, state)
-    with _on_device(k):
-        ref = C.byref(desc)
-        nbytes = ffi.lib().nlh_gated_delta_saved_bytes(ref)
-        if nbytes < 0:
-            ffi.check(ffi.lib().nlh_last_status(), where)
-        saved = torch.empty(max(nbytes, 1), dtype=torch.uint8, device=k.device)
-        y = (torch.zeros if n_seqs else torch.empty)(b, s, hv, dv, dtype=v.dtype, device=k.device)
-        m = torch.empty(state, dtype=torch.float32, device=k.device)
-        call("nlh_gated_delta_forward", desc=ref, k=k.data_ptr(), v=v.data_ptr(), q=q.data_ptr(),
-             log_retain=log_retain.data_ptr(), theta=theta.data_ptr(), m_initial=m0, seq_starts=seq_starts, y=y, m_final=m,
-             saved=saved, saved_bytes=nbytes)
+    nbytes = _bytes(where, ffi.lib().nlh_gated_delta_saved_bytes, desc)
+    saved = torch.empty(max(nbytes, 1), dtype=torch.uint8, device=k.device)
+    y = (torch.zeros if n_seqs else torch.empty)(v.shape, dtype=v.dtype, device=k.device)
+    m = torch.empty(state, dtype=torch.float32, device=k.device)
+    _run("nlh_gated_delta_forward", device, desc, k.data_ptr(), v.data_ptr(), q.data_ptr(), log_retain.data_ptr(),
+         theta.data_ptr(), _ptr(m0), _ptr(seq_starts), y.data_ptr(), m.data_ptr(), saved.data_ptr(), nbytes)
     return y, m, (saved if want_saved else None)
 
 
@@ -458,31 +477,25 @@ def gated_delta_backward(k, v, q, log_retain, theta, saved, d_y, d_m_final=None,
     dict(d_k, d_v, d_q, d_log_retain, d_theta, d_m_initial). d_y like v in type, any strides; d_m_final (gradient
     of m_final) may be None. Keys shared by several value heads get the sum of their gradients."""
     where = "gated_delta_backward"
-    _same_device(where, k, v=v, q=q, log_retain=log_retain, theta=theta, saved=saved, d_y=d_y, d_m_final=d_m_final,
-                 seq_starts=seq_starts)
+    device = _device_of(where, k, v, q, log_retain, theta, saved, d_y, d_m_final, seq_starts)
     log_retain, theta = _same_strides(log_retain, theta)
     if d_y.shape != v.shape or d_y.dtype != v.dtype:
         raise ValueError(f"{where}.d_y: need {v.dtype} {tuple(v.shape)}, got {d_y.dtype} {tuple(d_y.shape)}")
     n_seqs = _starts_of(where, seq_starts)
     desc = _gated_delta_desc(where, k, v, q, log_retain, theta, scale, n_seqs, d_y)
-    b, s, hv, dv = v.shape
-    state = (n_seqs or b, hv, dv, k.shape[3])
+    state = (n_seqs or k.shape[0], v.shape[2], v.shape[3], k.shape[3])
     if d_m_final is not None:
         _need(where, "d_m_final", d_m_final, torch.float32, state)
-    with _on_device(k):
-        ref = C.byref(desc)
-        lib = ffi.lib()
-        nbytes = lib.nlh_gated_delta_backward_bytes(ref)
-        if nbytes < 0:
-            ffi.check(lib.nlh_last_status(), where)
-        make = torch.zeros if n_seqs else torch.empty      # rows outside the sequences are not written
-        new = lambda t, dt=None: make(t.shape, dtype=dt or t.dtype, device=k.device)
-        work = make(max(nbytes, 1), dtype=torch.uint8, device=k.device)
-        g = dict(d_k=new(k), d_v=new(v), d_q=new(q), d_log_retain=new(theta), d_theta=new(theta))
-        g["d_m_initial"] = torch.empty(state, dtype=torch.float32, device=k.device) if want_initial else None
-        call("nlh_gated_delta_backward", desc=ref, k=k.data_ptr(), v=v.data_ptr(), q=q.data_ptr(),
-             log_retain=log_retain.data_ptr(), theta=theta.data_ptr(), seq_starts=seq_starts, saved=saved,
-             saved_bytes=saved.numel(), d_y=d_y.data_ptr(), d_m_final=d_m_final, workspace=work, workspace_bytes=nbytes, **g)
+    _need(where, "saved", saved, torch.uint8, saved.shape)
+    nbytes = _bytes(where, ffi.lib().nlh_gated_delta_backward_bytes, desc)
+    make = torch.zeros if n_seqs else torch.empty      # rows outside the sequences are not written
+    new = lambda t: make(t.shape, dtype=t.dtype, device=k.device)
+    work = make(max(nbytes, 1), dtype=torch.uint8, device=k.device)
+    g = dict(d_k=new(k), d_v=new(v), d_q=new(q), d_log_retain=new(theta), d_theta=new(theta))
+    g["d_m_initial"] = torch.empty(state, dtype=torch.float32, device=k.device) if want_initial else None
+    _run("nlh_gated_delta_backward", device, desc, k.data_ptr(), v.data_ptr(), q.data_ptr(), log_retain.data_ptr(),
+         theta.data_ptr(), _ptr(seq_starts), saved.data_ptr(), saved.numel(), d_y.data_ptr(), _ptr(d_m_final),
+         *[_ptr(t) for t in g.values()], work.data_ptr(), nbytes)
     return g
 
 
@@ -491,16 +504,15 @@ def gated_delta_step(k, v, q, log_retain, theta, m, slots=None, scale=1.0):
     (nlh_gated_delta_step). slots [B] int32: the state of each sequence (None: sequence i has state i); one outside
     [0, n_slots) marks an unused place of the batch, whose rows of y are zeros. Returns y like v."""
     where = "gated_delta_step"
-    _same_device(where, k, v=v, q=q, log_retain=log_retain, theta=theta, m=m, slots=slots)
+    device = _device_of(where, k, v, q, log_retain, theta, m, slots)
     log_retain, theta = _same_strides(log_retain, theta)
     desc = _gated_delta_desc(where, k, v, q, log_retain, theta, scale, 0)
     _need(where, "m", m, torch.float32, (m.shape[0], v.shape[2], v.shape[3], k.shape[3]))
     if slots is not None:
         _need(where, "slots", slots, torch.int32, (k.shape[0],))
-    with _on_device(k):
-        y = torch.empty(v.shape, dtype=v.dtype, device=k.device)
-        call("nlh_gated_delta_step", desc=C.byref(desc), k=k.data_ptr(), v=v.data_ptr(), q=q.data_ptr(),
-             log_retain=log_retain.data_ptr(), theta=theta.data_ptr(), m=m, slots=slots, n_slots=m.shape[0], y=y)
+    y = torch.empty(v.shape, dtype=v.dtype, device=k.device)
+    _run("nlh_gated_delta_step", device, desc, k.data_ptr(), v.data_ptr(), q.data_ptr(), log_retain.data_ptr(),
+         theta.data_ptr(), m.data_ptr(), _ptr(slots), m.shape[0], y.data_ptr())
     torch.autograd.graph.increment_version(m)    # written past autograd
     return y
 
@@ -515,14 +527,14 @@ def embedding_forward(w, ids, scale=1.0):
     """scale * w[ids] (nlh_embedding_forward): w [vocab, d] fp32 or bf16, ids int32 of any shape; returns [*ids.shape, d]
     in w's type. An id outside [0, vocab) gives a row of zeros."""
     where = "embedding_forward"
-    _same_device(where, w, ids=ids)
+    device = _device_of(where, w, ids)
     if w.dim() != 2 or w.dtype not in (torch.float32, torch.bfloat16) or not w.is_contiguous():
         raise ValueError(f"{where}.w: need a contiguous fp32 or bf16 [vocab, d]")
     _ids32(where, "ids", ids)
-    with _on_device(w):
-        out = torch.empty(*ids.shape, w.shape[1], dtype=w.dtype, device=w.device)
-        call("nlh_embedding_forward", w=w, w_is_bf16=int(w.dtype == torch.bfloat16), ids=ids, out=out, n=ids.numel(),
-             vocab=w.shape[0], d=w.shape[1], scale=scale)
+    vocab, d = w.shape
+    out = torch.empty(*ids.shape, d, dtype=w.dtype, device=w.device)
+    _run("nlh_embedding_forward", device, w.data_ptr(), w.dtype == torch.bfloat16, ids.data_ptr(), out.data_ptr(), ids.numel(),
+         vocab, d, scale)
     return out
 
 
@@ -530,7 +542,7 @@ def embedding_backward(d_out, ids, d_w, scale=1.0, accumulate=True):
     """Gradient of embedding_forward (nlh_embedding_backward): d_w [vocab, d] fp32 += scale * the sums of d_out's rows
     by id, or = with accumulate=False. The same inputs give the same bits. Returns d_w."""
     where = "embedding_backward"
-    _same_device(where, d_w, d_out=d_out, ids=ids)
+    device = _device_of(where, d_w, d_out, ids)
     if d_w.dim() != 2:
         raise ValueError(f"{where}.d_w: need [vocab, d]")
     _need(where, "d_w", d_w, torch.float32, d_w.shape)
@@ -538,20 +550,23 @@ def embedding_backward(d_out, ids, d_w, scale=1.0, accumulate=True):
     if d_out.dtype not in (torch.float32, torch.bfloat16) or d_out.shape != (*ids.shape, d) or not d_out.is_contiguous():
         raise ValueError(f"{where}.d_out: need a contiguous fp32 or bf16 {(*ids.shape, d)}, got {d_out.dtype} {tuple(d_out.shape)}")
     _ids32(where, "ids", ids)
-    with _on_device(d_w):
-        n = ids.numel()
-        nbytes = ffi.lib().nlh_embedding_backward_bytes(n, vocab, d)
-        work = torch.empty(nbytes, dtype=torch.uint8, device=d_w.device) if nbytes > 0 else None
-        call("nlh_embedding_backward", d_out=d_out, d_out_is_bf16=int(d_out.dtype == torch.bfloat16), ids=ids, d_w=d_w, n=n,
-             vocab=vocab, d=d, scale=scale, accumulate=int(accumulate), workspace=work, workspace_bytes=max(nbytes, 0))
+    n = ids.numel()
+    nbytes = _bytes(where, ffi.lib().nlh_embedding_backward_bytes, n, vocab, d)
+    work = torch.empty(nbytes, dtype=torch.uint8, device=d_w.device) if nbytes else None
+    _run("nlh_embedding_backward", device, d_out.data_ptr(), d_out.dtype == torch.bfloat16, ids.data_ptr(), d_w.data_ptr(), n, vocab,
+         d, scale, bool(accumulate), _ptr(work), nbytes)
     torch.autograd.graph.increment_version(d_w)      # written past autograd
     return d_w
 
 
 # ── distillation from a teacher's top logits (additive API) ────────────────
 class DistillSaved:
-    """What distill_backward needs of its forward: the forward's arguments and the rows' statistics."""
-    __slots__ = ("buffer", "shape", "dtype", "args")
+    """What distill_backward needs of its forward: the forward's tensors, the rows' statistics, sizes and weights."""
+    __slots__ = ("targets", "ids", "teacher", "buffer", "shape", "dtype", "k", "weights")
+
+
+def _row_stride(t):
+    return t.stride(0) if t.shape[0] > 1 else t.shape[1]
 
 
 def distill_forward(logits, teacher_ids, teacher_logits, targets=None, temperature=1.0, soft_weight=1.0, hard_weight=0.0):
@@ -560,7 +575,7 @@ def distill_forward(logits, teacher_ids, teacher_logits, targets=None, temperatu
     soft_weight * temperature^2 * mean KL(teacher || student at the temperature) + hard_weight * mean cross-entropy with
     targets [n] int32 (outside [0, vocab): none). Returns (loss, saved)."""
     where = "distill_forward"
-    _same_device(where, logits, teacher_ids=teacher_ids, teacher_logits=teacher_logits, targets=targets)
+    device = _device_of(where, logits, teacher_ids, teacher_logits, targets)
     if logits.dim() != 2 or logits.dtype not in (torch.float32, torch.bfloat16) or (logits.shape[1] > 1 and logits.stride(1) != 1):
         raise ValueError(f"{where}.logits: need fp32 or bf16 [n, vocab] with contiguous rows")
     n, vocab = logits.shape
@@ -572,19 +587,15 @@ def distill_forward(logits, teacher_ids, teacher_logits, targets=None, temperatu
         raise ValueError(f"{where}.teacher_logits: need contiguous fp32 or bf16")
     if targets is not None:
         _ids32(where, "targets", targets, n)
-    row_stride = logits.stride(0) if n > 1 else vocab
-    with _on_device(logits):
-        nbytes = ffi.lib().nlh_distill_saved_bytes(n, vocab)
-        s = DistillSaved()
-        s.buffer = torch.empty(max(nbytes, 16), dtype=torch.uint8, device=logits.device)
-        s.shape, s.dtype = logits.shape, logits.dtype
-        s.args = dict(logits_is_bf16=int(logits.dtype == torch.bfloat16), row_stride=row_stride, target_ids=targets,
-                      teacher_ids=teacher_ids, teacher_logits=teacher_logits,
-                      teacher_is_bf16=int(teacher_logits.dtype == torch.bfloat16), saved=s.buffer, saved_bytes=s.buffer.numel(),
-                      n=n, vocab=vocab, k=teacher_ids.shape[1], temperature=temperature, hard_weight=hard_weight,
-                      soft_weight=soft_weight)
-        loss = torch.empty((), dtype=torch.float32, device=logits.device)
-        call("nlh_distill_forward", logits=logits.data_ptr(), loss=loss, **s.args)
+    s = DistillSaved()
+    s.targets, s.ids, s.teacher, s.shape, s.dtype = targets, teacher_ids, teacher_logits, logits.shape, logits.dtype
+    s.k, s.weights = teacher_ids.shape[1], (temperature, hard_weight, soft_weight)
+    nbytes = _bytes(where, ffi.lib().nlh_distill_saved_bytes, n, vocab)
+    s.buffer = torch.empty(nbytes, dtype=torch.uint8, device=logits.device)
+    loss = torch.empty((), dtype=torch.float32, device=logits.device)
+    _run("nlh_distill_forward", device, logits.data_ptr(), logits.dtype == torch.bfloat16, _row_stride(logits), _ptr(targets),
+         teacher_ids.data_ptr(), teacher_logits.data_ptr(), teacher_logits.dtype == torch.bfloat16, loss.data_ptr(),
+         s.buffer.data_ptr(), nbytes, n, vocab, s.k, *s.weights)
     return loss, s
 
 
@@ -592,8 +603,9 @@ def distill_backward(logits, saved, grad=None, out=None):
     """Gradient of distill_forward with respect to logits, times the fp32 scalar tensor ``grad``. out (default: a new
     tensor) may be logits itself. The tensors given to the forward must not have changed."""
     where = "distill_backward"
-    _same_device(where, logits, grad=grad, out=out, saved=saved.buffer)
-    if logits.shape != saved.shape or logits.dtype != saved.dtype:
+    s = saved
+    device = _device_of(where, logits, s.buffer, grad, out)
+    if logits.shape != s.shape or logits.dtype != s.dtype or (logits.shape[1] > 1 and logits.stride(1) != 1):
         raise ValueError(f"{where}.logits: not what distill_forward was given")
     n, vocab = logits.shape
     if out is None:
@@ -602,10 +614,9 @@ def distill_backward(logits, saved, grad=None, out=None):
         raise ValueError(f"{where}.out: need {logits.dtype} {tuple(logits.shape)} with contiguous rows")
     if grad is not None and (grad.dtype != torch.float32 or grad.numel() != 1):
         raise ValueError(f"{where}.grad: need one fp32 value")
-    stride = lambda t: t.stride(0) if n > 1 else vocab
-    with _on_device(logits):
-        call("nlh_distill_backward", logits=logits.data_ptr(), grad_scale=None if grad is None else grad.data_ptr(),
-             d_logits=out.data_ptr(), d_row_stride=stride(out), **{**saved.args, "row_stride": stride(logits)})
+    _run("nlh_distill_backward", device, logits.data_ptr(), logits.dtype == torch.bfloat16, _row_stride(logits), _ptr(s.targets),
+         s.ids.data_ptr(), s.teacher.data_ptr(), s.teacher.dtype == torch.bfloat16, s.buffer.data_ptr(), s.buffer.numel(),
+         _ptr(grad), out.data_ptr(), _row_stride(out), n, vocab, s.k, *s.weights)
     torch.autograd.graph.increment_version(out)      # written past autograd
     return out
 

@@ -53,6 +53,7 @@ class StackedMAGConfig:
     vocab: int = 8192
     bf16: bool = True                 # bf16 activations for SWA and the dense projections
     exact_levels: tuple = (0,)        # tape strategy: level 0 exact, others frozen-M0 (proxy)
+    memory_rule: str = "titans"       # "gated_delta": every level on the gated delta rule (decay before the error, no momentum)
     exact_checkpoint: int = 0         # > 0: exact levels keep a checkpoint every this many tokens and
                                       # recompute the windows in the backward (less memory, more time)
     lr: float = 3e-4
@@ -62,6 +63,10 @@ class StackedMAGConfig:
     weight_decay: float = 0.1
     max_grad_norm: float = 1.0
     tie_embeddings: bool = True
+    embed_scale: float = 1.0          # factor of the embedding rows
+    embed_sorted_grad: bool = False   # embedding gradient by sorted tokens: the same bits every run (1.0 and False: gather / atomics)
+    distill_temperature: float = 2.0  # of the loss with a teacher's top logits (forward's `teacher`) ...
+    distill_weight: float = 0.5       # ... and its weight; the cross-entropy keeps 1 - distill_weight
     fused_glue: bool = True           # fused CUDA rule wrapper / MAG combine (CUDA only)
     level_streams: bool = True        # run CMS levels >= 1 on side streams next to level 0
     overlap_grad_sync: bool = True    # data-parallel: all-reduce each block's gradients under the rest of the backward
@@ -164,6 +169,32 @@ class _TitansMemory(torch.autograd.Function):
                                                    want_initial=False)
         return (g["d_k"], g["d_v"], g["d_q"], g["d_alpha"], g["d_theta"], g["d_eta"], None, None, None,
                 None, None)
+
+
+class _GatedDeltaMemory(torch.autograd.Function):
+    """Per-head gated delta rule over [N, S, hd] fp32 streams (nlh_gated_delta_forward / _backward) with the framework's
+    gates: retention 1 - alpha, learning rate theta. m0 [N, hd * hd]; returns y and the final memory."""
+
+    @staticmethod
+    def forward(ctx, k, v, q, alpha, theta, m0):
+        n, s, d = k.shape
+        heads = lambda t: t.unsqueeze(2)                 # one head per row of the batch
+        keep = 1.0 - alpha
+        args = (heads(k), heads(v), heads(q), heads(torch.log(keep)), heads(theta))
+        y, m, saved = D.gated_delta_forward(*args, m0=m0.view(n, 1, d, d))
+        ctx.save_for_backward(*args, saved, keep)
+        m = m.view(n, d * d)
+        ctx.mark_non_differentiable(m)
+        return y.view(n, s, d), m
+
+    @staticmethod
+    def backward(ctx, dy, _dm):
+        *args, saved, keep = ctx.saved_tensors
+        g = D.gated_delta_backward(*args, saved, dy.unsqueeze(2), want_initial=False)
+        # log(1 - alpha): the gradient of log_retain carries the factor 1 - alpha
+        d_alpha = -g["d_log_retain"].squeeze(2) / keep.clamp_min(1e-30)
+        sq = lambda x: g[x].squeeze(2)
+        return sq("d_k"), sq("d_v"), sq("d_q"), d_alpha, sq("d_theta"), None
 
 
 class _SWA(torch.autograd.Function):
@@ -593,6 +624,37 @@ class _CrossEntropy(torch.autograd.Function):
         return logits, None
 
 
+class _Distill(torch.autograd.Function):
+    """Distillation loss with a hard-target term on logits [n, vocab] (nlh_distill_forward / _backward). Like
+    _CrossEntropy's, the backward overwrites the logits with their gradient."""
+
+    @staticmethod
+    def forward(ctx, logits, teacher_ids, teacher_logits, targets, temperature, soft_weight, hard_weight):
+        loss, ctx.distill = D.distill_forward(logits, teacher_ids, teacher_logits, targets=targets, temperature=temperature,
+                                              soft_weight=soft_weight, hard_weight=hard_weight)
+        ctx.save_for_backward(logits)
+        return loss
+
+    @staticmethod
+    def backward(ctx, g):
+        (logits,) = ctx.saved_tensors
+        D.distill_backward(logits, ctx.distill, grad=g.float().reshape(1), out=logits)
+        return logits, None, None, None, None, None, None
+
+
+def _distill_plain(logits, teacher_ids, teacher_logits, targets, temperature, soft_weight, hard_weight):
+    """The same loss in PyTorch operators (fused_glue = False)."""
+    there = (teacher_ids >= 0) & (teacher_ids < logits.shape[1])
+    rows = there.any(1)
+    t = torch.where(there, teacher_logits.float() / temperature, -math.inf)[rows]
+    p = torch.where(there[rows], torch.softmax(t, 1), 0.0)
+    logq = torch.log_softmax(logits[rows] / temperature, 1).gather(1, teacher_ids[rows].clamp(0, logits.shape[1] - 1).long())
+    kl = (torch.special.xlogy(p, p) - p * logq).sum() / rows.sum().clamp_min(1)
+    ok = (targets >= 0) & (targets < logits.shape[1])
+    ce = F.cross_entropy(logits[ok], targets[ok].long(), reduction="sum") / ok.sum().clamp_min(1)
+    return soft_weight * temperature ** 2 * kl + hard_weight * ce
+
+
 class _Linear(torch.autograd.Function):
     """y = x W^T (or x W when transposed) on bf16 tensor cores, with the weight's bf16 copy taken
     from the model's per-step shadow arena (one cast of the whole arena per forward instead of one
@@ -625,19 +687,24 @@ class _Linear(torch.autograd.Function):
 
 
 class _Embedding(torch.autograd.Function):
-    """x[t] = w_embed[ids[t]] through embedding_gather_cuda; the backward scatter-adds the output
-    gradient straight into grad_out (the embedding's slice of the gradient arena,
-    embedding_scatter_add_cuda), so no dense [vocab, d] temporary and no accumulation pass exist.
+    """x[t] = scale * w_embed[ids[t]]; the backward adds the output gradient's rows straight into grad_out (the
+    embedding's slice of the gradient arena), so no dense [vocab, d] temporary and no accumulation pass exist. Scale 1 without
+    sorted_grad: embedding_gather_cuda and embedding_scatter_add_cuda (atomics); else nlh_embedding_forward and, by sorted
+    tokens, nlh_embedding_backward.
     Because of that side effect the Function returns no gradient for w_embed itself (w_embed is
     an input only so that the tape records the Function)."""
 
     @staticmethod
-    def forward(ctx, ids, w_embed, grad_out):
+    def forward(ctx, ids, w_embed, grad_out, scale=1.0, sorted_grad=False):
         B, S = ids.shape
         d = w_embed.shape[1]
         ids32 = ids.reshape(-1).to(torch.int32).contiguous()
-        out = torch.empty(B * S, d, dtype=torch.float32, device=w_embed.device)
-        D.call("embedding_gather_cuda", w_embed=w_embed, input_ids=ids32, output=out, seq_len=B * S, d=d)
+        ctx.scale, ctx.by_sort = scale, sorted_grad or scale != 1.0
+        if ctx.by_sort:
+            out = D.embedding_forward(w_embed.detach(), ids32, scale=scale)
+        else:
+            out = torch.empty(B * S, d, dtype=torch.float32, device=w_embed.device)
+            D.call("embedding_gather_cuda", w_embed=w_embed, input_ids=ids32, output=out, seq_len=B * S, d=d)
         ctx.save_for_backward(ids32)
         ctx.grad_out = grad_out
         ctx.mark_non_differentiable(ids32)
@@ -647,13 +714,21 @@ class _Embedding(torch.autograd.Function):
     def backward(ctx, d_x):
         (ids32,) = ctx.saved_tensors
         d_x = d_x.contiguous().float()
-        D.call("embedding_scatter_add_cuda", d_embedded=d_x.view(-1, d_x.shape[-1]), input_ids=ids32,
-               d_embed=ctx.grad_out, seq_len=ids32.numel(), d=d_x.shape[-1])
-        return None, None, None
+        if ctx.by_sort:
+            D.embedding_backward(d_x.view(-1, d_x.shape[-1]), ids32, ctx.grad_out, scale=ctx.scale)
+        else:
+            D.call("embedding_scatter_add_cuda", d_embedded=d_x.view(-1, d_x.shape[-1]), input_ids=ids32,
+                   d_embed=ctx.grad_out, seq_len=ids32.numel(), d=d_x.shape[-1])
+        return None, None, None, None, None
 
 
 def titans_memory(k, v, q, alpha, theta, eta, m0, chunk, slot=0, carry=None, ckpt=0):
     return _TitansMemory.apply(k, v, q, alpha, theta, eta, m0, chunk, slot, carry, ckpt)
+
+
+def gated_delta_memory(k, v, q, alpha, theta, eta, m0, chunk):
+    """The gated delta rule as a level's memory. It has no momentum (eta takes no part) and one form for every chunk."""
+    return _GatedDeltaMemory.apply(k, v, q, alpha, theta, m0)
 
 
 def swa(q, k, v, num_heads, head_dim, window):
@@ -666,6 +741,10 @@ class StackedMAG:
     def __init__(self, cfg: StackedMAGConfig, batch_per_rank: int, device="cuda", seed=42,
                  memory_fn=titans_memory, swa_fn=swa):
         self.cfg, self.device = cfg, torch.device(device)
+        if cfg.memory_rule not in ("titans", "gated_delta"):
+            raise ValueError(f"memory_rule {cfg.memory_rule!r}: need 'titans' or 'gated_delta'")
+        if cfg.memory_rule == "gated_delta" and memory_fn is titans_memory:
+            memory_fn = gated_delta_memory
         self.memory_fn, self.swa_fn = memory_fn, swa_fn
         d, v, k = cfg.d_model, cfg.vocab, cfg.k
         names, shapes, clamp, level_of = [], [], {}, []
@@ -872,16 +951,21 @@ class StackedMAG:
         out = F.layer_norm(x, (x.shape[-1],), p[name + "gamma"], p[name + "beta"], 1e-5)
         return (out, out) if mode == 2 else out
 
-    def forward(self, tokens, targets):
+    def forward(self, tokens, targets, teacher=None):
+        """Mean cross-entropy of the batch. teacher = (ids, logits), both [B, S, k]: the top entries of a teacher's
+        distribution at every position (ids int32, outside [0, vocab): unused); the loss is then the distillation loss
+        at cfg.distill_temperature with weight cfg.distill_weight, plus 1 - distill_weight times the cross-entropy."""
         cfg, p = self.cfg, self.p
         d, nh, hd = cfg.d_model, cfg.num_heads, cfg.head_dim
         fused = (cfg.fused_glue and tokens.is_cuda and cfg.k <= 4 and d <= 1024 and hd % 4 == 0)
         lp = 1 if (fused and cfg.bf16) else 0           # LayerNorm output feeding only a GEMM
         self._refresh_shadow()
         if fused and self._use_embed:
-            x = _Embedding.apply(tokens, p["w_embed"], self.g["w_embed"])
+            x = _Embedding.apply(tokens, p["w_embed"], self.g["w_embed"], cfg.embed_scale, cfg.embed_sorted_grad)
         else:
             x = F.embedding(tokens, p["w_embed"])
+            if cfg.embed_scale != 1.0:
+                x = x * cfg.embed_scale
         for b in range(cfg.n_blocks):
             pre = f"b{b}."
             self._mark_bucket(x, f"b{b}")            # fires once block b's backward has run
@@ -940,6 +1024,14 @@ class StackedMAG:
         self._mark_bucket(x, "tail")                 # unembedding and final LayerNorm
         x = self._ln(x, "ln_final_", lp, fused)
         logits = self._mm(x, "w_unembed", transposed=True)
+        if teacher is not None:
+            ids, top = (t.reshape(-1, t.shape[-1]) for t in teacher)
+            hard = targets.reshape(-1)
+            args = (cfg.distill_temperature, cfg.distill_weight, 1.0 - cfg.distill_weight)
+            if fused:
+                return _Distill.apply(logits.view(-1, cfg.vocab), ids.to(torch.int32).contiguous(), top.contiguous(),
+                                      hard.to(torch.int32).contiguous(), *args)
+            return _distill_plain(logits.float().view(-1, cfg.vocab), ids, top, hard, *args)
         if fused:
             return _CrossEntropy.apply(logits.view(-1, cfg.vocab), targets.reshape(-1).to(torch.int32))
         return F.cross_entropy(logits.float().view(-1, cfg.vocab), targets.reshape(-1))
@@ -950,8 +1042,8 @@ class StackedMAG:
         cfg = self.cfg
         return [self.global_step % cs == 0 or cfg.seq_len >= cs for cs in cfg.chunk_sizes]
 
-    def forward_backward(self, tokens, targets, process_group=None, world=1):
-        """Loss (mean over the local batch) and its gradients, accumulated into the arena.
+    def forward_backward(self, tokens, targets, process_group=None, world=1, teacher=None):
+        """Loss (mean over the local batch; see forward for `teacher`) and its gradients, accumulated into the arena.
         With world > 1 (and cfg.overlap_grad_sync) the gradients are also averaged over the
         ranks here: the arena is laid out in the order the backward completes it
         backwards (embedding | unembedding + final LayerNorm | block 0 | block 1 | ...), so each
@@ -962,7 +1054,7 @@ class StackedMAG:
                    and torch.distributed.is_initialized())
         self._sync_state = dict(pg=process_group, works=[], seen=set(), world=world,
                                 avg=tokens.is_cuda) if overlap else None
-        loss = self.forward(tokens, targets)
+        loss = self.forward(tokens, targets) if teacher is None else self.forward(tokens, targets, teacher)
         loss.backward()
         if overlap:
             st = self._sync_state
@@ -1053,28 +1145,32 @@ class StackedMAG:
         self._host_schedule()
         self._device_update()
 
-    def step(self, tokens, targets, process_group=None, world=1):
+    def step(self, tokens, targets, process_group=None, world=1, teacher=None):
         """forward + backward + gradient all-reduce + clip + AdamW. Returns the local loss."""
-        loss = self.forward_backward(tokens, targets, process_group, world)
+        more = () if teacher is None else (teacher,)
+        loss = self.forward_backward(tokens, targets, process_group, world, *more)
         self.sync_gradients(process_group, world)
         self.apply_update()
         return loss
 
-    def step_graphed(self, tokens, targets, process_group=None, world=1):
+    def step_graphed(self, tokens, targets, process_group=None, world=1, teacher=None):
         """Same as step(), replayed from one CUDA graph (forward, backward, gradient all-reduce,
         clip, AdamW, weight tying): removes the per-launch host cost, which dominates when the
         per-rank batch is small. The first call runs two eager steps (sizes every allocation and
         the library workspace) and captures; later calls copy the inputs into static buffers and
         replay. Shapes must not change between calls. The inputs have been read when the call returns:
-        a loader may refill its (pinned) buffers then. The step itself is only queued."""
+        a loader may refill its (pinned) buffers then. The step itself is only queued. A teacher is part of the
+        captured step: given on the first call, it is given on every call."""
         if getattr(self, "_graph", None) is None:
             self._static_tok = tokens.clone()
             self._static_tgt = targets.clone()
+            self._static_teacher = None if teacher is None else tuple(t.clone() for t in teacher)
+            more = () if teacher is None else (self._static_teacher,)
             side = torch.cuda.Stream()
             side.wait_stream(torch.cuda.current_stream())
             with torch.cuda.stream(side):
                 for _ in range(2):
-                    self.step(self._static_tok, self._static_tgt, process_group, world)
+                    self.step(self._static_tok, self._static_tgt, process_group, world, *more)
             torch.cuda.current_stream().wait_stream(side)
             torch.cuda.synchronize()
             torch.cuda.empty_cache()
@@ -1083,14 +1179,19 @@ class StackedMAG:
             self._graph = torch.cuda.CUDAGraph()
             with torch.cuda.graph(self._graph):
                 self._static_loss = self.forward_backward(self._static_tok, self._static_tgt,
-                                                          process_group, world)
+                                                          process_group, world, *more)
                 self.sync_gradients(process_group, world)
                 self._device_update()
             self._graph.replay()            # capture records only: run the scheduled step now
             self._inputs_read = torch.cuda.Event()
             return self._static_loss
+        if (teacher is None) != (self._static_teacher is None):
+            raise ValueError("step_graphed: the captured step was made " + ("without" if self._static_teacher is None else "with") +
+                             " a teacher")
         self._static_tok.copy_(tokens, non_blocking=True)
         self._static_tgt.copy_(targets, non_blocking=True)
+        for dst, src in zip(self._static_teacher or (), teacher or ()):
+            dst.copy_(src, non_blocking=True)
         self._inputs_read.record()
         # the descriptors go to the device ahead of the replay, stream-ordered: the host does not wait
         # for the previous step and its bookkeeping runs while the GPU is still busy with it
