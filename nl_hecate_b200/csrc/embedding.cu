@@ -5,13 +5,15 @@
 // The gradient's rows meet wherever an id repeats, and in text a few ids are much of it. Instead of atomics (whose
 // order, and so whose sum, changes from run to run, and which queue up on the hot rows) the tokens are sorted by id with a
 // stable radix sort, every sum then has one order, and every row of d_w is touched once, by one writer:
-//   sort    : least significant digit first, 9 bits a pass: a histogram per 2048 tokens, then ranks from it
+//   sort    : least significant digit first, 9 bits a pass at most: one cluster of CTAs, or for long lists a histogram per 2048 tokens and
+//             ranks from it
 //   reduce  : a run of sorted tokens per group of lanes; an id that lies inside the run is written at once, the pieces of one
 //             that crosses runs go to a buffer
 //   join    : those pieces, added in order by the run in which the id begins
 // Up to SMALL tokens one launch does it all: a CTA per token looks for its id in the whole list, and the first token of an id
 // adds up its rows.
 // Bound by HBM: d_out is read once, the touched rows of d_w once and written once.
+#include <cooperative_groups.h>
 #include <cuda_bf16.h>
 
 #include "nlh_common.cuh"
@@ -26,6 +28,10 @@ constexpr int SMALL = 2048;
 constexpr int THREADS = 128;
 
 template <typename T> struct Vec { static constexpr int N = 16 / sizeof(T); };
+// N elements as they came, and as floats
+template <typename T, int N> struct Raw { uint4 r; };
+template <> struct Raw<float, 1> { float r; };
+template <> struct Raw<__nv_bfloat16, 1> { __nv_bfloat16 r; };
 template <typename T, int N> __device__ __forceinline__ void load(const T* p, float* f);
 template <> __device__ __forceinline__ void load<float, 4>(const float* p, float* f)
 {
@@ -44,17 +50,21 @@ template <> __device__ __forceinline__ void load<__nv_bfloat16, 1>(const __nv_bf
 // N floats to / from fp32 memory
 template <int N> __device__ __forceinline__ void store_f32(float* p, const float* f)
 {
-    if (N == 1) { p[0] = f[0]; return; }
+    if constexpr (N == 1) p[0] = f[0];
+    else {
 #pragma unroll
-    for (int i = 0; i < N; i += 4) *reinterpret_cast<float4*>(p + i) = make_float4(f[i], f[i + 1], f[i + 2], f[i + 3]);
+        for (int i = 0; i < N; i += 4) *reinterpret_cast<float4*>(p + i) = make_float4(f[i], f[i + 1], f[i + 2], f[i + 3]);
+    }
 }
 template <int N> __device__ __forceinline__ void load_f32(const float* p, float* f)
 {
-    if (N == 1) { f[0] = p[0]; return; }
+    if constexpr (N == 1) f[0] = p[0];
+    else {
 #pragma unroll
-    for (int i = 0; i < N; i += 4) {
-        const float4 v = *reinterpret_cast<const float4*>(p + i);
-        f[i] = v.x; f[i + 1] = v.y; f[i + 2] = v.z; f[i + 3] = v.w;
+        for (int i = 0; i < N; i += 4) {
+            const float4 v = *reinterpret_cast<const float4*>(p + i);
+            f[i] = v.x; f[i + 1] = v.y; f[i + 2] = v.z; f[i + 3] = v.w;
+        }
     }
 }
 // One writer per row of d_w: a reduction without an answer, which no load waits for, has no other to race with.
@@ -183,15 +193,8 @@ __global__ void __launch_bounds__(SORT_THREADS) scatter_kernel(const int* ids, c
 #pragma unroll
     for (int e = 0; e < 2; e++) {
         const int digit = 2 * threadIdx.x + e;
-        if (total) { tot[e] = total[digit]; first[e] = hist[(long long)digit * blocks + blockIdx.x]; }
-        else {
-            tot[e] = first[e] = 0;
-            for (int b = 0; b < blocks; b++) {
-                const int c = hist[(long long)digit * blocks + b];
-                if (b < blockIdx.x) first[e] += c;
-                tot[e] += c;
-            }
-        }
+        tot[e] = total[digit];
+        first[e] = hist[(long long)digit * blocks + blockIdx.x];
     }
     int s = tot[0] + tot[1];
     for (int o = 1; o < 32; o <<= 1) { const int y = __shfl_up_sync(0xffffffffu, s, o); if (lane >= o) s += y; }
@@ -208,6 +211,97 @@ __global__ void __launch_bounds__(SORT_THREADS) scatter_kernel(const int* ids, c
 #pragma unroll
     for (int j = 0; j < SORT_ITEMS; j++)
         if (key[j] >= 0) out[s_cnt[w][(key[j] >> shift) & (BINS - 1)] + rank[j]] = make_int2(key[j], pos[j]);
+}
+
+// The whole sort in one launch up to 131072 tokens: a cluster of eight CTAs, a thread ITEMS tokens, the digits' totals exchanged
+// through distributed shared memory, digits only as wide as the passes need. 32768 tokens of a vocabulary of 8192 take 15 us
+// (the launches above: 27 and the gaps between them), 65521 of 50001 take 26 (37). Tokens of one digit in a warp are found by a
+// ballot per bit (a match instruction: 16 us). Sixteen CTAs, more than every part of the GPU promises to hold, would take 12 and 19.
+constexpr int CL = 8, CL_THREADS = 1024, CL_WARPS = CL_THREADS / 32;
+template <int ITEMS>
+__global__ void __cluster_dims__(CL, 1, 1) __launch_bounds__(CL_THREADS, 1) sort_cluster_kernel(const int* ids, int2* bufa, int2* bufb, int n,
+                                                                                               int vocab, int passes, int bits)
+{
+    extern __shared__ int s_dyn[];
+    int* s_cnt = s_dyn;                          // [CL_WARPS][BINS]
+    int* s_tot = s_dyn + CL_WARPS * BINS;        // [BINS] this CTA's tokens of each digit
+    int* s_first = s_tot + BINS;                 // [BINS] where they go
+    const int bins = 1 << bits;
+    __shared__ int s_scan[BINS / 32];
+    namespace cg = cooperative_groups;
+    cg::cluster_group cl = cg::this_cluster();
+    const int rank = (int)cl.block_rank(), tid = threadIdx.x, lane = tid & 31, w = tid >> 5;
+    const int base = (rank * CL_WARPS + w) * ITEMS * 32 + lane;    // warps hold stretches of the list, in order
+    const int2* in = nullptr;
+    int2* out = bufa;
+    for (int p = 0; p < passes; p++) {
+        const int shift = p * bits;
+        for (int i = tid; i < CL_WARPS * bins; i += CL_THREADS) s_cnt[i] = 0;
+        int key[ITEMS], pos[ITEMS], rnk[ITEMS];
+#pragma unroll
+        for (int j = 0; j < ITEMS; j++) {
+            const int i = base + j * 32;
+            key[j] = -1;
+            if (i < n) key[j] = key_of(ids, in, i, vocab, pos[j]);
+        }
+        __syncthreads();
+        int* mine = s_cnt + w * bins;
+#pragma unroll
+        for (int j = 0; j < ITEMS; j++) {
+            const int digit = key[j] < 0 ? -1 : (key[j] >> shift) & (bins - 1);
+            unsigned same = __ballot_sync(0xffffffffu, digit >= 0);
+            if (digit < 0) same = ~same;
+            for (int x = 0; x < bits; x++) {
+                const bool one = (digit >> x) & 1;
+                const unsigned m = __ballot_sync(0xffffffffu, one);
+                same &= one ? m : ~m;
+            }
+            int before = 0;
+            if (digit >= 0) before = mine[digit];
+            __syncwarp();
+            if (digit >= 0) {
+                rnk[j] = before + __popc(same & ((1u << lane) - 1));
+                if (lane == __ffs(same) - 1) mine[digit] = before + __popc(same);
+            }
+            __syncwarp();
+        }
+        __syncthreads();
+        if (tid < bins) {                        // tokens of the digit in the warps before
+            int at = 0;
+#pragma unroll 8
+            for (int j = 0; j < CL_WARPS; j++) { const int c = s_cnt[j * bins + tid]; s_cnt[j * bins + tid] = at; at += c; }
+            s_tot[tid] = at;
+        }
+        cl.sync();
+        int total = 0, first = 0;                // in all CTAs, in the CTAs before
+        if (tid < bins) {
+#pragma unroll
+            for (int r = 0; r < CL; r++) {
+                const int c = *cl.map_shared_rank(s_tot + tid, r);
+                total += c;
+                first += r < rank ? c : 0;
+            }
+            int s = total;
+            for (int o = 1; o < 32; o <<= 1) { const int y = __shfl_up_sync(0xffffffffu, s, o); if (lane >= o) s += y; }
+            if (lane == 31) s_scan[w] = s;
+            first += s - total;
+        }
+        __syncthreads();
+        if (tid < bins) {
+            for (int j = 0; j < w; j++) first += s_scan[j];
+            s_first[tid] = first;
+        }
+        __syncthreads();
+#pragma unroll
+        for (int j = 0; j < ITEMS; j++)
+            if (key[j] >= 0) {
+                const int digit = (key[j] >> shift) & (bins - 1);
+                out[s_first[digit] + mine[digit] + rnk[j]] = make_int2(key[j], pos[j]);
+            }
+        cl.sync();                               // the list is whole for the next pass, and every s_tot has been read
+        in = out;
+        out = out == bufa ? bufb : bufa;
+    }
 }
 
 // ── reduce ──
@@ -246,77 +340,94 @@ __global__ void __launch_bounds__(THREADS) reduce_kernel(const T* __restrict__ d
     };
     constexpr int U = 8;
     for (int i = 0; i < e; i += U) {
-        float f[U][N];
-        int key[U];
+        Raw<T, N> raw[U];
 #pragma unroll
-        for (int u = 0; u < U; u++) {
-            key[u] = vocab;
-            if (i + u < e) {
-                const int2 s = mine[i + u];
-                key[u] = s.x;
-                if (s.x < vocab) load<T, N>(dy + (long long)s.y * d + c, f[u]);
-            }
-        }
+        for (int u = 0; u < U; u++)
+            if (i + u < e && mine[i + u].x < vocab) raw[u] = *reinterpret_cast<const Raw<T, N>*>(dy + (long long)mine[i + u].y * d + c);
 #pragma unroll
         for (int u = 0; u < U; u++) {
             if (i + u >= e) break;
-            if (key[u] != cur) {
+            if (mine[i + u].x != cur) {
                 flush(false);
-                cur = key[u];
+                cur = mine[i + u].x;
                 head = false;
 #pragma unroll
                 for (int x = 0; x < N; x++) acc[x] = 0.f;
             }
             if (cur < vocab) {
+                float f[N];
+                load<T, N>(reinterpret_cast<const T*>(&raw[u]), f);
 #pragma unroll
-                for (int x = 0; x < N; x++) acc[x] += f[u][x];
+                for (int x = 0; x < N; x++) acc[x] += f[x];
             }
         }
     }
     flush(cur == next);
 }
-// Ids that cross runs: the run in which one begins adds its pieces up. A CTA per run and 32 N columns; most have nothing to do.
-// Its eight warps look 256 runs ahead at once for the last one that begins with the id, take a stretch of the pieces each and
-// join their sums in order. (One warp walking the pieces of the most frequent id of a text of 32768 tokens took 51 us.)
+// Ids that cross runs: the run in which one begins adds its pieces up, in their order. A warp per run and 32 N columns; most have
+// nothing to do. A warp looks 32 runs ahead at once for the last one that begins with the id. Up to LONG pieces it adds by itself;
+// for more the CTA's eight warps take a stretch each and join their sums (one warp walking the pieces of the most frequent id
+// of a text of 32768 tokens took 51 us).
+constexpr int LONG = 16;
+template <int N>
+__device__ __forceinline__ void add_pieces(float (&acc)[N], const float* part, long long r, long long i0, long long i1, int d, int c)
+{
+#pragma unroll
+    for (int i = 0; i < N; i++) acc[i] = 0.f;
+    if (c >= d) return;
+#pragma unroll 8
+    for (long long i = i0; i < i1; i++) {
+        float f[N];
+        load_f32<N>(part + ((r + i) * 2 + (i == 0)) * d + c, f);       // piece 0 is what run r left over, the others began before their runs
+#pragma unroll
+        for (int x = 0; x < N; x++) acc[x] += f[x];
+    }
+}
 template <int N, bool ADD>
 __global__ void __launch_bounds__(256) join_kernel(const int2* __restrict__ sorted, float* __restrict__ dw, const float* __restrict__ part,
                                                    int n, int vocab, int d, int run, float scale)
 {
     __shared__ float s_acc[8][32 * N];
+    __shared__ long long s_pieces[8];
+    __shared__ int s_key[8];
     const int lane = threadIdx.x & 31, w = threadIdx.x >> 5, c = (blockIdx.y * 32 + lane) * N;
-    const long long r = blockIdx.x, b = r * run, e = b + run;
-    if (e >= n) return;
-    const int key = sorted[e - 1].x;
-    if (key >= vocab || sorted[e].x != key) return;                    // nothing goes on behind this run
-    if (b > 0 && sorted[b].x == key && sorted[b - 1].x == key) return;  // it began before it
-    long long pieces = 0;                                              // runs behind r that begin with the id
-    for (;;) {
-        const long long q = r + 1 + pieces + threadIdx.x;
-        const int more = __syncthreads_count(q * run < n && sorted[q * run].x == key);    // sorted: they are the first ones
-        pieces += more;
-        if (more < 256) break;
-    }
-    const long long each = (pieces + 8) / 8, i0 = w * each, i1 = min(pieces + 1, i0 + each);   // piece 0 is run r's own
-    float acc[N];
-#pragma unroll
-    for (int i = 0; i < N; i++) acc[i] = 0.f;
-    if (c < d) {
-#pragma unroll 8
-        for (long long i = i0; i < i1; i++) {
-            float f[N];
-            load_f32<N>(part + ((r + i) * 2 + (i == 0)) * d + c, f);
-#pragma unroll
-            for (int x = 0; x < N; x++) acc[x] += f[x];
+    const long long r = (long long)blockIdx.x * 8 + w, b = r * run, e = b + run;
+    long long pieces = 0;                                              // runs behind r that begin with the id, if it begins in r
+    int key = -1;
+    if (e < n) {
+        key = sorted[e - 1].x;
+        if (key < vocab && sorted[e].x == key && !(b > 0 && sorted[b].x == key && sorted[b - 1].x == key)) {
+            for (;;) {
+                const long long q = r + 1 + pieces + lane;
+                const int more = __popc(__ballot_sync(0xffffffffu, q * run < n && sorted[q * run].x == key));    // sorted: the first ones
+                pieces += more;
+                if (more < 32) break;
+            }
         }
     }
-#pragma unroll
-    for (int i = 0; i < N; i++) s_acc[w][i * 32 + lane] = acc[i];
+    float acc[N];
+    if (pieces > 0 && pieces <= LONG) {
+        add_pieces<N>(acc, part, r, 0, pieces + 1, d, c);
+        if (c < d) add_row<N, ADD>(dw + (long long)key * d + c, acc, scale);
+    }
+    if (lane == 0) { s_pieces[w] = pieces > LONG ? pieces : 0; s_key[w] = key; }
     __syncthreads();
-    if (w != 0 || c >= d) return;
-    for (int j = 1; j < 8; j++)
+    for (int o = 0; o < 8; o++) {
+        const long long many = s_pieces[o];
+        if (many == 0) continue;
+        const long long each = (many + 8) / 8, i0 = w * each, i1 = min(many + 1, i0 + each);
+        add_pieces<N>(acc, part, (long long)blockIdx.x * 8 + o, i0, i1, d, c);
 #pragma unroll
-        for (int i = 0; i < N; i++) acc[i] += s_acc[j][i * 32 + lane];
-    add_row<N, ADD>(dw + (long long)key * d + c, acc, scale);
+        for (int i = 0; i < N; i++) s_acc[w][i * 32 + lane] = acc[i];
+        __syncthreads();
+        if (w == 0 && c < d) {
+            for (int j = 1; j < 8; j++)
+#pragma unroll
+                for (int i = 0; i < N; i++) acc[i] += s_acc[j][i * 32 + lane];
+            add_row<N, ADD>(dw + (long long)s_key[o] * d + c, acc, scale);
+        }
+        __syncthreads();
+    }
 }
 
 // ── few tokens ──
@@ -377,7 +488,7 @@ __global__ void __launch_bounds__(THREADS) small_kernel(const T* __restrict__ dy
 
 // ── host ──
 struct Plan {
-    int passes, blocks, run, runs;
+    int passes, bits, blocks, run, runs;              // bits: of a digit in the one-launch sort
     int2 *a, *b;
     int *hist, *total;
     float* part;
@@ -389,6 +500,8 @@ static int64_t place(Plan& P, char* base, int n, int vocab, int d)
     int bits = 1;
     while (bits < 31 && (vocab >> bits) != 0) bits++;          // keys 0 .. vocab
     P.passes = (bits + BITS - 1) / BITS;
+    P.bits = (bits + P.passes - 1) / P.passes;
+    if (P.bits < 5) P.bits = 5;                                // whole warps of digits
     P.blocks = (int)(((int64_t)n + SORT_TILE - 1) / SORT_TILE);
     // runs of 32 sorted tokens give every SM a few even at SMALL tokens; longer ones shorten the join of a hot id where there are plenty
     P.run = n <= (1 << 18) ? 32 : 128;
@@ -409,6 +522,15 @@ static int lanes_for(int d, int per, int most)
     return l;
 }
 
+template <int ITEMS> static bool sort_cluster(const int* ids, const Plan& P, int n, int vocab, const char* where)
+{
+    constexpr int bytes = (CL_WARPS + 2) * BINS * 4;
+    const cudaError_t e = cudaFuncSetAttribute(sort_cluster_kernel<ITEMS>, cudaFuncAttributeMaxDynamicSharedMemorySize, bytes);
+    if (e != cudaSuccess) { record_status(NLH_ERR_CUDA, where, cudaGetErrorString(e)); return false; }
+    sort_cluster_kernel<ITEMS><<<CL, CL_THREADS, bytes, current_stream()>>>(ids, P.a, P.b, n, vocab, P.passes, P.bits);
+    return check_launch(where);
+}
+
 template <typename T, int N, bool ADD>
 static bool backward(const T* dy, const int* ids, float* dw, int n, int vocab, int d, float scale, char* ws, const char* where)
 {
@@ -421,26 +543,29 @@ static bool backward(const T* dy, const int* ids, float* dw, int n, int vocab, i
         return check_launch(where);
     }
     const int2* in = nullptr;
-    int2* out = P.a;
-    for (int p = 0; p < P.passes; p++) {
-        hist_kernel<<<P.blocks, SORT_THREADS, 0, st>>>(ids, in, P.hist, n, vocab, p * BITS, P.blocks);
-        if (!check_launch(where)) return false;
-        // a scatter CTA adds up the histograms itself while they are few: one launch less
-        const bool scan = P.blocks > 64;
-        if (scan) {
+    if (n <= CL * CL_THREADS * 16) {
+        const int items = n <= CL * CL_THREADS * 4 ? 4 : n <= CL * CL_THREADS * 8 ? 8 : 16;
+        if (!(items == 4 ? sort_cluster<4>(ids, P, n, vocab, where) : items == 8 ? sort_cluster<8>(ids, P, n, vocab, where)
+                                                                                  : sort_cluster<16>(ids, P, n, vocab, where))) return false;
+        in = P.passes & 1 ? P.a : P.b;
+    } else {
+        int2* out = P.a;
+        for (int p = 0; p < P.passes; p++) {
+            hist_kernel<<<P.blocks, SORT_THREADS, 0, st>>>(ids, in, P.hist, n, vocab, p * BITS, P.blocks);
+            if (!check_launch(where)) return false;
             scan_kernel<<<BINS / 8, 256, 0, st>>>(P.hist, P.total, P.blocks);
             if (!check_launch(where)) return false;
+            scatter_kernel<<<P.blocks, SORT_THREADS, 0, st>>>(ids, in, out, P.hist, P.total, n, vocab, p * BITS, P.blocks);
+            if (!check_launch(where)) return false;
+            in = out;
+            out = out == P.a ? P.b : P.a;
         }
-        scatter_kernel<<<P.blocks, SORT_THREADS, 0, st>>>(ids, in, out, P.hist, scan ? P.total : nullptr, n, vocab, p * BITS, P.blocks);
-        if (!check_launch(where)) return false;
-        in = out;
-        out = out == P.a ? P.b : P.a;
     }
     const int per = THREADS / lanes;
     const dim3 grid((P.runs + per - 1) / per, (d + lanes * N - 1) / (lanes * N));
     reduce_kernel<T, N, ADD><<<grid, THREADS, per * (P.run + 2) * sizeof(int2), st>>>(dy, in, dw, P.part, n, vocab, d, lanes, P.run, scale);
     if (!check_launch(where)) return false;
-    join_kernel<N, ADD><<<dim3(P.runs, (d + 32 * N - 1) / (32 * N)), 256, 0, st>>>(in, dw, P.part, n, vocab, d, P.run, scale);
+    join_kernel<N, ADD><<<dim3((P.runs + 7) / 8, (d + 32 * N - 1) / (32 * N)), 256, 0, st>>>(in, dw, P.part, n, vocab, d, P.run, scale);
     return check_launch(where);
 }
 
