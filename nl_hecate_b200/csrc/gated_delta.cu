@@ -258,7 +258,6 @@ __global__ void __launch_bounds__(256, DKP == 64 ? 2 : 1) gd_state_fwd_kernel(Ar
         put_state(m);
     }
     Prefetch<T, DKP, 256> pk;
-    PrefetchT<256> pt;
     GateRow pg;
     Pair<T> pv[NT][2];
     const bool vpair = ((reinterpret_cast<uintptr_t>((const T*)A.v + n0) | (uintptr_t)((A.vb | A.vt | A.vh) * (long long)sizeof(T))) &
@@ -268,7 +267,6 @@ __global__ void __launch_bounds__(256, DKP == 64 ? 2 : 1) gd_state_fwd_kernel(Ar
         const Chunk ch = get_chunk(A, slot);
         const long long tile = (long long)slot * A.hv + h;
         pk.load((const T*)A.k + ch.b * A.kb + ch.t0 * A.kt + (h / A.share) * A.kh, A.kt, ch.len, A.dk);
-        pt.load(A.tmat + tile * T_BYTES);
         if (tid < C) { ldg(pg.g, reinterpret_cast<const float*>(A.gates + tile * C + tid)); ldg(pg.theta, A.theta_eff + tile * C + tid); }
         const T* vp = (const T*)A.v + ch.b * A.vb + ch.t0 * A.vt + h * A.vh + n0;
 #pragma unroll
@@ -282,10 +280,9 @@ __global__ void __launch_bounds__(256, DKP == 64 ? 2 : 1) gd_state_fwd_kernel(Ar
     auto commit = [&](int buf) {
         if (L::KB == 1) __syncthreads();              // the one buffer of K has been read
         pk.store(Kb + (L::KB == 1 ? 0 : buf) * IN * L::PK, LK, L::PK);
-        pt.store(Ts);
         if (tid < C) { s_gate[buf][tid] = pg.g; s_w[buf][tid] = pg.g.w * pg.theta; }
     };
-    if (count > 0) { fetch(0); commit(0); }
+    if (count > 0) { copy_t<256>(Ts, A.tmat + ((long long)slot0 * A.hv + h) * T_BYTES); fetch(0); commit(0); }
     __syncthreads();
     for (int c = 0; c < count; c++) {
         const int buf = c & 1;
@@ -315,6 +312,7 @@ __global__ void __launch_bounds__(256, DKP == 64 ? 2 : 1) gd_state_fwd_kernel(Ar
                 put2<3>(Rs + row * LS + H * hf + 8 * n + 2 * t, L::PR, x.x - s_gate[buf][row].z * acc[n][2 * r],
                         x.y - s_gate[buf][row].z * acc[n][2 * r + 1]);
             }
+        wait_t();
         __syncthreads();
         zero(acc);
         gemm<NT, false, true, 3, 3>(acc, Ts + 16 * rb * LP, LP, C * LP, Rs + H * hf, LS, L::PR, 0, 16 * (rb + 1));
@@ -329,6 +327,7 @@ __global__ void __launch_bounds__(256, DKP == 64 ? 2 : 1) gd_state_fwd_kernel(Ar
                 put2<3>(Us + row * LS + col, L::PR, wt * a, wt * b);
             }
         __syncthreads();
+        if (c + 1 < count) copy_t<256>(Ts, A.tmat + (tile + A.hv) * T_BYTES);
         const float gl = s_gate[buf][C - 1].z;
 #pragma unroll
         for (int m = 0; m < MT; m++) {
@@ -554,7 +553,6 @@ __global__ void __launch_bounds__(256, DKP == 64 ? 2 : 1) gd_state_bwd_kernel(Ar
         put_state(m);
     }
     Prefetch<T, DKP, 256> pk;
-    PrefetchT<256> pt;
     GateRow pg;
     float2 pf[NT][2], pn[MT][NT][2];
     auto fetch = [&](int c) {
@@ -562,7 +560,6 @@ __global__ void __launch_bounds__(256, DKP == 64 ? 2 : 1) gd_state_bwd_kernel(Ar
         const Chunk ch = get_chunk(A, slot);
         const long long tile = (long long)slot * A.hv + h;
         pk.load((const T*)A.k + ch.b * A.kb + ch.t0 * A.kt + (h / A.share) * A.kh, A.kt, ch.len, A.dk);
-        pt.load(A.tmat + tile * T_BYTES);
         if (tid < C) { ldg(pg.g, reinterpret_cast<const float*>(A.gates + tile * C + tid)); ldg(pg.theta, A.theta_eff + tile * C + tid); }
         const float* fp = A.f + tile * C * A.dvp + n0;
         const float* np = A.d_chunk + tile * DKP * A.dvp + n0;
@@ -579,10 +576,9 @@ __global__ void __launch_bounds__(256, DKP == 64 ? 2 : 1) gd_state_bwd_kernel(Ar
     auto commit = [&](int buf) {
         if (L::KB == 1) __syncthreads();
         pk.store(Kb + (L::KB == 1 ? 0 : buf) * IN * L::PK, LK, L::PK);
-        pt.store(Ts);
         if (tid < C) { s_gate[buf][tid] = pg.g; s_theta[buf][tid] = pg.theta; }
     };
-    if (count > 0) { fetch(count - 1); commit(0); }
+    if (count > 0) { copy_t<256>(Ts, A.tmat + ((long long)(slot0 + count - 1) * A.hv + h) * T_BYTES); fetch(count - 1); commit(0); }
     __syncthreads();
     for (int c = count - 1; c >= 0; c--) {
         const int buf = (count - 1 - c) & 1, slot = slot0 + c;
@@ -614,6 +610,7 @@ __global__ void __launch_bounds__(256, DKP == 64 ? 2 : 1) gd_state_bwd_kernel(Ar
                 const float wi = s_gate[buf][row].w, th = s_theta[buf][row];
                 put2<3>(Rs + row * LS + H * hf + 8 * n + 2 * t, L::PR, th * (f[n][r].x + wi * acc[n][2 * r]), th * (f[n][r].y + wi * acc[n][2 * r + 1]));
             }
+        wait_t();
         __syncthreads();
         zero(acc);
         gemm<NT, true, true, 3, 3>(acc, Ts + 16 * rb, LP, C * LP, Rs + H * hf, LS, L::PR, 16 * rb, C);
@@ -635,6 +632,7 @@ __global__ void __launch_bounds__(256, DKP == 64 ? 2 : 1) gd_state_bwd_kernel(Ar
                 }
             }
         __syncthreads();
+        if (c > 0) copy_t<256>(Ts, A.tmat + (tile - A.hv) * T_BYTES);
         const float gl = s_gate[buf][C - 1].z;
 #pragma unroll
         for (int m = 0; m < MT; m++) {
@@ -1080,7 +1078,10 @@ template <typename T, int DKP> static bool launch_states(const Args& A, bool bac
 {
     const long long heads = (long long)(A.n_seqs > 0 ? A.n_seqs : A.batch) * A.hv;
     if (heads == 0) return true;
-    if (heads * (A.dvp / 32) < 2 * 148) return launch_states_ns<T, DKP, 16>(A, heads, backward, st, where);
+    // 16 columns a CTA while 32 would leave SMs without one (2 x 8 heads of 128 x 128: 45 + 51 us against 65 + 76; at 128 CTAs of 32
+    // columns, 4 x 16 heads of 64 x 64, both take 440), and for packed batches longer, since their few longest sequences run
+    // alone in the end (13 prompts x 8 heads: 99 us against 138)
+    if (heads * (A.dvp / 32) < (A.n_seqs > 0 ? 4 * 148 : 128)) return launch_states_ns<T, DKP, 16>(A, heads, backward, st, where);
     return launch_states_ns<T, DKP, 32>(A, heads, backward, st, where);
 }
 

@@ -346,23 +346,16 @@ template <typename T, int COLS, int THREADS> struct Prefetch {
         }
     }
 };
-// The planes of T, copied as they are.
-template <int THREADS> struct PrefetchT {
-    static constexpr int N = (T_BYTES / 16 + THREADS - 1) / THREADS;
-    uint4 r[N];
-    __device__ __forceinline__ void load(const unsigned char* p)
-    {
-#pragma unroll
-        for (int i = 0; i < N; i++)
-            if ((int)threadIdx.x + i * THREADS < T_BYTES / 16) ldg(r[i], p + (threadIdx.x + i * THREADS) * 16);
-    }
-    __device__ __forceinline__ void store(bf* dst) const
-    {
-#pragma unroll
-        for (int i = 0; i < N; i++)
-            if ((int)threadIdx.x + i * THREADS < T_BYTES / 16) reinterpret_cast<uint4*>(dst)[threadIdx.x + i * THREADS] = r[i];
-    }
-};
+// The planes of T, copied as they are, straight into shared memory: issued when the chunk before has no more use for its T, waited
+// for when the next one needs it, half a chunk later.
+template <int THREADS> __device__ __forceinline__ void copy_t(bf* dst, const unsigned char* src)
+{
+    const unsigned d = smem_addr(dst);
+    for (int i = threadIdx.x; i < T_BYTES / 16; i += THREADS)
+        asm volatile("cp.async.cg.shared.global [%0], [%1], 16;\n" ::"r"(d + 16 * i), "l"(src + 16 * i) : "memory");
+    asm volatile("cp.async.commit_group;\n" ::: "memory");
+}
+__device__ __forceinline__ void wait_t() { asm volatile("cp.async.wait_group 0;\n" ::: "memory"); }
 
 }  // namespace gd
 }  // namespace nlh
