@@ -64,27 +64,29 @@ __device__ __forceinline__ int first_slot(const Args& A, int seq) { return A.sta
 __device__ __forceinline__ int chunk_count(const Args& A, int seq) { return A.starts ? A.off[seq + 1] - A.off[seq] : A.nc; }
 
 // ── prep: gates and T = (I + B diag(theta))^-1 of a chunk ──
-// One CTA of four warps per chunk and value head. T is built from the inverses of its 16 x 16 diagonal blocks
-// (forward substitution, a thread per column) by [[P, 0], [R, S]]^-1 = [[P', 0], [-S' R P', S']] twice, in fp32 FMA.
+// One CTA of eight warps per chunk and value head. T is built from the inverses of its 16 x 16 diagonal blocks (forward substitution,
+// a thread per column) by [[P, 0], [R, S]]^-1 = [[P', 0], [-S' R P', S']]: to 32 x 32 in fp32 FMA, to 64 x 64 on the tensor
+// cores, in the planes that leave for global memory. (All of it in FMA: 138 us for 4096 tiles of fp32 keys, against 99.)
 // A theta of 0 is taken as 2^-60: then u is 2^-60 e, which no sum of fp32 sees, and the gradient e.x / theta of
 // theta needs no case of its own (x, the gradient of v, carries the factor theta).
 template <typename T>
-__global__ void __launch_bounds__(128) gd_prep_kernel(Args A)
+__global__ void __launch_bounds__(256, 3) gd_prep_kernel(Args A)
 {
+    constexpr int IN = Pl<T>::in, PS = C * LP;
     extern __shared__ float4 smem4[];
-    float* Am = reinterpret_cast<float*>(smem4);
+    bf* Tp = reinterpret_cast<bf*>(smem4);        // K's planes, then T's
+    float* Am = reinterpret_cast<float*>(Tp + 3 * PS);
     float* Tm = Am + C * LD;
-    bf* Ks = reinterpret_cast<bf*>(Tm + C * LD);
-    float* Z = reinterpret_cast<float*>(Ks);
+    float* Z = Am + C / 2;                        // [32][LD] inside Am's upper right quarter, which no one reads
     __shared__ float2 s_g[C];
     __shared__ float s_theta[C];
     const int slot = blockIdx.x / A.hv, h = blockIdx.x - slot * A.hv;
     const Chunk ch = get_chunk(A, slot);
     if (ch.len <= 0) return;
     const long long tile = (long long)slot * A.hv + h;
-    const int tid = threadIdx.x, lane = tid & 31, w = tid >> 5, g = lane >> 2, t = lane & 3;
+    const int tid = threadIdx.x, lane = tid & 31, w = tid >> 5, rb = w & 3, hf = w >> 2, g = lane >> 2, t = lane & 3;
 
-    if (w == 0) {
+    if (w == 7) {                                 // a warp whose part of K K^T is upper triangle, or little else
         const long long at = ch.b * A.gb + ch.t0 * A.gt + h * A.gh;
         double x[2], th[2];
 #pragma unroll
@@ -110,34 +112,31 @@ __global__ void __launch_bounds__(128) gd_prep_kernel(Args A)
             s_theta[i] = (float)th[j];
         }
     }
-    constexpr int IN = Pl<T>::in, PS = C * LP;
-    float lo[4][4], hi[4][4];
-    zero(lo);
-    zero(hi);
+    float kk[4][4];
+    zero(kk);
+    const bool need = 32 * hf <= 16 * rb + 15;
     const T* kp = (const T*)A.k + ch.b * A.kb + ch.t0 * A.kt + (h / A.share) * A.kh;
     for (int c0 = 0; c0 < A.dk; c0 += 64) {
         __syncthreads();
-        load_tile<T, 64, 128>(Ks, LP, PS, kp + c0, A.kt, ch.len, A.dk - c0);
+        load_tile<T, 64, 256>(Tp, LP, PS, kp + c0, A.kt, ch.len, A.dk - c0);
         __syncthreads();
-        gemm<4, false, false, IN, IN>(lo, Ks + 16 * w * LP, LP, PS, Ks, LP, PS, 0, 64);
-        if (w >= 2) gemm<4, false, false, IN, IN>(hi, Ks + 16 * w * LP, LP, PS, Ks + 32 * LP, LP, PS, 0, 64);
+        if (need) gemm<4, false, false, IN, IN>(kk, Tp + 16 * rb * LP, LP, PS, Tp + 32 * hf * LP, LP, PS, 0, 64);
     }
-    for (int i = tid; i < C * LD / 4; i += 128) reinterpret_cast<float4*>(Tm)[i] = make_float4(0.f, 0.f, 0.f, 0.f);
+    if (need) {
 #pragma unroll
-    for (int half = 0; half < 2; half++)
-#pragma unroll
-        for (int n = 0; n < 4; n++)
+        for (int n = 0; n < 4; n++) {
+            if (32 * hf + 8 * n > 16 * rb + 15) continue;
 #pragma unroll
             for (int r = 0; r < 2; r++) {
-                const int i = 16 * w + g + 8 * r, j = 32 * half + 8 * n + 2 * t;
+                const int i = 16 * rb + g + 8 * r, j = 32 * hf + 8 * n + 2 * t;
+                const float2 gi = s_g[i];
                 float a[2];
 #pragma unroll
-                for (int c = 0; c < 2; c++) {
-                    const float kk = half ? hi[n][2 * r + c] : lo[n][2 * r + c];
-                    a[c] = j + c < i ? decay(s_g[i], s_g[j + c]) * kk * s_theta[j + c] : 0.f;
-                }
+                for (int e = 0; e < 2; e++) a[e] = j + e < i ? decay(gi, s_g[j + e]) * kk[n][2 * r + e] * s_theta[j + e] : 0.f;
                 st2(Am + i * LD + j, a[0], a[1]);
             }
+        }
+    }
     __syncthreads();
     if (tid < 64) {
         const int b = tid & ~15, j = tid & 15;
@@ -147,65 +146,68 @@ __global__ void __launch_bounds__(128) gd_prep_kernel(Args A)
             float s = i == j ? 1.f : 0.f;
             const float* row = Am + (b + i) * LD + b;
 #pragma unroll
-            for (int l = 0; l < i; l++) s = l < j ? s : fmaf(-row[l], col[l], s);
-            col[i] = i < j ? 0.f : s;
-            Tm[(b + i) * LD + b + j] = col[i];
+            for (int l = 0; l < i; l++) s = fmaf(-row[l], col[l], s);       // col[l] is 0 above the diagonal
+            col[i] = s;
+            Tm[(b + i) * LD + b + j] = s;
+        }
+    } else {
+        // meanwhile the planes' blocks that need no inverse: zeros, and B diag(theta) where T's lower left quarter will be
+        for (int i = tid - 64; i < C * 16; i += 192) {
+            const int r = i >> 4, c = (i & 15) * 4;
+            if (r < 32 && c >= 32) put4<3>(Tp + r * LP + c, PS, make_float4(0.f, 0.f, 0.f, 0.f));
+            if (r >= 32 && c < 32) put4<3>(Tp + r * LP + c, PS, *reinterpret_cast<const float4*>(Am + r * LD + c));
         }
     }
     __syncthreads();
-    {   // 16 -> 32, both pairs of blocks at once
-        const int p = tid >> 6, r = (tid >> 2) & 15, c = (tid & 3) * 4, r0 = 32 * p + 16, c0 = 32 * p;
-        float z[4] = {0.f, 0.f, 0.f, 0.f};
+    {   // 16 -> 32, both pairs of blocks at once, two columns a thread
+        const int p = tid >> 7, r = (tid >> 3) & 15, c = (tid & 7) * 2, r0 = 32 * p + 16, c0 = 32 * p;
+        float2 z = make_float2(0.f, 0.f);
+#pragma unroll
         for (int l = 0; l < 16; l++) {
             const float a = Am[(r0 + r) * LD + c0 + l];
-            const float4 b = *reinterpret_cast<const float4*>(Tm + (c0 + l) * LD + c0 + c);
-            // columns of T behind row l are 0 and must stay out: 0 times a later token's NaN would be a NaN
-            z[0] = c > l ? z[0] : fmaf(a, b.x, z[0]);
-            z[1] = c + 1 > l ? z[1] : fmaf(a, b.y, z[1]);
-            z[2] = c + 2 > l ? z[2] : fmaf(a, b.z, z[2]);
-            z[3] = c + 3 > l ? z[3] : fmaf(a, b.w, z[3]);
+            const float2 b = *reinterpret_cast<const float2*>(Tm + (c0 + l) * LD + c0 + c);
+            z.x = fmaf(a, b.x, z.x);
+            z.y = fmaf(a, b.y, z.y);
         }
-        *reinterpret_cast<float4*>(Z + (16 * p + r) * LD + c) = make_float4(z[0], z[1], z[2], z[3]);
+        *reinterpret_cast<float2*>(Z + (16 * p + r) * LD + c) = z;
         __syncthreads();
-        float o[4] = {0.f, 0.f, 0.f, 0.f};
-        for (int l = 0; l <= r; l++) {
+        float2 o = make_float2(0.f, 0.f);
+#pragma unroll
+        for (int l = 0; l < 16; l++) {
             const float a = -Tm[(r0 + r) * LD + r0 + l];
-            const float4 b = *reinterpret_cast<const float4*>(Z + (16 * p + l) * LD + c);
-            o[0] = fmaf(a, b.x, o[0]); o[1] = fmaf(a, b.y, o[1]); o[2] = fmaf(a, b.z, o[2]); o[3] = fmaf(a, b.w, o[3]);
+            const float2 b = *reinterpret_cast<const float2*>(Z + (16 * p + l) * LD + c);
+            o.x = fmaf(a, b.x, o.x);
+            o.y = fmaf(a, b.y, o.y);
         }
-        *reinterpret_cast<float4*>(Tm + (r0 + r) * LD + c0 + c) = make_float4(o[0], o[1], o[2], o[3]);
-        __syncthreads();
-    }
-    {   // 32 -> 64
-        const int r = tid >> 2, c = (tid & 3) * 8;
-        float z[8];
-#pragma unroll
-        for (int i = 0; i < 8; i++) z[i] = 0.f;
-        for (int l = c; l < 32; l++) {
-            const float a = Am[(32 + r) * LD + l];
-#pragma unroll
-            for (int i = 0; i < 8; i++) z[i] = c + i > l ? z[i] : fmaf(a, Tm[l * LD + c + i], z[i]);
-        }
-#pragma unroll
-        for (int i = 0; i < 8; i++) Z[r * LD + c + i] = z[i];
-        __syncthreads();
-#pragma unroll
-        for (int i = 0; i < 8; i++) z[i] = 0.f;
-        for (int l = 0; l <= r; l++) {
-            const float a = -Tm[(32 + r) * LD + 32 + l];
-#pragma unroll
-            for (int i = 0; i < 8; i++) z[i] = fmaf(a, Z[l * LD + c + i], z[i]);
-        }
-        __syncthreads();
-#pragma unroll
-        for (int i = 0; i < 8; i++) Tm[(32 + r) * LD + c + i] = z[i];
+        *reinterpret_cast<float2*>(Tm + (r0 + r) * LD + c0 + c) = o;
     }
     __syncthreads();
-    bf* out = reinterpret_cast<bf*>(A.tmat + tile * T_BYTES);
-    for (int i = tid; i < C * 16; i += 128) {
-        const int r = i >> 4, c = (i & 15) * 4;
-        put4<3>(out + r * LP + c, PS, *reinterpret_cast<const float4*>(Tm + r * LD + c));
+#pragma unroll
+    for (int i = 0; i < 2; i++) {                 // the 32 x 32 inverses into the planes
+        const int at = tid + i * 256, q = at >> 8, r = (at >> 3) & 31, c = (at & 7) * 4;
+        float4 v = *reinterpret_cast<const float4*>(Tm + (32 * q + r) * LD + 32 * q + c);
+        if (r < 16 && c >= 16) v = make_float4(0.f, 0.f, 0.f, 0.f);         // never written in Tm
+        put4<3>(Tp + (32 * q + r) * LP + 32 * q + c, PS, v);
     }
+    __syncthreads();
+    {   // 32 -> 64: warp = 16 x 8 of the lower left quarter
+        const int r0 = 32 + 16 * (w & 1), c0 = 8 * (w >> 1);
+        float z[1][4];
+        zero(z);
+        gemm<1, false, true, 3, 3>(z, Tp + r0 * LP, LP, PS, Tp + c0, LP, PS, 0, 32);
+        __syncthreads();
+        put2<3>(Tp + (r0 + g) * LP + c0 + 2 * t, PS, z[0][0], z[0][1]);
+        put2<3>(Tp + (r0 + g + 8) * LP + c0 + 2 * t, PS, z[0][2], z[0][3]);
+        __syncthreads();
+        zero(z);
+        gemm<1, false, true, 3, 3>(z, Tp + r0 * LP + 32, LP, PS, Tp + 32 * LP + c0, LP, PS, 0, 32);
+        __syncthreads();
+        put2<3>(Tp + (r0 + g) * LP + c0 + 2 * t, PS, -z[0][0], -z[0][1]);
+        put2<3>(Tp + (r0 + g + 8) * LP + c0 + 2 * t, PS, -z[0][2], -z[0][3]);
+    }
+    __syncthreads();
+    uint4* out = reinterpret_cast<uint4*>(A.tmat + tile * T_BYTES);
+    for (int i = tid; i < T_BYTES / 16; i += 256) out[i] = reinterpret_cast<const uint4*>(Tp)[i];
 }
 
 // ── forward states: the recurrence over chunks for NS columns of V ──
@@ -1093,9 +1095,9 @@ template <typename T> static bool run_forward(Args& A, cudaStream_t st, const ch
     }
     const unsigned tiles = (unsigned)((long long)A.slots * A.hv);
     if (tiles) {
-        constexpr int bytes = 2 * C * LD * 4 + Pl<T>::in * C * LP * 2 > 3 * C * LD * 4 ? 2 * C * LD * 4 + Pl<T>::in * C * LP * 2 : 3 * C * LD * 4;
+        constexpr int bytes = T_BYTES + 2 * C * LD * 4;
         if (!allow_smem(gd_prep_kernel<T>, bytes, where)) return false;
-        gd_prep_kernel<T><<<tiles, 128, bytes, st>>>(A);
+        gd_prep_kernel<T><<<tiles, 256, bytes, st>>>(A);
         if (!check_launch(where)) return false;
     }
     if (!(A.dkp == 64 ? launch_states<T, 64>(A, false, st, where) : launch_states<T, 128>(A, false, st, where))) return false;
