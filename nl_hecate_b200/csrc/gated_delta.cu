@@ -379,18 +379,20 @@ __device__ __forceinline__ void store_rows(T* out, const float (&acc)[4][4], int
 
 // ── forward outputs ──
 // Eight warps: warp = 16 tokens x 32 of the tile's 64 columns. For bf16 the state, P and U are two planes: y is rounded to bf16.
+// Two places in shared memory, Q then P, and K, then S, then U: four CTAs share an SM and cover each other's loads (4096 tiles
+// fp32: 151 us; three places and two CTAs 166, three CTAs with the next tile on its way in registers 174).
 template <typename T> struct OutFwdSmem {
-    static constexpr int PS = C * LP, IN = Pl<T>::in, O = Pl<T>::out, KP = IN > O ? IN : O;      // P goes where K was
-    static constexpr int BYTES = 2 * PS * (IN + KP + O);
+    static constexpr int PS = C * LP, IN = Pl<T>::in, O = Pl<T>::out, M = IN > O ? IN : O;
+    static constexpr int BYTES = 2 * PS * 2 * M;
 };
 template <typename T>
-__global__ void __launch_bounds__(256, Pl<T>::in == 1 ? 3 : 2) gd_out_fwd_kernel(Args A)
+__global__ void __launch_bounds__(256, 4) gd_out_fwd_kernel(Args A)
 {
     typedef OutFwdSmem<T> L;
     constexpr int PS = L::PS, IN = L::IN, O = L::O;
     extern __shared__ float4 smem4[];
     bf* Qs = reinterpret_cast<bf*>(smem4);
-    bf *Ks = Qs + IN * PS, *Ms = Ks + L::KP * PS;
+    bf* Ks = Qs + L::M * PS;
     __shared__ float4 s_gate[C];
     __shared__ float s_theta[C];
     const int slot = blockIdx.x / A.hv, h = blockIdx.x - slot * A.hv, n0 = blockIdx.y * 64;
@@ -409,13 +411,14 @@ __global__ void __launch_bounds__(256, Pl<T>::in == 1 ? 3 : 2) gd_out_fwd_kernel
         if (c0) __syncthreads();
         load_tile<T, 64, 256>(Qs, LP, PS, qp + c0, A.qt, ch.len, A.dk - c0);
         load_tile<T, 64, 256>(Ks, LP, PS, kp + c0, A.kt, ch.len, A.dk - c0);
-        load_own<O, 256>(Ms, A.m_chunk + (tile * A.dkp + c0) * A.dvp + n0, A.dvp);
         __syncthreads();
         if (need) gemm<4, false, false, IN, IN>(att, Qs + 16 * rb * LP, LP, PS, Ks + 32 * hf * LP, LP, PS, 0, 64);
-        gemm<4, false, true, IN, O>(y, Qs + 16 * rb * LP, LP, PS, Ms + 32 * hf, LP, PS, 0, 64);
+        __syncthreads();
+        load_own<O, 256>(Ks, A.m_chunk + (tile * A.dkp + c0) * A.dvp + n0, A.dvp);
+        __syncthreads();
+        gemm<4, false, true, IN, O>(y, Qs + 16 * rb * LP, LP, PS, Ks + 32 * hf, LP, PS, 0, 64);
     }
     __syncthreads();
-    bf *Ps = Ks, *Us = Ms;
 #pragma unroll
     for (int n = 0; n < 4; n++)
 #pragma unroll
@@ -429,27 +432,25 @@ __global__ void __launch_bounds__(256, Pl<T>::in == 1 ? 3 : 2) gd_out_fwd_kernel
                 x[e] = j + e <= i ? decay(make_float2(gi.x, gi.y), make_float2(gj.x, gj.y)) * A.scale * att[n][2 * r + e] : 0.f;
                 y[n][2 * r + e] *= A.scale * gi.z;
             }
-            put2<O>(Ps + i * LP + j, PS, x[0], x[1]);
+            put2<O>(Qs + i * LP + j, PS, x[0], x[1]);
         }
-    load_own<O, 256>(Us, A.e + tile * C * A.dvp + n0, A.dvp, s_theta);
+    load_own<O, 256>(Ks, A.e + tile * C * A.dvp + n0, A.dvp, s_theta);
     __syncthreads();
-    gemm<4, false, true, O, O>(y, Ps + 16 * rb * LP, LP, PS, Us + 32 * hf, LP, PS, 0, 16 * (rb + 1));
+    gemm<4, false, true, O, O>(y, Qs + 16 * rb * LP, LP, PS, Ks + 32 * hf, LP, PS, 0, 16 * (rb + 1));
     T* out = (T*)A.y + (ch.row0(A) * A.hv + h) * A.dv;
     store_rows<T>(out, y, 16 * rb, ch.len, n0 + 32 * hf, A.dv, (long long)A.hv * A.dv);
 }
 
 // ── backward, what needs no state gradient: F = P^T dY, and N = scale (e^G Q)^T dY into the place of D ──
-template <typename T> struct PreBwdSmem {
-    static constexpr int PS = C * LP, IN = Pl<T>::in, BYTES = 2 * PS * (2 * IN + 3 + 3);          // P^T goes where K was
-};
+// Two places in shared memory, Q then P^T, and K, then scale e^G dY, then dY: four CTAs share an SM.
+constexpr int PRE_BWD_BYTES = 2 * 3 * C * LP * 2;
 template <typename T>
-__global__ void __launch_bounds__(256, 2) gd_pre_bwd_kernel(Args A)
+__global__ void __launch_bounds__(256, 4) gd_pre_bwd_kernel(Args A)
 {
-    typedef PreBwdSmem<T> L;
-    constexpr int PS = L::PS, IN = L::IN;
+    constexpr int PS = C * LP, IN = Pl<T>::in;
     extern __shared__ float4 smem4[];
     bf* Qs = reinterpret_cast<bf*>(smem4);
-    bf *Ys = Qs + IN * PS, *Ks = Ys + IN * PS, *Yg = Ks + 3 * PS;
+    bf* Ks = Qs + 3 * PS;
     __shared__ float4 s_gate[C];
     const int slot = blockIdx.x / A.hv, h = blockIdx.x - slot * A.hv, n0 = blockIdx.y * 64;
     const Chunk ch = get_chunk(A, slot);
@@ -459,15 +460,7 @@ __global__ void __launch_bounds__(256, 2) gd_pre_bwd_kernel(Args A)
     if (tid < C) s_gate[tid] = A.gates[tile * C + tid];
     const T* kp = (const T*)A.k + ch.b * A.kb + ch.t0 * A.kt + (h / A.share) * A.kh;
     const T* qp = (const T*)A.q + ch.b * A.qb + ch.t0 * A.qt + (h / A.share) * A.qh;
-    load_tile<T, 64, 256>(Ys, LP, PS, (const T*)A.dy + ch.b * A.yb + ch.t0 * A.yt + h * A.yh + n0, A.yt, ch.len, A.dv - n0);
-    __syncthreads();
-#pragma unroll
-    for (int i = 0; i < C * 32 / 256; i++) {
-        const int at = tid + i * 256, r = at >> 5, c = (at & 31) * 2;
-        const float2 v = get2<IN>(Ys + r * LP + c, PS);
-        const float s = A.scale * s_gate[r].z;
-        put2<3>(Yg + r * LP + c, PS, s * v.x, s * v.y);
-    }
+    const T* yp = (const T*)A.dy + ch.b * A.yb + ch.t0 * A.yt + h * A.yh + n0;
     float att[4][4];                              // rows: j, columns: i >= j
     zero(att);
     const bool need = 32 * hf + 31 >= 16 * rb;
@@ -477,9 +470,12 @@ __global__ void __launch_bounds__(256, 2) gd_pre_bwd_kernel(Args A)
         load_tile<T, 64, 256>(Ks, LP, PS, kp + c0, A.kt, ch.len, A.dk - c0);
         __syncthreads();
         if (need) gemm<4, false, false, IN, IN>(att, Ks + 16 * rb * LP, LP, PS, Qs + 32 * hf * LP, LP, PS, 0, 64);
+        __syncthreads();
+        load_scaled<T, 256>(Ks, yp, A.yt, ch.len, A.dv - n0, A.scale, s_gate);
+        __syncthreads();
         float nn[4][4];                           // rows: dk, columns: dv
         zero(nn);
-        gemm<4, true, true, IN, 3>(nn, Qs + 16 * rb, LP, PS, Yg + 32 * hf, LP, PS, 0, C);
+        gemm<4, true, true, IN, 3>(nn, Qs + 16 * rb, LP, PS, Ks + 32 * hf, LP, PS, 0, C);
         float* np = A.d_chunk + (tile * A.dkp + c0) * A.dvp + n0 + 32 * hf;
 #pragma unroll
         for (int n = 0; n < 4; n++)
@@ -488,7 +484,8 @@ __global__ void __launch_bounds__(256, 2) gd_pre_bwd_kernel(Args A)
                 st2(np + (16 * rb + g + 8 * r) * A.dvp + 8 * n + 2 * t, nn[n][2 * r], nn[n][2 * r + 1]);
     }
     __syncthreads();
-    bf* Pt = Ks;                                  // [j][i]
+    load_tile<T, 64, 256>(Ks, LP, PS, yp, A.yt, ch.len, A.dv - n0);
+    bf* Pt = Qs;                                  // [j][i]
 #pragma unroll
     for (int n = 0; n < 4; n++)
 #pragma unroll
@@ -506,7 +503,7 @@ __global__ void __launch_bounds__(256, 2) gd_pre_bwd_kernel(Args A)
     __syncthreads();
     float f[4][4];
     zero(f);
-    gemm<4, false, true, 3, IN>(f, Pt + 16 * rb * LP, LP, PS, Ys + 32 * hf, LP, PS, 16 * rb, C);
+    gemm<4, false, true, 3, IN>(f, Pt + 16 * rb * LP, LP, PS, Ks + 32 * hf, LP, PS, 16 * rb, C);
     float* fp = A.f + tile * C * A.dvp + n0 + 32 * hf;
 #pragma unroll
     for (int n = 0; n < 4; n++)
@@ -1114,9 +1111,8 @@ template <typename T> static bool run_backward(Args& A, cudaStream_t st, const c
 {
     const unsigned tiles = (unsigned)((long long)A.slots * A.hv);
     if (tiles) {
-        constexpr int bytes = PreBwdSmem<T>::BYTES;
-        if (!allow_smem(gd_pre_bwd_kernel<T>, bytes, where)) return false;
-        gd_pre_bwd_kernel<T><<<dim3(tiles, A.dvp / 64), 256, bytes, st>>>(A);
+        if (!allow_smem(gd_pre_bwd_kernel<T>, PRE_BWD_BYTES, where)) return false;
+        gd_pre_bwd_kernel<T><<<dim3(tiles, A.dvp / 64), 256, PRE_BWD_BYTES, st>>>(A);
         if (!check_launch(where)) return false;
     }
     if (!(A.dkp == 64 ? launch_states<T, 64>(A, true, st, where) : launch_states<T, 128>(A, true, st, where))) return false;

@@ -184,6 +184,27 @@ __device__ __forceinline__ void load_tile(bf* dst, int ld, int ps, const T* base
         }
     }
 }
+// 64 x 64 of an input, each row times factor scale[row].z, in three planes.
+template <typename T, int THREADS>
+__device__ __forceinline__ void load_scaled(bf* dst, const T* base, long long stride, int rows, int cols, float factor, const float4* scale)
+{
+    if (vec_ok(base, stride, cols)) {
+#pragma unroll
+        for (int i = 0; i < C * 16 / THREADS; i++) {
+            const int at = threadIdx.x + i * THREADS, r = at >> 4, c = (at & 15) * 4;
+            float4 v = make_float4(0.f, 0.f, 0.f, 0.f);
+            if (r < rows && c < cols) v = ld4(base + r * stride + c);
+            const float s = factor * scale[r].z;
+            put4<3>(dst + r * LP + c, C * LP, make_float4(s * v.x, s * v.y, s * v.z, s * v.w));
+        }
+    } else {
+#pragma unroll 4
+        for (int i = 0; i < C * 64 / THREADS; i++) {
+            const int at = threadIdx.x + i * THREADS, r = at >> 6, c = at & 63;
+            put_one(dst + r * LP + c, C * LP, r < rows && c < cols ? factor * scale[r].z * to_f(base[r * stride + c]) : 0.f);
+        }
+    }
+}
 // 64 x 64 of a private, padded buffer, each row times scale[row] where a scale is given.
 template <int P, int THREADS>
 __device__ __forceinline__ void load_own(bf* dst, const float* base, int stride, const float* scale = nullptr)
