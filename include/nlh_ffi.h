@@ -518,7 +518,7 @@ int32_t nlh_transpose(const float* src, float* dst, int32_t rows, int32_t cols);
 /* ── Embedding lookup with scaling, gradient by sorted tokens (additive, no counterpart in the reference) ──
  * Beside embedding_gather_cuda / embedding_scatter_add_cuda above. out[t] = scale * w[ids[t]], w [vocab, d] and out [n, d] both
  * fp32 or both bf16; an id outside [0, vocab) gives a row of zeros and takes no part in the gradient. Backward: d_w [vocab, d] fp32,
- * accumulate != 0: d_w[r] += scale * sum of the rows of d_out [n, d] (fp32 or bf16) with id r; 0: d_w is overwritten, zeros in
+ * n up to 2^30, accumulate != 0: d_w[r] += scale * sum of the rows of d_out [n, d] (fp32 or bf16) with id r; 0: d_w is overwritten, zeros in
  * rows without a token. Sums are in fp32 and in one order that n, ids and d fix: the same call gives the same bits. workspace
  * (nlh_embedding_backward_bytes, 16-byte aligned) is the caller's. */
 int32_t nlh_embedding_forward(const void* w, int32_t w_is_bf16, const int32_t* ids, void* out, int32_t n, int32_t vocab,
@@ -555,8 +555,7 @@ int32_t nlh_distill_backward(const void* logits, int32_t logits_is_bf16, int64_t
  * y, d_k, d_v, d_q (in the inputs' type) and d_log_retain, d_theta (fp32) are contiguous in the inputs' shapes.
  * Packed batches: batch = 1, n_seqs > 0, seq_starts [n_seqs + 1] on the device, sequence i = tokens
  * seq_starts[i] .. seq_starts[i + 1] - 1. Starts are clamped to [0, seq] and to their running maximum; a sequence may be
- * empty (m_final = m_initial); tokens outside the sequences are not read, and their rows of y and of the gradients of v, log_retain
- * and theta are not written (those of k and q neither, unless heads are shared).
+ * empty (m_final = m_initial); tokens outside the sequences are not read, and their rows of y and of the gradients are not written.
  * A log_retain below -200 counts as -200 (e^-200 is 0 in fp32), a theta below 2^-60 in magnitude as 2^-60. A value that is not
  * finite, or above 4e34, may make any output of its sequence from the start of its chunk of 64 tokens a NaN (backward: of its whole sequence). */
 typedef struct nlh_gated_delta_desc {

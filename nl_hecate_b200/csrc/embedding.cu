@@ -608,7 +608,7 @@ int32_t nlh_embedding_forward(const void* w, int32_t w_is_bf16, const int32_t* i
 
 int64_t nlh_embedding_backward_bytes(int32_t n, int32_t vocab, int32_t d)
 {
-    if (n < 0 || vocab <= 0 || d <= 0) return -1;
+    if (n < 0 || n > (1 << 30) || vocab <= 0 || d <= 0) return -1;
     emb::Plan P;
     return emb::place(P, nullptr, n, vocab, d);
 }

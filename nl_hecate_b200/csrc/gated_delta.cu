@@ -838,11 +838,14 @@ __global__ void __launch_bounds__(128) gd_gate_bwd_kernel(Args A)
     if (2 * lane + 1 < ch.len) out[A.hv] = (float)(s - a);
 }
 
-// Gradients of shared keys and queries: the value heads of a group, added in their order.
+// Gradients of shared keys and queries: the value heads of a group, added in their order. Rows outside the sequences of a packed
+// batch have no sums and are left as they are.
 template <typename T>
 __global__ void __launch_bounds__(256) gd_group_kernel(Args A, long long n)
 {
-    for (long long i = (long long)blockIdx.x * 256 + threadIdx.x; i < n; i += (long long)gridDim.x * 256) {
+    const long long per_row = (long long)A.hk * A.dk;
+    const long long i0 = A.starts ? A.start[0] * per_row : 0, i1 = A.starts ? A.start[A.n_seqs] * per_row : n;
+    for (long long i = i0 + (long long)blockIdx.x * 256 + threadIdx.x; i < i1; i += (long long)gridDim.x * 256) {
         const long long rh = i / A.dk;                    // row * hk + key head
         const int c = (int)(i - rh * A.dk);
         const long long at = rh * A.share * A.dk + c;
@@ -1124,7 +1127,6 @@ template <typename T> static bool run_backward(Args& A, cudaStream_t st, const c
     gd_gate_bwd_kernel<<<(tiles + 3) / 4, 128, 0, st>>>(A);
     if (!check_launch(where)) return false;
     if (A.share > 1) {
-        // rows outside the sequences of a packed batch have no partial sums: their gradients are the caller's zeros
         const long long n = (long long)A.batch * A.seq * A.hk * A.dk;
         const long long need = (n + 255) / 256;
         gd_group_kernel<T><<<(unsigned)(need < 148 * 16 ? need : 148 * 16), 256, 0, st>>>(A, n);

@@ -13,6 +13,7 @@ from __future__ import annotations
 
 import ctypes as C
 import struct
+import threading
 
 import numpy as np
 import torch
@@ -20,6 +21,7 @@ import torch
 from . import ffi
 
 RULE_DELTA, RULE_TITANS, RULE_HEBBIAN = 0, 1, 2
+_LAUNCH = threading.Lock()   # the library has one launch stream: binding it and launching are one step for Python's threads
 _PLANS = {}      # entry name -> (function, ((argument, is pointer), ...), return type)
 
 
@@ -63,24 +65,25 @@ def call(name: str, **kw):
                 if not v.is_cuda or not v.is_contiguous():
                     raise ValueError(f"{name}.{an}: need a contiguous CUDA tensor")
                 args[i] = v.data_ptr()
-    bind_stream()
-    if ret is None:
-        ffi.lib().nlh_clear_status()   # void entries report through the recorded status
-    try:
-        rc = fn(*args)
-    except C.ArgumentError:
-        for at, v in zip(fn.argtypes, args):
-            if at is not C.c_void_p:
-                at(v)                      # a number of the wrong kind is a TypeError
-        raise
-    if ret is C.c_int32:
-        if rc:
-            ffi.check(rc, name)
-    elif ret is C.c_uint32:
-        if rc != 0:
-            raise RuntimeError(f"{name}: cudaError {rc}")
-    elif ret is None:
-        ffi.check_void(name)
+    with _LAUNCH:
+        bind_stream()
+        if ret is None:
+            ffi.lib().nlh_clear_status()   # void entries report through the recorded status
+        try:
+            rc = fn(*args)
+        except C.ArgumentError:
+            for at, v in zip(fn.argtypes, args):
+                if at is not C.c_void_p:
+                    at(v)                      # a number of the wrong kind is a TypeError
+            raise
+        if ret is C.c_int32:
+            if rc:
+                ffi.check(rc, name)
+        elif ret is C.c_uint32:
+            if rc != 0:
+                raise RuntimeError(f"{name}: cudaError {rc}")
+        elif ret is None:
+            ffi.check_void(name)
     return rc
 
 
@@ -364,16 +367,17 @@ _DESC = struct.Struct("8i15qf")          # nlh_gated_delta_desc (ffi.GatedDeltaD
 def _entry(name):
     """The C function of a status-returning entry, for calls with positional arguments as in the header: these
     operators run in microseconds, and call()'s keyword arguments would cost as much again."""
-    fn = getattr(ffi.lib(), name)
+    fn, set_stream = getattr(ffi.lib(), name), ffi.lib().nlh_set_stream
 
     def run(device, *args):
         if device != _CURRENT_DEVICE():                 # tensors of another device: its stream, under a guard
             with torch.cuda.device(device):
                 return run(device, *args)
-        ffi.lib().nlh_set_stream(_CURRENT_STREAM(device))
-        rc = fn(*args)
-        if rc:
-            ffi.check(rc, name)
+        with _LAUNCH:
+            set_stream(_CURRENT_STREAM(device))
+            rc = fn(*args)
+            if rc:
+                ffi.check(rc, name)
 
     _ENTRIES[name] = run
     return run
@@ -450,6 +454,16 @@ def _bytes(where, fn, *args):
     return n
 
 
+def _what(desc):
+    """The part of a packed descriptor that sizes the saved buffer: dimensions and type."""
+    return desc[:32]
+
+
+class GatedDeltaSaved:
+    """What gated_delta_backward needs of its forward, and the descriptor that it belongs to."""
+    __slots__ = ("buffer", "desc")
+
+
 def gated_delta_forward(k, v, q, log_retain, theta, m0=None, seq_starts=None, scale=1.0, want_saved=True):
     """Gated delta rule over whole sequences (nlh_gated_delta_forward): returns (y like v, m_final
     [sequences, Hv, dv, dk], saved). ``saved`` is what gated_delta_backward needs, None with want_saved=False.
@@ -463,12 +477,16 @@ def gated_delta_forward(k, v, q, log_retain, theta, m0=None, seq_starts=None, sc
     if m0 is not None:
         _need(where, "m0", m0, torch.float32, state)
     nbytes = _bytes(where, ffi.lib().nlh_gated_delta_saved_bytes, desc)
-    saved = torch.empty(max(nbytes, 1), dtype=torch.uint8, device=k.device)
+    buffer = torch.empty(max(nbytes, 1), dtype=torch.uint8, device=k.device)
     y = (torch.zeros if n_seqs else torch.empty)(v.shape, dtype=v.dtype, device=k.device)
     m = torch.empty(state, dtype=torch.float32, device=k.device)
     _run("nlh_gated_delta_forward", device, desc, k.data_ptr(), v.data_ptr(), q.data_ptr(), log_retain.data_ptr(),
-         theta.data_ptr(), _ptr(m0), _ptr(seq_starts), y.data_ptr(), m.data_ptr(), saved.data_ptr(), nbytes)
-    return y, m, (saved if want_saved else None)
+         theta.data_ptr(), _ptr(m0), _ptr(seq_starts), y.data_ptr(), m.data_ptr(), buffer.data_ptr(), nbytes)
+    if not want_saved:
+        return y, m, None
+    saved = GatedDeltaSaved()
+    saved.buffer, saved.desc = buffer, _what(desc)
+    return y, m, saved
 
 
 def gated_delta_backward(k, v, q, log_retain, theta, saved, d_y, d_m_final=None, seq_starts=None, scale=1.0,
@@ -477,7 +495,7 @@ def gated_delta_backward(k, v, q, log_retain, theta, saved, d_y, d_m_final=None,
     dict(d_k, d_v, d_q, d_log_retain, d_theta, d_m_initial). d_y like v in type, any strides; d_m_final (gradient
     of m_final) may be None. Keys shared by several value heads get the sum of their gradients."""
     where = "gated_delta_backward"
-    device = _device_of(where, k, v, q, log_retain, theta, saved, d_y, d_m_final, seq_starts)
+    device = _device_of(where, k, v, q, log_retain, theta, saved.buffer, d_y, d_m_final, seq_starts)
     log_retain, theta = _same_strides(log_retain, theta)
     if d_y.shape != v.shape or d_y.dtype != v.dtype:
         raise ValueError(f"{where}.d_y: need {v.dtype} {tuple(v.shape)}, got {d_y.dtype} {tuple(d_y.shape)}")
@@ -486,15 +504,16 @@ def gated_delta_backward(k, v, q, log_retain, theta, saved, d_y, d_m_final=None,
     state = (n_seqs or k.shape[0], v.shape[2], v.shape[3], k.shape[3])
     if d_m_final is not None:
         _need(where, "d_m_final", d_m_final, torch.float32, state)
-    _need(where, "saved", saved, torch.uint8, saved.shape)
+    if saved.desc != _what(desc):
+        raise ValueError(f"{where}.saved: from a forward of other shapes or another type")
     nbytes = _bytes(where, ffi.lib().nlh_gated_delta_backward_bytes, desc)
     make = torch.zeros if n_seqs else torch.empty      # rows outside the sequences are not written
     new = lambda t: make(t.shape, dtype=t.dtype, device=k.device)
-    work = make(max(nbytes, 1), dtype=torch.uint8, device=k.device)
+    work = torch.empty(max(nbytes, 1), dtype=torch.uint8, device=k.device)
     g = dict(d_k=new(k), d_v=new(v), d_q=new(q), d_log_retain=new(theta), d_theta=new(theta))
     g["d_m_initial"] = torch.empty(state, dtype=torch.float32, device=k.device) if want_initial else None
     _run("nlh_gated_delta_backward", device, desc, k.data_ptr(), v.data_ptr(), q.data_ptr(), log_retain.data_ptr(),
-         theta.data_ptr(), _ptr(seq_starts), saved.data_ptr(), saved.numel(), d_y.data_ptr(), _ptr(d_m_final),
+         theta.data_ptr(), _ptr(seq_starts), saved.buffer.data_ptr(), saved.buffer.numel(), d_y.data_ptr(), _ptr(d_m_final),
          *[_ptr(t) for t in g.values()], work.data_ptr(), nbytes)
     return g
 
@@ -599,6 +618,14 @@ def distill_forward(logits, teacher_ids, teacher_logits, targets=None, temperatu
     return loss, s
 
 
+def _overlap(a, b):
+    """Whether the memory of two [n, vocab] tensors meets, unless they are the same elements in the same places."""
+    if a.data_ptr() == b.data_ptr() and (a.stride(0) == b.stride(0) or a.shape[0] <= 1):
+        return False
+    end = lambda t: t.data_ptr() + ((t.shape[0] - 1) * t.stride(0) + t.shape[1]) * t.element_size()
+    return min(a.numel(), b.numel()) > 0 and a.data_ptr() < end(b) and b.data_ptr() < end(a)
+
+
 def distill_backward(logits, saved, grad=None, out=None):
     """Gradient of distill_forward with respect to logits, times the fp32 scalar tensor ``grad``. out (default: a new
     tensor) may be logits itself. The tensors given to the forward must not have changed."""
@@ -612,6 +639,8 @@ def distill_backward(logits, saved, grad=None, out=None):
         out = torch.empty(n, vocab, dtype=logits.dtype, device=logits.device)
     elif out.shape != logits.shape or out.dtype != logits.dtype or (vocab > 1 and out.stride(1) != 1):
         raise ValueError(f"{where}.out: need {logits.dtype} {tuple(logits.shape)} with contiguous rows")
+    elif out is not logits and _overlap(out, logits):
+        raise ValueError(f"{where}.out: overlaps logits without being logits")
     if grad is not None and (grad.dtype != torch.float32 or grad.numel() != 1):
         raise ValueError(f"{where}.grad: need one fp32 value")
     _run("nlh_distill_backward", device, logits.data_ptr(), logits.dtype == torch.bfloat16, _row_stride(logits), _ptr(s.targets),

@@ -181,16 +181,16 @@ class _GatedDeltaMemory(torch.autograd.Function):
         heads = lambda t: t.unsqueeze(2)                 # one head per row of the batch
         keep = 1.0 - alpha
         args = (heads(k), heads(v), heads(q), heads(torch.log(keep)), heads(theta))
-        y, m, saved = D.gated_delta_forward(*args, m0=m0.view(n, 1, d, d))
-        ctx.save_for_backward(*args, saved, keep)
+        y, m, ctx.chunks = D.gated_delta_forward(*args, m0=m0.view(n, 1, d, d))
+        ctx.save_for_backward(*args, keep)
         m = m.view(n, d * d)
         ctx.mark_non_differentiable(m)
         return y.view(n, s, d), m
 
     @staticmethod
     def backward(ctx, dy, _dm):
-        *args, saved, keep = ctx.saved_tensors
-        g = D.gated_delta_backward(*args, saved, dy.unsqueeze(2), want_initial=False)
+        *args, keep = ctx.saved_tensors
+        g = D.gated_delta_backward(*args, ctx.chunks, dy.contiguous().unsqueeze(2), want_initial=False)
         # log(1 - alpha): the gradient of log_retain carries the factor 1 - alpha
         d_alpha = -g["d_log_retain"].squeeze(2) / keep.clamp_min(1e-30)
         sq = lambda x: g[x].squeeze(2)

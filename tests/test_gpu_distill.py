@@ -143,6 +143,27 @@ def test_in_place_strided_and_scaled(n, vocab, dtype):
     assert torch.equal(wide[:, :vocab], d2) and bool((wide[:, vocab:] == 7).all())
 
 
+def test_refusals():
+    from nl_hecate_b200 import dispatch as D
+    z, ids, t, y = make(6, 50, 4, torch.float32)
+    for bad in ((z.half(), ids, t), (z[0], ids, t), (z, ids.long(), t), (z, ids[:5], t[:5]), (z, ids, t[:, :3]), (z, ids, t.half()),
+                (z.t().contiguous().t(), ids, t), (z, ids.cpu(), t)):
+        with pytest.raises(ValueError):
+            D.distill_forward(*bad)
+    with pytest.raises(ValueError):
+        D.distill_forward(z, ids, t, targets=y[:5])
+    with pytest.raises(RuntimeError, match="temperature"):
+        D.distill_forward(z, ids, t, temperature=0.0)
+    wide = torch.randn(6, 100, device="cuda")
+    loss, saved = D.distill_forward(wide[:, :50], ids, t)
+    with pytest.raises(ValueError, match="overlaps"):
+        D.distill_backward(wide[:, :50], saved, out=wide[:, 8:58])
+    with pytest.raises(ValueError):
+        D.distill_backward(z[:, :49], saved)
+    with pytest.raises(ValueError):
+        D.distill_backward(z, saved, grad=torch.ones(2, device="cuda"))
+
+
 def test_no_rows_and_repeatable_bits():
     from nl_hecate_b200 import dispatch as D
     z, ids, t, y = make(0, 100, 4, torch.float32)

@@ -203,6 +203,34 @@ def test_starts_that_are_out_of_order_or_range_stay_inside(bad):
     assert not out["y"][:, :at[0]].any() and not out["y"][:, at[-1]:].any()
 
 
+def test_rows_outside_the_sequences_are_left_as_they_were():
+    """The C entries themselves, which the wrapper hands zeroed buffers: shared heads, so that the sums over them are reached too."""
+    import ctypes as C
+    from nl_hecate_b200 import dispatch as D
+    from nl_hecate_b200 import ffi
+    p, starts, at = packed((70, 0, 5), 2, 4, 64, 48, torch.float32, before=3, behind=9)
+    total = p["k"].shape[1]
+    names = ("k", "v", "q", "log_retain", "theta")
+    want = run(p, starts=starts)
+    out = {x: torch.full_like(p[x], 7.0) for x in names} | {"y": torch.full_like(p["v"], 7.0)}
+    st = lambda t: t.stride()[:3]
+    d = ffi.GatedDeltaDesc(1, total, 2, 4, 64, 48, 3, 0, *st(p["k"]), *st(p["v"]), *st(p["q"]), *st(p["theta"]), *st(p["d_y"]), 1.0)
+    ref = C.byref(d)
+    saved = torch.empty(ffi.lib().nlh_gated_delta_saved_bytes(ref), dtype=torch.uint8, device="cuda")
+    work = torch.full((ffi.lib().nlh_gated_delta_backward_bytes(ref),), 255, dtype=torch.uint8, device="cuda")
+    m, dm = torch.empty_like(p["m0"]), torch.empty_like(p["m0"])
+    ins = {x: p[x] for x in names}
+    D.call("nlh_gated_delta_forward", desc=ref, **ins, m_initial=p["m0"], seq_starts=starts, y=out["y"], m_final=m, saved=saved,
+           saved_bytes=saved.numel())
+    D.call("nlh_gated_delta_backward", desc=ref, **ins, seq_starts=starts, saved=saved, saved_bytes=saved.numel(), d_y=p["d_y"],
+           d_m_final=p["d_m"], **{"d_" + x: out[x] for x in names}, d_m_initial=dm, workspace=work, workspace_bytes=work.numel())
+    assert torch.equal(m, want["m_final"]) and torch.equal(dm, want["d_m_initial"])
+    for x in out:
+        w = want["y" if x == "y" else "d_" + x]
+        assert torch.equal(out[x][:, at[0]:at[-1]], w[:, at[0]:at[-1]]), x
+        assert bool((out[x][:, :at[0]] == 7).all()) and bool((out[x][:, at[-1]:] == 7).all()), x
+
+
 def test_many_sequences():
     """More sequences than the threads that number them."""
     lengths = [(i * 7) % 5 for i in range(2500)]
@@ -370,8 +398,12 @@ def test_refusals():
     with pytest.raises(ValueError):
         D.gated_delta_forward(*a, seq_starts=torch.zeros(3, dtype=torch.int32, device="cuda"))     # batch 2
     y, m, saved = D.gated_delta_forward(*a)
+    with pytest.raises(ValueError, match="other shapes"):
+        D.gated_delta_backward(*[t[:1] for t in a], saved, p["d_y"][:1])
+    cut = D.GatedDeltaSaved()
+    cut.buffer, cut.desc = saved.buffer[:-256], saved.desc
     with pytest.raises(RuntimeError, match="too small"):
-        D.gated_delta_backward(*a, saved[:-256], p["d_y"])
+        D.gated_delta_backward(*a, cut, p["d_y"])
     with pytest.raises(ValueError):
         D.gated_delta_backward(*a, saved, p["d_y"].bfloat16())
     with pytest.raises(ValueError):
