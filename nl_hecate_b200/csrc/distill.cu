@@ -535,7 +535,8 @@ __device__ __forceinline__ void write_entries(const Entries& E, int k, T* d, con
     }
 }
 
-// Barrier that the two kinds of warps reach at different places: the entries' elements have been read.
+// Barrier that the two kinds of warps reach at different places, where the gradient goes over the logits: the entries' elements
+// have been read.
 template <int TH> __device__ __forceinline__ void entries_read() { asm volatile("bar.sync 1, %0;\n" ::"n"(TH + 32) : "memory"); }
 
 // TH threads write the row; one more warp has the entries. d_logits may be logits: a thread reads its elements before it writes
@@ -557,12 +558,14 @@ __global__ void __launch_bounds__(TH + 32, TH == 128 ? 12 : 5) bwd_kernel(Args A
     const RowGrad r = row_grad<MODE>(A, row);
     if (!r.hard && !r.soft) { zero_row<T, TH + 32>(d, s, threadIdx.x); return; }
     const int k = r.soft ? A.k : 0;
+    const bool in_place = A.d == A.z;             // else nothing that is written is still to be read
     if (threadIdx.x < TH) {
-        entries_read<TH>();
+        if (in_place) entries_read<TH>();
         write_row<T, MODE, TH>(z, d, s, u, r, cs, ch, threadIdx.x);
     } else {
         const float top = read_entries<T>(A, E, row, z, j0, j1, k, r);
-        entries_read<TH>();
+        if (in_place) entries_read<TH>();
+        else __syncwarp();
         weigh(E, k, top, r.ws);
     }
     __syncthreads();
