@@ -4,6 +4,8 @@
 // So a pass has three parts: what needs no state, for all chunks at once (prep); the states, one after the
 // other, divided over the columns of V, which never meet (state); what needs them, for all chunks at once
 // (out). The backward has the same three parts. Every sum has one order: no atomics.
+#include <atomic>
+
 #include "gated_delta.cuh"
 #include "nlh_common.cuh"
 #include "../../include/nlh_ffi.h"
@@ -1053,12 +1055,17 @@ static int64_t place_bwd(Args& A, char* base)
     return at;
 }
 
-template <typename K> static bool allow_smem(K kernel, int bytes, const char* where)
+// Opts a kernel in to its dynamic shared memory, once per device (the attribute belongs to the device that is current).
+template <auto KERNEL, int BYTES> static bool allow_smem(const char* where)
 {
-    const cudaError_t e = cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, bytes);
-    if (e == cudaSuccess) return true;
-    record_status(NLH_ERR_CUDA, where, cudaGetErrorString(e));
-    return false;
+    static std::atomic<uint64_t> done[2];        // devices 0 .. 127
+    int dev = 0;
+    if (cudaGetDevice(&dev) != cudaSuccess || dev < 0 || dev > 127) dev = -1;
+    if (dev >= 0 && (done[dev >> 6].load(std::memory_order_relaxed) >> (dev & 63) & 1)) return true;
+    const cudaError_t e = cudaFuncSetAttribute(KERNEL, cudaFuncAttributeMaxDynamicSharedMemorySize, BYTES);
+    if (e != cudaSuccess) { record_status(NLH_ERR_CUDA, where, cudaGetErrorString(e)); return false; }
+    if (dev >= 0) done[dev >> 6].fetch_or(1ull << (dev & 63), std::memory_order_relaxed);
+    return true;
 }
 
 template <typename T, int DKP, int NS>
@@ -1068,10 +1075,10 @@ static bool launch_states_ns(const Args& A, long long heads, bool backward, cuda
     if (grid >= (1LL << 31)) { record_status(NLH_ERR_INVALID_ARG, where, "too many sequences"); return false; }
     constexpr int bytes = StateSmem<T, DKP, NS>::BYTES;
     if (backward) {
-        if (!allow_smem(gd_state_bwd_kernel<T, DKP, NS>, bytes, where)) return false;
+        if (!allow_smem<gd_state_bwd_kernel<T, DKP, NS>, bytes>(where)) return false;
         gd_state_bwd_kernel<T, DKP, NS><<<(unsigned)grid, 256, bytes, st>>>(A);
     } else {
-        if (!allow_smem(gd_state_fwd_kernel<T, DKP, NS>, bytes, where)) return false;
+        if (!allow_smem<gd_state_fwd_kernel<T, DKP, NS>, bytes>(where)) return false;
         gd_state_fwd_kernel<T, DKP, NS><<<(unsigned)grid, 256, bytes, st>>>(A);
     }
     return check_launch(where);
@@ -1096,14 +1103,14 @@ template <typename T> static bool run_forward(Args& A, cudaStream_t st, const ch
     const unsigned tiles = (unsigned)((long long)A.slots * A.hv);
     if (tiles) {
         constexpr int bytes = T_BYTES + 2 * C * LD * 4;
-        if (!allow_smem(gd_prep_kernel<T>, bytes, where)) return false;
+        if (!allow_smem<gd_prep_kernel<T>, bytes>(where)) return false;
         gd_prep_kernel<T><<<tiles, 256, bytes, st>>>(A);
         if (!check_launch(where)) return false;
     }
     if (!(A.dkp == 64 ? launch_states<T, 64>(A, false, st, where) : launch_states<T, 128>(A, false, st, where))) return false;
     if (tiles) {
         constexpr int bytes = OutFwdSmem<T>::BYTES;
-        if (!allow_smem(gd_out_fwd_kernel<T>, bytes, where)) return false;
+        if (!allow_smem<gd_out_fwd_kernel<T>, bytes>(where)) return false;
         gd_out_fwd_kernel<T><<<dim3(tiles, A.dvp / 64), 256, bytes, st>>>(A);
         if (!check_launch(where)) return false;
     }
@@ -1114,14 +1121,14 @@ template <typename T> static bool run_backward(Args& A, cudaStream_t st, const c
 {
     const unsigned tiles = (unsigned)((long long)A.slots * A.hv);
     if (tiles) {
-        if (!allow_smem(gd_pre_bwd_kernel<T>, PRE_BWD_BYTES, where)) return false;
+        if (!allow_smem<gd_pre_bwd_kernel<T>, PRE_BWD_BYTES>(where)) return false;
         gd_pre_bwd_kernel<T><<<dim3(tiles, A.dvp / 64), 256, PRE_BWD_BYTES, st>>>(A);
         if (!check_launch(where)) return false;
     }
     if (!(A.dkp == 64 ? launch_states<T, 64>(A, true, st, where) : launch_states<T, 128>(A, true, st, where))) return false;
     if (!tiles) return true;
     constexpr int bytes = OutBwdSmem<T>::BYTES;
-    if (!allow_smem(gd_out_bwd_kernel<T>, bytes, where)) return false;
+    if (!allow_smem<gd_out_bwd_kernel<T>, bytes>(where)) return false;
     gd_out_bwd_kernel<T><<<dim3(tiles, A.dkp / 64), 256, bytes, st>>>(A);
     if (!check_launch(where)) return false;
     gd_gate_bwd_kernel<<<(tiles + 3) / 4, 128, 0, st>>>(A);

@@ -12,8 +12,8 @@
 // (24 significand bits) when it is written to shared memory, and a product of two such takes six passes, smallest terms
 // first; an operand that came in as bf16 is one plane, exact. A result that is rounded to bf16 is computed from two planes
 // (16 bits against the result's 8). Two tf32 numbers for a fp32 one take the same time on the tensor cores, but their splitting,
-// redone by every warp that reads them, and twice the instructions around each pass held the kernels at 40 % of it:
-// 64 sequences x 8 heads x 512 tokens fp32, forward and backward, TF32_TIME us against PLANE_TIME.
+// redone by every warp that reads them, and twice the instructions around each pass cost more: a training step of 64 sequences
+// x 8 heads x 512 tokens took 1435 us that way against 1308 (4 x 16 x 4096 in bf16: 1336 against 1122).
 // Why not tcgen05: the matrices are 64 x 64 x 64 and each depends on the one before it. One M64 N64 K16 tcgen05.mma takes 55
 // cycles (1190 multiply-adds a cycle), mma.sync does 983, and its results are in registers where the next product needs
 // them; tcgen05 needs a commit, a wait and a trip through TMEM and shared memory for each.
@@ -38,7 +38,7 @@ struct Args {
     const float *g, *theta, *m0;
     const int* starts;                 // [n_seqs + 1], NULL = dense batch
     long long kb, kt, kh, vb, vt, vh, qb, qt, qh, gb, gt, gh, yb, yt, yh;   // strides in elements: batch, token, head (y: d_y)
-    int batch, seq, hk, hv, share, dk, dv, n_seqs, dkp, dvp;   // dkp, dvp: padded to 64 and 32
+    int batch, seq, hk, hv, share, dk, dv, n_seqs, dkp, dvp;   // dkp, dvp: dk, dv padded to 64
     float scale;
     int slots, nc;                     // chunk slots; chunks per sequence of a dense batch
     // private buffers, one tile per slot and value head
