@@ -102,10 +102,12 @@ __global__ void __launch_bounds__(256, 3) gd_prep_kernel(Args A)
         double s = x[0] + x[1];
         for (int o = 1; o < 32; o <<= 1) { const double y = __shfl_up_sync(0xffffffffu, s, o); if (lane >= o) s += y; }
         const double last = __shfl_sync(0xffffffffu, s, 31);
+        double before = __shfl_up_sync(0xffffffffu, s, 1);       // not s - x[1]: a NaN there would reach the token before it
+        if (lane == 0) before = 0.;
 #pragma unroll
         for (int j = 0; j < 2; j++) {
             const int i = 2 * lane + j;
-            const double G = j == 1 ? s : s - x[1];
+            const double G = j == 1 ? s : before + x[0];
             const float hi = (float)G;
             const float4 o = make_float4(hi, (float)(G - hi), expf(hi), expf((float)(last - G)));
             A.gates[tile * C + i] = o;
@@ -124,6 +126,7 @@ __global__ void __launch_bounds__(256, 3) gd_prep_kernel(Args A)
         __syncthreads();
         if (need) gemm<4, false, false, IN, IN>(kk, Tp + 16 * rb * LP, LP, PS, Tp + 32 * hf * LP, LP, PS, 0, 64);
     }
+    bool any = false;
     if (need) {
 #pragma unroll
         for (int n = 0; n < 4; n++) {
@@ -135,11 +138,26 @@ __global__ void __launch_bounds__(256, 3) gd_prep_kernel(Args A)
                 float a[2];
 #pragma unroll
                 for (int e = 0; e < 2; e++) a[e] = j + e < i ? decay(gi, s_g[j + e]) * kk[n][2 * r + e] * s_theta[j + e] : 0.f;
+                any |= odd(a[0]) | odd(a[1]);
                 st2(Am + i * LD + j, a[0], a[1]);
             }
         }
     }
-    __syncthreads();
+    uint4* out = reinterpret_cast<uint4*>(A.tmat + tile * T_BYTES);
+    if (__syncthreads_or(any)) {                  // a value that is not finite: rows from the ones before them alone, see triangle_by_token
+        if (tid < 64)
+            for (int i = 0; i < C; i++) {
+                float s = i == tid ? 1.f : 0.f;
+                for (int l = tid; l < i; l++) s = fmaf(-Am[i * LD + l], Tm[l * LD + tid], s);
+                Tm[i * LD + tid] = s;
+            }
+        __syncthreads();
+        for (int i = tid; i < C * 16; i += 256)
+            put4<3>(Tp + (i >> 4) * LP + (i & 15) * 4, PS, *reinterpret_cast<const float4*>(Tm + (i >> 4) * LD + (i & 15) * 4));
+        __syncthreads();
+        for (int i = tid; i < T_BYTES / 16; i += 256) out[i] = reinterpret_cast<const uint4*>(Tp)[i];
+        return;
+    }
     if (tid < 64) {
         const int b = tid & ~15, j = tid & 15;
         float col[16];
@@ -208,7 +226,6 @@ __global__ void __launch_bounds__(256, 3) gd_prep_kernel(Args A)
         put2<3>(Tp + (r0 + g + 8) * LP + c0 + 2 * t, PS, -z[0][2], -z[0][3]);
     }
     __syncthreads();
-    uint4* out = reinterpret_cast<uint4*>(A.tmat + tile * T_BYTES);
     for (int i = tid; i < T_BYTES / 16; i += 256) out[i] = reinterpret_cast<const uint4*>(Tp)[i];
 }
 
@@ -307,19 +324,23 @@ __global__ void __launch_bounds__(256, DKP == 64 ? 2 : 1) gd_state_fwd_kernel(Ar
         float acc[NT][4];
         zero(acc);
         gemm<NT, false, true, IN, 3>(acc, Ks + 16 * rb * LK, LK, L::PK, Ms + H * hf, LS, L::PM, 0, DKP);
+        bool any = false;
 #pragma unroll
         for (int n = 0; n < NT; n++)
 #pragma unroll
             for (int r = 0; r < 2; r++) {
                 const int row = 16 * rb + g + 8 * r;
-                const float2 x = v[n][r].get();
-                put2<3>(Rs + row * LS + H * hf + 8 * n + 2 * t, L::PR, x.x - s_gate[buf][row].z * acc[n][2 * r],
-                        x.y - s_gate[buf][row].z * acc[n][2 * r + 1]);
+                float2 x = v[n][r].get();
+                x.x -= s_gate[buf][row].z * acc[n][2 * r];
+                x.y -= s_gate[buf][row].z * acc[n][2 * r + 1];
+                any |= odd(x.x) | odd(x.y);
+                put2<3>(Rs + row * LS + H * hf + 8 * n + 2 * t, L::PR, x.x, x.y);
             }
         wait_t();
-        __syncthreads();
+        any = __syncthreads_or(any);
         zero(acc);
-        gemm<NT, false, true, 3, 3>(acc, Ts + 16 * rb * LP, LP, C * LP, Rs + H * hf, LS, L::PR, 0, 16 * (rb + 1));
+        if (any) triangle_by_token<3, NT>(acc, Ts, C * LP, Rs, LS, L::PR, 16 * rb, H * hf);
+        else gemm<NT, false, true, 3, 3>(acc, Ts + 16 * rb * LP, LP, C * LP, Rs + H * hf, LS, L::PR, 0, 16 * (rb + 1));
         float* ep = A.e + tile * C * A.dvp + n0;
 #pragma unroll
         for (int n = 0; n < NT; n++)
@@ -436,9 +457,9 @@ __global__ void __launch_bounds__(256, 4) gd_out_fwd_kernel(Args A)
             }
             put2<O>(Qs + i * LP + j, PS, x[0], x[1]);
         }
-    load_own<O, 256>(Ks, A.e + tile * C * A.dvp + n0, A.dvp, s_theta);
-    __syncthreads();
-    gemm<4, false, true, O, O>(y, Qs + 16 * rb * LP, LP, PS, Ks + 32 * hf, LP, PS, 0, 16 * (rb + 1));
+    const bool any = load_own<O, 256>(Ks, A.e + tile * C * A.dvp + n0, A.dvp, s_theta);
+    if (__syncthreads_or(any)) triangle_by_token<O, 4>(y, Qs, PS, Ks, LP, PS, 16 * rb, 32 * hf);
+    else gemm<4, false, true, O, O>(y, Qs + 16 * rb * LP, LP, PS, Ks + 32 * hf, LP, PS, 0, 16 * (rb + 1));
     T* out = (T*)A.y + (ch.row0(A) * A.hv + h) * A.dv;
     store_rows<T>(out, y, 16 * rb, ch.len, n0 + 32 * hf, A.dv, (long long)A.hv * A.dv);
 }
@@ -874,8 +895,9 @@ __global__ void __launch_bounds__(256, 3) gd_step_kernel(Args A, float* M, const
     const int lane8 = threadIdx.x & 7, grp = threadIdx.x >> 3, end = min(A.dv, (part + 1) * rows);
     const int slot = slots ? slots[first] : first;
     if (slot < 0 || slot >= pool) {                       // no sequence in this place
-        for (int i = threadIdx.x; i < A.seq * rows; i += 256) {
-            const int tok = i / rows, row = part * rows + i - tok * rows;
+        for (long long i = threadIdx.x; i < (long long)A.seq * rows; i += 256) {
+            const long long tok = i / rows;
+            const int row = part * rows + (int)(i - tok * rows);
             if (row < A.dv) ((T*)A.y)[(((long long)first * A.seq + tok) * A.hv + h) * A.dv + row] = from_f<T>(0.f);
         }
         return;

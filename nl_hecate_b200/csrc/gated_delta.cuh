@@ -205,17 +205,46 @@ __device__ __forceinline__ void load_scaled(bf* dst, const T* base, long long st
         }
     }
 }
-// 64 x 64 of a private, padded buffer, each row times scale[row] where a scale is given.
-template <int P, int THREADS>
-__device__ __forceinline__ void load_own(bf* dst, const float* base, int stride, const float* scale = nullptr)
+__device__ __forceinline__ bool odd(float x) { return !(fabsf(x) <= 3.402823466e38f); }      // an infinity or a NaN
+// A lower triangle's 0 times a later token's infinity or NaN is a NaN. Where a chunk holds such a value the two triangular
+// products of the forward are formed again token by token: row `row` of lower (planes) times the rows j <= row of x's column.
+template <int P> __device__ __noinline__ float triangle_at(const bf* lower, int psl, const bf* x, int ldx, int psx, int row)
 {
+    float s = 0.f;
+    for (int j = 0; j <= row; j++) {
+        float a = 0.f, b = 0.f;
+        for (int q = P - 1; q >= 0; q--) {
+            a += __bfloat162float(lower[q * psl + row * LP + j]);
+            b += __bfloat162float(x[q * psx + j * ldx]);
+        }
+        s = fmaf(a, b, s);
+    }
+    return s;
+}
+template <int P, int NT>
+__device__ __forceinline__ void triangle_by_token(float (&acc)[NT][4], const bf* lower, int psl, const bf* x, int ldx, int psx, int r0, int c0)
+{
+    const int lane = threadIdx.x & 31, g = lane >> 2, t = lane & 3;
+#pragma unroll
+    for (int n = 0; n < NT; n++)
+#pragma unroll
+        for (int i = 0; i < 4; i++) acc[n][i] += triangle_at<P>(lower, psl, x + c0 + 8 * n + 2 * t + (i & 1), ldx, psx, r0 + g + 8 * (i >> 1));
+}
+
+// 64 x 64 of a private, padded buffer, each row times scale[row] where a scale is given; whether the thread's part is odd.
+template <int P, int THREADS>
+__device__ __forceinline__ bool load_own(bf* dst, const float* base, int stride, const float* scale = nullptr)
+{
+    bool any = false;
 #pragma unroll
     for (int i = 0; i < C * 16 / THREADS; i++) {
         const int at = threadIdx.x + i * THREADS, r = at >> 4, c = (at & 15) * 4;
         float4 v = *reinterpret_cast<const float4*>(base + (long long)r * stride + c);
         if (scale) { const float s = scale[r]; v.x *= s; v.y *= s; v.z *= s; v.w *= s; }
+        any |= odd(v.x) | odd(v.y) | odd(v.z) | odd(v.w);
         put4<P>(dst + r * LP + c, C * LP, v);
     }
+    return any;
 }
 
 // ── products ──

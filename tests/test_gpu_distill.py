@@ -36,7 +36,7 @@ def definition(z, ids, t, y, tau, sw, hw):
         if bool(ok.any()):
             ce = -torch.log_softmax(z[ok], 1).gather(1, y[ok].long().unsqueeze(1))
             loss = loss + hw * ce.sum() / ok.sum()
-            size += float(hw * ce.abs().mean())
+            size += float(hw * ce.detach().abs().mean())
     if sw:
         t = t.double() / tau
         ok = (ids >= 0) & (ids < vocab) & (t != -math.inf)
@@ -47,7 +47,7 @@ def definition(z, ids, t, y, tau, sw, hw):
             logq = torch.log_softmax(z[rows] / tau, 1).gather(1, ids[rows].clamp(0, vocab - 1).long())
             kl = (torch.special.xlogy(p, p) - torch.where(p > 0, p * logq, torch.zeros_like(p))).sum(1)
             loss = loss + sw * tau * tau * kl.sum() / rows.sum()
-            size += float(sw * tau * tau * (p * torch.where(p > 0, logq, torch.zeros_like(p)).abs()).sum(1).mean())
+            size += float(sw * tau * tau * (p * torch.where(p > 0, logq, torch.zeros_like(p)).abs()).sum(1).mean().detach())
     grad = torch.autograd.grad(loss, z)[0] if loss.requires_grad else torch.zeros_like(z)
     return loss.detach(), grad, size
 
@@ -141,6 +141,24 @@ def test_in_place_strided_and_scaled(n, vocab, dtype):
     loss, saved = D.distill_forward(wide[:, :vocab], ids, t, targets=y, temperature=2.0, soft_weight=0.5, hard_weight=0.5)
     D.distill_backward(wide[:, :vocab], saved, grad=grad, out=wide[:, :vocab])
     assert torch.equal(wide[:, :vocab], d2) and bool((wide[:, vocab:] == 7).all())
+
+
+def test_captured_pair_replays_on_new_inputs():
+    from nl_hecate_b200 import dispatch as D
+    z, ids, t, y = make(300, 400, 7, torch.bfloat16)
+    call = lambda a: D.distill_forward(a[0], a[1], a[2], targets=a[3], temperature=2.0, soft_weight=0.5, hard_weight=0.5)
+    D.distill_backward(z, call((z, ids, t, y))[1])
+    g = torch.cuda.CUDAGraph()
+    with torch.cuda.graph(g):
+        loss, saved = call((z, ids, t, y))
+        d = D.distill_backward(z, saved)
+    for seed in (1, 2):
+        fresh = make(300, 400, 7, torch.bfloat16, seed=seed)
+        for dst, src in zip((z, ids, t, y), fresh):
+            dst.copy_(src)
+        g.replay()
+        w, s = call(fresh)
+        assert torch.equal(loss, w) and torch.equal(d, D.distill_backward(fresh[0], s))
 
 
 def test_refusals():

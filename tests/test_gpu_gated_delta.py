@@ -309,19 +309,33 @@ def test_captured_pair_replays_on_new_inputs():
                 assert torch.equal(o[x], want[x]), x
 
 
-def test_values_that_are_not_finite_stay_in_their_sequence():
-    p = inputs(3, 130, 2, 2, 64, 64, torch.float32, seed=4)
+@pytest.mark.parametrize("dtype", DTYPES)
+@pytest.mark.parametrize("at", [0, 17, 63, 64, 100, 129])
+def test_values_that_are_not_finite_stay_behind_their_token(dtype, at):
+    """A NaN or an infinity at one token (what padding may hold) leaves the tokens before it and the other sequences as they were;
+    one in V stays in its column of y and its row of M."""
+    p = inputs(3, 130, 2, 2, 64, 64, dtype, seed=4)
     clean = run(p)
-    for x, bad in (("k", float("nan")), ("v", float("inf")), ("q", float("nan")), ("log_retain", float("nan")), ("theta", float("nan"))):
+    want = reference(p, 1.0)
+    for x, bad in (("k", float("nan")), ("v", float("inf")), ("v", float("nan")), ("q", float("nan")), ("log_retain", float("nan")),
+                   ("theta", float("nan"))):
         q = {**p, x: p[x].clone()}
-        q[x][1, 100] = bad
+        if x in ("k", "v", "q"):
+            q[x][1, at, :, 5] = bad
+        else:
+            q[x][1, at] = bad
         out = run(q)
         for name in clean:
-            t, c = out[name], clean[name]
-            keep = [0, 2]
-            assert torch.equal(t[keep], c[keep]), (x, name)
-        # chunks of 64 tokens in front of the value are not reached by it in the forward
-        assert torch.equal(out["y"][1, :64], clean["y"][1, :64]) and bool(torch.isnan(out["y"][1, 100]).any()), x
+            assert torch.equal(out[name][[0, 2]], clean[name][[0, 2]]), (x, name)
+        check({"y": out["y"][1:2, :at]}, {"y": want["y"][1:2, :at]}, dtype, x)
+        assert not bool(torch.isfinite(out["y"][1, at, :, 5]).any()), x
+        if x == "v":
+            other = [c for c in range(64) if c != 5]
+            check({"y": out["y"][1:2][..., other], "m_final": out["m_final"][1:2][:, :, other]},
+                  {"y": want["y"][1:2][..., other], "m_final": want["m_final"][1:2][:, :, other]}, dtype, x)
+        if x == "q":
+            check({"y": out["y"][1:2, at + 1:], "m_final": out["m_final"][1:2]},
+                  {"y": want["y"][1:2, at + 1:], "m_final": want["m_final"][1:2]}, dtype, x)
 
 
 # ── recurrent step ──
@@ -354,6 +368,57 @@ def test_step_slots():
         want = reference(q, 1.0)
         got = torch.cat([y[i:i + 1] for i in who], 1)
         check({"y": got, "m_final": pool[slot:slot + 1]}, want, torch.float32, f"slot {slot}")
+
+
+def test_captured_step_and_inference_mode():
+    """A captured step advances the stored states at every replay, on the inputs of that replay; the same calls in inference mode."""
+    from nl_hecate_b200 import dispatch as D
+    names = ("k", "v", "q", "log_retain", "theta")
+    toks = [inputs(4, 1, 2, 2, 64, 64, torch.bfloat16, seed=s) for s in range(3)]
+    slots = torch.tensor([2, 0, 5, 1], dtype=torch.int32, device="cuda")
+    start = torch.randn(6, 2, 64, 64, device="cuda")
+    with torch.inference_mode():
+        want_m, want = start.clone(), []
+        for p in toks:
+            want.append(D.gated_delta_step(*[p[x] for x in names], want_m, slots=slots))
+    pool, cur = start.clone(), {x: toks[0][x].clone() for x in names}
+    g = torch.cuda.CUDAGraph()
+    with torch.cuda.graph(g):
+        y = D.gated_delta_step(*[cur[x] for x in names], pool, slots=slots)
+    for p, w in zip(toks, want):
+        for x in names:
+            cur[x].copy_(p[x])
+        g.replay()
+        assert torch.equal(y, w)
+    assert torch.equal(pool, want_m)
+
+
+def test_two_threads_with_streams_of_their_own():
+    import threading
+    sets = [inputs(2, 150, 2, 2, 64, 64, torch.float32, seed=s) for s in (1, 2)]
+    want, got, failed = [run(p) for p in sets], [[], []], []
+
+    def work(i):
+        try:
+            st = torch.cuda.Stream()
+            with torch.cuda.stream(st):
+                for _ in range(20):
+                    got[i].append(run(sets[i]))
+            st.synchronize()
+        except Exception as e:           # noqa: BLE001 - shown by the assertion below
+            failed.append(e)
+
+    torch.cuda.synchronize()
+    threads = [threading.Thread(target=work, args=(i,)) for i in range(2)]
+    for t in threads:
+        t.start()
+    for t in threads:
+        t.join()
+    assert not failed, failed
+    for w, outs in zip(want, got):
+        for o in outs:
+            for x in w:
+                assert torch.equal(o[x], w[x]), x
 
 
 def test_prompt_then_tokens():

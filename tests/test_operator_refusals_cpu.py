@@ -51,6 +51,7 @@ def test_sizes(lib):
     assert lib.nlh_gated_delta_saved_bytes(C.byref(desc(seq=0))) == 0
     assert lib.nlh_gated_delta_saved_bytes(C.byref(desc(batch=1, seq=100, n_seqs=7))) > 0
     assert lib.nlh_embedding_backward_bytes(100, 1000, 64) == 0 and lib.nlh_embedding_backward_bytes(5000, 1000, 64) >= 5000 * 16
+    assert lib.nlh_embedding_backward_bytes((1 << 30) + 1, 10, 4) == -1
     assert lib.nlh_embedding_backward_bytes(-1, 10, 4) == -1 and lib.nlh_embedding_backward_bytes(1, 0, 4) == -1
     assert lib.nlh_distill_saved_bytes(0, 10) >= 0 and lib.nlh_distill_saved_bytes(-1, 10) == -1
     # bytes that pass 32 bits
@@ -113,7 +114,7 @@ def test_distill_refuses(lib):
         return lib.nlh_distill_forward(logits, 0, stride, targets, ids, top, 0, loss, saved, nbytes, rows, vocab, k, tau, hard, soft)
 
     for kw in (dict(logits=None), dict(stride=49), dict(top=None), dict(loss=None), dict(saved=None), dict(nbytes=n - 1), dict(rows=-1),
-               dict(vocab=0), dict(k=-1), dict(k=1025), dict(tau=0.0), dict(tau=-1.0), dict(tau=float("nan")), dict(tau=float("inf")),
+               dict(vocab=0), dict(vocab=(1 << 30) + 1, stride=1 << 31), dict(k=-1), dict(k=1025), dict(tau=0.0), dict(tau=-1.0), dict(tau=float("nan")), dict(tau=float("inf")),
                dict(saved=C.c_void_p(4104))):
         assert fwd(**kw) == BAD, kw
     b = lib.nlh_distill_backward
