@@ -401,15 +401,16 @@ __device__ __forceinline__ void store_rows(T* out, const float (&acc)[4][4], int
 }
 
 // ── forward outputs ──
-// Eight warps: warp = 16 tokens x 32 of the tile's 64 columns. For bf16 the state, P and U are two planes: y is rounded to bf16.
-// Two places in shared memory, Q then P, and K, then S, then U: four CTAs share an SM and cover each other's loads (4096 tiles
-// fp32: 151 us; three places and two CTAs 166, three CTAs with the next tile on its way in registers 174).
+// Four warps: warp = 32 tokens x 32 of the tile's 64 columns. For bf16 the state, P and U are two planes: y is rounded to bf16.
+// Two places in shared memory, Q then P, and K, then S, then U: four CTAs share an SM and cover each other's loads. 4096 tiles
+// fp32: 143 us (bf16: 92); eight warps of 16 x 32, which read a third more from shared memory, 152 (106); those with three places and two
+// CTAs 166, with three CTAs and the next tile on its way in registers 174.
 template <typename T> struct OutFwdSmem {
     static constexpr int PS = C * LP, IN = Pl<T>::in, O = Pl<T>::out, M = IN > O ? IN : O;
     static constexpr int BYTES = 2 * PS * 2 * M;
 };
 template <typename T>
-__global__ void __launch_bounds__(256, 4) gd_out_fwd_kernel(Args A)
+__global__ void __launch_bounds__(128, 4) gd_out_fwd_kernel(Args A)
 {
     typedef OutFwdSmem<T> L;
     constexpr int PS = L::PS, IN = L::IN, O = L::O;
@@ -422,46 +423,49 @@ __global__ void __launch_bounds__(256, 4) gd_out_fwd_kernel(Args A)
     const Chunk ch = get_chunk(A, slot);
     if (ch.len <= 0) return;
     const long long tile = (long long)slot * A.hv + h;
-    const int tid = threadIdx.x, lane = tid & 31, w = tid >> 5, rb = w & 3, hf = w >> 2, g = lane >> 2, t = lane & 3;
+    const int tid = threadIdx.x, lane = tid & 31, w = tid >> 5, rb = w & 1, hf = w >> 1, g = lane >> 2, t = lane & 3;
     if (tid < C) { s_gate[tid] = A.gates[tile * C + tid]; s_theta[tid] = A.theta_eff[tile * C + tid]; }
     const T* kp = (const T*)A.k + ch.b * A.kb + ch.t0 * A.kt + (h / A.share) * A.kh;
     const T* qp = (const T*)A.q + ch.b * A.qb + ch.t0 * A.qt + (h / A.share) * A.qh;
-    float att[4][4], y[4][4];
-    zero(att);
-    zero(y);
-    const bool need = 32 * hf <= 16 * rb + 15;
+    float att[2][4][4], y[2][4][4];
+    zero(att[0]); zero(att[1]);
+    zero(y[0]); zero(y[1]);
+    const bool need = hf <= rb;
     for (int c0 = 0; c0 < A.dk; c0 += 64) {
         if (c0) __syncthreads();
-        load_tile<T, 64, 256>(Qs, LP, PS, qp + c0, A.qt, ch.len, A.dk - c0);
-        load_tile<T, 64, 256>(Ks, LP, PS, kp + c0, A.kt, ch.len, A.dk - c0);
+        load_tile<T, 64, 128>(Qs, LP, PS, qp + c0, A.qt, ch.len, A.dk - c0);
+        load_tile<T, 64, 128>(Ks, LP, PS, kp + c0, A.kt, ch.len, A.dk - c0);
         __syncthreads();
-        if (need) gemm<4, false, false, IN, IN>(att, Qs + 16 * rb * LP, LP, PS, Ks + 32 * hf * LP, LP, PS, 0, 64);
+        if (need) gemm_2<4, false, false, IN, IN>(att, Qs + 32 * rb * LP, LP, PS, Ks + 32 * hf * LP, LP, PS, 0, 64);
         __syncthreads();
-        load_own<O, 256>(Ks, A.m_chunk + (tile * A.dkp + c0) * A.dvp + n0, A.dvp);
+        load_own<O, 128>(Ks, A.m_chunk + (tile * A.dkp + c0) * A.dvp + n0, A.dvp);
         __syncthreads();
-        gemm<4, false, true, IN, O>(y, Qs + 16 * rb * LP, LP, PS, Ks + 32 * hf, LP, PS, 0, 64);
+        gemm_2<4, false, true, IN, O>(y, Qs + 32 * rb * LP, LP, PS, Ks + 32 * hf, LP, PS, 0, 64);
     }
     __syncthreads();
 #pragma unroll
     for (int n = 0; n < 4; n++)
 #pragma unroll
-        for (int r = 0; r < 2; r++) {
-            const int i = 16 * rb + g + 8 * r, j = 32 * hf + 8 * n + 2 * t;
+        for (int r = 0; r < 4; r++) {
+            const int i = 32 * rb + g + 8 * r, j = 32 * hf + 8 * n + 2 * t, m = r >> 1, o = 2 * (r & 1);
             const float4 gi = s_gate[i];
             float x[2];
 #pragma unroll
             for (int e = 0; e < 2; e++) {
                 const float4 gj = s_gate[j + e];
-                x[e] = j + e <= i ? decay(make_float2(gi.x, gi.y), make_float2(gj.x, gj.y)) * A.scale * att[n][2 * r + e] : 0.f;
-                y[n][2 * r + e] *= A.scale * gi.z;
+                x[e] = j + e <= i ? decay(make_float2(gi.x, gi.y), make_float2(gj.x, gj.y)) * A.scale * att[m][n][o + e] : 0.f;
+                y[m][n][o + e] *= A.scale * gi.z;
             }
             put2<O>(Qs + i * LP + j, PS, x[0], x[1]);
         }
-    const bool any = load_own<O, 256>(Ks, A.e + tile * C * A.dvp + n0, A.dvp, s_theta);
-    if (__syncthreads_or(any)) triangle_by_token<O, 4>(y, Qs, PS, Ks, LP, PS, 16 * rb, 32 * hf);
-    else gemm<4, false, true, O, O>(y, Qs + 16 * rb * LP, LP, PS, Ks + 32 * hf, LP, PS, 0, 16 * (rb + 1));
+    const bool any = load_own<O, 128>(Ks, A.e + tile * C * A.dvp + n0, A.dvp, s_theta);
+    if (__syncthreads_or(any)) {
+        triangle_by_token<O, 4>(y[0], Qs, PS, Ks, LP, PS, 32 * rb, 32 * hf);
+        triangle_by_token<O, 4>(y[1], Qs, PS, Ks, LP, PS, 32 * rb + 16, 32 * hf);
+    } else gemm_2<4, false, true, O, O>(y, Qs + 32 * rb * LP, LP, PS, Ks + 32 * hf, LP, PS, 0, 32 * (rb + 1));
     T* out = (T*)A.y + (ch.row0(A) * A.hv + h) * A.dv;
-    store_rows<T>(out, y, 16 * rb, ch.len, n0 + 32 * hf, A.dv, (long long)A.hv * A.dv);
+    store_rows<T>(out, y[0], 32 * rb, ch.len, n0 + 32 * hf, A.dv, (long long)A.hv * A.dv);
+    store_rows<T>(out, y[1], 32 * rb + 16, ch.len, n0 + 32 * hf, A.dv, (long long)A.hv * A.dv);
 }
 
 // ── backward, what needs no state gradient: F = P^T dY, and N = scale (e^G Q)^T dY into the place of D ──
@@ -1133,7 +1137,7 @@ template <typename T> static bool run_forward(Args& A, cudaStream_t st, const ch
     if (tiles) {
         constexpr int bytes = OutFwdSmem<T>::BYTES;
         if (!allow_smem<gd_out_fwd_kernel<T>, bytes>(where)) return false;
-        gd_out_fwd_kernel<T><<<dim3(tiles, A.dvp / 64), 256, bytes, st>>>(A);
+        gd_out_fwd_kernel<T><<<dim3(tiles, A.dvp / 64), 128, bytes, st>>>(A);
         if (!check_launch(where)) return false;
     }
     return true;

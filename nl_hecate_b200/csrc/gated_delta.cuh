@@ -307,6 +307,42 @@ __device__ __forceinline__ void gemm(float (&acc)[NT][4], const bf* A, int lda, 
         }
     }
 }
+// The same for 32 rows: every B fragment serves two A fragments.
+template <int NT, bool AK, bool BK, int PA, int PB>
+__device__ __forceinline__ void gemm_2(float (&acc)[2][NT][4], const bf* A, int lda, int psa, const bf* B, int ldb, int psb, int k0, int k1)
+{
+    constexpr int TOP = (PA > PB ? PA : PB) - 1;
+    const int l = threadIdx.x & 31, l8 = l & 7, q = l >> 3;
+    const unsigned a0 = smem_addr(AK ? A + ((q >> 1) * 8 + l8) * lda + (q & 1) * 8 : A + ((q & 1) * 8 + l8) * lda + (q >> 1) * 8);
+    const unsigned b0 = smem_addr(BK ? B + ((q & 1) * 8 + l8) * ldb + (q >> 1) * 8 : B + ((q >> 1) * 8 + l8) * ldb + (q & 1) * 8);
+#pragma unroll 1
+    for (int k = k0; k < k1; k += 16) {
+        unsigned a[2][PA][4];
+#pragma unroll
+        for (int m = 0; m < 2; m++)
+#pragma unroll
+            for (int i = 0; i < PA; i++) ldsm4<AK>(a[m][i], a0 + 2 * (i * psa + (AK ? k * lda + 16 * m : k + 16 * m * lda)));
+#pragma unroll
+        for (int n = 0; n < NT; n += 2) {
+            unsigned b[PB][4];
+#pragma unroll
+            for (int j = 0; j < PB; j++) ldsm4<BK>(b[j], b0 + 2 * (j * psb + (BK ? k * ldb + n * 8 : k + n * 8 * ldb)));
+#pragma unroll
+            for (int m = 0; m < 2; m++)
+#pragma unroll
+                for (int e = 0; e < 2; e++) {
+                    float s[4] = {0.f, 0.f, 0.f, 0.f};
+#pragma unroll
+                    for (int o = TOP; o >= 0; o--)
+#pragma unroll
+                        for (int i = 0; i < PA; i++)
+                            if (o - i >= 0 && o - i < PB) mma_bf16(s, a[m][i], b[o - i][2 * e], b[o - i][2 * e + 1]);
+#pragma unroll
+                    for (int x = 0; x < 4; x++) acc[m][n + e][x] += s[x];
+                }
+        }
+    }
+}
 template <int NT> __device__ __forceinline__ void zero(float (&acc)[NT][4])
 {
 #pragma unroll
