@@ -689,6 +689,19 @@ __global__ void __launch_bounds__(256, DKP == 64 ? 2 : 1) gd_state_bwd_kernel(Ar
     }
 }
 
+// One warp: the gradient of log_retain of a chunk, sums of the gradient of G (a, b: of tokens 2 lane, 2 lane + 1) from each token to the
+// chunk's end, in 64 bits. `last` belongs to the last G; rows behind the chunk's last token are 0.
+__device__ __forceinline__ void gate_gradient(const Args& A, const Chunk& ch, int h, double a, double b, double last)
+{
+    const int lane = threadIdx.x & 31;
+    if (lane == 31) b += last;
+    double s = a + b;
+    for (int o = 1; o < 32; o <<= 1) { const double y = __shfl_down_sync(0xffffffffu, s, o); if (lane + o < 32) s += y; }
+    float* out = A.d_g + (ch.row0(A) + 2 * lane) * A.hv + h;
+    if (2 * lane < ch.len) out[0] = (float)s;
+    if (2 * lane + 1 < ch.len) out[A.hv] = (float)(s - a);
+}
+
 // ── backward outputs: d_q, d_k, d_theta and the gradient of G, for 64 columns of dk ──
 //   Mq_ij = scale e^{G_i - G_j} (dy_i.e_j) theta_j (j <= i),  Mb_ij = -e^{G_i - G_j} (x_i.e_j) theta_j (j < i)
 //   d_q = scale e^G dY M_0 + Mq K;  k as a query: -e^G X M_0 + Mb K;  k as a key: theta e^{G_L - G} E D + Mq^T Q + Mb^T K
@@ -825,12 +838,20 @@ __global__ void __launch_bounds__(256, 2) gd_out_bwd_kernel(Args A)
     gsum = warp_sum(gsum);
     if (lane == 0) s_red[w] = gsum;
     __syncthreads();
-    const long long part = (long long)kt * A.slots * A.hv + tile;
-    if (tid < C) A.dg_part[part * C + tid] = s_row[0][tid] + s_row[1][tid];
-    if (tid == 0) {
-        float s = 0.f;
-        for (int i = 0; i < 8; i++) s += s_red[i];
-        A.dgl_part[part] = s;
+    if (gridDim.y == 1) {                         // all of dk is here: so are the sums over the chunk
+        if (w == 0) {
+            float last = 0.f;
+            for (int i = 0; i < 8; i++) last += s_red[i];
+            gate_gradient(A, ch, h, (double)s_row[0][2 * lane] + s_row[1][2 * lane], (double)s_row[0][2 * lane + 1] + s_row[1][2 * lane + 1], last);
+        }
+    } else {
+        const long long part = (long long)kt * A.slots * A.hv + tile;
+        if (tid < C) A.dg_part[part * C + tid] = s_row[0][tid] + s_row[1][tid];
+        if (tid == 0) {
+            float s = 0.f;
+            for (int i = 0; i < 8; i++) s += s_red[i];
+            A.dgl_part[part] = s;
+        }
     }
     if (A.share == 1) {
         const long long at = (ch.row0(A) * A.hk + h) * A.dk, st = (long long)A.hk * A.dk;
@@ -843,7 +864,7 @@ __global__ void __launch_bounds__(256, 2) gd_out_bwd_kernel(Args A)
     }
 }
 
-// Gradient of log_retain: sums of the gradient of G from each token to the chunk's end. One warp per chunk and head.
+// Where dk takes two CTAs of the kernel above: their parts of the gradient of G. One warp per chunk and head.
 __global__ void __launch_bounds__(128) gd_gate_bwd_kernel(Args A)
 {
     const long long tile = (long long)blockIdx.x * 4 + (threadIdx.x >> 5);
@@ -851,18 +872,14 @@ __global__ void __launch_bounds__(128) gd_gate_bwd_kernel(Args A)
     const int slot = (int)(tile / A.hv), h = (int)(tile - (long long)slot * A.hv), lane = threadIdx.x & 31;
     const Chunk ch = get_chunk(A, slot);
     if (ch.len <= 0) return;
-    double a = 0., b = 0.;
+    double a = 0., b = 0., last = 0.;
     for (int kt = 0; kt < A.dkp / 64; kt++) {
         const long long part = (long long)kt * A.slots * A.hv + tile;
         a += A.dg_part[part * C + 2 * lane];
         b += A.dg_part[part * C + 2 * lane + 1];
-        if (lane == 31) b += A.dgl_part[part];       // rows behind the chunk's last token are 0
+        last += A.dgl_part[part];
     }
-    double s = a + b;
-    for (int o = 1; o < 32; o <<= 1) { const double y = __shfl_down_sync(0xffffffffu, s, o); if (lane + o < 32) s += y; }
-    float* out = A.d_g + (ch.row0(A) + 2 * lane) * A.hv + h;
-    if (2 * lane < ch.len) out[0] = (float)s;
-    if (2 * lane + 1 < ch.len) out[A.hv] = (float)(s - a);
+    gate_gradient(A, ch, h, a, b, last);
 }
 
 // Gradients of shared keys and queries: the value heads of a group, added in their order. Rows outside the sequences of a packed
@@ -1157,8 +1174,10 @@ template <typename T> static bool run_backward(Args& A, cudaStream_t st, const c
     if (!allow_smem<gd_out_bwd_kernel<T>, bytes>(where)) return false;
     gd_out_bwd_kernel<T><<<dim3(tiles, A.dkp / 64), 256, bytes, st>>>(A);
     if (!check_launch(where)) return false;
-    gd_gate_bwd_kernel<<<(tiles + 3) / 4, 128, 0, st>>>(A);
-    if (!check_launch(where)) return false;
+    if (A.dkp > 64) {
+        gd_gate_bwd_kernel<<<(tiles + 3) / 4, 128, 0, st>>>(A);
+        if (!check_launch(where)) return false;
+    }
     if (A.share > 1) {
         const long long n = (long long)A.batch * A.seq * A.hk * A.dk;
         const long long need = (n + 255) / 256;

@@ -115,3 +115,28 @@ def test_captured_gradient_replays():
         g.replay()
         want = D.embedding_backward(d2, i2, torch.zeros_like(dw))
         assert torch.equal(dw, want)
+
+
+@pytest.mark.parametrize("n,vocab", [(2500, 1), (3000, 7), (40000, 2), (70000, 300), (131072, 40), (131073, 40)])
+def test_tiny_vocabularies_and_borders_of_the_sorts(n, vocab):
+    """Fewer ids than a warp has lanes; the largest list that one launch sorts, and the first that it does not."""
+    from nl_hecate_b200 import dispatch as D
+    ids, dy, dw = make(n, vocab, 4, torch.float32, "hot", seed=vocab)
+    old = dw.clone()
+    D.embedding_backward(dy, ids, dw)
+    s, mag, count = sums(ids, dy, vocab)
+    tol = 2.0 ** -24 * ((count + 2) * mag + old.double().abs() + (old.double() + s).abs())
+    assert bool(((dw.double() - old.double() - s).abs() <= tol).all())
+
+
+def test_refusals():
+    from nl_hecate_b200 import dispatch as D
+    ids, dy, dw = make(30, 50, 8, torch.float32, "spread")
+    w = dw.clone()
+    for bad in ((w.half(), ids), (w.t(), ids), (w[0], ids), (w, ids.long()), (w, ids.cpu()), (w, ids[::2])):
+        with pytest.raises(ValueError):
+            D.embedding_forward(*bad)
+    for bad in ((dy.half(), ids, dw), (dy[:29], ids, dw), (dy[:, :4], ids, dw), (dy, ids.long(), dw), (dy, ids, dw.bfloat16()),
+                (dy, ids, dw.t()), (dy.t().contiguous().t(), ids, dw), (dy.cpu(), ids, dw)):
+        with pytest.raises(ValueError):
+            D.embedding_backward(*bad)
