@@ -13,6 +13,7 @@
 // Up to SMALL tokens one launch does it all: a CTA per token looks for its id in the whole list, and the first token of an id
 // adds up its rows.
 // Bound by HBM: d_out is read once, the touched rows of d_w once and written once.
+#include <atomic>
 #include <cooperative_groups.h>
 #include <cuda_bf16.h>
 
@@ -213,13 +214,13 @@ __global__ void __launch_bounds__(SORT_THREADS) scatter_kernel(const int* ids, c
         if (key[j] >= 0) out[s_cnt[w][(key[j] >> shift) & (BINS - 1)] + rank[j]] = make_int2(key[j], pos[j]);
 }
 
-// The whole sort in one launch up to 131072 tokens: a cluster of eight CTAs, a thread ITEMS tokens, the digits' totals exchanged
-// through distributed shared memory, digits only as wide as the passes need. 32768 tokens of a vocabulary of 8192 take 15 us
-// (the launches above: 27 and the gaps between them), 65521 of 50001 take 26 (37). Tokens of one digit in a warp are found by a
-// ballot per bit (a match instruction: 16 us). Sixteen CTAs, more than every part of the GPU promises to hold, would take 12 and 19.
-constexpr int CL = 8, CL_THREADS = 1024, CL_WARPS = CL_THREADS / 32;
-template <int ITEMS>
-__global__ void __cluster_dims__(CL, 1, 1) __launch_bounds__(CL_THREADS, 1) sort_cluster_kernel(const int* ids, int2* bufa, int2* bufb, int n,
+// The whole sort in one launch up to 131072 tokens: a cluster of CL CTAs, a thread ITEMS tokens, the digits' totals exchanged
+// through distributed shared memory, digits only as wide as the passes need. CL is 16 where the device can hold such a cluster,
+// else 8. 32768 tokens of a vocabulary of 8192 take 12 us (8 CTAs: 15; the launches above: 27 and the gaps between them), 65521 of
+// 50001 take 19 (26; 37). Tokens of one digit in a warp are found by a ballot per bit (a match instruction: 16 us with 8 CTAs).
+constexpr int CL_THREADS = 1024, CL_WARPS = CL_THREADS / 32, CL_MOST = 131072;
+template <int ITEMS, int CL>
+__global__ void __launch_bounds__(CL_THREADS, 1) sort_cluster_kernel(const int* ids, int2* bufa, int2* bufb, int n,
                                                                                                int vocab, int passes, int bits)
 {
     extern __shared__ int s_dyn[];
@@ -522,13 +523,56 @@ static int lanes_for(int d, int per, int most)
     return l;
 }
 
-template <int ITEMS> static bool sort_cluster(const int* ids, const Plan& P, int n, int vocab, const char* where)
+template <int ITEMS, int CL> static cudaError_t sort_cluster(const int* ids, const Plan& P, int n, int vocab, bool* fits)
 {
     constexpr int bytes = (CL_WARPS + 2) * BINS * 4;
-    const cudaError_t e = cudaFuncSetAttribute(sort_cluster_kernel<ITEMS>, cudaFuncAttributeMaxDynamicSharedMemorySize, bytes);
-    if (e != cudaSuccess) { record_status(NLH_ERR_CUDA, where, cudaGetErrorString(e)); return false; }
-    sort_cluster_kernel<ITEMS><<<CL, CL_THREADS, bytes, current_stream()>>>(ids, P.a, P.b, n, vocab, P.passes, P.bits);
-    return check_launch(where);
+    const auto kernel = sort_cluster_kernel<ITEMS, CL>;
+    cudaError_t e = cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, bytes);
+    if (e == cudaSuccess && CL > 8) e = cudaFuncSetAttribute(kernel, cudaFuncAttributeNonPortableClusterSizeAllowed, 1);
+    if (e != cudaSuccess) return e;
+    cudaLaunchAttribute at;
+    at.id = cudaLaunchAttributeClusterDimension;
+    at.val.clusterDim.x = CL;
+    at.val.clusterDim.y = at.val.clusterDim.z = 1;
+    cudaLaunchConfig_t c = {};
+    c.gridDim = dim3(CL);
+    c.blockDim = dim3(CL_THREADS);
+    c.dynamicSmemBytes = bytes;
+    c.stream = current_stream();
+    c.attrs = &at;
+    c.numAttrs = 1;
+    if (fits) {
+        int clusters = 0;
+        *fits = cudaOccupancyMaxActiveClusters(&clusters, kernel, &c) == cudaSuccess && clusters > 0;
+        cudaGetLastError();                      // a size that the device does not take is an answer, not an error
+        return cudaSuccess;
+    }
+    return cudaLaunchKernelEx(&c, kernel, ids, P.a, P.b, n, vocab, P.passes, P.bits);
+}
+template <int CL> static bool sort_with(const int* ids, const Plan& P, int n, int vocab, const char* where)
+{
+    constexpr int MOST = CL_MOST / (CL * CL_THREADS);           // tokens a thread of the longest list
+    const int items = (n + CL * CL_THREADS - 1) / (CL * CL_THREADS);
+    const cudaError_t e = items <= 2 ? sort_cluster<2, CL>(ids, P, n, vocab, nullptr)
+                          : items <= MOST / 2 ? sort_cluster<MOST / 2, CL>(ids, P, n, vocab, nullptr)
+                                              : sort_cluster<MOST, CL>(ids, P, n, vocab, nullptr);
+    if (e != cudaSuccess) record_status(NLH_ERR_CUDA, where, cudaGetErrorString(e));
+    return e == cudaSuccess;
+}
+// Whether the current device holds a cluster of sixteen of these CTAs; asked once per device.
+static bool wide_clusters(const Plan& P)
+{
+    static std::atomic<int> known[64];           // 0: not asked, 1: no, 2: yes
+    int dev = 0;
+    if (cudaGetDevice(&dev) != cudaSuccess || dev < 0 || dev >= 64) return false;
+    int k = known[dev].load(std::memory_order_relaxed);
+    if (k == 0) {
+        bool fits = false;
+        if (sort_cluster<8, 16>(nullptr, P, 0, 1, &fits) != cudaSuccess) { cudaGetLastError(); fits = false; }
+        k = fits ? 2 : 1;
+        known[dev].store(k, std::memory_order_relaxed);
+    }
+    return k == 2;
 }
 
 template <typename T, int N, bool ADD>
@@ -543,10 +587,8 @@ static bool backward(const T* dy, const int* ids, float* dw, int n, int vocab, i
         return check_launch(where);
     }
     const int2* in = nullptr;
-    if (n <= CL * CL_THREADS * 16) {
-        const int items = n <= CL * CL_THREADS * 4 ? 4 : n <= CL * CL_THREADS * 8 ? 8 : 16;
-        if (!(items == 4 ? sort_cluster<4>(ids, P, n, vocab, where) : items == 8 ? sort_cluster<8>(ids, P, n, vocab, where)
-                                                                                  : sort_cluster<16>(ids, P, n, vocab, where))) return false;
+    if (n <= CL_MOST) {
+        if (!(wide_clusters(P) ? sort_with<16>(ids, P, n, vocab, where) : sort_with<8>(ids, P, n, vocab, where))) return false;
         in = P.passes & 1 ? P.a : P.b;
     } else {
         int2* out = P.a;
