@@ -518,8 +518,8 @@ int32_t nlh_transpose(const float* src, float* dst, int32_t rows, int32_t cols);
 /* ── Embedding lookup with scaling, gradient by sorted tokens (additive, no counterpart in the reference) ──
  * Beside embedding_gather_cuda / embedding_scatter_add_cuda above. out[t] = scale * w[ids[t]], w [vocab, d] and out [n, d] both
  * fp32 or both bf16; an id outside [0, vocab) gives a row of zeros and takes no part in the gradient. Backward: d_w [vocab, d] fp32,
- * n up to 2^30, accumulate != 0: d_w[r] += scale * sum of the rows of d_out [n, d] (fp32 or bf16) with id r; 0: d_w is overwritten, zeros in
- * rows without a token. Sums are in fp32 and in one order that n, ids and d fix: the same call gives the same bits. workspace
+ * n up to 2^30, d up to 2^20, accumulate != 0: d_w[r] += scale * sum of the rows of d_out [n, d] (fp32 or bf16) with id r; 0: d_w is overwritten, zeros in
+ * rows without a token. Sums are in fp32 and in one order that n, ids, d and the alignment of d_out and d_w fix: the same call gives the same bits. workspace
  * (nlh_embedding_backward_bytes, 16-byte aligned) is the caller's. */
 int32_t nlh_embedding_forward(const void* w, int32_t w_is_bf16, const int32_t* ids, void* out, int32_t n, int32_t vocab,
     int32_t d, float scale);

@@ -60,7 +60,9 @@ def test_lookup(dtype, n, vocab, d):
 @pytest.mark.parametrize("n,vocab,d,dtype", [
     (1, 1, 1, torch.float32), (5, 9, 3, torch.bfloat16), (64, 256, 64, torch.float32), (2048, 300, 40, torch.bfloat16),
     (2049, 300, 40, torch.bfloat16), (2049, 70000, 9, torch.float32), (5000, 513, 512, torch.float32), (4096, 31, 1032, torch.bfloat16),
-    (140000, 1000, 8, torch.float32), (270000, 300000, 4, torch.float32), (6007, 511, 1, torch.float32), (6007, 512, 2, torch.float32)])
+    (140000, 1000, 8, torch.float32), (270000, 300000, 4, torch.float32), (6007, 511, 1, torch.float32), (6007, 512, 2, torch.float32),
+    (4096, 300, 40, torch.bfloat16), (4097, 300, 40, torch.float32), (1024, 90, 1024, torch.float32), (1025, 90, 1024, torch.bfloat16),
+    (30, 11, 35003, torch.float32), (1, 2, 1 << 20, torch.bfloat16), (2, 2, 1 << 20, torch.float32)])
 def test_gradient(n, vocab, d, dtype, kind, accumulate):
     from nl_hecate_b200 import dispatch as D
     ids, dy, dw = make(n, vocab, d, dtype, kind, seed=n)

@@ -1,11 +1,12 @@
 """Gated delta rule (chunked forward and backward, recurrent step) against the token-by-token recurrence and its
 adjoint in 64 bits.
 
-Tolerances, relative to the largest value of a tensor. fp32: operands of the products carry 22 bits (2^-23 = 1.2e-7 a
-factor), about eight products follow one another, sums of up to 128 terms in fp32 between them: 8 x 2 x 1.2e-7 = 2e-6;
+Tolerances, relative to the largest value of a tensor. fp32: operands of the products carry 24 bits (three bf16
+parts; the parts of the product that are left out and the operand's own rounding stay below 2^-23 = 1.2e-7 a factor), about
+eight products follow one another, sums of up to 128 terms in fp32 between them: 8 x 2 x 1.2e-7 = 2e-6;
 gradients pass twice as many: 4e-6; gate gradients are sums of up to 64 of those with both signs: 2e-5. Results in bf16:
-half a step, 2^-9 of the value's binade = 2^-8 relative at most, and the same again in y for its one-pass products
-(2^-12 an operand, far less)."""
+half a step, 2^-9 of the value's binade = 2^-8 relative at most, and the same again in y for its products of
+operands in two bf16 parts (2^-17 an operand, far less)."""
 import os
 import sys
 

@@ -52,6 +52,7 @@ def test_sizes(lib):
     assert lib.nlh_gated_delta_saved_bytes(C.byref(desc(batch=1, seq=100, n_seqs=7))) > 0
     assert lib.nlh_embedding_backward_bytes(100, 1000, 64) == 0 and lib.nlh_embedding_backward_bytes(5000, 1000, 64) >= 5000 * 16
     assert lib.nlh_embedding_backward_bytes((1 << 30) + 1, 10, 4) == -1
+    assert lib.nlh_embedding_backward_bytes(1, 10, (1 << 20) + 1) == -1 and lib.nlh_embedding_backward_bytes(0, 10, 1 << 20) == 0
     assert lib.nlh_embedding_backward_bytes(-1, 10, 4) == -1 and lib.nlh_embedding_backward_bytes(1, 0, 4) == -1
     assert lib.nlh_distill_saved_bytes(0, 10) >= 0 and lib.nlh_distill_saved_bytes(-1, 10) == -1
     # bytes that pass 32 bits
