@@ -517,10 +517,10 @@ int32_t nlh_transpose(const float* src, float* dst, int32_t rows, int32_t cols);
 
 /* ── Embedding lookup with scaling, gradient by sorted tokens (additive, no counterpart in the reference) ──
  * Beside embedding_gather_cuda / embedding_scatter_add_cuda above. out[t] = scale * w[ids[t]], w [vocab, d] and out [n, d] both
- * fp32 or both bf16; an id outside [0, vocab) gives a row of zeros and takes no part in the gradient. Backward: d_w [vocab, d] fp32,
- * n up to 2^30, d up to 2^20, accumulate != 0: d_w[r] += scale * sum of the rows of d_out [n, d] (fp32 or bf16) with id r; 0: d_w is overwritten, zeros in
- * rows without a token. Sums are in fp32 and in one order that n, ids, d and the alignment of d_out and d_w fix: the same call gives the same bits. workspace
- * (nlh_embedding_backward_bytes, 16-byte aligned) is the caller's. */
+ * fp32 or both bf16, d up to 2^20; an id outside [0, vocab) gives a row of zeros and takes no part in the gradient. Backward:
+ * d_w [vocab, d] fp32, n up to 2^30, accumulate != 0: d_w[r] += scale * sum of the rows of d_out [n, d] (fp32 or bf16) with id r;
+ * 0: d_w is overwritten, zeros in rows without a token. Sums are in fp32 and in one order that n, ids, d and the alignment of
+ * d_out and d_w fix: the same call gives the same bits. workspace (nlh_embedding_backward_bytes, 16-byte aligned) is the caller's. */
 int32_t nlh_embedding_forward(const void* w, int32_t w_is_bf16, const int32_t* ids, void* out, int32_t n, int32_t vocab,
     int32_t d, float scale);
 int64_t nlh_embedding_backward_bytes(int32_t n, int32_t vocab, int32_t d);
@@ -529,7 +529,7 @@ int32_t nlh_embedding_backward(const void* d_out, int32_t d_out_is_bf16, const i
 
 /* ── Distillation from a teacher's top logits (additive, no counterpart in the reference) ──────
  * Beside the cross-entropy above. logits [n, vocab] fp32 or bf16, rows row_stride elements apart; teacher_ids [n, k] and
- * teacher_logits [n, k] (fp32 or bf16), k <= 1024: p = softmax(teacher / temperature) over a row's valid entries (an id outside
+ * teacher_logits [n, k] (fp32 or bf16), k <= 1024, n and vocab <= 2^30: p = softmax(teacher / temperature) over a row's valid entries (an id outside
  * [0, vocab) or a logit of -infinity marks an unused one; an id may occur more than once). target_ids [n] as in the
  * cross-entropy. With n_hard rows that have a target and n_soft rows that have a teacher entry:
  *   loss[0] = hard_weight / n_hard sum (lse(z) - z_target)
@@ -551,7 +551,7 @@ int32_t nlh_distill_backward(const void* logits, int32_t logits_is_bf16, int64_t
  * beside the Delta rule above (core/src/delta_rule.rs), which takes its error before the decay. M [dv, dk]
  * fp32, g = log_retain. k, q [batch, seq, heads_k, dk], v [batch, seq, heads_v, dv] and d_y like v, all bf16 or all fp32
  * (is_bf16), log_retain and theta [batch, seq, heads_v] fp32; strides in elements, the last axis contiguous. Value head
- * h reads key head h / (heads_v / heads_k). dk, dv in 1..128. m_initial [sequences, heads_v, dv, dk] or NULL (zeros).
+ * h reads key head h / (heads_v / heads_k). dk, dv in 1..128, batch * seq <= 2^30. m_initial [sequences, heads_v, dv, dk] or NULL (zeros).
  * y, d_k, d_v, d_q (in the inputs' type) and d_log_retain, d_theta (fp32) are contiguous in the inputs' shapes.
  * Packed batches: batch = 1, n_seqs > 0, seq_starts [n_seqs + 1] on the device, sequence i = tokens
  * seq_starts[i] .. seq_starts[i + 1] - 1. Starts are clamped to [0, seq] and to their running maximum; a sequence may be

@@ -17,7 +17,7 @@
 namespace nlh {
 namespace distill {
 
-constexpr int MAX_K = 1024, MAX_VOCAB = 1 << 30;
+constexpr int MAX_K = 1024, MAX_N = 1 << 30;          // MAX_N: rows, and vocabulary; strided loops stay in 32 bits
 constexpr float LOG2E = 1.4426950408889634f;
 
 struct Args {
@@ -599,8 +599,8 @@ static bool fill(const char* where, Args& A, const void* logits, int64_t row_str
     const char* bad = nullptr;
     A.hard = targets != nullptr && hard_weight != 0.f;
     A.soft = teacher_ids != nullptr && soft_weight != 0.f;
-    if (n < 0 || vocab <= 0 || vocab > MAX_VOCAB || k < 0 || k > MAX_K || row_stride < vocab)
-        bad = "bad dimensions (k is at most 1024, vocab 2^30)";
+    if (n < 0 || n > MAX_N || vocab <= 0 || vocab > MAX_N || k < 0 || k > MAX_K || row_stride < vocab)
+        bad = "bad dimensions (k is at most 1024, n and vocab 2^30)";
     else if (!(temperature > 0.f) || temperature > 1e6f || temperature < 1e-6f) bad = "the temperature must be in [1e-6, 1e6]";
     else if (n > 0 && (!logits || (A.soft && k > 0 && !teacher_logits))) bad = "NULL pointer";
     if (bad) { record_status(NLH_ERR_INVALID_ARG, where, bad); return false; }
@@ -660,7 +660,7 @@ extern "C" {
 
 int64_t nlh_distill_saved_bytes(int32_t n, int32_t vocab)
 {
-    if (n < 0 || vocab <= 0 || vocab > distill::MAX_VOCAB) return -1;
+    if (n < 0 || n > distill::MAX_N || vocab <= 0 || vocab > distill::MAX_N) return -1;
     distill::Args A{};
     A.n = n; A.vocab = vocab;
     distill::divide(A);

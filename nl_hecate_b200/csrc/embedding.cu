@@ -27,6 +27,7 @@ constexpr int BITS = 9, BINS = 1 << BITS;
 constexpr int SORT_THREADS = 256, SORT_ITEMS = 8, SORT_TILE = SORT_THREADS * SORT_ITEMS;
 constexpr int SMALL = 2048;
 constexpr int THREADS = 128;
+constexpr int MAX_N = 1 << 30, MAX_D = 1 << 20;       // tokens, width: strided loops and grids stay in their ranges
 
 template <typename T> struct Vec { static constexpr int N = 16 / sizeof(T); };
 // N elements as they came, and as floats
@@ -635,7 +636,7 @@ int32_t nlh_embedding_forward(const void* w, int32_t w_is_bf16, const int32_t* i
     float scale)
 {
     const char* where = "nlh_embedding_forward";
-    if (n < 0 || vocab <= 0 || d <= 0 || (n > 0 && (!w || !ids || !out))) {
+    if (n < 0 || vocab <= 0 || d <= 0 || d > emb::MAX_D || (n > 0 && (!w || !ids || !out))) {
         record_status(NLH_ERR_INVALID_ARG, where, "bad dimensions or NULL pointer");
         return NLH_ERR_INVALID_ARG;
     }
@@ -655,7 +656,7 @@ int32_t nlh_embedding_forward(const void* w, int32_t w_is_bf16, const int32_t* i
 
 int64_t nlh_embedding_backward_bytes(int32_t n, int32_t vocab, int32_t d)
 {
-    if (n < 0 || n > (1 << 30) || vocab <= 0 || d <= 0 || d > (1 << 20)) return -1;
+    if (n < 0 || n > emb::MAX_N || vocab <= 0 || d <= 0 || d > emb::MAX_D) return -1;
     emb::Plan P;
     return emb::place(P, nullptr, n, vocab, d);
 }

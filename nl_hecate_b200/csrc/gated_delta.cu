@@ -1036,6 +1036,7 @@ __global__ void __launch_bounds__(256, 3) gd_step_kernel(Args A, float* M, const
 }
 
 // ── host ──
+constexpr int MAX_N = 1 << 30;       // tokens, and chunks of all heads: strided loops stay in 32 bits
 static bool fill(const char* where, const nlh_gated_delta_desc* d, Args& A)
 {
     A = Args{};
@@ -1045,7 +1046,7 @@ static bool fill(const char* where, const nlh_gated_delta_desc* d, Args& A)
     else if (d->heads_v % d->heads_k != 0) bad = "heads_v is no multiple of heads_k";
     else if (d->dk < 1 || d->dk > 128 || d->dv < 1 || d->dv > 128) bad = "dk and dv must be in 1..128";
     else if (d->n_seqs > 0 && d->batch != 1) bad = "a packed batch has batch = 1";
-    else if ((long long)d->batch * d->seq >= (1LL << 31)) bad = "batch * seq must stay below 2^31";
+    else if ((long long)d->batch * d->seq > MAX_N || d->n_seqs > MAX_N) bad = "batch * seq and n_seqs are 2^30 at most";
     if (bad) { record_status(NLH_ERR_INVALID_ARG, where, bad); return false; }
     A.batch = d->batch; A.seq = d->seq; A.hk = d->heads_k; A.hv = d->heads_v; A.share = d->heads_v / d->heads_k;
     A.dk = d->dk; A.dv = d->dv; A.n_seqs = d->n_seqs;
@@ -1058,7 +1059,7 @@ static bool fill(const char* where, const nlh_gated_delta_desc* d, Args& A)
     A.scale = d->scale;
     A.nc = (d->seq + C - 1) / C;
     const long long slots = d->n_seqs > 0 ? (long long)d->seq / C + d->n_seqs : (long long)d->batch * A.nc;
-    if (slots * d->heads_v >= (1LL << 31)) { record_status(NLH_ERR_INVALID_ARG, where, "too many chunks"); return false; }
+    if (slots * d->heads_v > MAX_N) { record_status(NLH_ERR_INVALID_ARG, where, "too many chunks"); return false; }
     A.slots = (int)slots;
     return true;
 }

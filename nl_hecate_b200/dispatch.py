@@ -492,7 +492,7 @@ def gated_delta_forward(k, v, q, log_retain, theta, m0=None, seq_starts=None, sc
 def gated_delta_backward(k, v, q, log_retain, theta, saved, d_y, d_m_final=None, seq_starts=None, scale=1.0,
                          want_initial=True):
     """Gradients of gated_delta_forward, which has returned ``saved`` for the same inputs and scale:
-    dict(d_k, d_v, d_q, d_log_retain, d_theta, d_m_initial). d_y like v in type, any strides; d_m_final (gradient
+    dict(d_k, d_v, d_q, d_log_retain, d_theta, d_m_initial). d_y like v in type, strided as v may be; d_m_final (gradient
     of m_final) may be None. Keys shared by several value heads get the sum of their gradients."""
     where = "gated_delta_backward"
     device = _device_of(where, k, v, q, log_retain, theta, saved.buffer, d_y, d_m_final, seq_starts)

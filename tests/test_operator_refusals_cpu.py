@@ -55,12 +55,14 @@ def test_sizes(lib):
     assert lib.nlh_embedding_backward_bytes(1, 10, (1 << 20) + 1) == -1 and lib.nlh_embedding_backward_bytes(0, 10, 1 << 20) == 0
     assert lib.nlh_embedding_backward_bytes(-1, 10, 4) == -1 and lib.nlh_embedding_backward_bytes(1, 0, 4) == -1
     assert lib.nlh_distill_saved_bytes(0, 10) >= 0 and lib.nlh_distill_saved_bytes(-1, 10) == -1
+    assert lib.nlh_distill_saved_bytes((1 << 30) + 1, 1) == -1 and lib.nlh_distill_saved_bytes(1, (1 << 30) + 1) == -1
     # bytes that pass 32 bits
     assert lib.nlh_gated_delta_saved_bytes(C.byref(desc(batch=64, seq=65536, heads_k=16, heads_v=16, dk=128, dv=128))) > 1 << 36
 
 
 @pytest.mark.parametrize("bad", [dict(batch=-1), dict(seq=-1), dict(heads_k=0), dict(heads_v=3), dict(dk=0), dict(dk=129), dict(dv=200),
-                                 dict(n_seqs=-1), dict(n_seqs=3), dict(batch=1 << 20, seq=1 << 12)])
+                                 dict(n_seqs=-1), dict(n_seqs=3), dict(batch=1 << 20, seq=1 << 12),
+                                 dict(batch=1 << 15, seq=(1 << 15) + 1), dict(batch=1, seq=10, n_seqs=(1 << 30) + 1), dict(batch=1 << 29, seq=1)])
 def test_gated_delta_refuses(lib, bad):
     d = desc(**bad)
     p = C.c_void_p(4096)                   # never followed: the descriptor is refused first
@@ -97,7 +99,7 @@ def test_gated_delta_refuses_buffers(lib):
 def test_embedding_refuses(lib):
     p = C.c_void_p(4096)
     assert lib.nlh_embedding_forward(p, 0, p, p, -1, 10, 4, 1.0) == BAD and lib.nlh_embedding_forward(None, 0, p, p, 3, 10, 4, 1.0) == BAD
-    assert lib.nlh_embedding_forward(p, 0, p, p, 3, 0, 4, 1.0) == BAD
+    assert lib.nlh_embedding_forward(p, 0, p, p, 3, 0, 4, 1.0) == BAD and lib.nlh_embedding_forward(p, 0, p, p, 3, 10, (1 << 20) + 1, 1.0) == BAD
     assert lib.nlh_embedding_forward(None, 0, None, None, 0, 10, 4, 1.0) == OK
     f = lib.nlh_embedding_backward
     need = lib.nlh_embedding_backward_bytes(5000, 10, 4)
