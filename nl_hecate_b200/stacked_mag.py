@@ -1188,6 +1188,9 @@ class StackedMAG:
         if (teacher is None) != (self._static_teacher is None):
             raise ValueError("step_graphed: the captured step was made " + ("without" if self._static_teacher is None else "with") +
                              " a teacher")
+        if teacher is not None and [t.shape for t in teacher] != [t.shape for t in self._static_teacher]:
+            raise ValueError(f"step_graphed: the captured step's teacher has shapes {[tuple(t.shape) for t in self._static_teacher]}, "
+                             f"got {[tuple(t.shape) for t in teacher]}")
         self._static_tok.copy_(tokens, non_blocking=True)
         self._static_tgt.copy_(targets, non_blocking=True)
         for dst, src in zip(self._static_teacher or (), teacher or ()):

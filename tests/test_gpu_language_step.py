@@ -76,6 +76,9 @@ def test_graphed_step_equals_eager(with_teacher):
         assert abs(float(la) - float(lb)) <= 1e-3 * abs(float(la))
     with pytest.raises(ValueError, match="teacher"):
         b.step_graphed(tok, tgt, **({} if with_teacher else {"teacher": teacher}))
+    if with_teacher:      # one entry would be broadcast to all of the captured step's
+        with pytest.raises(ValueError, match="shapes"):
+            b.step_graphed(tok, tgt, teacher=tuple(t[..., :1] for t in teacher))
 
 
 def test_unknown_rule_is_refused():
