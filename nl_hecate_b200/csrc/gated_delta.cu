@@ -254,6 +254,7 @@ __global__ void __launch_bounds__(256, DKP == 64 ? 2 : 1) gd_state_fwd_kernel(Ar
     bf *Rs = Ms + 3 * L::PM, *Us = Rs + 3 * L::PR;      // [64][LS]
     __shared__ float4 s_gate[2][C];
     __shared__ float s_w[2][C];
+    __shared__ __align__(8) unsigned long long s_bar;
     const int nsl = A.dvp / NS, sl = blockIdx.x % nsl, p = blockIdx.x / nsl, h = p % A.hv, seq = p / A.hv;
     const int n0 = sl * NS, tid = threadIdx.x, lane = tid & 31, w = tid >> 5, rb = w & 3, hf = w >> 2, g = lane >> 2, t = lane & 3;
     const int slot0 = first_slot(A, seq), count = chunk_count(A, seq);
@@ -303,7 +304,12 @@ __global__ void __launch_bounds__(256, DKP == 64 ? 2 : 1) gd_state_fwd_kernel(Ar
         pk.store(Kb + (L::KB == 1 ? 0 : buf) * IN * L::PK, LK, L::PK);
         if (tid < C) { s_gate[buf][tid] = pg.g; s_w[buf][tid] = pg.g.w * pg.theta; }
     };
-    if (count > 0) { copy_t<256>(Ts, A.tmat + ((long long)slot0 * A.hv + h) * T_BYTES); fetch(0); commit(0); }
+    if (tid == 0) {
+        init_t(&s_bar);
+        if (count > 0) copy_t(Ts, A.tmat + ((long long)slot0 * A.hv + h) * T_BYTES, &s_bar);
+    }
+    bool dead = false;
+    if (count > 0) { fetch(0); commit(0); }
     __syncthreads();
     for (int c = 0; c < count; c++) {
         const int buf = c & 1;
@@ -336,7 +342,7 @@ __global__ void __launch_bounds__(256, DKP == 64 ? 2 : 1) gd_state_fwd_kernel(Ar
                 any |= odd(x.x) | odd(x.y);
                 put2<3>(Rs + row * LS + H * hf + 8 * n + 2 * t, L::PR, x.x, x.y);
             }
-        wait_t();
+        wait_t(&s_bar, buf, dead);
         any = __syncthreads_or(any);
         zero(acc);
         if (any) triangle_by_token<3, NT>(acc, Ts, C * LP, Rs, LS, L::PR, 16 * rb, H * hf);
@@ -352,7 +358,7 @@ __global__ void __launch_bounds__(256, DKP == 64 ? 2 : 1) gd_state_fwd_kernel(Ar
                 put2<3>(Us + row * LS + col, L::PR, wt * a, wt * b);
             }
         __syncthreads();
-        if (c + 1 < count) copy_t<256>(Ts, A.tmat + (tile + A.hv) * T_BYTES);
+        if (tid == 0 && c + 1 < count) copy_t(Ts, A.tmat + (tile + A.hv) * T_BYTES, &s_bar);
         const float gl = s_gate[buf][C - 1].z;
 #pragma unroll
         for (int m = 0; m < MT; m++) {
@@ -554,6 +560,7 @@ __global__ void __launch_bounds__(256, DKP == 64 ? 2 : 1) gd_state_bwd_kernel(Ar
     bf *Rs = Ds + 3 * L::PM, *Us = Rs + 3 * L::PR;
     __shared__ float4 s_gate[2][C];
     __shared__ float s_theta[2][C];
+    __shared__ __align__(8) unsigned long long s_bar;
     const int nsl = A.dvp / NS, sl = blockIdx.x % nsl, p = blockIdx.x / nsl, h = p % A.hv, seq = p / A.hv;
     const int n0 = sl * NS, tid = threadIdx.x, lane = tid & 31, w = tid >> 5, rb = w & 3, hf = w >> 2, g = lane >> 2, t = lane & 3;
     const int slot0 = first_slot(A, seq), count = chunk_count(A, seq);
@@ -604,7 +611,12 @@ __global__ void __launch_bounds__(256, DKP == 64 ? 2 : 1) gd_state_bwd_kernel(Ar
         pk.store(Kb + (L::KB == 1 ? 0 : buf) * IN * L::PK, LK, L::PK);
         if (tid < C) { s_gate[buf][tid] = pg.g; s_theta[buf][tid] = pg.theta; }
     };
-    if (count > 0) { copy_t<256>(Ts, A.tmat + ((long long)(slot0 + count - 1) * A.hv + h) * T_BYTES); fetch(count - 1); commit(0); }
+    if (tid == 0) {
+        init_t(&s_bar);
+        if (count > 0) copy_t(Ts, A.tmat + ((long long)(slot0 + count - 1) * A.hv + h) * T_BYTES, &s_bar);
+    }
+    bool dead = false;
+    if (count > 0) { fetch(count - 1); commit(0); }
     __syncthreads();
     for (int c = count - 1; c >= 0; c--) {
         const int buf = (count - 1 - c) & 1, slot = slot0 + c;
@@ -636,7 +648,7 @@ __global__ void __launch_bounds__(256, DKP == 64 ? 2 : 1) gd_state_bwd_kernel(Ar
                 const float wi = s_gate[buf][row].w, th = s_theta[buf][row];
                 put2<3>(Rs + row * LS + H * hf + 8 * n + 2 * t, L::PR, th * (f[n][r].x + wi * acc[n][2 * r]), th * (f[n][r].y + wi * acc[n][2 * r + 1]));
             }
-        wait_t();
+        wait_t(&s_bar, buf, dead);
         __syncthreads();
         zero(acc);
         gemm<NT, true, true, 3, 3>(acc, Ts + 16 * rb, LP, C * LP, Rs + H * hf, LS, L::PR, 16 * rb, C);
@@ -658,7 +670,7 @@ __global__ void __launch_bounds__(256, DKP == 64 ? 2 : 1) gd_state_bwd_kernel(Ar
                 }
             }
         __syncthreads();
-        if (c > 0) copy_t<256>(Ts, A.tmat + (tile - A.hv) * T_BYTES);
+        if (tid == 0 && c > 0) copy_t(Ts, A.tmat + (tile - A.hv) * T_BYTES, &s_bar);
         const float gl = s_gate[buf][C - 1].z;
 #pragma unroll
         for (int m = 0; m < MT; m++) {
@@ -1259,6 +1271,13 @@ int32_t nlh_gated_delta_backward(const nlh_gated_delta_desc* desc, const void* k
     A.d_g = d_log_retain; A.d_theta = d_theta; A.d_m0 = d_m_initial;
     const bool ok = desc->is_bf16 ? run_backward<__nv_bfloat16>(A, current_stream(), where) : run_backward<float>(A, current_stream(), where);
     return ok ? NLH_OK : NLH_ERR_CUDA;
+}
+
+int32_t nlh_gated_delta_timeout_flag(void)
+{
+    int v = 0;
+    if (cudaMemcpyFromSymbol(&v, g_gd_timeout, sizeof(int)) != cudaSuccess) return -1;
+    return v;
 }
 
 int32_t nlh_gated_delta_step(const nlh_gated_delta_desc* desc, const void* k, const void* v, const void* q,

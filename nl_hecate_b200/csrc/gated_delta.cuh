@@ -432,16 +432,33 @@ template <typename T, int COLS, int THREADS> struct Prefetch {
         }
     }
 };
-// The planes of T, copied as they are, straight into shared memory: issued when the chunk before has no more use for its T, waited
-// for when the next one needs it, half a chunk later.
-template <int THREADS> __device__ __forceinline__ void copy_t(bf* dst, const unsigned char* src)
+// The planes of T, copied as they are, straight into shared memory: one bulk copy by one thread, issued when the chunk before has no
+// more use for its T, waited for when the next one needs it, half a chunk later. (As 16-byte cp.async by all threads the
+// issue alone held the warps up for some 900 cycles of a chunk's 4000.) The wait is bounded: where it runs out the CTA sets
+// g_gd_timeout and carries on with wrong results.
+__device__ int g_gd_timeout = 0;
+constexpr unsigned T_WAIT_LIMIT = 1u << 22;
+__device__ __forceinline__ void init_t(unsigned long long* bar)
 {
-    const unsigned d = smem_addr(dst);
-    for (int i = threadIdx.x; i < T_BYTES / 16; i += THREADS)
-        asm volatile("cp.async.cg.shared.global [%0], [%1], 16;\n" ::"r"(d + 16 * i), "l"(src + 16 * i) : "memory");
-    asm volatile("cp.async.commit_group;\n" ::: "memory");
+    asm volatile("mbarrier.init.shared::cta.b64 [%0], 1;\n" ::"r"(smem_addr(bar)) : "memory");
+    asm volatile("fence.mbarrier_init.release.cluster;\n" ::: "memory");
 }
-__device__ __forceinline__ void wait_t() { asm volatile("cp.async.wait_group 0;\n" ::: "memory"); }
+__device__ __forceinline__ void copy_t(bf* dst, const unsigned char* src, unsigned long long* bar)
+{
+    asm volatile("mbarrier.arrive.expect_tx.shared::cta.b64 _, [%0], %1;\n" ::"r"(smem_addr(bar)), "r"(T_BYTES) : "memory");
+    asm volatile("cp.async.bulk.shared::cluster.global.mbarrier::complete_tx::bytes [%0], [%1], %2, [%3];\n"
+                 ::"r"(smem_addr(dst)), "l"(src), "r"(T_BYTES), "r"(smem_addr(bar)) : "memory");
+}
+__device__ __forceinline__ void wait_t(unsigned long long* bar, unsigned parity, bool& dead)
+{
+    for (unsigned i = 0; !dead; i++) {
+        unsigned ok;
+        asm volatile("{\n\t.reg .pred P;\n\tmbarrier.try_wait.parity.shared::cta.b64 P, [%1], %2;\n\tselp.u32 %0, 1, 0, P;\n\t}\n"
+                     : "=r"(ok) : "r"(smem_addr(bar)), "r"(parity) : "memory");
+        if (ok) return;
+        if (i == T_WAIT_LIMIT) { dead = true; atomicExch(&g_gd_timeout, 1); }
+    }
+}
 
 }  // namespace gd
 }  // namespace nlh
