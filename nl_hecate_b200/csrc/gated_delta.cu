@@ -241,6 +241,14 @@ template <typename T, int DKP, int NS> struct StateSmem {
     static constexpr int BYTES = T_BYTES + 2 * (KB * Pl<T>::in * PK + 3 * PM + 6 * PR);
 };
 struct GateRow { float4 g; float theta; };
+// A sequence: its first token in its batch, its length.
+struct Seq { int b, t0, len; };
+__device__ __forceinline__ Seq get_seq(const Args& A, int seq)
+{
+    if (!A.starts) return Seq{seq, 0, A.seq};
+    const int t0 = A.start[seq];
+    return Seq{0, t0, A.start[seq + 1] - t0};
+}
 
 template <typename T, int DKP, int NS>
 __global__ void __launch_bounds__(256, DKP == 64 ? 2 : 1) gd_state_fwd_kernel(Args A)
@@ -284,20 +292,30 @@ __global__ void __launch_bounds__(256, DKP == 64 ? 2 : 1) gd_state_fwd_kernel(Ar
     Pair<T> pv[NT][2];
     const bool vpair = ((reinterpret_cast<uintptr_t>((const T*)A.v + n0) | (uintptr_t)((A.vb | A.vt | A.vh) * (long long)sizeof(T))) &
                         (2 * sizeof(T) - 1)) == 0 && (A.dv & 1) == 0;
+    const Seq sq = get_seq(A, seq);
+    const long long tile0 = (long long)slot0 * A.hv + h, tok0 = sq.b * A.vb + sq.t0 * A.vt;
+    const int row0 = 16 * rb + g, col0 = H * hf + 2 * t;
+    const T* vp0 = (const T*)A.v + tok0 + h * A.vh + n0 + row0 * A.vt + col0;
+    const float4* gp0 = A.gates + tile0 * C + tid;
+    const float* tp0 = A.theta_eff + tile0 * C + tid;
+    float* mc = A.m_chunk + (tile0 * DKP + row0) * A.dvp + n0 + col0;
+    float* ep = A.e + (tile0 * C + row0) * A.dvp + n0 + col0;
+    const long long v_step = C * A.vt, g_step = (long long)A.hv * C, m_step = (long long)A.hv * DKP * A.dvp, e_step = g_step * A.dvp;
+    pk.init((const T*)A.k + sq.b * A.kb + sq.t0 * A.kt + (h / A.share) * A.kh, A.kt, A.dk);
     auto fetch = [&](int c) {
-        const int slot = slot0 + c;
-        const Chunk ch = get_chunk(A, slot);
-        const long long tile = (long long)slot * A.hv + h;
-        pk.load((const T*)A.k + ch.b * A.kb + ch.t0 * A.kt + (h / A.share) * A.kh, A.kt, ch.len, A.dk);
-        if (tid < C) { ldg(pg.g, reinterpret_cast<const float*>(A.gates + tile * C + tid)); ldg(pg.theta, A.theta_eff + tile * C + tid); }
-        const T* vp = (const T*)A.v + ch.b * A.vb + ch.t0 * A.vt + h * A.vh + n0;
+        const int len = min(C, sq.len - c * C);
+        pk.load(c, len);
+        if (tid < C) { ldg(pg.g, reinterpret_cast<const float*>(gp0 + c * g_step)); ldg(pg.theta, tp0 + c * g_step); }
+        const T* vp = vp0 + c * v_step;
 #pragma unroll
-        for (int n = 0; n < NT; n++)
+        for (int r = 0; r < 2; r++) {
 #pragma unroll
-            for (int r = 0; r < 2; r++) {
-                const int row = 16 * rb + g + 8 * r, col = H * hf + 8 * n + 2 * t;
-                pv[n][r].load(vp + row * A.vt + col, row < ch.len && n0 + col < A.dv, row < ch.len && n0 + col + 1 < A.dv, vpair);
+            for (int n = 0; n < NT; n++) {
+                const int col = n0 + col0 + 8 * n;
+                pv[n][r].load(vp + 8 * n, row0 + 8 * r < len && col < A.dv, row0 + 8 * r < len && col + 1 < A.dv, vpair);
             }
+            vp += 8 * A.vt;
+        }
     };
     auto commit = [&](int buf) {
         if (L::KB == 1) __syncthreads();              // the one buffer of K has been read
@@ -306,26 +324,24 @@ __global__ void __launch_bounds__(256, DKP == 64 ? 2 : 1) gd_state_fwd_kernel(Ar
     };
     if (tid == 0) {
         init_t(&s_bar);
-        if (count > 0) copy_t(Ts, A.tmat + ((long long)slot0 * A.hv + h) * T_BYTES, &s_bar);
+        if (count > 0) copy_t(Ts, A.tmat + tile0 * T_BYTES, &s_bar);
     }
     bool dead = false;
     if (count > 0) { fetch(0); commit(0); }
     __syncthreads();
     for (int c = 0; c < count; c++) {
         const int buf = c & 1;
-        const long long tile = (long long)(slot0 + c) * A.hv + h;
         const bf* Ks = Kb + (L::KB == 1 ? 0 : buf) * IN * L::PK;
         Pair<T> v[NT][2];
-        float* mc = A.m_chunk + tile * DKP * A.dvp + n0;
 #pragma unroll
         for (int n = 0; n < NT; n++)
 #pragma unroll
             for (int r = 0; r < 2; r++) {
                 v[n][r] = pv[n][r];
 #pragma unroll
-                for (int m = 0; m < MT; m++)
-                    st2(mc + (64 * m + 16 * rb + g + 8 * r) * A.dvp + H * hf + 8 * n + 2 * t, S[m][n][2 * r], S[m][n][2 * r + 1]);
+                for (int m = 0; m < MT; m++) st2(mc + (64 * m + 8 * r) * A.dvp + 8 * n, S[m][n][2 * r], S[m][n][2 * r + 1]);
             }
+        mc += m_step;
         if (c + 1 < count) fetch(c + 1);
         float acc[NT][4];
         zero(acc);
@@ -347,18 +363,18 @@ __global__ void __launch_bounds__(256, DKP == 64 ? 2 : 1) gd_state_fwd_kernel(Ar
         zero(acc);
         if (any) triangle_by_token<3, NT>(acc, Ts, C * LP, Rs, LS, L::PR, 16 * rb, H * hf);
         else gemm<NT, false, true, 3, 3>(acc, Ts + 16 * rb * LP, LP, C * LP, Rs + H * hf, LS, L::PR, 0, 16 * (rb + 1));
-        float* ep = A.e + tile * C * A.dvp + n0;
 #pragma unroll
         for (int n = 0; n < NT; n++)
 #pragma unroll
             for (int r = 0; r < 2; r++) {
-                const int row = 16 * rb + g + 8 * r, col = H * hf + 8 * n + 2 * t;
+                const int row = row0 + 8 * r, col = col0 + 8 * n;
                 const float a = acc[n][2 * r], b = acc[n][2 * r + 1], wt = s_w[buf][row];
-                st2(ep + (long long)row * A.dvp + col, a, b);
+                st2(ep + 8 * r * A.dvp + 8 * n, a, b);
                 put2<3>(Us + row * LS + col, L::PR, wt * a, wt * b);
             }
         __syncthreads();
-        if (tid == 0 && c + 1 < count) copy_t(Ts, A.tmat + (tile + A.hv) * T_BYTES, &s_bar);
+        ep += e_step;
+        if (tid == 0 && c + 1 < count) copy_t(Ts, A.tmat + (tile0 + (long long)(c + 1) * A.hv) * T_BYTES, &s_bar);
         const float gl = s_gate[buf][C - 1].z;
 #pragma unroll
         for (int m = 0; m < MT; m++) {
@@ -588,22 +604,28 @@ __global__ void __launch_bounds__(256, DKP == 64 ? 2 : 1) gd_state_bwd_kernel(Ar
     Prefetch<T, DKP, 256> pk;
     GateRow pg;
     float2 pf[NT][2], pn[MT][NT][2];
+    const Seq sq = get_seq(A, seq);
+    const long long tile0 = (long long)slot0 * A.hv + h;
+    const int row0 = 16 * rb + g, col0 = H * hf + 2 * t;
+    const float4* gp0 = A.gates + tile0 * C + tid;
+    const float* tp0 = A.theta_eff + tile0 * C + tid;
+    float* dc0 = A.d_chunk + (tile0 * DKP + row0) * A.dvp + n0 + col0;
+    const float* fp0 = A.f + (tile0 * C + row0) * A.dvp + n0 + col0;
+    float* xp0 = A.x + (tile0 * C + row0) * A.dvp + n0 + col0;
+    const long long dv_row = (long long)A.hv * A.dv, g_step = (long long)A.hv * C, m_step = (long long)A.hv * DKP * A.dvp, e_step = g_step * A.dvp;
+    T* dv0 = (T*)A.d_v + ((long long)sq.b * A.seq + sq.t0 + row0) * dv_row + h * A.dv + n0 + col0;
+    pk.init((const T*)A.k + sq.b * A.kb + sq.t0 * A.kt + (h / A.share) * A.kh, A.kt, A.dk);
     auto fetch = [&](int c) {
-        const int slot = slot0 + c;
-        const Chunk ch = get_chunk(A, slot);
-        const long long tile = (long long)slot * A.hv + h;
-        pk.load((const T*)A.k + ch.b * A.kb + ch.t0 * A.kt + (h / A.share) * A.kh, A.kt, ch.len, A.dk);
-        if (tid < C) { ldg(pg.g, reinterpret_cast<const float*>(A.gates + tile * C + tid)); ldg(pg.theta, A.theta_eff + tile * C + tid); }
-        const float* fp = A.f + tile * C * A.dvp + n0;
-        const float* np = A.d_chunk + tile * DKP * A.dvp + n0;
+        pk.load(c, min(C, sq.len - c * C));
+        if (tid < C) { ldg(pg.g, reinterpret_cast<const float*>(gp0 + c * g_step)); ldg(pg.theta, tp0 + c * g_step); }
+        const float *fp = fp0 + c * e_step, *np = dc0 + c * m_step;
 #pragma unroll
         for (int n = 0; n < NT; n++)
 #pragma unroll
             for (int r = 0; r < 2; r++) {
-                const int row = 16 * rb + g + 8 * r, col = H * hf + 8 * n + 2 * t;
-                ldg(pf[n][r], fp + (long long)row * A.dvp + col);
+                ldg(pf[n][r], fp + 8 * r * A.dvp + 8 * n);
 #pragma unroll
-                for (int m = 0; m < MT; m++) ldg(pn[m][n][r], np + (64 * m + row) * A.dvp + col);
+                for (int m = 0; m < MT; m++) ldg(pn[m][n][r], np + (64 * m + 8 * r) * A.dvp + 8 * n);
             }
     };
     auto commit = [&](int buf) {
@@ -613,18 +635,16 @@ __global__ void __launch_bounds__(256, DKP == 64 ? 2 : 1) gd_state_bwd_kernel(Ar
     };
     if (tid == 0) {
         init_t(&s_bar);
-        if (count > 0) copy_t(Ts, A.tmat + ((long long)(slot0 + count - 1) * A.hv + h) * T_BYTES, &s_bar);
+        if (count > 0) copy_t(Ts, A.tmat + (tile0 + (long long)(count - 1) * A.hv) * T_BYTES, &s_bar);
     }
     bool dead = false;
     if (count > 0) { fetch(count - 1); commit(0); }
     __syncthreads();
     for (int c = count - 1; c >= 0; c--) {
-        const int buf = (count - 1 - c) & 1, slot = slot0 + c;
-        const Chunk ch = get_chunk(A, slot);
-        const long long tile = (long long)slot * A.hv + h;
+        const int buf = (count - 1 - c) & 1, len = min(C, sq.len - c * C);
         const bf* Ks = Kb + (L::KB == 1 ? 0 : buf) * IN * L::PK;
         float2 f[NT][2], nn[MT][NT][2];
-        float* dc = A.d_chunk + tile * DKP * A.dvp + n0;
+        float* dc = dc0 + c * m_step;
 #pragma unroll
         for (int n = 0; n < NT; n++)
 #pragma unroll
@@ -633,7 +653,7 @@ __global__ void __launch_bounds__(256, DKP == 64 ? 2 : 1) gd_state_bwd_kernel(Ar
 #pragma unroll
                 for (int m = 0; m < MT; m++) {
                     nn[m][n][r] = pn[m][n][r];
-                    st2(dc + (64 * m + 16 * rb + g + 8 * r) * A.dvp + H * hf + 8 * n + 2 * t, S[m][n][2 * r], S[m][n][2 * r + 1]);
+                    st2(dc + (64 * m + 8 * r) * A.dvp + 8 * n, S[m][n][2 * r], S[m][n][2 * r + 1]);
                 }
             }
         if (c > 0) fetch(c - 1);
@@ -652,25 +672,25 @@ __global__ void __launch_bounds__(256, DKP == 64 ? 2 : 1) gd_state_bwd_kernel(Ar
         __syncthreads();
         zero(acc);
         gemm<NT, true, true, 3, 3>(acc, Ts + 16 * rb, LP, C * LP, Rs + H * hf, LS, L::PR, 16 * rb, C);
-        float* xp = A.x + tile * C * A.dvp + n0;
-        T* dv = (T*)A.d_v + (ch.row0(A) * A.hv + h) * A.dv + n0;
+        float* xp = xp0 + c * e_step;
+        T* dv = dv0 + c * (C * dv_row);
 #pragma unroll
         for (int n = 0; n < NT; n++)
 #pragma unroll
             for (int r = 0; r < 2; r++) {
-                const int row = 16 * rb + g + 8 * r, col = H * hf + 8 * n + 2 * t;
+                const int row = row0 + 8 * r, col = col0 + 8 * n;
                 const float a = acc[n][2 * r], b = acc[n][2 * r + 1], eg = -s_gate[buf][row].z;
-                st2(xp + (long long)row * A.dvp + col, a, b);
+                st2(xp + 8 * r * A.dvp + 8 * n, a, b);
                 put2<3>(Us + row * LS + col, L::PR, eg * a, eg * b);
-                if (row < ch.len) {
+                if (row < len) {
                     const bool none = fabsf(s_theta[buf][row]) <= THETA_TINY;     // theta was 0: so is the gradient of v
-                    T* o = dv + (long long)row * A.hv * A.dv + col;
+                    T* o = dv + 8 * r * dv_row + 8 * n;
                     if (n0 + col < A.dv) o[0] = from_f<T>(none ? 0.f : a);
                     if (n0 + col + 1 < A.dv) o[1] = from_f<T>(none ? 0.f : b);
                 }
             }
         __syncthreads();
-        if (tid == 0 && c > 0) copy_t(Ts, A.tmat + (tile - A.hv) * T_BYTES, &s_bar);
+        if (tid == 0 && c > 0) copy_t(Ts, A.tmat + (tile0 + (long long)(c - 1) * A.hv) * T_BYTES, &s_bar);
         const float gl = s_gate[buf][C - 1].z;
 #pragma unroll
         for (int m = 0; m < MT; m++) {

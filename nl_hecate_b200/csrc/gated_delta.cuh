@@ -401,35 +401,40 @@ template <> struct Pair<bf> {
 };
 
 // A tile of an input on its way from global to shared memory, in registers: loaded while the chunk before it is computed. Rows
-// that do not allow vector loads are read when they are stored instead.
+// that do not allow vector loads are read when they are stored instead. Addresses are a thread's own, made once: with 64-bit products and
+// divisions in the loop they were a quarter of a chunk's time, since few warps share a scheduler.
 template <typename T, int COLS, int THREADS> struct Prefetch {
     typedef typename Raw<T>::type R;
-    static constexpr int PER_ROW = COLS / 4, N = C * PER_ROW / THREADS;
+    static constexpr int PER_ROW = COLS / 4, ROWS = THREADS / PER_ROW, N = C / ROWS;
     R r[N];
-    const T* base;
+    const T *base, *mine;                // chunk 0; this thread's part of it
     long long stride;
-    int rows, cols;
-    bool vec;
-    __device__ __forceinline__ void load(const T* b, long long st, int nr, int nc)
+    int cols, chunk, rows;
+    bool vec, has;
+    __device__ __forceinline__ void init(const T* b, long long st, int nc)
     {
-        base = b; stride = st; rows = nr; cols = nc;
+        base = b; stride = st; cols = nc;
         vec = vec_ok(b, st, nc);
-        if (!vec) return;
+        const int c = (threadIdx.x % PER_ROW) * 4;
+        has = vec && c < nc;
+        mine = b + threadIdx.x / PER_ROW * st + c;
+    }
+    __device__ __forceinline__ void load(int c, int nr)
+    {
+        chunk = c; rows = nr;
+        const T* p = mine + c * (C * stride);
 #pragma unroll
         for (int i = 0; i < N; i++) {
-            const int at = threadIdx.x + i * THREADS, row = at / PER_ROW, c = (at - row * PER_ROW) * 4;
             r[i] = R{};
-            if (row < rows && c < cols) ldg(r[i], base + row * stride + c);
+            if (has && threadIdx.x / PER_ROW + i * ROWS < nr) ldg(r[i], p);
+            p += ROWS * stride;
         }
     }
     __device__ __forceinline__ void store(bf* dst, int ld, int ps) const
     {
-        if (!vec) { load_tile<T, COLS, THREADS>(dst, ld, ps, base, stride, rows, cols); return; }
+        if (!vec) { load_tile<T, COLS, THREADS>(dst, ld, ps, base + chunk * (C * stride), stride, rows, cols); return; }
 #pragma unroll
-        for (int i = 0; i < N; i++) {
-            const int at = threadIdx.x + i * THREADS, row = at / PER_ROW, c = (at - row * PER_ROW) * 4;
-            put_raw(dst + row * ld + c, ps, r[i]);
-        }
+        for (int i = 0; i < N; i++) put_raw(dst + (threadIdx.x / PER_ROW + i * ROWS) * ld + (threadIdx.x % PER_ROW) * 4, ps, r[i]);
     }
 };
 // The planes of T, copied as they are, straight into shared memory: one bulk copy by one thread, issued when the chunk before has no
