@@ -605,20 +605,16 @@ __global__ void __launch_bounds__(256, DKP == 64 ? 2 : 1) gd_state_bwd_kernel(Ar
     GateRow pg;
     float2 pf[NT][2], pn[MT][NT][2];
     const Seq sq = get_seq(A, seq);
-    const long long tile0 = (long long)slot0 * A.hv + h;
     const int row0 = 16 * rb + g, col0 = H * hf + 2 * t;
-    const float4* gp0 = A.gates + tile0 * C + tid;
-    const float* tp0 = A.theta_eff + tile0 * C + tid;
-    float* dc0 = A.d_chunk + (tile0 * DKP + row0) * A.dvp + n0 + col0;
-    const float* fp0 = A.f + (tile0 * C + row0) * A.dvp + n0 + col0;
-    float* xp0 = A.x + (tile0 * C + row0) * A.dvp + n0 + col0;
     const long long dv_row = (long long)A.hv * A.dv, g_step = (long long)A.hv * C, m_step = (long long)A.hv * DKP * A.dvp, e_step = g_step * A.dvp;
-    T* dv0 = (T*)A.d_v + ((long long)sq.b * A.seq + sq.t0 + row0) * dv_row + h * A.dv + n0 + col0;
+    long long tile = (long long)(slot0 + count - 1) * A.hv + h, g_at = tile * C + tid;     // of the chunk that is computed
+    long long m_at = (tile * DKP + row0) * A.dvp + n0 + col0, e_at = (tile * C + row0) * A.dvp + n0 + col0;
+    T* dv = (T*)A.d_v + ((long long)sq.b * A.seq + sq.t0 + (long long)(count - 1) * C + row0) * dv_row + h * A.dv + n0 + col0;
     pk.init((const T*)A.k + sq.b * A.kb + sq.t0 * A.kt + (h / A.share) * A.kh, A.kt, A.dk);
-    auto fetch = [&](int c) {
+    auto fetch = [&](int c, long long ga, long long ea, long long ma) {
         pk.load(c, min(C, sq.len - c * C));
-        if (tid < C) { ldg(pg.g, reinterpret_cast<const float*>(gp0 + c * g_step)); ldg(pg.theta, tp0 + c * g_step); }
-        const float *fp = fp0 + c * e_step, *np = dc0 + c * m_step;
+        if (tid < C) { ldg(pg.g, reinterpret_cast<const float*>(A.gates + ga)); ldg(pg.theta, A.theta_eff + ga); }
+        const float *fp = A.f + ea, *np = A.d_chunk + ma;
 #pragma unroll
         for (int n = 0; n < NT; n++)
 #pragma unroll
@@ -635,16 +631,16 @@ __global__ void __launch_bounds__(256, DKP == 64 ? 2 : 1) gd_state_bwd_kernel(Ar
     };
     if (tid == 0) {
         init_t(&s_bar);
-        if (count > 0) copy_t(Ts, A.tmat + (tile0 + (long long)(count - 1) * A.hv) * T_BYTES, &s_bar);
+        if (count > 0) copy_t(Ts, A.tmat + tile * T_BYTES, &s_bar);
     }
     bool dead = false;
-    if (count > 0) { fetch(count - 1); commit(0); }
+    if (count > 0) { fetch(count - 1, g_at, e_at, m_at); commit(0); }
     __syncthreads();
     for (int c = count - 1; c >= 0; c--) {
         const int buf = (count - 1 - c) & 1, len = min(C, sq.len - c * C);
         const bf* Ks = Kb + (L::KB == 1 ? 0 : buf) * IN * L::PK;
         float2 f[NT][2], nn[MT][NT][2];
-        float* dc = dc0 + c * m_step;
+        float* dc = A.d_chunk + m_at;
 #pragma unroll
         for (int n = 0; n < NT; n++)
 #pragma unroll
@@ -656,7 +652,7 @@ __global__ void __launch_bounds__(256, DKP == 64 ? 2 : 1) gd_state_bwd_kernel(Ar
                     st2(dc + (64 * m + 8 * r) * A.dvp + 8 * n, S[m][n][2 * r], S[m][n][2 * r + 1]);
                 }
             }
-        if (c > 0) fetch(c - 1);
+        if (c > 0) fetch(c - 1, g_at - g_step, e_at - e_step, m_at - m_step);
         float acc[NT][4];
         zero(acc);
         gemm<NT, false, true, IN, 3>(acc, Ks + 16 * rb * LK, LK, L::PK, Ds + H * hf, LS, L::PM, 0, DKP);
@@ -672,8 +668,7 @@ __global__ void __launch_bounds__(256, DKP == 64 ? 2 : 1) gd_state_bwd_kernel(Ar
         __syncthreads();
         zero(acc);
         gemm<NT, true, true, 3, 3>(acc, Ts + 16 * rb, LP, C * LP, Rs + H * hf, LS, L::PR, 16 * rb, C);
-        float* xp = xp0 + c * e_step;
-        T* dv = dv0 + c * (C * dv_row);
+        float* xp = A.x + e_at;
 #pragma unroll
         for (int n = 0; n < NT; n++)
 #pragma unroll
@@ -690,7 +685,12 @@ __global__ void __launch_bounds__(256, DKP == 64 ? 2 : 1) gd_state_bwd_kernel(Ar
                 }
             }
         __syncthreads();
-        if (tid == 0 && c > 0) copy_t(Ts, A.tmat + (tile0 + (long long)(c - 1) * A.hv) * T_BYTES, &s_bar);
+        tile -= A.hv;
+        g_at -= g_step;
+        e_at -= e_step;
+        m_at -= m_step;
+        dv -= C * dv_row;
+        if (tid == 0 && c > 0) copy_t(Ts, A.tmat + tile * T_BYTES, &s_bar);
         const float gl = s_gate[buf][C - 1].z;
 #pragma unroll
         for (int m = 0; m < MT; m++) {
