@@ -587,6 +587,8 @@ int32_t nlh_gated_delta_backward(const nlh_gated_delta_desc* desc, const void* k
  * [0, n_slots) is no sequence: its rows of y are zeros. A slot named more than once is stepped in the order of the batch. */
 int32_t nlh_gated_delta_step(const nlh_gated_delta_desc* desc, const void* k, const void* v, const void* q,
     const float* log_retain, const float* theta, float* m, const int32_t* slots, int32_t n_slots, void* y);
+/* 1 once a wait of the state kernels for their copies has run out (its results are wrong), 0 otherwise; synchronous. */
+int32_t nlh_gated_delta_timeout_flag(void);
 
 /* ── Host-slice dispatch layer (compiled counterpart of core/src/dispatch.rs `*_dispatch`) ────
  * Same argument order and meaning as the reference functions its kernel tests call

@@ -28,6 +28,7 @@ __device__ __forceinline__ int block_scan(int v, bool take_max, int* s_warp)
     for (int j = 0; j < w; j++) v = take_max ? max(v, s_warp[j]) : v + s_warp[j];
     return v;
 }
+constexpr int RANKED = 256;
 __global__ void __launch_bounds__(1024) gd_map_kernel(Args A)
 {
     __shared__ int s_warp[32], s_last;
@@ -46,6 +47,20 @@ __global__ void __launch_bounds__(1024) gd_map_kernel(Args A)
             carry = s_last;
             __syncthreads();
         }
+    }
+    // The state kernels begin long sequences first: their chains are what a pass waits for. (13 prompts x 8 heads, the longest the last in
+    // the batch: 72 + 80 us against 84 + 94 in the batch's order; 40 prompts: 94 + 114 against 122 + 145.) Many sequences even out by themselves.
+    __shared__ int s_len[RANKED];
+    const bool ranked = A.n_seqs <= RANKED;
+    if (ranked && threadIdx.x < A.n_seqs) s_len[threadIdx.x] = A.off[threadIdx.x + 1] - A.off[threadIdx.x];
+    __syncthreads();
+    for (int i = threadIdx.x; i < A.n_seqs; i += 1024) {
+        int rank = i;
+        if (ranked) {
+            rank = 0;
+            for (int j = 0; j < A.n_seqs; j++) rank += s_len[j] > s_len[i] || (s_len[j] == s_len[i] && j < i);
+        }
+        A.order[rank] = i;
     }
     for (int slot = threadIdx.x; slot < A.slots; slot += 1024) {
         int lo = 0, hi = A.n_seqs;                  // off[lo] <= slot; the last such lo
@@ -231,8 +246,8 @@ __global__ void __launch_bounds__(256, 3) gd_prep_kernel(Args A)
 
 // ── forward states: the recurrence over chunks for NS columns of V ──
 // Eight warps: warp = 16 rows (tokens; state rows of each 64 of dk in the update) x half of the columns. The state (transposed, S
-// [dk, dv]) stays in the update's accumulators from chunk to chunk. While a chunk is computed the next one's K, T, V and gates are
-// on their way in registers. Bound by the chain of three products of 64 x NS x 64 a chunk: NS = 32 shares the loads of K and T
+// [dk, dv]) stays in the update's accumulators from chunk to chunk. While a chunk is computed the next one's K, V and gates are
+// on their way in registers, and its T in a bulk copy. Bound by the chain of three products of 64 x NS x 64 a chunk: NS = 32 shares the loads of K and T
 // among more columns, NS = 16 gives twice the CTAs where heads are few. A bf16 K has two buffers, so that only the
 // products' own barriers are left; three planes of a fp32 one have one buffer, which lets two CTAs share an SM.
 template <typename T, int DKP, int NS> struct StateSmem {
@@ -263,7 +278,7 @@ __global__ void __launch_bounds__(256, DKP == 64 ? 2 : 1) gd_state_fwd_kernel(Ar
     __shared__ float4 s_gate[2][C];
     __shared__ float s_w[2][C];
     __shared__ __align__(8) unsigned long long s_bar;
-    const int nsl = A.dvp / NS, sl = blockIdx.x % nsl, p = blockIdx.x / nsl, h = p % A.hv, seq = p / A.hv;
+    const int nsl = A.dvp / NS, sl = blockIdx.x % nsl, p = blockIdx.x / nsl, h = p % A.hv, seq = A.starts ? A.order[p / A.hv] : p / A.hv;
     const int n0 = sl * NS, tid = threadIdx.x, lane = tid & 31, w = tid >> 5, rb = w & 3, hf = w >> 2, g = lane >> 2, t = lane & 3;
     const int slot0 = first_slot(A, seq), count = chunk_count(A, seq);
 
@@ -577,7 +592,7 @@ __global__ void __launch_bounds__(256, DKP == 64 ? 2 : 1) gd_state_bwd_kernel(Ar
     __shared__ float4 s_gate[2][C];
     __shared__ float s_theta[2][C];
     __shared__ __align__(8) unsigned long long s_bar;
-    const int nsl = A.dvp / NS, sl = blockIdx.x % nsl, p = blockIdx.x / nsl, h = p % A.hv, seq = p / A.hv;
+    const int nsl = A.dvp / NS, sl = blockIdx.x % nsl, p = blockIdx.x / nsl, h = p % A.hv, seq = A.starts ? A.order[p / A.hv] : p / A.hv;
     const int n0 = sl * NS, tid = threadIdx.x, lane = tid & 31, w = tid >> 5, rb = w & 3, hf = w >> 2, g = lane >> 2, t = lane & 3;
     const int slot0 = first_slot(A, seq), count = chunk_count(A, seq);
 
@@ -1111,6 +1126,7 @@ static int64_t place_saved(Args& A, char* base)
         A.map = (int4*)take((int64_t)A.slots * 16);
         A.start = (int*)take((int64_t)(A.n_seqs + 1) * 4);
         A.off = (int*)take((int64_t)(A.n_seqs + 1) * 4);
+        A.order = (int*)take((int64_t)A.n_seqs * 4);
     }
     return at;
 }
@@ -1163,10 +1179,10 @@ template <typename T, int DKP> static bool launch_states(const Args& A, bool bac
 {
     const long long heads = (long long)(A.n_seqs > 0 ? A.n_seqs : A.batch) * A.hv;
     if (heads == 0) return true;
-    // 16 columns a CTA while 32 would leave SMs without one (2 x 8 heads of 128 x 128: 45 + 51 us against 65 + 76; at 128 CTAs of 32
-    // columns, 4 x 16 heads of 64 x 64, both take 440), and for packed batches longer, since their few longest sequences run
-    // alone in the end (13 prompts x 8 heads: 99 us against 138)
-    if (heads * (A.dvp / 32) < (A.n_seqs > 0 ? 4 * 148 : 128)) return launch_states_ns<T, DKP, 16>(A, heads, backward, st, where);
+    // 16 columns a CTA while each of those CTAs finds an SM of its own (forward + backward, 2 x 8 heads of 128 x 128: 39 + 43 us against
+    // 60 + 69 with 32 columns; 3 x 16 of 64 x 64, which does not: 83 + 99 against 80 + 93), and for packed batches longer, since
+    // their few longest sequences run alone in the end (13 prompts x 8 heads: 72 + 80 us against 95 + 111)
+    if (A.n_seqs > 0 ? heads * (A.dvp / 32) < 4 * 148 : heads * (A.dvp / 16) <= 148) return launch_states_ns<T, DKP, 16>(A, heads, backward, st, where);
     return launch_states_ns<T, DKP, 32>(A, heads, backward, st, where);
 }
 

@@ -49,6 +49,7 @@ struct Args {
     float* m_chunk;                    // [slot, hv, dkp, dvp] state in front of the chunk, transposed
     int4* map;                         // [slot] {sequence, first token, length, -} of a ragged batch
     int *start, *off;                  // [n_seqs + 1] first token and first slot of each sequence
+    int *order;                        // [n_seqs] sequences in the order in which the state kernels begin them
     void* y;
     float* m_final;
     // backward

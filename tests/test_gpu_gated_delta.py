@@ -479,3 +479,19 @@ def test_refusals():
     with pytest.raises(RuntimeError, match="fewer states"):
         D.gated_delta_step(*a, m[:1])
     D.gated_delta_step(*a, m)          # and the library goes on working
+
+
+def test_sequences_of_many_lengths_in_any_order_and_no_wait_ran_out():
+    """The order in which sequences are begun (longest first up to 256 of them, else as they come) does not show: the same bits as
+    each sequence by itself."""
+    from nl_hecate_b200 import dispatch as D, ffi
+    for n in (5, 256, 257):
+        lengths = tuple((37 * i) % 200 for i in range(n))
+        p, starts, at = packed(lengths, 1, 1, 64, 64, torch.bfloat16)
+        y, m, _ = D.gated_delta_forward(p["k"], p["v"], p["q"], p["log_retain"], p["theta"], m0=p["m0"], seq_starts=starts)
+        begin = starts.tolist()
+        for i in {0, 1, n // 2, n - 1}:
+            cut = lambda x: p[x][:, begin[i]:begin[i + 1]].contiguous()
+            y1, m1, _ = D.gated_delta_forward(cut("k"), cut("v"), cut("q"), cut("log_retain"), cut("theta"), m0=p["m0"][i:i + 1].contiguous())
+            assert torch.equal(y[:, begin[i]:begin[i + 1]], y1) and torch.equal(m[i:i + 1], m1)
+    assert ffi.lib().nlh_gated_delta_timeout_flag() == 0
