@@ -438,22 +438,17 @@ __device__ __forceinline__ void store_rows(T* out, const float (&acc)[4][4], int
 }
 
 // ── forward outputs ──
-// Four warps: warp = 32 tokens x 32 of the tile's 64 columns. For bf16 the state, P and U are two planes: y is rounded to bf16.
-// Two places in shared memory, Q then P, and K, then S, then U: four CTAs share an SM and cover each other's loads. 4096 tiles
-// fp32: 143 us (bf16: 92); eight warps of 16 x 32, which read a third more from shared memory, 152 (106); those with three places and two
+// Four warps: warp = 32 tokens x 32 of the tile's 64 columns. Two places in shared memory, Q then P, and K, then S, then U: four
+// CTAs share an SM and cover each other's loads. 4096 tiles fp32: 143 us; eight warps of 16 x 32, which read a third more from shared memory, 152; those with three places and two
 // CTAs 166, with three CTAs and the next tile on its way in registers 174.
-template <typename T> struct OutFwdSmem {
-    static constexpr int PS = C * LP, IN = Pl<T>::in, O = Pl<T>::out, M = IN > O ? IN : O;
-    static constexpr int BYTES = 2 * PS * 2 * M;
-};
+constexpr int OUT_FWD_BYTES = 2 * 3 * C * LP * 2;
 template <typename T>
 __global__ void __launch_bounds__(128, 4) gd_out_fwd_kernel(Args A)
 {
-    typedef OutFwdSmem<T> L;
-    constexpr int PS = L::PS, IN = L::IN, O = L::O;
+    constexpr int PS = C * LP, IN = Pl<T>::in;
     extern __shared__ float4 smem4[];
     bf* Qs = reinterpret_cast<bf*>(smem4);
-    bf* Ks = Qs + L::M * PS;
+    bf* Ks = Qs + 3 * PS;
     __shared__ float4 s_gate[C];
     __shared__ float s_theta[C];
     const int slot = blockIdx.x / A.hv, h = blockIdx.x - slot * A.hv, n0 = blockIdx.y * 64;
@@ -475,9 +470,9 @@ __global__ void __launch_bounds__(128, 4) gd_out_fwd_kernel(Args A)
         __syncthreads();
         if (need) gemm_2<4, false, false, IN, IN>(att, Qs + 32 * rb * LP, LP, PS, Ks + 32 * hf * LP, LP, PS, 0, 64);
         __syncthreads();
-        load_own<O, 128>(Ks, A.m_chunk + (tile * A.dkp + c0) * A.dvp + n0, A.dvp);
+        load_own<3, 128>(Ks, A.m_chunk + (tile * A.dkp + c0) * A.dvp + n0, A.dvp);
         __syncthreads();
-        gemm_2<4, false, true, IN, O>(y, Qs + 32 * rb * LP, LP, PS, Ks + 32 * hf, LP, PS, 0, 64);
+        gemm_2<4, false, true, IN, 3>(y, Qs + 32 * rb * LP, LP, PS, Ks + 32 * hf, LP, PS, 0, 64);
     }
     __syncthreads();
 #pragma unroll
@@ -493,13 +488,13 @@ __global__ void __launch_bounds__(128, 4) gd_out_fwd_kernel(Args A)
                 x[e] = j + e <= i ? decay(make_float2(gi.x, gi.y), make_float2(gj.x, gj.y)) * A.scale * att[m][n][o + e] : 0.f;
                 y[m][n][o + e] *= A.scale * gi.z;
             }
-            put2<O>(Qs + i * LP + j, PS, x[0], x[1]);
+            put2<3>(Qs + i * LP + j, PS, x[0], x[1]);
         }
-    const bool any = load_own<O, 128>(Ks, A.e + tile * C * A.dvp + n0, A.dvp, s_theta);
+    const bool any = load_own<3, 128>(Ks, A.e + tile * C * A.dvp + n0, A.dvp, s_theta);
     if (__syncthreads_or(any)) {
-        triangle_by_token<O, 4>(y[0], Qs, PS, Ks, LP, PS, 32 * rb, 32 * hf);
-        triangle_by_token<O, 4>(y[1], Qs, PS, Ks, LP, PS, 32 * rb + 16, 32 * hf);
-    } else gemm_2<4, false, true, O, O>(y, Qs + 32 * rb * LP, LP, PS, Ks + 32 * hf, LP, PS, 0, 32 * (rb + 1));
+        triangle_by_token<3, 4>(y[0], Qs, PS, Ks, LP, PS, 32 * rb, 32 * hf);
+        triangle_by_token<3, 4>(y[1], Qs, PS, Ks, LP, PS, 32 * rb + 16, 32 * hf);
+    } else gemm_2<4, false, true, 3, 3>(y, Qs + 32 * rb * LP, LP, PS, Ks + 32 * hf, LP, PS, 0, 32 * (rb + 1));
     T* out = (T*)A.y + (ch.row0(A) * A.hv + h) * A.dv;
     store_rows<T>(out, y[0], 32 * rb, ch.len, n0 + 32 * hf, A.dv, (long long)A.hv * A.dv);
     store_rows<T>(out, y[1], 32 * rb + 16, ch.len, n0 + 32 * hf, A.dv, (long long)A.hv * A.dv);
@@ -1201,9 +1196,8 @@ template <typename T> static bool run_forward(Args& A, cudaStream_t st, const ch
     }
     if (!(A.dkp == 64 ? launch_states<T, 64>(A, false, st, where) : launch_states<T, 128>(A, false, st, where))) return false;
     if (tiles) {
-        constexpr int bytes = OutFwdSmem<T>::BYTES;
-        if (!allow_smem<gd_out_fwd_kernel<T>, bytes>(where)) return false;
-        gd_out_fwd_kernel<T><<<dim3(tiles, A.dvp / 64), 128, bytes, st>>>(A);
+        if (!allow_smem<gd_out_fwd_kernel<T>, OUT_FWD_BYTES>(where)) return false;
+        gd_out_fwd_kernel<T><<<dim3(tiles, A.dvp / 64), 128, OUT_FWD_BYTES, st>>>(A);
         if (!check_launch(where)) return false;
     }
     return true;

@@ -10,8 +10,9 @@
 //
 // Products run on the tensor cores in bf16 (mma.sync m16n8k16) with fp32 sums. A fp32 operand is split into three bf16 planes
 // (24 significand bits) when it is written to shared memory, and a product of two such takes six passes, smallest terms
-// first; an operand that came in as bf16 is one plane, exact. A result that is rounded to bf16 is computed from two planes
-// (16 bits against the result's 8). Two tf32 numbers for a fp32 one take the same time on the tensor cores, but their splitting,
+// first; an operand that came in as bf16 is one plane, exact. So the bf16 form computes what the fp32 form computes from the same
+// values, and rounds it once. (Two planes for the operands of a bf16 y, whose own rounding hides the difference, saved 1 to 4 % of a
+// pass, but then a prompt's y and the recurrent step's, which works in fp32, were of different accuracy.) Two tf32 numbers for a fp32 one take the same time on the tensor cores, but their splitting,
 // redone by every warp that reads them, and twice the instructions around each pass cost more: a training step of 64 sequences
 // x 8 heads x 512 tokens took 1435 us that way against 1308 (4 x 16 x 4096 in bf16: 1336 against 1122).
 // Why not tcgen05: the matrices are 64 x 64 x 64 and each depends on the one before it. One M64 N64 K16 tcgen05.mma takes 55
@@ -105,8 +106,8 @@ __device__ __forceinline__ float4 ld4(const __nv_bfloat16* p)
 
 // ── bf16 planes in shared memory ──
 typedef __nv_bfloat16 bf;
-template <typename T> struct Pl { static constexpr int in = 3, out = 3; };      // planes of an input, of an operand of y
-template <> struct Pl<__nv_bfloat16> { static constexpr int in = 1, out = 2; };
+template <typename T> struct Pl { static constexpr int in = 3; };      // planes of an input
+template <> struct Pl<__nv_bfloat16> { static constexpr int in = 1; };
 
 __device__ __forceinline__ unsigned pack2(float x, float y)
 {
