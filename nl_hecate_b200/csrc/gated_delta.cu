@@ -1221,8 +1221,8 @@ template <typename T> static bool run_backward(Args& A, cudaStream_t st, const c
         gd_gate_bwd_kernel<<<(tiles + 3) / 4, 128, 0, st>>>(A);
         if (!check_launch(where)) return false;
     }
-    if (A.share > 1) {
-        const long long n = (long long)A.batch * A.seq * A.hk * A.dk;
+    const long long n = (long long)A.batch * A.seq * A.hk * A.dk;
+    if (A.share > 1 && n > 0) {                   // a packed batch without a token has chunk slots, but no rows
         const long long need = (n + 255) / 256;
         gd_group_kernel<T><<<(unsigned)(need < 148 * 16 ? need : 148 * 16), 256, 0, st>>>(A, n);
         if (!check_launch(where)) return false;

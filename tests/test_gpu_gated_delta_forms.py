@@ -23,3 +23,15 @@ def test_bf16_is_the_fp32_form_rounded_once(b, s, hk, hv, dk, dv):
     got, want = run(p, 0.5), run(wide, 0.5)
     for x in want:
         assert torch.equal(got[x], want[x].to(got[x].dtype)), (x, float((got[x].double() - want[x].double()).abs().max()))
+
+
+@pytest.mark.parametrize("dtype", [torch.float32, torch.bfloat16])
+@pytest.mark.parametrize("hk,hv", [(2, 2), (2, 4)])
+def test_packed_batch_without_a_token(hk, hv, dtype):
+    """Sequences that are all empty, in a batch of no tokens: the states and their gradients pass through."""
+    p = inputs(1, 0, hk, hv, 64, 48, dtype)
+    p["m0"], p["d_m"] = torch.randn(2, hv, 48, 64, device="cuda"), torch.randn(2, hv, 48, 64, device="cuda")
+    out = run(p, starts=torch.zeros(3, dtype=torch.int32, device="cuda"))
+    assert torch.equal(out["m_final"], p["m0"]) and torch.equal(out["d_m_initial"], p["d_m"])
+    for x in ("y", "d_k", "d_v", "d_q", "d_log_retain", "d_theta"):
+        assert out[x].numel() == 0, x
