@@ -1273,7 +1273,8 @@ int32_t nlh_gated_delta_forward(const nlh_gated_delta_desc* desc, const void* k,
     Args A;
     if (!gd_inputs(where, A, desc, k, v, q, log_retain, theta, seq_starts)) return NLH_ERR_INVALID_ARG;
     const bool tokens = (long long)A.batch * A.seq > 0;
-    if ((tokens && !y) || (!m_final && (A.n_seqs > 0 || A.batch > 0)) || ((uintptr_t)saved & 15) || saved_bytes < place_saved(A, (char*)saved) || (tokens && !saved)) {
+    const int64_t need = place_saved(A, (char*)saved);       // a packed batch has chunk slots without a token too
+    if ((tokens && !y) || (!m_final && (A.n_seqs > 0 || A.batch > 0)) || ((uintptr_t)saved & 15) || saved_bytes < need || (need > 0 && !saved)) {
         record_status(NLH_ERR_INVALID_ARG, where, "NULL output, or a saved buffer that is too small or not 16-byte aligned");
         return NLH_ERR_INVALID_ARG;
     }
@@ -1291,9 +1292,9 @@ int32_t nlh_gated_delta_backward(const nlh_gated_delta_desc* desc, const void* k
     Args A;
     if (!gd_inputs(where, A, desc, k, v, q, log_retain, theta, seq_starts)) return NLH_ERR_INVALID_ARG;
     const bool tokens = (long long)A.batch * A.seq > 0;
-    if ((tokens && (!d_y || !d_k || !d_v || !d_q || !d_log_retain || !d_theta || !saved || !workspace)) ||
-        (((uintptr_t)saved | (uintptr_t)workspace) & 15) || saved_bytes < place_saved(A, (char*)saved) ||
-        workspace_bytes < place_bwd(A, (char*)workspace)) {
+    const int64_t need_saved = place_saved(A, (char*)saved), need_work = place_bwd(A, (char*)workspace);
+    if ((tokens && (!d_y || !d_k || !d_v || !d_q || !d_log_retain || !d_theta)) || (need_saved > 0 && !saved) || (need_work > 0 && !workspace) ||
+        (((uintptr_t)saved | (uintptr_t)workspace) & 15) || saved_bytes < need_saved || workspace_bytes < need_work) {
         record_status(NLH_ERR_INVALID_ARG, where, "NULL pointer, or a buffer that is too small or not 16-byte aligned");
         return NLH_ERR_INVALID_ARG;
     }

@@ -96,6 +96,18 @@ def test_gated_delta_refuses_buffers(lib):
     assert s(C.byref(d), p, p, p, p, p, p, p, -1, p) == BAD
 
 
+def test_packed_batch_without_a_token_needs_its_buffers(lib):
+    """It has chunk slots to number although it has no rows: a NULL buffer of the right size is refused."""
+    d, p = desc(batch=1, seq=0, n_seqs=2), C.c_void_p(4096)
+    n, w = lib.nlh_gated_delta_saved_bytes(C.byref(d)), lib.nlh_gated_delta_backward_bytes(C.byref(d))
+    assert n > 0 and w > 0
+    none = (None,) * 5
+    assert lib.nlh_gated_delta_forward(C.byref(d), *none, p, p, None, p, None, n) == BAD
+    b = lib.nlh_gated_delta_backward
+    assert b(C.byref(d), *none, p, None, n, None, None, *none, p, p, w) == BAD
+    assert b(C.byref(d), *none, p, p, n, None, None, *none, p, None, w) == BAD
+
+
 def test_embedding_refuses(lib):
     p = C.c_void_p(4096)
     assert lib.nlh_embedding_forward(p, 0, p, p, -1, 10, 4, 1.0) == BAD and lib.nlh_embedding_forward(None, 0, p, p, 3, 10, 4, 1.0) == BAD
