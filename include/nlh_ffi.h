@@ -336,6 +336,9 @@ int32_t nlh_swa_backward_f32(const float* q, const float* k, const float* v, con
  * nonzero if a bounded mbarrier wait of these kernels, or of the matrix-form ones
  * (NLH_OPT_CHUNK_MATRIX), ever ran out. */
 #define NLH_OPT_BULK_STAGING 5
+/* NLH_OPT_GATED_DELTA_WAIT (default 1): 0 gives the bounded waits of nlh_gated_delta_forward / _backward no time at all, so
+ * that a caller can see what a copy that does not arrive leads to. */
+#define NLH_OPT_GATED_DELTA_WAIT 6
 int32_t nlh_bulk_timeout_flag(void);
 int32_t nlh_set_option(int32_t option, int32_t value);
 /* How the last tcgen05 SWA forward of this process staged its operand tiles: 1 = tiled TMA copies,
@@ -587,8 +590,11 @@ int32_t nlh_gated_delta_backward(const nlh_gated_delta_desc* desc, const void* k
  * [0, n_slots) is no sequence: its rows of y are zeros. A slot named more than once is stepped in the order of the batch. */
 int32_t nlh_gated_delta_step(const nlh_gated_delta_desc* desc, const void* k, const void* v, const void* q,
     const float* log_retain, const float* theta, float* m, const int32_t* slots, int32_t n_slots, void* y);
-/* 1 once a wait of the state kernels for their copies has run out (its results are wrong), 0 otherwise; synchronous. */
+/* The state kernels wait for their copies for a second or so. Where a wait runs out, what is still to be computed of the state, of y
+ * and of the gradients that depend on it is NaN, and a flag of the device is set: 1 once that has happened, 0 if not, -1 if it
+ * cannot be read. Both calls wait for the launch stream (nlh_set_stream) first, and may not be captured. */
 int32_t nlh_gated_delta_timeout_flag(void);
+int32_t nlh_gated_delta_timeout_clear(void);
 
 /* ── Host-slice dispatch layer (compiled counterpart of core/src/dispatch.rs `*_dispatch`) ────
  * Same argument order and meaning as the reference functions its kernel tests call

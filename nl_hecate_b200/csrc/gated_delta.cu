@@ -278,6 +278,7 @@ __global__ void __launch_bounds__(256, DKP == 64 ? 2 : 1) gd_state_fwd_kernel(Ar
     __shared__ float4 s_gate[2][C];
     __shared__ float s_w[2][C];
     __shared__ __align__(8) unsigned long long s_bar;
+    __shared__ int s_dead;
     const int nsl = A.dvp / NS, sl = blockIdx.x % nsl, p = blockIdx.x / nsl, h = p % A.hv, seq = A.starts ? A.order[p / A.hv] : p / A.hv;
     const int n0 = sl * NS, tid = threadIdx.x, lane = tid & 31, w = tid >> 5, rb = w & 3, hf = w >> 2, g = lane >> 2, t = lane & 3;
     const int slot0 = first_slot(A, seq), count = chunk_count(A, seq);
@@ -338,10 +339,10 @@ __global__ void __launch_bounds__(256, DKP == 64 ? 2 : 1) gd_state_fwd_kernel(Ar
         if (tid < C) { s_gate[buf][tid] = pg.g; s_w[buf][tid] = pg.g.w * pg.theta; }
     };
     if (tid == 0) {
+        s_dead = 0;
         init_t(&s_bar);
         if (count > 0) copy_t(Ts, A.tmat + tile0 * T_BYTES, &s_bar);
     }
-    bool dead = false;
     if (count > 0) { fetch(0); commit(0); }
     __syncthreads();
     for (int c = 0; c < count; c++) {
@@ -373,11 +374,12 @@ __global__ void __launch_bounds__(256, DKP == 64 ? 2 : 1) gd_state_fwd_kernel(Ar
                 any |= odd(x.x) | odd(x.y);
                 put2<3>(Rs + row * LS + H * hf + 8 * n + 2 * t, L::PR, x.x, x.y);
             }
-        wait_t(&s_bar, buf, dead);
+        if (s_dead == 0 && !wait_t(&s_bar, buf, A.wait_cycles)) s_dead = 1;
         any = __syncthreads_or(any);
         zero(acc);
         if (any) triangle_by_token<3, NT>(acc, Ts, C * LP, Rs, LS, L::PR, 16 * rb, H * hf);
         else gemm<NT, false, true, 3, 3>(acc, Ts + 16 * rb * LP, LP, C * LP, Rs + H * hf, LS, L::PR, 0, 16 * (rb + 1));
+        if (lost_t(&s_dead, &s_bar, buf)) fill_nan(acc);
 #pragma unroll
         for (int n = 0; n < NT; n++)
 #pragma unroll
@@ -389,7 +391,7 @@ __global__ void __launch_bounds__(256, DKP == 64 ? 2 : 1) gd_state_fwd_kernel(Ar
             }
         __syncthreads();
         ep += e_step;
-        if (tid == 0 && c + 1 < count) copy_t(Ts, A.tmat + (tile0 + (long long)(c + 1) * A.hv) * T_BYTES, &s_bar);
+        if (tid == 0 && c + 1 < count && s_dead == 0) copy_t(Ts, A.tmat + (tile0 + (long long)(c + 1) * A.hv) * T_BYTES, &s_bar);
         const float gl = s_gate[buf][C - 1].z;
 #pragma unroll
         for (int m = 0; m < MT; m++) {
@@ -587,6 +589,7 @@ __global__ void __launch_bounds__(256, DKP == 64 ? 2 : 1) gd_state_bwd_kernel(Ar
     __shared__ float4 s_gate[2][C];
     __shared__ float s_theta[2][C];
     __shared__ __align__(8) unsigned long long s_bar;
+    __shared__ int s_dead;
     const int nsl = A.dvp / NS, sl = blockIdx.x % nsl, p = blockIdx.x / nsl, h = p % A.hv, seq = A.starts ? A.order[p / A.hv] : p / A.hv;
     const int n0 = sl * NS, tid = threadIdx.x, lane = tid & 31, w = tid >> 5, rb = w & 3, hf = w >> 2, g = lane >> 2, t = lane & 3;
     const int slot0 = first_slot(A, seq), count = chunk_count(A, seq);
@@ -640,10 +643,10 @@ __global__ void __launch_bounds__(256, DKP == 64 ? 2 : 1) gd_state_bwd_kernel(Ar
         if (tid < C) { s_gate[buf][tid] = pg.g; s_theta[buf][tid] = pg.theta; }
     };
     if (tid == 0) {
+        s_dead = 0;
         init_t(&s_bar);
         if (count > 0) copy_t(Ts, A.tmat + tile * T_BYTES, &s_bar);
     }
-    bool dead = false;
     if (count > 0) { fetch(count - 1, g_at, e_at, m_at); commit(0); }
     __syncthreads();
     for (int c = count - 1; c >= 0; c--) {
@@ -674,10 +677,11 @@ __global__ void __launch_bounds__(256, DKP == 64 ? 2 : 1) gd_state_bwd_kernel(Ar
                 const float wi = s_gate[buf][row].w, th = s_theta[buf][row];
                 put2<3>(Rs + row * LS + H * hf + 8 * n + 2 * t, L::PR, th * (f[n][r].x + wi * acc[n][2 * r]), th * (f[n][r].y + wi * acc[n][2 * r + 1]));
             }
-        wait_t(&s_bar, buf, dead);
+        if (s_dead == 0 && !wait_t(&s_bar, buf, A.wait_cycles)) s_dead = 1;
         __syncthreads();
         zero(acc);
         gemm<NT, true, true, 3, 3>(acc, Ts + 16 * rb, LP, C * LP, Rs + H * hf, LS, L::PR, 16 * rb, C);
+        if (lost_t(&s_dead, &s_bar, buf)) fill_nan(acc);
         float* xp = A.x + e_at;
 #pragma unroll
         for (int n = 0; n < NT; n++)
@@ -700,7 +704,7 @@ __global__ void __launch_bounds__(256, DKP == 64 ? 2 : 1) gd_state_bwd_kernel(Ar
         e_at -= e_step;
         m_at -= m_step;
         dv -= C * dv_row;
-        if (tid == 0 && c > 0) copy_t(Ts, A.tmat + tile * T_BYTES, &s_bar);
+        if (tid == 0 && c > 0 && s_dead == 0) copy_t(Ts, A.tmat + tile * T_BYTES, &s_bar);
         const float gl = s_gate[buf][C - 1].z;
 #pragma unroll
         for (int m = 0; m < MT; m++) {
@@ -1099,6 +1103,7 @@ static bool fill(const char* where, const nlh_gated_delta_desc* d, Args& A)
     A.gb = d->gate_batch; A.gt = d->gate_token; A.gh = d->gate_head;
     A.yb = d->dy_batch; A.yt = d->dy_token; A.yh = d->dy_head;
     A.scale = d->scale;
+    A.wait_cycles = option_value(NLH_OPT_GATED_DELTA_WAIT) ? T_WAIT_CYCLES : 0u;
     A.nc = (d->seq + C - 1) / C;
     const long long slots = d->n_seqs > 0 ? (long long)d->seq / C + d->n_seqs : (long long)d->batch * A.nc;
     if (slots * d->heads_v > MAX_N) { record_status(NLH_ERR_INVALID_ARG, where, "too many chunks"); return false; }
@@ -1307,8 +1312,18 @@ int32_t nlh_gated_delta_backward(const nlh_gated_delta_desc* desc, const void* k
 int32_t nlh_gated_delta_timeout_flag(void)
 {
     int v = 0;
-    if (cudaMemcpyFromSymbol(&v, g_gd_timeout, sizeof(int)) != cudaSuccess) return -1;
+    if (cudaStreamSynchronize(current_stream()) != cudaSuccess || cudaMemcpyFromSymbol(&v, g_gd_timeout, sizeof(int)) != cudaSuccess) return -1;
     return v;
+}
+
+int32_t nlh_gated_delta_timeout_clear(void)
+{
+    const int v = 0;
+    if (cudaStreamSynchronize(current_stream()) != cudaSuccess || cudaMemcpyToSymbol(g_gd_timeout, &v, sizeof(int)) != cudaSuccess) {
+        record_status(NLH_ERR_CUDA, "nlh_gated_delta_timeout_clear", cudaGetErrorString(cudaGetLastError()));
+        return NLH_ERR_CUDA;
+    }
+    return NLH_OK;
 }
 
 int32_t nlh_gated_delta_step(const nlh_gated_delta_desc* desc, const void* k, const void* v, const void* q,

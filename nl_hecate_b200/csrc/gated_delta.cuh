@@ -61,6 +61,7 @@ struct Args {
     float *dk_part, *dq_part;          // [batch * seq, hv, dk] when heads share keys
     void *d_k, *d_v, *d_q;
     float *d_g, *d_theta, *d_m0;
+    unsigned wait_cycles;              // of the state kernels' waits for T
 };
 
 struct Chunk {
@@ -441,10 +442,11 @@ template <typename T, int COLS, int THREADS> struct Prefetch {
 };
 // The planes of T, copied as they are, straight into shared memory: one bulk copy by one thread, issued when the chunk before has no
 // more use for its T, waited for when the next one needs it, half a chunk later. (As 16-byte cp.async by all threads the
-// issue alone held the warps up for some 900 cycles of a chunk's 4000.) The wait is bounded: where it runs out the CTA sets
-// g_gd_timeout and carries on with wrong results.
+// issue alone held the warps up for some 900 cycles of a chunk's 4000.) The wait is bounded by the clock: a second or so, where
+// a copy takes a microsecond. Where it runs out, in any thread, the CTA gives the copy in flight as long again, issues no
+// more, sets g_gd_timeout, and takes NaN for the product with T: so is its share of the state from there on, and all that follows.
 __device__ int g_gd_timeout = 0;
-constexpr unsigned T_WAIT_LIMIT = 1u << 22;
+constexpr unsigned T_WAIT_CYCLES = 2000000000u;
 __device__ __forceinline__ void init_t(unsigned long long* bar)
 {
     asm volatile("mbarrier.init.shared::cta.b64 [%0], 1;\n" ::"r"(smem_addr(bar)) : "memory");
@@ -456,15 +458,38 @@ __device__ __forceinline__ void copy_t(bf* dst, const unsigned char* src, unsign
     asm volatile("cp.async.bulk.shared::cluster.global.mbarrier::complete_tx::bytes [%0], [%1], %2, [%3];\n"
                  ::"r"(smem_addr(dst)), "l"(src), "r"(T_BYTES), "r"(smem_addr(bar)) : "memory");
 }
-__device__ __forceinline__ void wait_t(unsigned long long* bar, unsigned parity, bool& dead)
+__device__ __forceinline__ bool test_t(unsigned long long* bar, unsigned parity)
 {
-    for (unsigned i = 0; !dead; i++) {
-        unsigned ok;
-        asm volatile("{\n\t.reg .pred P;\n\tmbarrier.try_wait.parity.shared::cta.b64 P, [%1], %2;\n\tselp.u32 %0, 1, 0, P;\n\t}\n"
-                     : "=r"(ok) : "r"(smem_addr(bar)), "r"(parity) : "memory");
-        if (ok) return;
-        if (i == T_WAIT_LIMIT) { dead = true; atomicExch(&g_gd_timeout, 1); }
+    unsigned ok;
+    asm volatile("{\n\t.reg .pred P;\n\tmbarrier.try_wait.parity.shared::cta.b64 P, [%1], %2;\n\tselp.u32 %0, 1, 0, P;\n\t}\n"
+                 : "=r"(ok) : "r"(smem_addr(bar)), "r"(parity) : "memory");
+    return ok != 0;
+}
+// Whether the copy has arrived before `cycles` have passed.
+__device__ __forceinline__ bool wait_t(unsigned long long* bar, unsigned parity, unsigned cycles)
+{
+    if (cycles > 0 && test_t(bar, parity)) return true;
+    for (const unsigned t0 = (unsigned)clock(); (unsigned)clock() - t0 < cycles;)
+        if (test_t(bar, parity)) return true;
+    return false;
+}
+template <int NT> __device__ __forceinline__ void fill_nan(float (&acc)[NT][4])
+{
+#pragma unroll
+    for (int n = 0; n < NT; n++)
+#pragma unroll
+        for (int i = 0; i < 4; i++) acc[n][i] = __int_as_float(0x7fffffff);
+}
+// Behind the barrier that follows the wait: whether the copy has not come (the same for all threads, and from now on).
+__device__ __forceinline__ bool lost_t(int* dead, unsigned long long* bar, unsigned parity)
+{
+    const int d = *dead;                          // 1: not reported yet
+    if (threadIdx.x == 0 && d == 1) {
+        wait_t(bar, parity, T_WAIT_CYCLES);
+        atomicExch(&g_gd_timeout, 1);
+        *dead = 2;
     }
+    return d != 0;
 }
 
 }  // namespace gd

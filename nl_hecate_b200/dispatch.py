@@ -536,6 +536,19 @@ def gated_delta_step(k, v, q, log_retain, theta, m, slots=None, scale=1.0):
     return y
 
 
+def gated_delta_check():
+    """Raises RuntimeError if a copy of the gated delta rule's state kernels did not arrive on the current device since the
+    last check; results that depend on it are NaN. Waits for the current stream."""
+    with _LAUNCH:
+        bind_stream()
+        flag = ffi.lib().nlh_gated_delta_timeout_flag()
+        if flag == 1:
+            ffi.check(ffi.lib().nlh_gated_delta_timeout_clear(), "gated_delta_check")
+    if flag:
+        raise RuntimeError("gated_delta_check: " + ("a copy did not arrive in time; the states, outputs and gradients behind it are NaN"
+                                                    if flag == 1 else "the device's flag cannot be read"))
+
+
 # ── embedding with scaling, gradient by sorted tokens (additive API) ───────
 def _ids32(where, name, ids, numel=None):
     if ids.dtype != torch.int32 or not ids.is_contiguous() or (numel is not None and ids.numel() != numel):

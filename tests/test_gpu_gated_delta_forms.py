@@ -7,7 +7,7 @@ import pytest
 import torch
 
 sys.path.insert(0, os.path.dirname(os.path.abspath(__file__)))
-from test_gpu_gated_delta import inputs, run  # noqa: E402
+from test_gpu_gated_delta import inputs, packed, run  # noqa: E402
 
 pytestmark = pytest.mark.gpu
 
@@ -35,3 +35,46 @@ def test_packed_batch_without_a_token(hk, hv, dtype):
     assert torch.equal(out["m_final"], p["m0"]) and torch.equal(out["d_m_initial"], p["d_m"])
     for x in ("y", "d_k", "d_v", "d_q", "d_log_retain", "d_theta"):
         assert out[x].numel() == 0, x
+
+
+WAIT = 6      # NLH_OPT_GATED_DELTA_WAIT
+
+
+@pytest.mark.parametrize("dtype", [torch.float32, torch.bfloat16])
+def test_a_wait_that_runs_out_shows(dtype):
+    """With no time for the waits of the state kernels every copy counts as lost: NaN in the states, outputs and gradients that
+    depend on it, the flag set until it is cleared, and the next call right again."""
+    from nl_hecate_b200 import dispatch as D
+    from nl_hecate_b200 import ffi
+    lib = ffi.lib()
+    nan = lambda t: bool(torch.isnan(t).all())
+    cases = [(inputs(2, 150, 2, 2, 64, 48, dtype, seed=1), None), (inputs(2, 70, 1, 1, 128, 128, dtype, seed=2), None),
+             packed((130, 0, 7), 1, 2, 64, 64, dtype)[:2]]
+    D.gated_delta_check()
+    for p, starts in cases:
+        a = [p[x] for x in ("k", "v", "q", "log_retain", "theta")]
+        want = run(p, starts=starts)
+        y, m, saved = D.gated_delta_forward(*a, m0=p["m0"], seq_starts=starts)
+        try:
+            assert lib.nlh_set_option(WAIT, 0) == 0
+            ynan, mnan, _ = D.gated_delta_forward(*a, m0=p["m0"], seq_starts=starts)
+            with pytest.raises(RuntimeError, match="did not arrive"):
+                D.gated_delta_check()
+            D.gated_delta_check()                     # raised once
+            g = D.gated_delta_backward(*a, saved, p["d_y"], d_m_final=p["d_m"], seq_starts=starts)
+            assert lib.nlh_gated_delta_timeout_flag() == 1 and lib.nlh_gated_delta_timeout_flag() == 1
+        finally:
+            lib.nlh_set_option(WAIT, 1)
+        assert lib.nlh_gated_delta_timeout_clear() == 0 and lib.nlh_gated_delta_timeout_flag() == 0
+        here = [0, 2] if starts is not None else slice(None)      # the empty sequence has no copy to wait for
+        assert nan(ynan) and nan(mnan[here])
+        if starts is not None:
+            assert torch.equal(mnan[1], p["m0"][1]) and torch.equal(g["d_m_initial"][1], p["d_m"][1])
+        for x in ("d_k", "d_v", "d_log_retain", "d_theta"):
+            assert nan(g[x]), x
+        assert nan(g["d_m_initial"][here])
+        assert torch.equal(g["d_q"], want["d_q"])     # needs the forward's states alone
+        again = run(p, starts=starts)
+        for x in want:
+            assert torch.equal(again[x], want[x]), x
+    D.gated_delta_check()
