@@ -644,12 +644,12 @@ class _Distill(torch.autograd.Function):
 
 def _distill_plain(logits, teacher_ids, teacher_logits, targets, temperature, soft_weight, hard_weight):
     """The same loss in PyTorch operators (fused_glue = False)."""
-    there = (teacher_ids >= 0) & (teacher_ids < logits.shape[1])
+    there = (teacher_ids >= 0) & (teacher_ids < logits.shape[1]) & (teacher_logits != -math.inf)
     rows = there.any(1)
     t = torch.where(there, teacher_logits.float() / temperature, -math.inf)[rows]
     p = torch.where(there[rows], torch.softmax(t, 1), 0.0)
     logq = torch.log_softmax(logits[rows] / temperature, 1).gather(1, teacher_ids[rows].clamp(0, logits.shape[1] - 1).long())
-    kl = (torch.special.xlogy(p, p) - p * logq).sum() / rows.sum().clamp_min(1)
+    kl = (torch.special.xlogy(p, p) - torch.where(p > 0, p * logq, 0.0)).sum() / rows.sum().clamp_min(1)
     ok = (targets >= 0) & (targets < logits.shape[1])
     ce = F.cross_entropy(logits[ok], targets[ok].long(), reduction="sum") / ok.sum().clamp_min(1)
     return soft_weight * temperature ** 2 * kl + hard_weight * ce

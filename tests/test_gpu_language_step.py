@@ -61,6 +61,19 @@ def test_model_step_matches_plain_operators():
             assert float((x - y).abs().max()) <= 1e-3 * max(float(y.abs().max()), 1e-6)
 
 
+def test_teacher_entries_without_mass():
+    """Teacher logits of -infinity, a whole position of them among others: unused for the kernels and for the plain operators alike."""
+    from nl_hecate_b200.stacked_mag import StackedMAG
+    ours = StackedMAG(config(), 3, seed=7)
+    ref = StackedMAG(config(fused=False), 3, seed=7, memory_fn=gated_delta_ref, swa_fn=swa_ref)
+    tok, tgt, (ids, top) = data(3)
+    top[:, ::5] = -float("inf")
+    top[:, 1::5, ::2] = -float("inf")
+    with torch.no_grad():
+        a, b = ours.forward(tok, tgt, (ids, top)), ref.forward(tok, tgt, (ids, top))
+    assert abs(float(a) - float(b)) <= 1e-5 * abs(float(b))
+
+
 @pytest.mark.parametrize("with_teacher", [True, False])
 def test_graphed_step_equals_eager(with_teacher):
     from nl_hecate_b200.stacked_mag import StackedMAG
