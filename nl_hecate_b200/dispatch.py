@@ -359,8 +359,8 @@ def titans_frozen_stream_backward(k, v, q, alpha, theta, eta, ms, d_y, chunk, wa
 # k, q [B, S, Hk, dk], v [B, S, Hv, dv], log_retain, theta [B, S, Hv] fp32, any strides with a contiguous last
 # axis; Hk divides Hv. States m [B, Hv, dv, dk] fp32 (y = M q). A packed batch has B = 1 and seq_starts [n + 1] int32.
 
-_CURRENT_DEVICE = torch._C._cuda_getDevice
-_CURRENT_STREAM = torch._C._cuda_getCurrentRawStream
+_CURRENT_DEVICE = getattr(torch._C, "_cuda_getDevice", None)       # a PyTorch without CUDA has neither, and no tensor to call them for
+_CURRENT_STREAM = getattr(torch._C, "_cuda_getCurrentRawStream", None)
 _DESC = struct.Struct("8i15qf")          # nlh_gated_delta_desc (ffi.GatedDeltaDesc), packed in one call
 
 

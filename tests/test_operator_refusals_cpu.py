@@ -150,3 +150,25 @@ def test_host_tensors_are_refused():
         D.distill_forward(z(3, 9), z(3, 2, dtype=torch.int32), z(3, 2))
     with pytest.raises(ValueError, match="CUDA"):
         D.gated_delta_step(z(1, 1, 1, 8), z(1, 1, 1, 8), z(1, 1, 1, 8), z(1, 1, 1), z(1, 1, 1), z(1, 1, 8, 8))
+
+
+def test_package_imports_and_refuses_without_cuda_bindings():
+    """A PyTorch built without CUDA has no device and stream queries: importing works, and the operators refuse its tensors."""
+    import subprocess
+    code = """
+import torch
+for x in ("_cuda_getDevice", "_cuda_getCurrentRawStream"):
+    delattr(torch._C, x)
+import nl_hecate_b200.stacked_mag
+from nl_hecate_b200 import dispatch as D
+z = torch.zeros
+try:
+    D.embedding_forward(z(4, 8), z(3, dtype=torch.int32))
+except ValueError as e:
+    assert "CUDA" in str(e)
+else:
+    raise SystemExit("not refused")
+"""
+    root = os.path.dirname(os.path.dirname(os.path.abspath(__file__)))
+    r = subprocess.run([sys.executable, "-c", code], cwd=root, capture_output=True, text=True, timeout=300)
+    assert r.returncode == 0, r.stderr[-800:]
