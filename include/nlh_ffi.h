@@ -538,7 +538,8 @@ int32_t nlh_embedding_backward(const void* d_out, int32_t d_out_is_bf16, const i
  *   loss[0] = hard_weight / n_hard sum (lse(z) - z_target)
  *           + soft_weight temperature^2 / n_soft sum_rows sum_k p_k (log p_k - z_k / temperature + lse(z / temperature)).
  * A weight of 0 or NULL ids leave a term out. The backward writes d loss / d logits * grad_scale[0] (NULL = 1) in the logits'
- * type, zeros in rows without a term; d_logits may be logits itself. saved (nlh_distill_saved_bytes, 16-byte
+ * type, zeros in rows without a term; d_logits may be logits itself (with the same row stride), and may
+ * lie between its rows, but shares no element with it otherwise. saved (nlh_distill_saved_bytes, 16-byte
  * aligned, the caller's) carries the rows' maxima and sums; the backward's other arguments are the forward's. */
 int64_t nlh_distill_saved_bytes(int32_t n, int32_t vocab);
 int32_t nlh_distill_forward(const void* logits, int32_t logits_is_bf16, int64_t row_stride, const int32_t* target_ids,

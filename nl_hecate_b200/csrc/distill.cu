@@ -621,6 +621,20 @@ static bool fill(const char* where, Args& A, const void* logits, int64_t row_str
     divide(A);
     return true;
 }
+// Whether the gradient's rows share an element with the logits', other than as the same elements in the same places: exact for rows
+// of one stride, else whether the address ranges meet.
+static bool overlaps(const Args& A, int64_t size)
+{
+    const int64_t n = A.n, width = A.vocab, apart = ((intptr_t)A.d - (intptr_t)A.z) / size, row = n > 1 ? A.z_row : 0;
+    if (n > 1 && A.d_row != row) return apart > -((n - 1) * A.d_row + width) && apart < (n - 1) * row + width;
+    int64_t k = 0;                       // rows of logits that a row of the gradient can meet: this far ahead, and the next
+    if (row) { k = apart / row; if (k * row > apart) k--; }
+    for (int i = 0; i < 2; i++, k++) {
+        const int64_t off = apart - k * row;
+        if (apart != 0 && k < n && -k < n && off < width && -off < width) return true;
+    }
+    return false;
+}
 static int mode_of(const Args& A) { return !(A.hard && A.soft) || A.tau == 1.f ? ONE : A.tau == 2.f ? SQUARE : BOTH; }
 
 // Who reads a row in the forward: with many short rows a warp, which waits at no barrier (32768 x 8192 bf16 at tau 2: 110 us
@@ -714,6 +728,10 @@ int32_t nlh_distill_backward(const void* logits, int32_t logits_is_bf16, int64_t
     }
     if (n == 0) return NLH_OK;
     A.d = d_logits; A.d_row = d_row_stride; A.grad = grad_scale;
+    if (distill::overlaps(A, logits_is_bf16 ? 2 : 4)) {
+        record_status(NLH_ERR_INVALID_ARG, where, "d_logits overlaps logits without being logits");
+        return NLH_ERR_INVALID_ARG;
+    }
     return (logits_is_bf16 ? distill::launch<__nv_bfloat16>(A, true, where) : distill::launch<float>(A, true, where)) ? NLH_OK : NLH_ERR_CUDA;
 }
 

@@ -632,11 +632,16 @@ def distill_forward(logits, teacher_ids, teacher_logits, targets=None, temperatu
 
 
 def _overlap(a, b):
-    """Whether the memory of two [n, vocab] tensors meets, unless they are the same elements in the same places."""
-    if a.data_ptr() == b.data_ptr() and (a.stride(0) == b.stride(0) or a.shape[0] <= 1):
+    """Whether two [n, vocab] tensors share an element, other than as the same elements in the same places. Exact where both have
+    one row stride; else whether their address ranges meet."""
+    n, width, size = a.shape[0], a.shape[1], a.element_size()
+    if n == 0 or width == 0:
         return False
-    end = lambda t: t.data_ptr() + ((t.shape[0] - 1) * t.stride(0) + t.shape[1]) * t.element_size()
-    return min(a.numel(), b.numel()) > 0 and a.data_ptr() < end(b) and b.data_ptr() < end(a)
+    apart, row = (b.data_ptr() - a.data_ptr()) // size, a.stride(0) if n > 1 else 0
+    if n > 1 and b.stride(0) != row:
+        return -((n - 1) * b.stride(0) + width) < apart < (n - 1) * row + width
+    first = apart // row if row else 0                # rows of a that a row of b can meet: this far ahead, and the next
+    return apart != 0 and any(abs(k) < n and abs(apart - k * row) < width for k in (first, first + 1))
 
 
 def distill_backward(logits, saved, grad=None, out=None):

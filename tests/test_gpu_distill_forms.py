@@ -81,3 +81,26 @@ def test_an_infinite_logit_at_an_entry_is_not_left_out(tau, n, vocab):
         assert math.isnan(float(loss)) and bool(torch.isnan(d[1]).all())
         if hw:
             assert torch.equal(d[2:], want[2:]) and torch.equal(d[:1], want[:1])
+
+
+@pytest.mark.parametrize("dtype", [torch.float32, torch.bfloat16])
+def test_gradient_between_the_rows_of_its_logits(dtype):
+    """Logits and gradient as the two halves of one buffer's rows: no element in common, so no refusal, and neither touches the other."""
+    from nl_hecate_b200 import dispatch as D
+    z, ids, t, y = make(40, 300, 5, dtype)
+    both = torch.full((40, 600), 7.0, dtype=dtype, device="cuda")
+    both[:, :300] = z
+    _, saved = D.distill_forward(both[:, :300], ids, t, targets=y, temperature=2.0, hard_weight=0.5)
+    want = D.distill_backward(both[:, :300], saved)
+    got = D.distill_backward(both[:, :300], saved, out=both[:, 300:])
+    assert torch.equal(got, want) and torch.equal(both[:, :300], z)
+    with pytest.raises(ValueError, match="overlaps"):
+        D.distill_backward(both[:, :300], saved, out=both[:, 299:599])
+    with pytest.raises(ValueError, match="overlaps"):
+        D.distill_backward(both[:20, :300], saved_of(both[:20, :300], ids, t, y), out=both[1:21, :300])
+
+
+def saved_of(z, ids, t, y):
+    from nl_hecate_b200 import dispatch as D
+    n = z.shape[0]
+    return D.distill_forward(z, ids[:n].contiguous(), t[:n].contiguous(), targets=y[:n].contiguous(), temperature=2.0, hard_weight=0.5)[1]

@@ -172,3 +172,32 @@ else:
     root = os.path.dirname(os.path.dirname(os.path.abspath(__file__)))
     r = subprocess.run([sys.executable, "-c", code], cwd=root, capture_output=True, text=True, timeout=300)
     assert r.returncode == 0, r.stderr[-800:]
+
+
+def test_gradients_that_overlap_their_logits(lib):
+    """Rows of both as sets of elements, against the wrapper's and the C entry's answers: the same elements in the same places are
+    allowed, rows that lie between each other's, and nothing that shares an element otherwise."""
+    import torch
+    from nl_hecate_b200 import dispatch as D
+    store = torch.zeros(400)
+    base = store.data_ptr()
+    n, need = 0, lib.nlh_distill_saved_bytes(4, 7)
+    p = C.c_void_p(4096)
+    for rows in (1, 2, 4):
+        for width, za, zr, dr in ((7, 40, 20, 20), (7, 40, 14, 14), (7, 40, 7, 7), (5, 100, 9, 9), (7, 60, 20, 10), (7, 60, 7, 20)):
+            for da in range(0, 200):
+                if da + (rows - 1) * dr + width > 400:
+                    continue
+                z = store.as_strided((rows, width), (zr, 1), za)
+                d = store.as_strided((rows, width), (dr, 1), da)
+                at = lambda a, r: [a + i * r + j for i in range(rows) for j in range(width)]
+                same = at(za, zr) == at(da, dr)
+                shares = not same and bool(set(at(za, zr)) & set(at(da, dr)))
+                got = D._overlap(z, d)
+                assert got == shares or (got and rows > 1 and zr != dr), (rows, width, za, zr, da, dr)
+                if shares:
+                    rc = lib.nlh_distill_backward(C.c_void_p(base + 4 * za), 0, zr, p, p, p, 0, p, need, None, C.c_void_p(base + 4 * da), dr,
+                                                  rows, width, 2, 2.0, 0.5, 0.5)
+                    assert rc == BAD, (rows, width, za, zr, da, dr)
+                    n += 1
+    assert n > 500
