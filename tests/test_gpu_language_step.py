@@ -98,3 +98,24 @@ def test_unknown_rule_is_refused():
     from nl_hecate_b200.stacked_mag import StackedMAG, StackedMAGConfig
     with pytest.raises(ValueError, match="memory_rule"):
         StackedMAG(StackedMAGConfig(d_model=64, num_heads=1, n_blocks=1, k=1, chunk_sizes=(1,), memory_rule="delta2"), 1)
+
+
+def test_sizes_of_more_than_32_bits_are_refused():
+    """Sizes go to the C entries in 32 bits: 2^32 + 2 rows would count as two. The buffers are allocated, not touched."""
+    from nl_hecate_b200 import dispatch as D
+    n = 2 ** 32 + 2
+    few = torch.zeros(3, dtype=torch.int32, device="cuda")
+    row = torch.empty(n, 1, dtype=torch.bfloat16, device="cuda")
+    with pytest.raises(ValueError, match="2\\^31"):
+        D.embedding_forward(row, few)
+    with pytest.raises(ValueError, match="2\\^31"):
+        D.distill_forward(row, few.new_zeros(n, 0), row[:, :0].contiguous())
+    ids = torch.empty(n, dtype=torch.int32, device="cuda")
+    with pytest.raises(ValueError, match="2\\^31"):
+        D.embedding_forward(row[:4], ids)
+    with pytest.raises(ValueError, match="2\\^31"):
+        D.embedding_backward(row, ids, torch.zeros(4, 1, device="cuda"))
+    one = torch.zeros(1, 1, 1, 1, device="cuda")
+    pool = torch.empty(n, 1, 1, 1, device="cuda")
+    with pytest.raises(ValueError, match="2\\^31"):
+        D.gated_delta_step(one, one, one, one[0], one[0], pool)
