@@ -56,8 +56,7 @@ struct Args {
     // backward
     const float* d_m_final;
     float *f, *x, *d_chunk;            // like e, e, m_chunk
-    float* dg_part;                    // [dkp / 64, slot, hv, 64] gradient of G, then [dkp / 64, slot, hv] of the chunk's last G
-    float* dgl_part;
+    float* dg_part;                    // [dkp / 64, slot, hv, 64] parts of the gradient of log_retain, where there are two
     float *dk_part, *dq_part;          // [batch * seq, hv, dk] when heads share keys
     void *d_k, *d_v, *d_q;
     float *d_g, *d_theta, *d_m0;

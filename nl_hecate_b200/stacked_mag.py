@@ -171,6 +171,9 @@ class _TitansMemory(torch.autograd.Function):
                 None, None)
 
 
+_KEEP_TINY = 2.0 ** -60     # a retention of 0 is taken as this one, which no fp32 state sees: log and the division below stay finite
+
+
 class _GatedDeltaMemory(torch.autograd.Function):
     """Per-head gated delta rule over [N, S, hd] fp32 streams (nlh_gated_delta_forward / _backward) with the framework's
     gates: retention 1 - alpha, learning rate theta. m0 [N, hd * hd]; returns y and the final memory."""
@@ -179,8 +182,9 @@ class _GatedDeltaMemory(torch.autograd.Function):
     def forward(ctx, k, v, q, alpha, theta, m0):
         n, s, d = k.shape
         heads = lambda t: t.unsqueeze(2)                 # one head per row of the batch
-        keep = 1.0 - alpha
-        args = (heads(k), heads(v), heads(q), heads(torch.log(keep)), heads(theta))
+        keep = (1.0 - alpha).clamp_min(_KEEP_TINY)
+        log_retain = torch.log1p(-alpha).clamp_min(math.log(_KEEP_TINY))
+        args = (heads(k), heads(v), heads(q), heads(log_retain), heads(theta))
         y, m, ctx.chunks = D.gated_delta_forward(*args, m0=m0.view(n, 1, d, d))
         ctx.save_for_backward(*args, keep)
         m = m.view(n, d * d)
@@ -191,8 +195,8 @@ class _GatedDeltaMemory(torch.autograd.Function):
     def backward(ctx, dy, _dm):
         *args, keep = ctx.saved_tensors
         g = D.gated_delta_backward(*args, ctx.chunks, dy.contiguous().unsqueeze(2), want_initial=False)
-        # log(1 - alpha): the gradient of log_retain carries the factor 1 - alpha
-        d_alpha = -g["d_log_retain"].squeeze(2) / keep.clamp_min(1e-30)
+        # log(1 - alpha): the gradient of log_retain carries the factor 1 - alpha, in each of the terms that the kernel adds up
+        d_alpha = -g["d_log_retain"].squeeze(2) / keep
         sq = lambda x: g[x].squeeze(2)
         return sq("d_k"), sq("d_v"), sq("d_q"), d_alpha, sq("d_theta"), None
 

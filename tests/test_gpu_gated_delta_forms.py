@@ -1,5 +1,6 @@
 """Gated delta rule: the kernels' variants at the sizes that choose them, against the recurrence in 64 bits with the tolerances of
 test_gpu_gated_delta.py, and what the variants have in common bit by bit."""
+import math
 import os
 import sys
 
@@ -7,7 +8,8 @@ import pytest
 import torch
 
 sys.path.insert(0, os.path.dirname(os.path.abspath(__file__)))
-from test_gpu_gated_delta import inputs, packed, run  # noqa: E402
+from test_gpu_gated_delta import TOL, inputs, packed, reference, run  # noqa: E402
+from test_gpu_language_step import gated_delta_ref  # noqa: E402
 
 pytestmark = pytest.mark.gpu
 
@@ -78,3 +80,43 @@ def test_a_wait_that_runs_out_shows(dtype):
         for x in want:
             assert torch.equal(again[x], want[x]), x
     D.gated_delta_check()
+
+
+RETAIN = (0.01, 1e-4, 1e-6, 6e-8, 1e-12)
+
+
+@pytest.mark.parametrize("dtype", [torch.float32, torch.bfloat16])
+@pytest.mark.parametrize("b,s,hk,hv,dk,dv", [(2, 150, 2, 2, 64, 64), (1, 130, 1, 2, 128, 40), (1, 64, 1, 1, 24, 128)])
+def test_gate_gradient_keeps_its_factor(b, s, hk, hv, dk, dv, dtype):
+    """The gradient of log_retain divided by the retention, which it carries as a factor, is the gradient of the retention: as
+    accurate, at retentions of any size, as the gate gradients' tolerance says of the largest one."""
+    p = inputs(b, s, hk, hv, dk, dv, dtype, seed=8)
+    for i, t in enumerate((0, 5, 6, 20, 40, 62, 63, 64, 100, 101, 127, 128)):
+        if t < s:
+            p["log_retain"][:, t] = math.log(RETAIN[i % 5])
+    r = torch.exp(p["log_retain"].double())
+    want = reference(p, 0.5, p["d_y"], p["d_m"])["d_log_retain"] / r
+    got = run(p, 0.5)["d_log_retain"].double() / r
+    assert float((got - want).abs().max()) <= TOL["d_log_retain"] * float(want.abs().max())
+
+
+@pytest.mark.parametrize("retain", [0.5, *RETAIN[:4], 0.0])
+def test_memory_gradient_at_saturated_gates(retain):
+    """gated_delta_memory for alpha near and at 1: the gradient of alpha against 64 bits, and small alphas that 1 - alpha would lose."""
+    from nl_hecate_b200.stacked_mag import gated_delta_memory
+    g = torch.Generator(device="cuda").manual_seed(3)
+    n = lambda *sh: torch.randn(*sh, generator=g, device="cuda")
+    unit = lambda t: torch.nn.functional.normalize(t, dim=-1)
+    a = dict(k=unit(n(4, 150, 32)), v=n(4, 150, 32), q=unit(n(4, 150, 32)), alpha=0.3 * torch.sigmoid(n(4, 150)), theta=torch.sigmoid(n(4, 150)))
+    a["alpha"][:, [0, 9, 10, 50, 63, 64, 130]] = 1.0 - retain
+    a["alpha"][:, 70:110] = 1e-9
+    m0, d_y = 0.3 * n(4, 32 * 32), n(4, 150, 32)
+    leaves = {x: t.clone().requires_grad_(True) for x, t in a.items()}
+    exact = {x: t.double().requires_grad_(True) for x, t in a.items()}
+    y, _ = gated_delta_memory(*leaves.values(), None, m0, 64)
+    w, _ = gated_delta_ref(*exact.values(), None, m0.double(), 64)
+    got, want = torch.autograd.grad(y, list(leaves.values()), d_y), torch.autograd.grad(w, list(exact.values()), d_y.double())
+    for x, u, v in zip(a, got, want):
+        tol = TOL["d_log_retain"] if x == "alpha" else TOL["d_" + x]
+        assert float((u.double() - v).abs().max()) <= tol * float(v.abs().max()), x
+    assert float((y.detach().double() - w.detach()).abs().max()) <= TOL["y"] * float(w.detach().abs().max())
