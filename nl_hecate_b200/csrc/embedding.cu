@@ -215,12 +215,12 @@ __global__ void __launch_bounds__(SORT_THREADS) scatter_kernel(const int* ids, c
         if (key[j] >= 0) out[s_cnt[w][(key[j] >> shift) & (BINS - 1)] + rank[j]] = make_int2(key[j], pos[j]);
 }
 
-// The whole sort in one launch up to 131072 tokens: a cluster of CL CTAs, a thread ITEMS tokens, the digits' totals exchanged
-// through distributed shared memory, digits only as wide as the passes need. CL is 16 where the device can hold such a cluster,
-// else 8. 32768 tokens of a vocabulary of 8192 take 12 us (8 CTAs: 15; the launches above: 27 and the gaps between them), 65521 of
-// 50001 take 19 (26; 37). Tokens of one digit in a warp are found by a ballot per bit (a match instruction: 16 us with 8 CTAs).
-constexpr int CL_THREADS = 1024, CL_WARPS = CL_THREADS / 32, CL_MOST = 131072;
-template <int ITEMS, int CL>
+// The whole sort in one launch up to 131072 tokens: a cluster of sixteen CTAs, a thread ITEMS tokens, the digits' totals exchanged
+// through distributed shared memory, digits only as wide as the passes need. A device (or a part of one) that cannot hold such a
+// cluster takes the launches above. 32768 tokens of a vocabulary of 8192 take 12 us (the launches above: 27 and the gaps between
+// them), 65521 of 50001 take 19 (37). Tokens of one digit in a warp are found by a ballot per bit, which beat a match instruction.
+constexpr int CL = 16, CL_THREADS = 1024, CL_WARPS = CL_THREADS / 32, CL_MOST = CL * CL_THREADS * 8;
+template <int ITEMS>
 __global__ void __launch_bounds__(CL_THREADS, 1) sort_cluster_kernel(const int* ids, int2* bufa, int2* bufb, int n,
                                                                                                int vocab, int passes, int bits)
 {
@@ -529,12 +529,12 @@ static int lanes_for(int d, int per, int most)
     return l;
 }
 
-template <int ITEMS, int CL> static cudaError_t sort_cluster(const int* ids, const Plan& P, int n, int vocab, bool* fits)
+template <int ITEMS> static cudaError_t sort_cluster(const int* ids, const Plan& P, int n, int vocab, bool* fits)
 {
     constexpr int bytes = (CL_WARPS + 2) * BINS * 4;
-    const auto kernel = sort_cluster_kernel<ITEMS, CL>;
+    const auto kernel = sort_cluster_kernel<ITEMS>;
     cudaError_t e = cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, bytes);
-    if (e == cudaSuccess && CL > 8) e = cudaFuncSetAttribute(kernel, cudaFuncAttributeNonPortableClusterSizeAllowed, 1);
+    if (e == cudaSuccess) e = cudaFuncSetAttribute(kernel, cudaFuncAttributeNonPortableClusterSizeAllowed, 1);
     if (e != cudaSuccess) return e;
     cudaLaunchAttribute at;
     at.id = cudaLaunchAttributeClusterDimension;
@@ -555,13 +555,11 @@ template <int ITEMS, int CL> static cudaError_t sort_cluster(const int* ids, con
     }
     return cudaLaunchKernelEx(&c, kernel, ids, P.a, P.b, n, vocab, P.passes, P.bits);
 }
-template <int CL> static bool sort_with(const int* ids, const Plan& P, int n, int vocab, const char* where)
+static bool sort_in_one(const int* ids, const Plan& P, int n, int vocab, const char* where)
 {
-    constexpr int MOST = CL_MOST / (CL * CL_THREADS);           // tokens a thread of the longest list
     const int items = (n + CL * CL_THREADS - 1) / (CL * CL_THREADS);
-    const cudaError_t e = items <= 2 ? sort_cluster<2, CL>(ids, P, n, vocab, nullptr)
-                          : items <= MOST / 2 ? sort_cluster<MOST / 2, CL>(ids, P, n, vocab, nullptr)
-                                              : sort_cluster<MOST, CL>(ids, P, n, vocab, nullptr);
+    const cudaError_t e = items <= 2 ? sort_cluster<2>(ids, P, n, vocab, nullptr)
+                          : items <= 4 ? sort_cluster<4>(ids, P, n, vocab, nullptr) : sort_cluster<8>(ids, P, n, vocab, nullptr);
     if (e != cudaSuccess) record_status(NLH_ERR_CUDA, where, cudaGetErrorString(e));
     return e == cudaSuccess;
 }
@@ -574,7 +572,7 @@ static bool wide_clusters(const Plan& P)
     int k = known[dev].load(std::memory_order_relaxed);
     if (k == 0) {
         bool fits = false;
-        if (sort_cluster<8, 16>(nullptr, P, 0, 1, &fits) != cudaSuccess) { cudaGetLastError(); fits = false; }
+        if (sort_cluster<8>(nullptr, P, 0, 1, &fits) != cudaSuccess) { cudaGetLastError(); fits = false; }
         k = fits ? 2 : 1;
         known[dev].store(k, std::memory_order_relaxed);
     }
@@ -593,8 +591,8 @@ static bool backward(const T* dy, const int* ids, float* dw, int n, int vocab, i
         return check_launch(where);
     }
     const int2* in = nullptr;
-    if (n <= CL_MOST) {
-        if (!(wide_clusters(P) ? sort_with<16>(ids, P, n, vocab, where) : sort_with<8>(ids, P, n, vocab, where))) return false;
+    if (n <= CL_MOST && wide_clusters(P)) {
+        if (!sort_in_one(ids, P, n, vocab, where)) return false;
         in = P.passes & 1 ? P.a : P.b;
     } else {
         int2* out = P.a;
