@@ -495,10 +495,13 @@ struct Plan {
     int *hist, *total;
     float* part;
 };
-// The single launch adds the rows of a frequent id one after the other, the sorted path costs 18 to 27 us whatever its size. us, one
-// launch | sorted (ids drawn as 1 / rank^1.1, vocabulary 256): width 64, 2048 tokens 10.4 | 21.6; 512, 2048: 22.1 | 20.6;
-// 1024, 1024: 20.5 | 20.6 and 2048: 39.3 | 20.6. With the tokens every CTA's search of the list grows (width 64, 8192: 30.9 | 20.6).
-static bool one_launch(int n, int d) { return n <= SMALL && (int64_t)n * d <= (1 << 20); }
+// The single launch adds the rows of one id by one CTA, so its time goes by the most frequent id; the sorted path takes 15 to 23 us
+// whatever the ids. us, one launch | sorted, fp32, for ids drawn as 1 / rank^1.1 of 256, and for a list of one id (padding, at worst):
+//   tokens x width  512 x 64      1024 x 64     256 x 512     1024 x 128    256 x 1024    2048 x 512
+//   drawn           5.2 | 16.9    7.7 | 17.0    8.1 | 15.7    9.7 | 16.7    12.9 | 15.6   43.1 | 18.6
+//   one id          8.8 | 15.4    15.6 | 15.8   24.8 | 14.7   26.2 | 15.6   47.6 | 14.9   184 | 17.1
+// (bf16 within a tenth of these.) Up to 2^17 elements it gains more on drawn ids than it loses on one.
+static bool one_launch(int n, int d) { return n <= SMALL && (int64_t)n * d <= (1 << 17); }
 
 static int64_t place(Plan& P, char* base, int n, int vocab, int d)
 {
