@@ -1227,9 +1227,12 @@ template <typename T, int DKP> static bool launch_states(const Args& A, bool bac
     const long long heads = (long long)(A.n_seqs > 0 ? A.n_seqs : A.batch) * A.hv;
     if (heads == 0) return true;
     // 16 columns a CTA while each of those CTAs finds an SM of its own (forward + backward, 2 x 8 heads of 128 x 128: 39 + 43 us against
-    // 60 + 69 with 32 columns; 3 x 16 of 64 x 64, which does not: 83 + 99 against 80 + 93), and for packed batches longer, since
-    // their few longest sequences run alone in the end (13 prompts x 8 heads: 72 + 80 us against 95 + 111)
-    if (A.n_seqs > 0 ? heads * (A.dvp / 32) < 4 * 148 : heads * (A.dvp / 16) <= 148) return launch_states_ns<T, DKP, 16>(A, heads, backward, st, where);
+    // 60 + 69 with 32 columns; 3 x 16 of 64 x 64, which does not: 83 + 99 against 80 + 93). For packed batches longer, since their few
+    // longest sequences run alone in the end: up to three CTAs of 32 columns an SM where two fit one, up to two where one does. Whole pass,
+    // 16 | 32 columns, bf16, lengths drawn from x^3 (CTAs of 32 columns): dk 64: 495 | 539 us (208), 420 | 476 (416), 167 | 155 (600),
+    // 440 | 414 (640); dk 128: 322 | 420 (104), 280 | 336 (208), 291 | 274 (320), 855 | 793 (416). Equal lengths: 0 to 8 % the other way.
+    const bool narrow = A.n_seqs > 0 ? heads * (A.dvp / 32) < (DKP == 64 ? 3 : 2) * 148 : heads * (A.dvp / 16) <= 148;
+    if (narrow) return launch_states_ns<T, DKP, 16>(A, heads, backward, st, where);
     return launch_states_ns<T, DKP, 32>(A, heads, backward, st, where);
 }
 
