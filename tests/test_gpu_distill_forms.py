@@ -104,3 +104,13 @@ def saved_of(z, ids, t, y):
     from nl_hecate_b200 import dispatch as D
     n = z.shape[0]
     return D.distill_forward(z, ids[:n].contiguous(), t[:n].contiguous(), targets=y[:n].contiguous(), temperature=2.0, hard_weight=0.5)[1]
+
+
+@pytest.mark.parametrize("dtype", [torch.float32, torch.bfloat16])
+@pytest.mark.parametrize("tau,sw,hw", MODES)
+@pytest.mark.parametrize("n,vocab,k", [(4096, 12288, 7), (4097, 12289, 7), (5001, 513, 40), (150, 16400, 33), (149, 40003, 5), (150, 16384, 3)])
+def test_the_sizes_that_choose_a_kernel(n, vocab, k, tau, sw, hw, dtype):
+    """A warp per row (4096 rows and more, up to 12288 columns), a CTA of 128 or (above 16384 columns) 256 threads per row, none of them
+    divided."""
+    z, ids, t, y = make(n, vocab, k, dtype, seed=vocab)
+    close(z, ids, t, y, tau, sw, hw)

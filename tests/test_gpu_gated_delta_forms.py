@@ -8,7 +8,7 @@ import pytest
 import torch
 
 sys.path.insert(0, os.path.dirname(os.path.abspath(__file__)))
-from test_gpu_gated_delta import TOL, inputs, packed, reference, run  # noqa: E402
+from test_gpu_gated_delta import TOL, check, inputs, packed, reference, run  # noqa: E402
 from test_gpu_language_step import gated_delta_ref  # noqa: E402
 
 pytestmark = pytest.mark.gpu
@@ -120,3 +120,53 @@ def test_memory_gradient_at_saturated_gates(retain):
         tol = TOL["d_log_retain"] if x == "alpha" else TOL["d_" + x]
         assert float((u.double() - v).abs().max()) <= tol * float(v.abs().max()), x
     assert float((y.detach().double() - w.detach()).abs().max()) <= TOL["y"] * float(w.detach().abs().max())
+
+
+DTYPES = [torch.float32, torch.bfloat16]
+STREAM_NAMES = ("k", "v", "q", "log_retain", "theta")
+
+
+@pytest.mark.parametrize("dtype", DTYPES)
+@pytest.mark.parametrize("b,s,hk,hv,dk,dv", [(10, 150, 4, 4, 64, 64), (5, 130, 2, 4, 128, 128), (38, 70, 1, 1, 128, 64), (38, 66, 1, 1, 64, 128),
+                                             (38, 200, 1, 1, 7, 5), (13, 65, 1, 3, 100, 33)])
+def test_pair_with_many_heads(b, s, hk, hv, dk, dv, dtype):
+    """More than 148 CTAs of 16 columns: the state kernels of 32 columns, over several chunks, in both directions."""
+    p = inputs(b, s, hk, hv, dk, dv, dtype, seed=s)
+    check(run(p, 0.5), reference(p, 0.5, p["d_y"], p["d_m"]), dtype)
+
+
+@pytest.mark.parametrize("dtype", DTYPES)
+@pytest.mark.parametrize("n,hk,hv,dk,dv", [(230, 1, 2, 64, 64), (300, 1, 1, 64, 40), (80, 1, 2, 128, 64), (75, 2, 2, 96, 128)])
+def test_packed_batch_of_many_sequences(n, hk, hv, dk, dv, dtype):
+    """The same kernels for packed batches, up to 256 sequences and more, some empty, some of three chunks."""
+    lengths = tuple((53 * i) % 140 if i % 9 else 0 for i in range(n))
+    p, starts, at = packed(lengths, hk, hv, dk, dv, dtype, before=2, behind=3)
+    out = run(p, 0.5, starts=starts)
+    for x in ("y", "d_k", "d_v", "d_q", "d_log_retain", "d_theta"):
+        assert not out[x][:, :2].any() and not out[x][:, at[-1]:].any(), x
+    for i in {1, 2, n // 2 + 1, n - 1, lengths.index(max(lengths)), lengths.index(0)}:
+        e = slice(at[i], at[i + 1])
+        if lengths[i] == 0:
+            assert torch.equal(out["m_final"][i], p["m0"][i]) and torch.equal(out["d_m_initial"][i], p["d_m"][i])
+            continue
+        q = {x: p[x][:, e] for x in STREAM_NAMES} | {"m0": p["m0"][i:i + 1]}
+        got = {x: out[x][:, e] for x in ("y", "d_k", "d_v", "d_q", "d_log_retain", "d_theta")}
+        got |= {"m_final": out["m_final"][i:i + 1], "d_m_initial": out["d_m_initial"][i:i + 1]}
+        check(got, reference(q, 0.5, p["d_y"][:, e], p["d_m"][i:i + 1]), dtype, f"sequence {i}")
+
+
+@pytest.mark.parametrize("dtype", DTYPES)
+@pytest.mark.parametrize("b,s,hk,hv,dk,dv", [(75, 1, 2, 4, 128, 128), (150, 2, 1, 2, 72, 100), (300, 1, 1, 1, 97, 64)])
+def test_step_of_a_full_batch(b, s, hk, hv, dk, dv, dtype):
+    """64 rows of a state a CTA where that gives every SM two."""
+    from nl_hecate_b200 import dispatch as D
+    p = inputs(b, s, hk, hv, dk, dv, dtype, seed=b)
+    want = reference(p, 0.5)
+    slots = torch.randperm(b + 3, device="cuda")[:b].to(torch.int32)
+    pool = torch.full((b + 3, hv, dv, dk), 3.0, device="cuda")
+    pool[slots.long()] = p["m0"]
+    y = D.gated_delta_step(*[p[x] for x in STREAM_NAMES], pool, slots=slots, scale=0.5)
+    check({"y": y, "m_final": pool[slots.long()]}, want, dtype)
+    free = torch.ones(b + 3, dtype=torch.bool, device="cuda")
+    free[slots.long()] = False
+    assert bool((pool[free] == 3.0).all())
