@@ -103,7 +103,7 @@ __global__ void __launch_bounds__(256, 3) gd_prep_kernel(Args A)
     const long long tile = (long long)slot * A.hv + h;
     const int tid = threadIdx.x, lane = tid & 31, w = tid >> 5, rb = w & 3, hf = w >> 2, g = lane >> 2, t = lane & 3;
 
-    if (w == 7) {                                 // a warp whose part of K K^T is upper triangle, or little else
+    if (w == 4) {                                 // all of its part of K K^T is above the diagonal
         const long long at = ch.b * A.gb + ch.t0 * A.gt + h * A.gh;
         double x[2], th[2];
 #pragma unroll
