@@ -560,7 +560,8 @@ int32_t nlh_distill_backward(const void* logits, int32_t logits_is_bf16, int64_t
  * Packed batches: batch = 1, n_seqs > 0, seq_starts [n_seqs + 1] on the device, sequence i = tokens
  * seq_starts[i] .. seq_starts[i + 1] - 1. Starts are clamped to [0, seq] and to their running maximum; a sequence may be
  * empty (m_final = m_initial); tokens outside the sequences are not read, and their rows of y and of the gradients are not written.
- * A log_retain below -200 counts as -200 (e^-200 is 0 in fp32), a theta below 2^-60 in magnitude as 2^-60. In the forward a NaN or an
+ * A log_retain below -200 counts as -200 (e^-200 is 0 in fp32), a theta below 2^-60 in magnitude as 2^-60. Positive ones whose sum
+ * over 64 tokens passes 88 overflow (e^88), also where the state they multiply is 0. In the forward a NaN or an
  * infinity reaches the outputs that it reaches token by token, and no others; an infinity, or a value above 3.39e38, may arrive as a
  * NaN. In the backward it may make any gradient of its sequence a NaN. */
 typedef struct nlh_gated_delta_desc {

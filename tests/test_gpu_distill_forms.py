@@ -114,3 +114,10 @@ def test_the_sizes_that_choose_a_kernel(n, vocab, k, tau, sw, hw, dtype):
     divided."""
     z, ids, t, y = make(n, vocab, k, dtype, seed=vocab)
     close(z, ids, t, y, tau, sw, hw)
+
+
+@pytest.mark.parametrize("tau", [1e-6, 1e-4, 1e-2, 1e4, 1e6])
+def test_temperatures_at_their_limits(tau):
+    """At the lowest the softmax is its maximum's alone, at the highest uniform; exponents are rounded relative to themselves."""
+    z, ids, t, y = make(70, 200, 6, torch.float32, seed=5)
+    close(10 * z, ids, t, y, tau, 0.5, 0.5)
