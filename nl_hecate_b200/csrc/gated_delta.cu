@@ -374,12 +374,14 @@ __global__ void __launch_bounds__(256, DKP == 64 ? 2 : 1) gd_state_fwd_kernel(Ar
                 any |= odd(x.x) | odd(x.y);
                 put2<3>(Rs + row * LS + H * hf + 8 * n + 2 * t, L::PR, x.x, x.y);
             }
-        if (s_dead == 0 && !wait_t(&s_bar, buf, A.wait_cycles)) s_dead = 1;
+        any |= not_arrived(&s_dead, &s_bar, buf, A.wait_cycles);
         any = __syncthreads_or(any);
         zero(acc);
-        if (any) triangle_by_token<3, NT>(acc, Ts, C * LP, Rs, LS, L::PR, 16 * rb, H * hf);
+        if (any) {
+            if (lost_t(&s_dead, &s_bar, buf)) fill_nan(acc);
+            else triangle_by_token<3, NT>(acc, Ts, C * LP, Rs, LS, L::PR, 16 * rb, H * hf);
+        }
         else gemm<NT, false, true, 3, 3>(acc, Ts + 16 * rb * LP, LP, C * LP, Rs + H * hf, LS, L::PR, 0, 16 * (rb + 1));
-        if (lost_t(&s_dead, &s_bar, buf)) fill_nan(acc);
 #pragma unroll
         for (int n = 0; n < NT; n++)
 #pragma unroll
@@ -677,11 +679,10 @@ __global__ void __launch_bounds__(256, DKP == 64 ? 2 : 1) gd_state_bwd_kernel(Ar
                 const float wi = s_gate[buf][row].w, th = s_theta[buf][row];
                 put2<3>(Rs + row * LS + H * hf + 8 * n + 2 * t, L::PR, th * (f[n][r].x + wi * acc[n][2 * r]), th * (f[n][r].y + wi * acc[n][2 * r + 1]));
             }
-        if (s_dead == 0 && !wait_t(&s_bar, buf, A.wait_cycles)) s_dead = 1;
-        __syncthreads();
+        const bool lost = __syncthreads_or(not_arrived(&s_dead, &s_bar, buf, A.wait_cycles));
         zero(acc);
-        gemm<NT, true, true, 3, 3>(acc, Ts + 16 * rb, LP, C * LP, Rs + H * hf, LS, L::PR, 16 * rb, C);
-        if (lost_t(&s_dead, &s_bar, buf)) fill_nan(acc);
+        if (lost) { lost_t(&s_dead, &s_bar, buf); fill_nan(acc); }
+        else gemm<NT, true, true, 3, 3>(acc, Ts + 16 * rb, LP, C * LP, Rs + H * hf, LS, L::PR, 16 * rb, C);
         float* xp = A.x + e_at;
 #pragma unroll
         for (int n = 0; n < NT; n++)

@@ -479,7 +479,15 @@ template <int NT> __device__ __forceinline__ void fill_nan(float (&acc)[NT][4])
 #pragma unroll
         for (int i = 0; i < 4; i++) acc[n][i] = __int_as_float(0x7fffffff);
 }
-// Behind the barrier that follows the wait: whether the copy has not come (the same for all threads, and from now on).
+// The wait of a chunk: whether its copy, or one before it, has not come. The answers of a CTA's threads meet in the barrier behind it.
+__device__ __forceinline__ bool not_arrived(int* dead, unsigned long long* bar, unsigned parity, unsigned cycles)
+{
+    if (cycles > 0 && test_t(bar, parity)) return false;
+    if (*dead == 0 && wait_t(bar, parity, cycles)) return false;
+    if (*dead == 0) *dead = 1;
+    return true;
+}
+// Behind that barrier, where a thread answered so: whether a copy is lost (the same for all threads, and from now on).
 __device__ __forceinline__ bool lost_t(int* dead, unsigned long long* bar, unsigned parity)
 {
     const int d = *dead;                          // 1: not reported yet
