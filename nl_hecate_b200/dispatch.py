@@ -412,11 +412,11 @@ def _need(where, name, t, dtype, shape):
                          f"got {t.dtype} {tuple(t.shape)}")
 
 
-def _int32(where, **sizes):
-    """The C entries' sizes are 32 bits wide, and ctypes would cut a larger one off."""
-    for name, x in sizes.items():
-        if x >= 1 << 31:
-            raise ValueError(f"{where}: {name} is {x}, need less than 2^31")
+_INT32 = 2 ** 31 - 1     # the C entries' sizes are 32 bits wide, and ctypes would cut a larger one off
+
+
+def _too_large(where, **sizes):
+    raise ValueError(f"{where}: need sizes below 2^31, got {sizes}")
 
 
 def _gated_delta_desc(where, k, v, q, log_retain, theta, scale, n_seqs, d_y=None):
@@ -536,7 +536,8 @@ def gated_delta_step(k, v, q, log_retain, theta, m, slots=None, scale=1.0):
     _need(where, "m", m, torch.float32, (m.shape[0], v.shape[2], v.shape[3], k.shape[3]))
     if slots is not None:
         _need(where, "slots", slots, torch.int32, (k.shape[0],))
-    _int32(where, states=m.shape[0])
+    if m.shape[0] > _INT32:
+        _too_large(where, states=m.shape[0])
     y = torch.empty(v.shape, dtype=v.dtype, device=k.device)
     _run("nlh_gated_delta_step", device, desc, k.data_ptr(), v.data_ptr(), q.data_ptr(), log_retain.data_ptr(),
          theta.data_ptr(), m.data_ptr(), _ptr(slots), m.shape[0], y.data_ptr())
@@ -572,7 +573,8 @@ def embedding_forward(w, ids, scale=1.0):
         raise ValueError(f"{where}.w: need a contiguous fp32 or bf16 [vocab, d]")
     _ids32(where, "ids", ids)
     vocab, d = w.shape
-    _int32(where, ids=ids.numel(), vocab=vocab, d=d)
+    if ids.numel() > _INT32 or vocab > _INT32 or d > _INT32:
+        _too_large(where, ids=ids.numel(), vocab=vocab, d=d)
     out = torch.empty(*ids.shape, d, dtype=w.dtype, device=w.device)
     _run("nlh_embedding_forward", device, w.data_ptr(), w.dtype == torch.bfloat16, ids.data_ptr(), out.data_ptr(), ids.numel(),
          vocab, d, scale)
@@ -592,7 +594,8 @@ def embedding_backward(d_out, ids, d_w, scale=1.0, accumulate=True):
         raise ValueError(f"{where}.d_out: need a contiguous fp32 or bf16 {(*ids.shape, d)}, got {d_out.dtype} {tuple(d_out.shape)}")
     _ids32(where, "ids", ids)
     n = ids.numel()
-    _int32(where, ids=n, vocab=vocab, d=d)
+    if n > _INT32 or vocab > _INT32 or d > _INT32:
+        _too_large(where, ids=n, vocab=vocab, d=d)
     nbytes = _bytes(where, ffi.lib().nlh_embedding_backward_bytes, n, vocab, d)
     work = torch.empty(nbytes, dtype=torch.uint8, device=d_w.device) if nbytes else None
     _run("nlh_embedding_backward", device, d_out.data_ptr(), d_out.dtype == torch.bfloat16, ids.data_ptr(), d_w.data_ptr(), n, vocab,
@@ -629,7 +632,8 @@ def distill_forward(logits, teacher_ids, teacher_logits, targets=None, temperatu
         raise ValueError(f"{where}.teacher_logits: need contiguous fp32 or bf16")
     if targets is not None:
         _ids32(where, "targets", targets, n)
-    _int32(where, rows=n, vocab=vocab, entries=teacher_ids.shape[1])
+    if n > _INT32 or vocab > _INT32 or teacher_ids.shape[1] > _INT32:
+        _too_large(where, rows=n, vocab=vocab, entries=teacher_ids.shape[1])
     s = DistillSaved()
     s.targets, s.ids, s.teacher, s.shape, s.dtype = targets, teacher_ids, teacher_logits, logits.shape, logits.dtype
     s.k, s.weights = teacher_ids.shape[1], (temperature, hard_weight, soft_weight)
