@@ -15,9 +15,12 @@
 // pass, but then a prompt's y and the recurrent step's, which works in fp32, were of different accuracy.) Two tf32 numbers for a fp32 one take the same time on the tensor cores, but their splitting,
 // redone by every warp that reads them, and twice the instructions around each pass cost more: a training step of 64 sequences
 // x 8 heads x 512 tokens took 1435 us that way against 1308 (4 x 16 x 4096 in bf16: 1336 against 1122).
-// Why not tcgen05: the matrices are 64 x 64 x 64 and each depends on the one before it. One M64 N64 K16 tcgen05.mma takes 55
-// cycles (1190 multiply-adds a cycle), mma.sync does 983, and its results are in registers where the next product needs
-// them; tcgen05 needs a commit, a wait and a trip through TMEM and shared memory for each.
+// Why not tcgen05: in the kernels that walk the states the matrices are 64 x 64 x 64 and each depends on the one before it. One M64
+// N64 K16 tcgen05.mma takes 55 cycles (1190 multiply-adds a cycle), mma.sync does 983, and its results are in registers where the
+// next product needs them; tcgen05 needs a commit, a wait and a trip through TMEM and shared memory for each. That does not
+// hold for the kernels that form the outputs of all chunks: there tiles could be stacked to 128 x 128, and no product waits for
+// another chunk's. They run on mma.sync too, bound by the shared-memory path and latency; what stands against tcgen05 there is the sum of
+// many k-steps in one accumulator, which the tensor core cuts off instead of rounding (see gemm), for fp32 streams.
 #pragma once
 
 #include <cuda_bf16.h>
